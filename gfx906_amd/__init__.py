@@ -7,6 +7,9 @@ strided views with a contiguous head dim are read in place) and returns a new
 tensor of the input dtype, or writes ``out``. It raises if the HIP libraries
 are not built or the inputs are not accepted; there is no fallback
 implementation.
+
+``gfx906_amd.kv4`` holds a paged key/value cache in 4 bits with the attention over
+it, ``gfx906_amd.sparse`` attention over the key blocks that a score selects.
 """
 
 from .loader import (KERNEL_LIB, EXT_LIB, NotBuiltError, capi, extension,  # noqa: F401

@@ -3,12 +3,12 @@
 Two shared objects and one program are produced under ``gfx906_amd/lib/``:
 
 * ``libgfx906_amd_attn.so`` -- the HIP kernels and the C ABIs declared in
-  ``include/gfx906_amd_attn.h`` and ``include/gfx906_amd_conv3d.h``, compiled
-  by ``hipcc --offload-arch=gfx950``. It plays the part of the reference's
+  ``include/gfx906_amd_attn.h``, ``gfx906_amd_conv3d.h``, ``gfx906_amd_kv4.h``
+  and ``gfx906_amd_sparse.h``, compiled by ``hipcc --offload-arch=gfx950``. It plays the part of the reference's
   separately compiled kernel objects (``attn_kernel.gfx906.o``,
   ``conv3d_kernel.<arch>.o``; README.md:12, deploy/gfx906_attn.py:40-59).
-* ``gfx906_amd_attn_ext.so`` -- the PyTorch binding (``attn(q, k, v, scale)``
-  and ``conv3d(...)``), built the way the reference builds its own
+* ``gfx906_amd_attn_ext.so`` -- the PyTorch binding (``attn(q, k, v, scale)``,
+  ``conv3d(...)`` and the ops of ``kv4`` and ``sparse``), built the way the reference builds its own
   (README.md:13, deploy/gfx906_attn.py:77-83): ``torch.utils.cpp_extension
   .load`` over the plain C++ binding sources with the kernel library in
   ``extra_ldflags``. The build directory is ``gfx906_amd/lib`` itself, so the
@@ -59,12 +59,14 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-mfma-vgpr-form=1",
 ]
 
-KERNEL_SOURCES = [CSRC / "attn_kernel.hip", CSRC / "conv3d_kernel.hip", CSRC / "scratch.hip"]
+KERNEL_SOURCES = [CSRC / "attn_kernel.hip", CSRC / "conv3d_kernel.hip", CSRC / "scratch.hip",
+                  CSRC / "kv4_kernel.hip", CSRC / "sparse_kernel.hip"]
 # A torch-free C caller of launch() (the reference's micro3.hip pattern),
 # linked against the kernel library.
 HARNESS_SOURCE = CSRC / "launch_harness.cpp"
 HARNESS = LIB / "launch_harness"
-BINDING_SOURCES = [CSRC / "attn.cpp", CSRC / "conv3d.cpp", CSRC / "module.cpp"]
+BINDING_SOURCES = [CSRC / "attn.cpp", CSRC / "conv3d.cpp", CSRC / "kv4.cpp", CSRC / "sparse.cpp",
+                   CSRC / "module.cpp"]
 # The binding is host C++ only; HIP types come from the runtime headers.
 EXT_CFLAGS = ["-O2", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
 EXT_LDFLAGS = [f"-L{LIB}", "-lgfx906_amd_attn", "-lc10_hip", "-ltorch_hip",
@@ -146,7 +148,7 @@ def _newest_mtime(paths) -> float:
 
 
 def kernel_lib_inputs() -> list:
-    return [*KERNEL_SOURCES, CSRC / "scratch.h", *sorted(CSRC.glob("*.inc")),
+    return [*KERNEL_SOURCES, CSRC / "scratch.h", CSRC / "longctx.h", *sorted(CSRC.glob("*.inc")),
             *sorted(INCLUDE.glob("*.h"))]
 
 

@@ -1,0 +1,474 @@
+"""The 4-bit cache on the GPU against the CPU oracle in 64 bits: pages and slots,
+storing and reading, attention over it, and a run of them together."""
+
+import math
+
+import pytest
+import torch
+
+from gfx906_amd import kv4
+from oracle import longctx as oc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# -- pages and slots ----------------------------------------------------------------------
+
+PLANS = [  # lens, new, page, table width, free pages, used, extra slots
+    ([0], [1], 64, 1, 1, 0, 0),
+    ([0, 0], [0, 0], 64, 2, 0, 0, 3),
+    ([63, 64, 65], [1, 1, 1], 64, 3, 2, 1, 0),
+    ([5, 0, 700, 128, 1], [300, 1, 0, 129, 64], 128, 7, 12, 2, 9),
+    ([0, 10, 20], [1000, 2000, 3], 256, 20, 30, 0, 0),
+    ([0, 100, 60], [500, 100, 300], 64, 4, 6, 0, 2),      # list and rows end early
+    ([-3, 7], [5, -2], 64, 2, 2, 0, 0),                   # negative counts are 0
+    (list(range(300)), [k % 5 for k in range(300)], 64, 8, 300, 0, 5),
+    ([17] * 4096, [1] * 4096, 64, 1, 0, 0, 0),
+]
+
+
+@pytest.mark.parametrize("case", range(len(PLANS)))
+def test_plan_pages(case):
+    lens, new, page, W, n_free, used, extra = PLANS[case]
+    print(f"plan {case}", flush=True)
+    g = torch.Generator().manual_seed(case)
+    phys = torch.randperm(n_free + len(lens) * W, generator=g).tolist()
+    free, phys = phys[:n_free], phys[n_free:]
+    table = [[phys[b * W + k] if k < -(-max(0, n) // page) else -1 for k in range(W)]
+             for b, n in enumerate(lens)]
+    tokens = sum(max(0, n) for n in new) + extra
+    wide = torch.full((len(lens), W + 3), -7, dtype=torch.int32, device=DEV)  # strided rows
+    wide[:, :W] = i32(table)
+    plan = kv4.plan_pages(i32(lens), i32(new), wide[:, :W], i32(free), i32([used]), page, tokens)
+    want = oc.plan_pages(lens, new, table, free, used, page, tokens)
+    for got, ref in zip((*plan, wide[:, :W]), (want[0], want[1], want[2], [want[3]], [want[4]],
+                                               want[5])):
+        assert got.tolist() == ref
+    assert wide[:, W:].eq(-7).all()
+    # The call reads what it does not write: again with the same arguments, the same result.
+    again = kv4.plan_pages(i32(lens), i32(new), wide[:, :W], i32(free), i32([used]), page, tokens)
+    assert all(torch.equal(a, b) for a, b in zip(plan, again))
+
+
+def test_plan_pages_with_a_short_slot_list():
+    plan = kv4.plan_pages(i32([0, 0]), i32([70, 3]), i32([[-1, -1], [-1, -1]]), i32([4, 5, 6]),
+                          i32([0]), 64, 10)
+    assert plan.slots.tolist() == list(range(256, 266)) and plan.cu_new.tolist() == [0, 70, 73]
+
+
+def test_plan_pages_refuses():
+    a = dict(lens=i32([1]), new_lens=i32([1]), table=i32([[0]]), free_pages=i32([1]), used=i32([0]),
+             page=64, tokens=1)
+    for bad in (dict(lens=i32([1]).long()), dict(new_lens=i32([1, 2])), dict(page=100),
+                dict(tokens=-1), dict(table=i32([0])), dict(table=i32([[0], [1]])),
+                dict(used=i32([0, 0])), dict(free_pages=torch.zeros(2, dtype=torch.int32)),
+                dict(lens=i32([1, 1]), new_lens=i32([1, 1]), table=i32([[0]]).expand(2, 1)),
+                dict(free_pages=None)):
+        with pytest.raises((RuntimeError, TypeError)):
+            kv4.plan_pages(**(a | bad))
+    t = i32([[0]])
+    with pytest.raises(RuntimeError):
+        kv4.plan_pages(**(a | dict(table=t, free_pages=t[0])))
+
+
+# -- storing and reading ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,D,page", [(1, 1, 64, 64), (5, 3, 128, 64), (130, 2, 64, 128),
+                                        (300, 5, 128, 256)])
+def test_store_is_exact(T, H, D, page, dtype):
+    print(f"store T{T} H{H} D{D} page {page} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(T + H)
+    pages = T // page + 3
+    x = torch.randn(2, T, H, D, generator=g) * torch.exp2(
+        torch.randint(-12, 9, (2, T, H, 1), generator=g).float())
+    x[0, 0, 0, :32] = 0
+    x[1, -1, -1, 32:40] = torch.tensor([6.0, 7.0, 5.0, 2.5, 0.75, 0.25, 3.5, 1.25])
+    if T > 4:   # special blocks
+        x[0, 1, 0, 3], x[0, 2, 0, 33], x[0, 3, 0, 0] = math.nan, math.inf, -math.inf
+        x[1, 1, 0, :32] = 2.0 ** -24
+        x[1, 2, 0, :32] = 65504.0 if dtype == torch.float16 else 3.0e38
+    k, v = (t.to(dtype) for t in x)
+    slots = torch.randperm(pages * page, generator=g)[:T].int()
+    cache = kv4.new_cache(pages, page, H, D)
+    kv4.store(cache, k.to(DEV), v.to(DEV), slots.to(DEV))
+    host = kv4.Cache(*(t.cpu() for t in cache))
+    for x, codes, scales in ((k, host.k, host.k_scale), (v, host.v, host.v_scale)):
+        c, e = oc.quantise(x)
+        held = torch.zeros(pages, page, dtype=torch.bool)
+        for t, s in enumerate(slots.tolist()):
+            gc, ge = oc.read_cache(codes, scales, s // page, s % page)
+            ok = (ge != 255).repeat_interleave(32, -1)
+            assert torch.equal(ge, e[t]) and torch.equal(gc[ok], c[t].int()[ok]), (t, s)
+            held[s // page, s % page] = True
+        assert codes.transpose(1, 2)[~held].eq(0).all()   # other tokens untouched
+    gk, gv = kv4.load(cache, slots.to(DEV), dtype)
+    for x, got in ((k, gk), (v, gv)):
+        want = oc.dequantise(*oc.quantise(x)).to(dtype)
+        assert torch.equal(got.cpu().nan_to_num(9.0, 8.0, 7.0), want.nan_to_num(9.0, 8.0, 7.0))
+
+
+def test_store_and_load_pass_over_slots_outside_and_read_strided_rows():
+    T, H, D, page = 70, 2, 64, 64
+    big = torch.randn(T, 3, 3, 96, device=DEV).half()
+    k, v = big[:, 0, :H, :D], big[:, 1, 1:, 3:3 + D]   # v: not 16-byte aligned, copied
+    slots = torch.arange(T, dtype=torch.int32, device=DEV)
+    slots[3], slots[4], slots[5] = -1, 2 * page, 2 ** 31 - 1
+    cache = kv4.new_cache(2, page, H, D)
+    kv4.store(cache, k, v, slots)
+    gk, gv = kv4.load(cache, slots)
+    for x, got in ((k, gk), (v, gv)):
+        want = oc.dequantise(*oc.quantise(x.cpu())).half()
+        want[3:6] = 0
+        assert torch.equal(got.cpu(), want)
+    empty = torch.empty(0, dtype=torch.int32, device=DEV)
+    kv4.store(cache, k[:0], v[:0], empty)
+    assert kv4.load(cache, empty)[0].shape == (0, H, D)
+
+
+def test_store_and_load_refuse():
+    cache = kv4.new_cache(2, 64, 2, 64)
+    x, s = torch.zeros(3, 2, 64, device=DEV).half(), i32([0, 1, 2])
+    for k, v, slots in ((x.float(), x.float(), s), (x, x.bfloat16(), s), (x, x[:2], s),
+                        (x, x, s[:2]), (x, x, s.long()), (x[:, :1], x[:, :1], s),
+                        (x.cpu(), x, s), (x, x, s.cpu())):
+        with pytest.raises(RuntimeError):
+            kv4.store(cache, k, v, slots)
+    for bad in (cache._replace(k=cache.k.int()), cache._replace(v=cache.v[:1]),
+                cache._replace(k_scale=cache.k_scale[:, :1]), cache._replace(v=cache.v[:, :, ::2])):
+        with pytest.raises(RuntimeError):
+            kv4.load(bad, s)
+    with pytest.raises(RuntimeError):
+        kv4.load(cache, s, torch.float32)
+
+
+# -- attention ----------------------------------------------------------------------------
+
+def filled(lens, page, Hkv, D, dtype, seed, spare=2, gain=2.0):
+    """(cache on the GPU, its CPU copy, table) of random rows in shuffled pages. What no
+    token fills holds NaN scales: nothing may read it."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + spare
+    phys = torch.randperm(pages, generator=g).tolist()
+    W = max(max(need, default=0), 1) + 1
+    table = torch.full((len(lens), W), -1, dtype=torch.int32)
+    cache = kv4.new_cache(pages, page, Hkv, D)
+    for t in cache:
+        t.fill_(255)
+    at, slots = 0, []
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = torch.tensor(phys[at:at + need[b]], dtype=torch.int32)
+        slots += [phys[at + t // page] * page + t % page for t in range(n)]
+        at += need[b]
+    T = len(slots)
+    if T:
+        k = (torch.randn(T, Hkv, D, generator=g) * gain).to(dtype)
+        v = torch.randn(T, Hkv, D, generator=g).to(dtype)
+        kv4.store(cache, k.to(DEV), v.to(DEV), i32(slots))
+    return cache, [t.cpu() for t in cache], table
+
+
+def check(out, rows, untouched=None):
+    """Computed rows within the bound, the others as they were."""
+    out = out.double().cpu()
+    worst = 0.0
+    for r in range(out.shape[0]):
+        if r not in rows:
+            if untouched is not None:
+                assert torch.equal(out[r], untouched[r].double().cpu()), f"row {r} written"
+            continue
+        o, tol = rows[r]
+        nan = o.isnan()
+        assert torch.equal(out[r].isnan(), nan), f"row {r}: NaN"
+        err = ((out[r] - o).abs() / tol)[~nan]
+        if err.numel():
+            worst = max(worst, err.max().item())
+            assert worst <= 1.0, f"row {r}: {worst} of the bound"
+    print(f"  worst {worst:.3f} of the bound", flush=True)
+
+
+HEADS = [(1, 1), (8, 2), (5, 5), (16, 1), (24, 2), (40, 1), (6, 2)]
+DECODES = [[1], [0, 5], [63, 64, 65], [0, 1, 130, 700, 33], [2050, 1, 300]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,page", [(64, 64), (128, 64), (128, 128), (64, 256), (128, 256)])
+@pytest.mark.parametrize("lens", DECODES)
+def test_single_tokens(lens, D, page, dtype):
+    Hq, Hkv = HEADS[(len(lens) + D // 64 + page // 64) % len(HEADS)]
+    print(f"decode lens {lens} heads {Hq}/{Hkv} D{D} page {page} {dtype}", flush=True)
+    cache, host, table = filled(lens, page, Hkv, D, dtype, seed=sum(lens))
+    q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(7)).to(dtype)
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), D ** -0.5)
+    check(out, oc.cache_attn(q, host, page, table, lens, D ** -0.5))
+
+
+CHUNKS = [  # lens, queries of each request, rows behind the last
+    ([1], [1], 0), ([64], [64], 0), ([130, 77, 300], [130, 1, 45], 5),
+    ([500, 0, 20, 9], [3, 0, 20, 0], 1), ([5, 200], [9, 2], 0),   # more queries than tokens
+    ([700], [300], 0), ([129, 1025], [2, 17], 3),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(4, 4), (6, 2), (8, 1)])
+@pytest.mark.parametrize("case", range(len(CHUNKS)))
+def test_chunks(case, heads, dtype, causal):
+    lens, news, behind = CHUNKS[case]
+    Hq, Hkv = heads
+    D, page = (64, 128)[case % 2], (64, 128, 256)[(case + Hq) % 3]
+    print(f"chunks {case} heads {heads} D{D} page {page} {dtype} causal {causal}", flush=True)
+    cache, host, table = filled(lens, page, Hkv, D, dtype, seed=case)
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    T = cu[-1] + behind
+    q = torch.randn(T, Hq, D, generator=torch.Generator().manual_seed(case)).to(dtype)
+    out = torch.full((T, Hq, D), 3.0, dtype=dtype, device=DEV)
+    before = out.clone()
+    got = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), D ** -0.5, cu_q=i32(cu),
+                   max_q=max(news), causal=causal, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check(out, oc.cache_attn(q, host, page, table, lens, D ** -0.5, cu, causal=causal), before)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_scales(scale):
+    lens = [200, 3]
+    cache, host, table = filled(lens, 64, 2, 64, torch.float16, seed=5)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(5)).half()
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), scale)
+    check(out, oc.cache_attn(q, host, 64, table, lens, scale))
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [40, 3, 90]])
+def test_bad_pages_narrow_tables_and_hostile_lengths(news):
+    lens, page, D = [300, 150, 200], 64, 128
+    cache, host, table = filled(lens, page, 2, D, torch.bfloat16, seed=11)
+    table[0, 1], table[0, 3], table[1, 0], table[1, 1], table[1, 2] = -1, 10 ** 9, -5, 10 ** 6, -1
+    table = table[:, :4].contiguous()          # request 0 has 5 pages
+    for lens in ([300, 150, 200], [2 ** 31 - 1, -4, 10 ** 6]):
+        cu = [0]
+        for m in news:
+            cu.append(cu[-1] + m)
+        q = torch.randn(cu[-1], 4, D, generator=torch.Generator().manual_seed(3)).bfloat16()
+        print(f"bad pages, lens {lens}", flush=True)
+        # Tokens past what was stored hold NaN; a causal row past the table sees all of it.
+        host_lens = [min(n, 4 * page) for n in lens]
+        out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.1, cu_q=i32(cu),
+                       max_q=max(news), causal=False)
+        check(out, oc.cache_attn(q, host, page, table, host_lens, 0.1, cu, causal=False))
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 3, 9], [-4, 2, 100, 200], [7, 7, 7, 7], [9, 0, 0, 9]])
+def test_query_bounds_out_of_order_are_safe(cu):
+    lens = [100, 70, 64]
+    cache, host, table = filled(lens, 64, 1, 64, torch.float16, seed=2)
+    q = torch.randn(9, 2, 64, generator=torch.Generator().manual_seed(1)).half()
+    out = torch.full((9, 2, 64), 3.0, dtype=torch.float16, device=DEV)
+    before = out.clone()
+    kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.1, cu_q=i32(cu), out=out)
+    if cu == [0, 5, 3, 9]:
+        return   # rows 3 and 4 belong to two requests: either's result
+    check(out, oc.cache_attn(q, host, 64, table, lens, 0.1, cu), before)
+
+
+def test_queries_past_max_q_are_left():
+    lens, cu = [100, 90], [0, 40, 43]
+    cache, host, table = filled(lens, 64, 2, 128, torch.float16, seed=4)
+    q = torch.randn(43, 2, 128, generator=torch.Generator().manual_seed(1)).half()
+    for max_q in (0, 1, 3, 33):
+        out = torch.full((43, 2, 128), 3.0, dtype=torch.float16, device=DEV)
+        before = out.clone()
+        kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.1, cu_q=i32(cu), max_q=max_q, out=out)
+        check(out, oc.cache_attn(q, host, 64, table, lens, 0.1, cu, max_q=max_q), before)
+
+
+def test_infinite_and_nan_blocks():
+    """A NaN or infinite key block makes the rows that see it NaN and no others; values
+    likewise; where no row sees them they change nothing."""
+    lens, D = [70, 70], 64
+    g = torch.Generator().manual_seed(8)
+    for where in ("k", "v"):
+        cache, host, table = filled(lens, 64, 1, D, torch.float16, seed=8)
+        bad = torch.randn(1, 1, D, generator=g).half()
+        bad[0, 0, 40] = math.inf
+        ok = torch.randn(1, 1, D, generator=g).half()
+        slot = i32([table[0, 1].item() * 64 + 3])      # token 67 of request 0
+        kv4.store(cache, (bad if where == "k" else ok).to(DEV), (bad if where == "v" else ok).to(DEV),
+                  slot)
+        q = torch.randn(10, 2, D, generator=g).half()
+        out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.1, cu_q=i32([0, 5, 10]),
+                       max_q=5).cpu()
+        nan = out.isnan()
+        dims = slice(0, D) if where == "k" else slice(32, D)
+        assert nan[2:5, :, dims].all() and not nan[:2].any() and not nan[5:].any()
+        if where == "v":
+            assert not nan[:, :, :32].any()
+
+
+def test_strided_queries_and_outputs():
+    lens, D = [90, 300], 64
+    cache, host, table = filled(lens, 64, 2, D, torch.bfloat16, seed=9)
+    big = torch.randn(3, 8, 4, D, device=DEV).bfloat16()
+    for q in (big[0, :4].transpose(0, 1)[:2], big[1, :2, :, :], big[:2, 1, :, :],
+              torch.randn(2, 4, D + 1, device=DEV).bfloat16()[:, :, 1:]):
+        hold = torch.full((4, 2, D + 4), 3.0, dtype=torch.bfloat16, device=DEV)
+        out = hold.transpose(0, 1)[:, :, :D]
+        kv4.attn(q, cache, table.to(DEV), i32(lens), 0.1, out=out)
+        check(out, oc.cache_attn(q.cpu(), host, 64, table, lens, 0.1))
+        assert hold[:, :, D:].eq(3.0).all()
+    q = big[0, :2].clone()
+    want = kv4.attn(q, cache, table.to(DEV), i32(lens), 0.1)
+    kv4.attn(q, cache, table.to(DEV), i32(lens), 0.1, out=q)   # in place
+    assert torch.equal(q, want)
+
+
+def test_attention_refuses():
+    cache, _, table = filled([70], 64, 2, 64, torch.float16, seed=1)
+    table = table.to(DEV)
+    q = torch.zeros(1, 4, 64, device=DEV).half()
+    n = i32([70])
+    for kw in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[:, :, :32]), dict(q=q.cpu()),
+               dict(lens=n.long()), dict(lens=i32([70, 70])), dict(table=table[0]),
+               dict(table=table.long()), dict(cu_q=i32([0])), dict(out=q.float()),
+               dict(out=q.bfloat16()), dict(out=torch.zeros(1, 1, 64, device=DEV).half().expand(1, 4, 64)),
+               dict(scale=math.nan), dict(scale=math.inf)):
+        a = dict(q=q, cache=cache, table=table, lens=n, scale=0.1) | kw
+        with pytest.raises(RuntimeError):
+            kv4.attn(**a)
+    x = torch.zeros(2, 4, 64, device=DEV).half()
+    with pytest.raises(RuntimeError):   # out partly q
+        kv4.attn(x[:1], cache, table, n, 0.1, out=x.view(-1)[64:320].view(1, 4, 64))
+
+
+def test_no_queries_and_an_empty_cache():
+    cache = kv4.new_cache(0, 64, 2, 64)
+    table = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    assert kv4.attn(q, cache, table, i32([0, 9]), 0.1).eq(0).all()
+    assert kv4.attn(q[:0], cache, table[:0], i32([]), 0.1).shape == (0, 4, 64)
+
+
+# -- together -----------------------------------------------------------------------------
+
+def serve(steps, dtype, D=128, Hq=8, Hkv=2, page=64, seed=0):
+    """Prompts and then single tokens through plan, store and attention; returns every
+    step's output and what the oracle needs."""
+    g = torch.Generator().manual_seed(seed)
+    B, W, pages = 3, 6, 14
+    cache = kv4.new_cache(pages, page, Hkv, D)
+    table = torch.full((B, W), -1, dtype=torch.int32, device=DEV)
+    free = torch.randperm(pages, generator=g).int().to(DEV)
+    lens, used = i32([0] * B), i32([0])
+    done = []
+    for news in steps:
+        T = sum(news) + 2                       # padded batch
+        q, k, v = (torch.randn(T, h, D, generator=g).to(dtype).to(DEV) for h in (Hq, Hkv, Hkv))
+        plan = kv4.plan_pages(lens, i32(news), table, free, used, page, T)
+        kv4.store(cache, k, v, plan.slots)
+        out = torch.full((T, Hq, D), 3.0, dtype=dtype, device=DEV)
+        kv4.attn(q, cache, table, plan.lens, D ** -0.5, cu_q=plan.cu_new, max_q=max(news), out=out)
+        lens, used = plan.lens, plan.used
+        done.append((out, q, [t.cpu() for t in cache], table.cpu(), lens.tolist(),
+                     plan.cu_new.tolist()))
+        assert plan.missing.item() == 0
+    return done
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_then_single_tokens(dtype):
+    steps = [[100, 1, 37], [1, 1, 1], [1, 64, 1], [1, 0, 1], [5, 1, 2]]
+    for out, q, host, table, lens, cu in serve(steps, dtype):
+        rows = oc.cache_attn(q.cpu(), host, 64, table, lens, 128 ** -0.5, cu)
+        check(out, rows, torch.full_like(out, 3.0))
+
+
+def test_captured_step_replays():
+    """Plan, store and attention in one graph, replayed with new inputs in the same
+    buffers and eager work in between, against eager calls."""
+    D, Hq, Hkv, page, B = 128, 8, 2, 64, 5
+    g = torch.Generator(device=DEV).manual_seed(3)
+    lens0 = [100, 63, 0, 700, 128]
+    cache, _, table = filled(lens0, page, Hkv, D, torch.float16, seed=3, spare=9)
+    table = table.to(DEV)
+    taken = set(table[table >= 0].tolist())
+    free = i32([p for p in range(cache.k.shape[0]) if p not in taken])
+    lens, new, used = i32(lens0), i32([1] * B), i32([0])
+    q, k, v = (torch.randn(B, h, D, device=DEV, generator=g).half() for h in (Hq, Hkv, Hkv))
+    out = torch.zeros(B, Hq, D, device=DEV).half()
+
+    def step():
+        plan = kv4.plan_pages(lens, new, table, free, used, page, B)
+        kv4.store(cache, k, v, plan.slots)
+        kv4.attn(q, cache, table, plan.lens, 0.1, cu_q=plan.cu_new, max_q=1, out=out)
+        return plan
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, device=DEV, generator=g).half())
+        graph.replay()
+        got = out.clone()
+        torch.randn(1 << 18, device=DEV).sum().item()
+        out.zero_()
+        plan = step()
+        assert torch.equal(out, got), f"replay {i}"
+        lens.copy_(plan.lens)
+        used.copy_(plan.used)
+        torch.cuda.synchronize()
+
+
+def test_two_streams_at_once():
+    lens = [3000, 500, 1]
+    cache, host, table = filled(lens, 128, 2, 64, torch.float16, seed=6)
+    table, n = table.to(DEV), i32(lens)
+    qs = [torch.randn(3, 8, 64, device=DEV).half() for _ in range(6)]
+    want = [kv4.attn(q, cache, table, n, 0.1) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for i, q in enumerate(qs):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(kv4.attn(q, cache, table, n, 0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits():
+    """Rows whose codes start past 2^32 bytes."""
+    page, D, Hkv = 256, 128, 8
+    pages = 2 ** 32 // (Hkv * page * D // 2) + 3
+    cache = kv4.new_cache(pages, page, Hkv, D)
+    k, v = (torch.randn(300, Hkv, D, device=DEV).half() for _ in range(2))
+    at = torch.arange(300, dtype=torch.int32, device=DEV)
+    table = i32([[pages - 1, pages - 2]])
+    slots = table[0, (at // page).long()] * page + at % page
+    kv4.store(cache, k, v, slots)
+    want = [oc.dequantise(*oc.quantise(x.cpu())) for x in (k, v)]
+    for got, ref in zip(kv4.load(cache, slots), want):
+        assert torch.equal(got.cpu().double(), ref)
+    q = torch.randn(300, 8, D).half()
+    small = kv4.new_cache(2, page, Hkv, D)
+    kv4.store(small, k, v, at)
+    for cu, m, n in ((None, 1, 1), (i32([0, 300]), 300, 300)):
+        x = q[:n].to(DEV)
+        far = kv4.attn(x, cache, table, i32([300]), 0.1, cu_q=cu, max_q=m)
+        near = kv4.attn(x, small, i32([[0, 1]]), i32([300]), 0.1, cu_q=cu, max_q=m)
+        assert torch.equal(far, near)
