@@ -148,7 +148,7 @@ def _newest_mtime(paths) -> float:
 
 
 def kernel_lib_inputs() -> list:
-    return [*KERNEL_SOURCES, CSRC / "scratch.h", CSRC / "longctx.h", *sorted(CSRC.glob("*.inc")),
+    return [*KERNEL_SOURCES, *sorted(CSRC.glob("*.h")), *sorted(CSRC.glob("*.inc")),
             *sorted(INCLUDE.glob("*.h"))]
 
 

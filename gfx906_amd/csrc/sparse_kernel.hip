@@ -7,7 +7,7 @@
 // exact, and rounded once to fp32; products of two fp32 are exact in fp64 and add
 // up there. Scores of different blocks closer than 1e-15 relative are as good as
 // never seen; equal ones go by the index.
-#include "longctx.h"
+#include "longctx_tile.h"
 
 #include <algorithm>
 
@@ -132,60 +132,325 @@ struct AttnArgs {
     Strides sq, sk, sv, so;
     const int* index;
     int Hq, Hkv, Sq, Skv, D, block, nq, nk, count, causal;
-    float scale;
+    float c, qsign;  // |scale| log2(e), at least 1e-30; a negative scale negates q
+    // Lists are split in nsplit ranges of a query block's entries; a range writes its
+    // unnormalised O (fp32) and (m, l) to the workspace, at row range * rows + row of
+    // all heads' rows, and combine_kernel merges them.
+    int nsplit;
+    long long rows;
+    float* ws_o;
+    float* ws_ml;
 };
 
-// One wave per query row: 64 keys at a time, a score per lane, then a pair of dims
-// per lane.
-template <class T>
-__global__ void __launch_bounds__(64) attn_rows_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float qs[128], ps[64];
-    const int row = blockIdx.x, bh = blockIdx.y, lane = threadIdx.x;
-    const int b = bh / a.Hq, h = bh - b * a.Hq, hk = h / (a.Hq / a.Hkv);
-    const T* q = (const T*)a.q + b * a.sq.b + h * a.sq.h + row * a.sq.s;
-    const T* k = (const T*)a.k + b * a.sk.b + hk * a.sk.h;
-    const T* v = (const T*)a.v + b * a.sv.b + hk * a.sv.h;
-    T* o = (T*)a.o + b * a.so.b + h * a.so.h + row * a.so.s;
-    const int* list = a.index + ((long long)bh * a.nq + row / kQBlock) * a.count;
-    for (int d = lane; d < a.D; d += 64) qs[d] = (float)q[d];
-    __syncthreads();
-    const long long seen = a.causal ? (long long)row + a.Skv - a.Sq + 1 : a.Skv;
+// Where the results of one row go: the output, or the workspace of a split range.
+template <class T>
+__device__ __forceinline__ void store_pair(const AttnArgs& a, T* orow, long long wrow, int d,
+                                           float x, float y, float inv, bool split) {
+    if (split) {
+        *reinterpret_cast<f32x2*>(a.ws_o + wrow * a.D + d) = f32x2{x, y};
+    } else {
+        *reinterpret_cast<typename Elem<T>::x2*>(orow + d) = Elem<T>::cvt2(x * inv, y * inv);
+    }
+}
+
+// One row over the blocks list[e0..e1), by one wave: 64 keys at a time, a score per
+// lane, then a pair of dims per lane. Keys the row does not see are not touched at
+// all, so that what they hold cannot reach it.
+template <int D, class T>
+__device__ __attribute__((noinline)) void attend_row(const AttnArgs& a, const T* q, const T* k,
+                                                     const T* v, T* orow, long long wrow,
+                                                     const uint16_t* list, int e0, int e1,
+                                                     int seen) {
+    const int lane = threadIdx.x & 63;
     float m = kNoMax, l = 0.f, o0 = 0.f, o1 = 0.f;
-    int last = -1;
-    for (int e = 0; e < a.count; ++e) {
-        const int blk = list[e];
-        if (blk <= last || blk >= a.nk) continue;
-        last = blk;
+    for (int e = e0; e < e1; ++e)
         for (int u = 0; u < a.block; u += 64) {
-            const long long j0 = (long long)blk * a.block + u, j = j0 + lane;
-            const long long end = min(seen, (long long)a.Skv);
+            const int j0 = list[e] * a.block + u, j = j0 + lane;
             float s = -INFINITY;
-            if (j < end) {
+            if (j < seen) {
                 s = 0.f;
-                for (int d = 0; d < a.D; ++d) s += qs[d] * (float)k[j * a.sk.s + d];
-                s *= a.scale * kLog2e;
+                for (int d = 0; d < D; ++d) s = fmaf((float)q[d], (float)k[j * a.sk.s + d], s);
+                s *= a.c * a.qsign;
             }
-            const float mn = fmaxf(m, wave_max(s)), w = exp2f(m - mn), p = exp2f(s - mn);
+            const float mn = max2(m, wave_max(s)), w = exp2f(m - mn), p = exp2f(s - mn);
             l = l * w + wave_sum(p);
             o0 *= w;
             o1 *= w;
             m = mn;
-            ps[lane] = p;
-            __syncthreads();
-            if (2 * lane < a.D)
-                for (int i = 0; i < 64 && j0 + i < end; ++i) {
-                    o0 += ps[i] * (float)v[(j0 + i) * a.sv.s + 2 * lane];
-                    o1 += ps[i] * (float)v[(j0 + i) * a.sv.s + 2 * lane + 1];
+            for (int i = 0; i < 64 && j0 + i < seen; ++i) {
+                const float pi = __shfl(p, i);
+                if (2 * lane < D) {
+                    o0 = fmaf(pi, (float)v[(j0 + i) * a.sv.s + 2 * lane], o0);
+                    o1 = fmaf(pi, (float)v[(j0 + i) * a.sv.s + 2 * lane + 1], o1);
                 }
-            __syncthreads();
+            }
+        }
+    if (2 * lane < D)
+        store_pair(a, orow, wrow, 2 * lane, o0, o1, l != 0.f ? 1.f / l : 0.f, a.nsplit > 1);
+    if (a.nsplit > 1 && lane == 0) *reinterpret_cast<f32x2*>(a.ws_ml + 2 * wrow) = f32x2{m, l};
+}
+
+// Workgroup w's place in a grid of n: the dispatcher deals workgroups out to the 8
+// XCDs in turn; where 8 divides n, consecutive units go to one XCD, whose L2 then
+// streams the keys of as few heads as possible.
+__device__ __forceinline__ int xcd_order(int w, int n) {
+    return (n & 7) == 0 ? (w & 7) * (n >> 3) + (w >> 3) : w;
+}
+#endif
+
+// Attention of one query block (128 rows, 32 a wave) over its listed key blocks.
+//
+// The list is read first and its valid entries gathered in LDS. Then the waves walk
+// the listed keys in tiles of 32, software-pipelined as attn_fwd_pipe: the step of
+// tile j issues the PV products of tile j-1 and the QK products of tile j+1 around
+// the softmax of tile j. K and V tiles come by loads to LDS into rings of four, K
+// three and V two steps ahead, whose waits are counted: one barrier a step. Tiles of
+// 32 (16 KB of K and V at D = 128) instead of attn_fwd_pipe's 64 let two
+// workgroups of four waves share a CU's LDS, for lists of 128 rows instead of 256.
+//
+// Tiles past the list load zeros (empty range) and are masked, so that loads and
+// waits stay static. A tile with masked keys is checked for infinite and NaN values
+// of V (which a weight of 0 would not keep out of the sums); where there are any
+// the wave does its rows again by attend_row.
+template <int D, class T>
+__global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using W = Tile<D, T>;
+    using x8 = typename W::x8;
+    constexpr int NU = W::NU, RB = W::RB, BYTES = W::BYTES;
+    constexpr int LPT = BYTES / 1024 / 4;  // loads a wave and tile
+    constexpr int kWait = 0x0F70 | ((4 * LPT) & 15) | (((4 * LPT) >> 4) << 14);
+    __shared__ __attribute__((aligned(1024))) char k0[BYTES];
+    __shared__ __attribute__((aligned(1024))) char k1[BYTES];
+    __shared__ __attribute__((aligned(1024))) char k2[BYTES];
+    __shared__ __attribute__((aligned(1024))) char k3[BYTES];
+    __shared__ __attribute__((aligned(1024))) char v0[BYTES];
+    __shared__ __attribute__((aligned(1024))) char v1[BYTES];
+    __shared__ __attribute__((aligned(1024))) char v2[BYTES];
+    __shared__ __attribute__((aligned(1024))) char v3[BYTES];
+    __shared__ uint16_t list[SPARSE_MAX_COUNT];
+    __shared__ int n_list;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    // (uniform, and kept in scalar registers: divisions run on the vector unit, and
+    // descriptors made from vector registers would be read in loops)
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int unit = xcd_order(blockIdx.x, gridDim.x);
+    const int qi = uni(unit / a.nsplit), range = unit - qi * a.nsplit;
+    const int bh = uni(qi / a.nq), qb = qi - bh * a.nq;
+    const int b = uni(bh / a.Hq), h = bh - b * a.Hq, hk = uni(h / uni(a.Hq / a.Hkv));
+    const T* Q = (const T*)a.q + b * a.sq.b + h * a.sq.h;
+    const T* K = (const T*)a.k + b * a.sk.b + hk * a.sk.h;
+    const T* V = (const T*)a.v + b * a.sv.b + hk * a.sv.h;
+    const int row0 = qb * kQBlock + wave * 32;  // this lane's rows: row0 + 16 nb + i
+    const bool active = row0 < a.Sq;            // (wave-uniform)
+
+    W w;
+    w.init(lane);
+    const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
+    int lim[2];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+        const int row = row0 + 16 * nb + i;
+        lim[nb] = a.causal ? min(a.Skv, row + a.Skv - a.Sq + 1) : a.Skv;
+#pragma unroll
+        for (int s = 0; s < W::NQ; ++s) {
+            u32x4 x = {};
+            if (row < a.Sq)
+                x = *reinterpret_cast<const u32x4*>(Q + row * a.sq.s + 32 * s + 8 * g);
+            w.qf[nb][s] = __builtin_bit_cast(x8, x ^ neg);
         }
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    if (2 * lane < a.D) {
-        o[2 * lane] = (T)(o0 * inv);
-        o[2 * lane + 1] = (T)(o1 * inv);
+    // Keys below this one are seen by every row of the wave.
+    const int all_see = a.causal ? min(a.Skv, row0 + a.Skv - a.Sq + 1) : a.Skv;
+
+    // The valid entries of the list: above every valid one before them, in range, and
+    // (causal) not behind every row of the query block.
+    if (wave == 0) {
+        const int* src = a.index + ((long long)bh * a.nq + qb) * a.count;
+        const int reach = a.causal
+                              ? min(a.nk, (int)((min(a.Sq, (qb + 1) * kQBlock) - 1LL + a.Skv - a.Sq +
+                                                 a.block) / a.block))
+                              : a.nk;
+        int last = -1, n = 0;
+        for (int e0 = 0; e0 < a.count; e0 += 64) {
+            const int e = e0 + lane;
+            const int x = e < a.count ? src[e] : -1;
+            const bool in = x >= 0 && x < a.nk;
+            int top = in ? x : -1;  // running max, inclusive
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(top, o);
+                if (lane >= o) top = max(top, y);
+            }
+            int before = __shfl_up(top, 1);
+            before = max(last, lane ? before : -1);
+            const bool take = in && x > before && x < reach;
+            const unsigned long long mk = __ballot(take);
+            if (take) list[n + __popcll(mk & ((1ull << lane) - 1))] = (uint16_t)x;
+            n += __popcll(mk);
+            last = max(last, __shfl(top, 63));
+        }
+        if (lane == 0) n_list = n;
     }
+    for (int z = tid; z < BYTES / 16; z += 256) *reinterpret_cast<u32x4*>(v3 + 16 * z) = u32x4{};
+    __syncthreads();
+    const int n_all = __builtin_amdgcn_readfirstlane(n_list);
+    // (at most 2048 entries and 512 ranges)
+    const int e0 = uni(n_all * range / a.nsplit), e1 = uni(n_all * (range + 1) / a.nsplit);
+    const int bshift = a.block == 64 ? 1 : 2;  // log2 of the tiles in a block
+    const int ntiles = (e1 - e0) << bshift;
+
+    // First key of tile t (past the list: past every key).
+    auto key_of = [&](int t) __attribute__((always_inline)) {
+        const int e = min(e0 + (t >> bshift), SPARSE_MAX_COUNT - 1);
+        const int k = (int)list[e] * a.block + (t & ((1 << bshift) - 1)) * 32;
+        return __builtin_amdgcn_readfirstlane(t < ntiles ? k : 0x7fffff00);
+    };
+    int koff[LPT], voff[LPT];
+#pragma unroll
+    for (int n = 0; n < LPT; ++n) {
+        const int u = (wave + 4 * n) * 64 + lane, r = u / NU, s = u % NU;
+        koff[n] = (int)(r * a.sk.s + (s ^ kswz<NU>(r)) * 8) * 2;
+        voff[n] = (int)(r * a.sv.s + (s ^ vswz<NU>(r)) * 8) * 2;
+    }
+    auto issue = [&](const T* X, long long ss, int key, char* dst, const int (&off)[LPT])
+        __attribute__((always_inline)) {
+        const int rows = min(a.Skv - key, 32);
+        const int bytes =
+            __builtin_amdgcn_readfirstlane(rows > 0 ? (int)(((rows - 1) * ss + D) * 2) : 0);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(X + (rows > 0 ? key : 0) * ss), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int n = 0; n < LPT; ++n)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (GFX906_LDS void*)(dst + (wave + 4 * n) * 1024), 16, off[n], 0, 0, 0);
+    };
+
+    bool redo = false;
+    if (ntiles > 0) {
+        f32x4 Sa[2][2], Sb[2][2];
+        x8 Pa[2], Pb[2];
+        Pb[0] = x8{};
+        Pb[1] = x8{};
+        // Keys of tiles j .. j+4 and of V's tiles; shifted every step.
+        int q0 = key_of(0), q1 = key_of(1), q2 = key_of(2), q3 = key_of(3), q4 = key_of(4);
+        bool hidden = false;  // tile j-1 had masked keys
+        issue(K, a.sk.s, q0, k0, koff);
+        issue(K, a.sk.s, q1, k1, koff);
+        issue(K, a.sk.s, q2, k2, koff);
+        issue(V, a.sv.s, q0, v0, voff);
+        issue(K, a.sk.s, q3, k3, koff);
+        issue(V, a.sv.s, q1, v1, voff);
+        __builtin_amdgcn_s_waitcnt(kWait);
+        lds_barrier();
+        if (active) w.qk(k0, Sa);
+        lds_barrier();
+        issue(K, a.sk.s, q4, k0, koff);
+        issue(V, a.sv.s, q2, v2, voff);
+
+        // Tile j: V of tile j-1 in vp, K of tile j+1 in kn; tile j+5 of K and j+3 of V
+        // go where those were.
+        auto step = [&](int j, const char* vp, const char* kn, char* kfree, char* vfree,
+                        f32x4 (&S)[2][2], f32x4 (&Sn)[2][2], const x8 (&Pp)[2], x8 (&P)[2])
+            __attribute__((always_inline)) {
+            const int q5 = key_of(j + 5);
+            if (active) {
+                if (__builtin_expect(hidden, 0)) redo |= not_finite<D, T>(vp, lane);
+                hidden = q0 + 32 > all_see;
+                if (hidden) w.mask(S, q0, lim, g);
+                w.pv(vp, Pp);
+                w.qk(kn, Sn);
+                w.softmax(S, P, a.c);
+            }
+            __builtin_amdgcn_s_waitcnt(kWait);
+            lds_barrier();
+            issue(K, a.sk.s, q5, kfree, koff);
+            issue(V, a.sv.s, q3, vfree, voff);
+            q0 = q1;
+            q1 = q2;
+            q2 = q3;
+            q3 = q4;
+            q4 = q5;
+        };
+        for (int j = 0; j < ntiles; j += 4) {
+            step(j + 0, v3, k1, k1, v3, Sa, Sb, Pb, Pa);
+            step(j + 1, v0, k2, k2, v0, Sb, Sa, Pa, Pb);
+            step(j + 2, v1, k3, k3, v1, Sa, Sb, Pb, Pa);
+            step(j + 3, v2, k0, k0, v2, Sb, Sa, Pa, Pb);
+        }
+        if (active) {
+            if (hidden) redo |= not_finite<D, T>(v3, lane);
+            w.pv(v3, Pb);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // loads past the end, before LDS is released
+    }
+    if (!active) return;
+
+    T* O = (T*)a.o + b * a.so.b + h * a.so.h;
+    const long long wbase = range * a.rows + (long long)bh * a.Sq;
+    if (__builtin_expect(redo, 0)) {
+        // The arguments where they lie (a reference to `a` would put it in memory).
+        const AttnArgs& ka = *(const AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+        for (int r = row0; r < min(row0 + 32, a.Sq); ++r)
+            attend_row<D, T>(ka, Q + r * a.sq.s, K, V, O + r * a.so.s, wbase + r, list, e0, e1,
+                             a.causal ? min(a.Skv, r + a.Skv - a.Sq + 1) : a.Skv);
+        return;
+    }
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+        const int row = row0 + 16 * nb + i;
+        const float l = quad_sum(w.lacc[nb][0]);
+        if (row >= a.Sq) continue;
+        if (a.nsplit > 1) {
+            float* wo = a.ws_o + (wbase + row) * D;
+#pragma unroll
+            for (int ob = 0; ob < W::NO; ++ob)
+                *reinterpret_cast<f32x4*>(wo + 16 * ob + 4 * g) = w.oacc[ob][nb];
+            if (g == 0) *reinterpret_cast<f32x2*>(a.ws_ml + 2 * (wbase + row)) = f32x2{w.m[nb], l};
+            continue;
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        T* op = O + row * a.so.s;
+#pragma unroll
+        for (int ob = 0; ob < W::NO; ++ob) {
+            const f32x4 x = w.oacc[ob][nb] * inv;
+            const auto lo = Elem<T>::cvt2(x[0], x[1]), hi = Elem<T>::cvt2(x[2], x[3]);
+            *reinterpret_cast<u32x2*>(op + 16 * ob + 4 * g) =
+                u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
+        }
+    }
+#endif
+}
+
+// Merges the ranges of a row, four dims a lane.
+template <class T>
+__global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int dq = a.D / 4;
+    const long long row = id / dq;
+    const int d = (int)(id - row * dq) * 4;
+    if (row >= a.rows) return;
+    float mx = kNoMax;
+    for (int s = 0; s < a.nsplit; ++s) mx = max2(mx, a.ws_ml[2 * (s * a.rows + row)]);
+    f32x4 acc = {};
+    float l = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) {
+        const long long r = s * a.rows + row;
+        const float w = __builtin_amdgcn_exp2f(a.ws_ml[2 * r] - mx);
+        acc += w * *reinterpret_cast<const f32x4*>(a.ws_o + r * a.D + d);
+        l += w * a.ws_ml[2 * r + 1];
+    }
+    acc *= l != 0.f ? 1.f / l : 0.f;
+    const int bh = (int)(row / a.Sq), r = (int)(row - (long long)bh * a.Sq), b = bh / a.Hq;
+    T* o = (T*)a.o + b * a.so.b + (bh - b * a.Hq) * a.so.h + r * a.so.s + d;
+    const auto lo = Elem<T>::cvt2(acc[0], acc[1]), hi = Elem<T>::cvt2(acc[2], acc[3]);
+    *reinterpret_cast<u32x2*>(o) =
+        u32x2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
 #endif
 }
 
@@ -201,6 +466,15 @@ int check_sizes(int B, int H, int S, int D, int block, const char* who) {
 }
 
 int blocks_of(int S, int block) { return (S + block - 1) / block; }
+
+// Ranges the lists are split in: enough for two workgroups a CU, of 4 tiles or more.
+int split_count(int B, int Hq, int Sq, int Skv, int block, int count) {
+    const long long units = (long long)B * Hq * blocks_of(Sq, kQBlock);
+    const int entries = std::min(count, blocks_of(Skv, block));
+    if (units >= 256 || entries <= 1) return 1;
+    const int most = std::max(1, entries * (block / 32) / 4);
+    return (int)std::min<long long>(most, 512 / units);
+}
 
 int check_strides(const long long* s, const void* p, size_t bytes, int mult, const char* who) {
     for (int i = 0; i < 3; ++i)
@@ -271,8 +545,9 @@ extern "C" int sparse_select(const float* q_means, const float* k_means, int B, 
 
 extern "C" size_t sparse_attn_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block,
                                               int count) {
-    (void)B, (void)Hq, (void)Sq, (void)Skv, (void)D, (void)block, (void)count;
-    return 0;
+    if (B <= 0 || Hq <= 0 || Sq <= 0 || Skv <= 0 || D <= 0 || block <= 0 || count <= 0) return 0;
+    const int n = split_count(B, Hq, Sq, Skv, block, count);
+    return n <= 1 ? 0 : (size_t)n * B * Hq * Sq * (D + 2) * sizeof(float);
 }
 
 extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
@@ -308,14 +583,34 @@ extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
         return g_err.fail("sparse_attn: k/v sequence stride above 2^22 elements");
     const long long oe[3] = {B, Hq, Sq};
     if (!rows_apart(o_strides, oe, 3, D)) return g_err.fail("sparse_attn: o's rows overlap");
-    (void)workspace, (void)workspace_bytes;
+    const size_t need = sparse_attn_workspace_bytes(B, Hq, Sq, Skv, D, block, count);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return g_err.fail("sparse_attn: workspace misaligned or smaller than "
+                          "sparse_attn_workspace_bytes()");
     auto st = [](const long long* s) { return Strides{s[0], s[1], s[2]}; };
-    const AttnArgs a{q, k, v, o, st(q_strides), st(k_strides), st(v_strides), st(o_strides), index,
-                     Hq, Hkv, Sq, Skv, D, block, blocks_of(Sq, kQBlock), blocks_of(Skv, block),
-                     count, causal, scale};
-    if (dtype == SPARSE_DTYPE_F16)
-        hipLaunchKernelGGL(attn_rows_kernel<f16>, dim3(Sq, B * Hq), dim3(64), 0, stream, a);
-    else
-        hipLaunchKernelGGL(attn_rows_kernel<bf16>, dim3(Sq, B * Hq), dim3(64), 0, stream, a);
+    AttnArgs a{q, k, v, o, st(q_strides), st(k_strides), st(v_strides), st(o_strides), index,
+               Hq, Hkv, Sq, Skv, D, block, blocks_of(Sq, kQBlock), blocks_of(Skv, block), count,
+               causal, fmaxf(fabsf(scale) * kLog2e, 1e-30f), scale < 0.f ? -1.f : 1.f,
+               Skv > 0 ? split_count(B, Hq, Sq, Skv, block, count) : 1, (long long)B * Hq * Sq,
+               nullptr, nullptr};
+    if (a.nsplit > 1) {
+        a.ws_o = (float*)workspace;
+        a.ws_ml = a.ws_o + (size_t)a.nsplit * a.rows * D;
+    }
+    const long long grid = (long long)a.nq * B * Hq * a.nsplit;
+    if (grid >= (1LL << 31)) return g_err.fail("sparse_attn: too many query blocks");
+    auto go = [&](auto kernel, auto combine) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
+        if (a.nsplit > 1)
+            hipLaunchKernelGGL(combine, dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256),
+                               0, stream, a);
+    };
+    if (dtype == SPARSE_DTYPE_F16) {
+        if (D == 64) go(attn_tile_kernel<64, f16>, combine_kernel<f16>);
+        else go(attn_tile_kernel<128, f16>, combine_kernel<f16>);
+    } else {
+        if (D == 64) go(attn_tile_kernel<64, bf16>, combine_kernel<bf16>);
+        else go(attn_tile_kernel<128, bf16>, combine_kernel<bf16>);
+    }
     return g_err.launched("sparse_attn", hipGetLastError());
 }

@@ -95,10 +95,14 @@ def softmax_rows(q, k, v, scale, hide):
     l = w.sum(1, keepdim=True)
     inv = torch.where(l > 0, 1 / l, torch.zeros_like(l))
     inv = torch.where(torch.isnan(l), l, inv)
-    used = torch.where((~hide).any(0)[:, None], v, torch.zeros_like(v))
+    # A key that a row does not see adds nothing to it, whatever the key holds.
+    bad = ~torch.isfinite(v).all(1) & (~hide).any(0)
+    used = torch.where((torch.isfinite(v).all(1) & (~hide).any(0))[:, None], v, torch.zeros_like(v))
+    more = sum((torch.where(hide[:, j:j + 1], 0.0, w[:, j:j + 1] * v[j]) for j in bad.nonzero()),
+               torch.zeros(()))
     size = ((q.abs() @ k.abs().T) * abs(scale)).masked_fill(hide, 0.0)
     size = size.nan_to_num(0.0, 0.0, 0.0).max().item() if z.numel() else 0.0
-    return w @ used * inv, w @ used.abs() * inv, size
+    return (w @ used + more) * inv, w @ used.abs() * inv, size
 
 
 def tolerance(o, spread, size, dtype, D, keys, vmax):

@@ -186,7 +186,8 @@ def test_what_no_row_sees_changes_nothing(D, Sq):
     if Sq > 1:   # the last key is seen by the last row only
         k2[:, :, -1], v2[:, :, -1] = math.nan, math.nan
         got = sparse.attn_blocks(q.to(DEV), k2.to(DEV), v2.to(DEV), 0.1, index.to(DEV), 64, True)
-        assert got[:, :, -1].isnan().all() and torch.equal(got[:, :, :-1], want[:, :, :-1])
+        assert got[:, :, -1].isnan().all()
+        check(got, *oc.sparse_attn(q, k2, v2, 0.1, index, 64, True))
 
 
 def test_very_low_and_high_scores():
