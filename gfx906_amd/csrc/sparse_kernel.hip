@@ -27,20 +27,54 @@ struct MeansArgs {
     const void* x;
     long long sb, sh, ss;
     float* means;
-    int H, S, D, block, nb;
+    int H, S, block, nb;
+    long long blocks;  // of all heads
 };
 
-// One wave per block of rows and 64 dims.
-template <class T>
-__global__ void __launch_bounds__(64) means_kernel(const MeansArgs a) {
+// One wave per block of rows: a lane reads 16 bytes (8 dims) of a row, so that a load
+// takes 4 (D = 128) or 8 (D = 64) whole rows, 16 loads in flight; the lanes that hold
+// the same dims add up at the end. Bound by the bytes of x.
+template <int D, class T>
+__global__ void __launch_bounds__(256) means_kernel(const MeansArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int j = blockIdx.x, bh = blockIdx.y, d = blockIdx.z * 64 + threadIdx.x;
-    const int b = bh / a.H, h = bh - b * a.H;
-    const int r0 = j * a.block, r1 = min(a.S, r0 + a.block);
-    const T* x = (const T*)a.x + b * a.sb + h * a.sh + d;
-    double sum = 0.0;
-    for (int r = r0; r < r1; ++r) sum += (double)(float)x[r * a.ss];
-    a.means[((long long)bh * a.nb + j) * a.D + d] = (float)(sum / (r1 - r0));
+    using x8 = typename Elem<T>::x8;
+    constexpr int LPR = D / 8, RPL = 64 / LPR, N = 16;
+    const int lane = threadIdx.x & 63;
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= a.blocks) return;
+    const int j = (int)(id % a.nb), bh = (int)(id / a.nb), b = bh / a.H, h = bh - b * a.H;
+    const int r0 = j * a.block, rows = min(a.block, a.S - r0);
+    const int c = lane % LPR, r = lane / LPR;
+    const T* x = (const T*)a.x + b * a.sb + h * a.sh + r0 * a.ss + c * 8;
+    double sum[8] = {};
+    for (int t = 0; t < rows; t += N * RPL) {
+        x8 v[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int row = t + n * RPL + r;
+            v[n] = x8{};
+            if (row < rows) v[n] = *reinterpret_cast<const x8*>(x + row * a.ss);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += (double)(float)v[n][e];
+    }
+#pragma unroll
+    for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], o);
+    if (r == 0) {
+        float* m = a.means + id * D + c * 8;
+        f32x4 lo, hi;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            lo[e] = (float)(sum[e] / rows);
+            hi[e] = (float)(sum[e + 4] / rows);
+        }
+        *reinterpret_cast<f32x4*>(m) = lo;
+        *reinterpret_cast<f32x4*>(m + 4) = hi;
+    }
 #endif
 }
 
@@ -52,6 +86,7 @@ struct SelectArgs {
     double* score;
     int* index;
     int Hq, Hkv, Sq, Skv, D, block, nq, nk, count, causal;
+    long long rows;  // query blocks of all heads
 };
 
 // Key blocks a query block may take (the first `seen`), and the first of those that
@@ -69,52 +104,154 @@ __host__ __device__ inline Reach reach(int i, int Sq, int Skv, int block, int nk
     return {(int)(last / block) + 1, (int)((first < 0 ? 0 : first) / block)};
 }
 
-// One workgroup per query block: all scores, then every block counts those ranked
-// before it, then the chosen ones are written in order.
-__global__ void __launch_bounds__(256) select_kernel(const SelectArgs a) {
+// Scores of a kv head's query rows (row r: query block r / G of query head r % G of the
+// head's group) and key blocks, on the fp64 matrix pipe: a wave keeps 16 rows and goes
+// through tiles of 16 key blocks. In step s of a tile lane group g supplies dim
+// g D/4 + s, so that a lane reads D/4 consecutive floats of its row.
+//
+// grid: row tiles, kv heads of all batches, shares of the key tiles; 4 waves.
+template <int D>
+__global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float qs[128];
-    __shared__ int base, wave_n[4];
-    const int i = blockIdx.x, bh = blockIdx.y, t = threadIdx.x;
-    const int b = bh / a.Hq, h = bh - b * a.Hq, kvh = b * a.Hkv + h / (a.Hq / a.Hkv);
-    const Reach r = reach(i, a.Sq, a.Skv, a.block, a.nk, a.causal);
-    const long long row = (long long)bh * a.nq + i;
-    double* score = a.score + row * a.nk;
-    int* out = a.index + row * a.count;
-    if (t < a.D) qs[t] = a.qm[row * a.D + t];
-    if (t == 0) base = 0;
-    __syncthreads();
-    for (int j = t; j < r.seen; j += 256) {
-        const float* k = a.km + ((long long)kvh * a.nk + j) * a.D;
-        double s = 0.0;
-        for (int d = 0; d < a.D; ++d) s = fma((double)qs[d], (double)k[d], s);
-        score[j] = s != s || j >= r.own ? INFINITY : s;
-    }
-    __syncthreads();
-    __threadfence_block();
-    for (int j0 = 0; j0 < r.seen; j0 += 256) {
-        const int j = j0 + t;
-        bool take = false;
-        if (j < r.seen) {
-            const double s = score[j];
-            int before = 0;
-            for (int u = 0; u < r.seen; ++u) {
-                const bool mine = u >= r.own, me = j >= r.own;
-                before += mine != me ? mine : score[u] > s || (score[u] == s && u < j);
-            }
-            take = before < a.count;
+    constexpr int N = D / 4;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int G = a.Hq / a.Hkv, rows = G * a.nq, r0 = blockIdx.x * 16;
+    const int b = blockIdx.y / a.Hkv, hk = blockIdx.y - b * a.Hkv;
+    const int tiles = (a.nk + 15) / 16, step = 4 * gridDim.z;
+    // Row of the score matrix (of all heads) that tile row r stands for.
+    auto row_of = [&](int r) {
+        const int qb = r / G;
+        return ((long long)b * a.Hq + hk * G + (r - qb * G)) * a.nq + qb;
+    };
+    double q[N];
+    {
+        const int r = min(r0 + i, rows - 1);
+        const float* p = a.qm + row_of(r) * D + g * N;
+#pragma unroll
+        for (int s = 0; s < N; s += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p + s);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[s + e] = x[e];
         }
-        const unsigned long long m = __ballot(take);
-        if ((t & 63) == 0) wave_n[t >> 6] = __popcll(m);
-        __syncthreads();
-        int at = base + __popcll(m & ((1ull << (t & 63)) - 1));
-        for (int w = 0; w < t >> 6; ++w) at += wave_n[w];
-        if (take && at < a.count) out[at] = j;
-        __syncthreads();
-        if (t == 0) base += wave_n[0] + wave_n[1] + wave_n[2] + wave_n[3];
-        __syncthreads();
     }
-    for (int j = base + t; j < a.count; j += 256) out[j] = -1;
+    const float* km = a.km + (long long)blockIdx.y * a.nk * D + g * N;
+    for (int t = blockIdx.z * 4 + (threadIdx.x >> 6); t < tiles; t += step) {
+        const float* p = km + (long long)min(16 * t + i, a.nk - 1) * D;
+        f32x4 k[N / 4];
+#pragma unroll
+        for (int s = 0; s < N / 4; ++s) k[s] = *reinterpret_cast<const f32x4*>(p + 4 * s);
+        f64x4 c = {};
+#pragma unroll
+        for (int s = 0; s < N; ++s)
+            c = __builtin_amdgcn_mfma_f64_16x16x4f64(q[s], (double)k[s / 4][s % 4], c, 0, 0, 0);
+        // (accumulator element e: row 4 e + l/16, column l%16)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = r0 + 4 * e + g, j = 16 * t + i;
+            if (r < rows && j < a.nk) a.score[row_of(r) * a.nk + j] = c[e];
+        }
+    }
+#endif
+}
+
+// The choice of one row by WAVES waves, K scores a lane (wave w: the w-th run of 64 K
+// key blocks). Scores become 64-bit integers of the same order (0: not to be taken;
+// all ones: always), and the count-th largest is found bit by bit from the top, until
+// exactly `count` lie at or above the bits so far, or their last bit is set: then
+// scores equal to it fill up in the order of their index. Everything stays in
+// registers; a step is a compare and a population count per 64 scores (and, with
+// several waves, an exchange through LDS).
+template <int WAVES, int K>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef unsigned long long u64;
+    __shared__ int part[2][WAVES];
+    const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
+    const long long row = WAVES == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= a.rows) return;  // (a whole wave; with several, never)
+    const int i = (int)(row % a.nq);
+    const Reach r = reach(i, a.Sq, a.Skv, a.block, a.nk, a.causal);
+    const double* score = a.score + row * a.nk;
+    int* out = a.index + row * a.count;
+    const int base = wave * 64 * K + lane;
+    u64 key[K];
+#pragma unroll
+    for (int n = 0; n < K; ++n) {
+        const int j = base + 64 * n;
+        key[n] = 0;
+        if (j < r.seen) {
+            const double s = score[j] + 0.0;  // -0 becomes +0
+            const u64 bits = (u64)__double_as_longlong(s != s ? INFINITY : s);
+            key[n] = j >= r.own ? ~0ull : bits >> 63 ? ~bits : bits | 1ull << 63;
+        }
+    }
+    int turn = 0;
+    auto popc = [](u64 x) { return (int)__popcll(x); };  // (unsigned, else)
+    // Sum over the waves of a wave-uniform count; `before`: that of the waves before.
+    auto total = [&](int mine, int* before) {
+        if (WAVES == 1) {
+            if (before) *before = 0;
+            return mine;
+        }
+        if (lane == 0) part[turn][wave] = mine;
+        __syncthreads();
+        int sum = 0, pre = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const int x = part[turn][w];
+            sum += x;
+            pre += w < wave ? x : 0;
+        }
+        turn ^= 1;
+        if (before) *before = pre;
+        return sum;
+    };
+    auto at_least = [&](u64 x) {
+        int n = 0;
+#pragma unroll
+        for (int m = 0; m < K; ++m) n += popc(__ballot(key[m] >= x));
+        return total(n, nullptr);
+    };
+    // All scores above `bar`, and `ties` of those equal to it.
+    u64 bar = 0;
+    int ties = 0;
+    if (at_least(1) > a.count) {
+        u64 top = 0;
+        bool done = false;
+        for (int bit = 63; bit >= 0 && !done; --bit) {
+            const u64 x = top | 1ull << bit;
+            const int n = at_least(x);
+            if (n >= a.count) top = x;
+            done = n == a.count;
+        }
+        bar = done ? top - 1 : top;
+        if (!done) ties = a.count - (top == ~0ull ? 0 : at_least(top + 1));
+    }
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int n = 0; n < K; ++n) {
+        above += popc(__ballot(key[n] > bar));
+        equal += popc(__ballot(bar && key[n] == bar));
+    }
+    int ties_before;
+    total(equal, &ties_before);
+    const int mine = above + min(equal, max(0, ties - ties_before));
+    int at;
+    const int all = total(mine, &at);
+    const u64 below = (1ull << lane) - 1;
+    int ties_left = max(0, ties - ties_before);
+#pragma unroll
+    for (int n = 0; n < K; ++n) {
+        const u64 eq = __ballot(bar && key[n] == bar);
+        const bool take = key[n] > bar ||
+                          (bar && key[n] == bar && popc(eq & below) < ties_left);
+        const u64 mk = __ballot(take);
+        if (take) out[at + popc(mk & below)] = base + 64 * n;
+        at += popc(mk);
+        ties_left = max(0, ties_left - popc(eq));
+    }
+    for (int e = all + (WAVES == 1 ? lane : (int)threadIdx.x); e < a.count; e += 64 * WAVES)
+        out[e] = -1;
 #endif
 }
 
@@ -290,8 +427,8 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
             before = max(last, lane ? before : -1);
             const bool take = in && x > before && x < reach;
             const unsigned long long mk = __ballot(take);
-            if (take) list[n + __popcll(mk & ((1ull << lane) - 1))] = (uint16_t)x;
-            n += __popcll(mk);
+            if (take) list[n + (int)__popcll(mk & ((1ull << lane) - 1))] = (uint16_t)x;
+            n += (int)__popcll(mk);
             last = max(last, __shfl(top, 63));
         }
         if (lane == 0) n_list = n;
@@ -498,12 +635,15 @@ extern "C" int sparse_block_means(const void* x, const long long* strides, int d
     if (!x || !strides || !means) return g_err.fail("sparse_block_means: null argument");
     if (check_strides(strides, x, 16, 8, "sparse_block_means")) return 1;
     const int nb = blocks_of(S, block);
-    const MeansArgs a{x, strides[0], strides[1], strides[2], means, H, S, D, block, nb};
-    const dim3 grid(nb, B * H, D / 64);
+    const long long blocks = (long long)B * H * nb;
+    const MeansArgs a{x, strides[0], strides[1], strides[2], means, H, S, block, nb, blocks};
+    if ((blocks + 3) / 4 >= (1LL << 31)) return g_err.fail("sparse_block_means: too many blocks");
+    const dim3 grid((unsigned)((blocks + 3) / 4));
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
     if (dtype == SPARSE_DTYPE_F16)
-        hipLaunchKernelGGL(means_kernel<f16>, grid, dim3(64), 0, stream, a);
+        D == 64 ? go(means_kernel<64, f16>) : go(means_kernel<128, f16>);
     else
-        hipLaunchKernelGGL(means_kernel<bf16>, grid, dim3(64), 0, stream, a);
+        D == 64 ? go(means_kernel<64, bf16>) : go(means_kernel<128, bf16>);
     return g_err.launched("sparse_block_means", hipGetLastError());
 }
 
@@ -538,8 +678,29 @@ extern "C" int sparse_select(const float* q_means, const float* k_means, int B, 
         return g_err.fail("sparse_select: workspace misaligned or smaller than "
                           "sparse_select_workspace_bytes()");
     SelectArgs a{q_means, k_means, (double*)workspace, index, Hq, Hkv, Sq, Skv, D, block,
-                 blocks_of(Sq, kQBlock), blocks_of(Skv, block), count, causal};
-    hipLaunchKernelGGL(select_kernel, dim3(a.nq, B * Hq), dim3(256), 0, stream, a);
+                 blocks_of(Sq, kQBlock), blocks_of(Skv, block), count, causal, 0};
+    a.rows = (long long)B * Hq * a.nq;
+    if (a.rows >= (1LL << 31)) return g_err.fail("sparse_select: too many query blocks");
+    if (a.nk > 0) {
+        const int x = (Hq / Hkv * a.nq + 15) / 16, y = B * Hkv, tiles = (a.nk + 15) / 16;
+        // Shares of the key tiles: enough workgroups for the GPU, a tile a wave at least.
+        const int z = (int)std::max<long long>(
+            1, std::min<long long>((tiles + 3) / 4, 1024 / std::max(1LL, (long long)x * y)));
+        const dim3 grid(x, y, z);
+        if (D == 64)
+            hipLaunchKernelGGL(score_kernel<64>, grid, dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL(score_kernel<128>, grid, dim3(256), 0, stream, a);
+    }
+    const dim3 quads((unsigned)((a.rows + 3) / 4)), singles((unsigned)a.rows);
+    if (a.nk <= 256)
+        hipLaunchKernelGGL((select_kernel<1, 4>), quads, dim3(256), 0, stream, a);
+    else if (a.nk <= 1024)
+        hipLaunchKernelGGL((select_kernel<1, 16>), quads, dim3(256), 0, stream, a);
+    else if (a.nk <= 16384)
+        hipLaunchKernelGGL((select_kernel<16, 16>), singles, dim3(1024), 0, stream, a);
+    else
+        hipLaunchKernelGGL((select_kernel<16, 32>), singles, dim3(1024), 0, stream, a);
     return g_err.launched("sparse_select", hipGetLastError());
 }
 

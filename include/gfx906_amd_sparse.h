@@ -20,7 +20,7 @@ extern "C" {
 #define SPARSE_DTYPE_F16 0
 #define SPARSE_DTYPE_BF16 1
 #define SPARSE_Q_BLOCK 128
-#define SPARSE_MAX_BLOCKS 65535 /* key blocks of a head */
+#define SPARSE_MAX_BLOCKS 32768 /* key blocks of a head */
 #define SPARSE_MAX_COUNT 2048   /* blocks chosen for a query block */
 
 /* means[b][h][j][:] = mean of rows j*block .. of x [B, H, S, D] (the last block

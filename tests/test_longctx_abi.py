@@ -123,7 +123,7 @@ def sparse_attn(lib, **kw):
 @pytest.mark.parametrize("bad,word", [
     (dict(D=72), b"head dim"), (dict(block=32), b"blocks"), (dict(Hkv=3), b"multiple"),
     (dict(Hkv=0), b"multiple"), (dict(dtype=2), b"dtype"), (dict(Sq=-1), b"negative"),
-    (dict(Skv=1 << 30), b"2^30"), (dict(Skv=(1 << 22) + 64), b"key blocks"),
+    (dict(Skv=1 << 30), b"2^30"), (dict(Skv=(1 << 21) + 64), b"key blocks"),
     (dict(count=0), b"count"), (dict(count=2049), b"count"), (dict(scale=float("inf")), b"finite"),
     (dict(index=None), b"null"), (dict(k=None), b"null"), (dict(q=FAKE + 8), b"aligned"),
     (dict(ks=strides(1 << 20, 1 << 16, 100)), b"multiples of 8"),
