@@ -5,9 +5,10 @@
 // gfx950 converts between E2M1 pairs with an E8M0 scale and fp16, bf16 or fp32
 // in one instruction (v_cvt_scalef32_*), rounding to nearest even and
 // saturating, so the format costs half an instruction a value to read.
-#include "longctx.h"
+#include "longctx_tile.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gfx906_amd_kv4.h"
 
@@ -249,94 +250,504 @@ __global__ void __launch_bounds__(256) load_kernel(const RowArgs a) {
 struct AttnArgs {
     const void* q;
     void* o;
-    long long qt, qh, ot, oh;
+    long long qt, qh, ot, oh;  // strides: token, head
     Cache c;
     const int* table;
     long long table_stride;
     const int* lens;
     const int* cu;  // NULL: one query a request
-    int W, T, B, Hq, max_q, causal;
-    float scale;
+    int W, T, B, Hq, G, max_q, causal;
+    float scale, qsign;  // |scale| log2(e), at least 1e-30; a negative scale negates q
+    int few_rows;  // requests of at most so many query rows a kv head go to attn_few_kernel
+    // attn_few_kernel's partial results: two slots a workgroup (below).
+    int groups, min_units;
+    long long* starts;  // [B + 1]: first unit of every request; units a workgroup
+    float* ws_o;        // [slot][row][D]
+    float* ws_ml;       // [slot][row][2]
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
 __device__ __forceinline__ int cu_at(const AttnArgs& a, int b) {
     return a.cu ? min(max(a.cu[b], 0), a.T) : b;
 }
-#endif
 
-// One wave per query row and head: 64 keys at a time, a score per lane, then a
-// pair of dims per lane (D = 64: one).
+// A request: its query rows first .. first + n - 1 of which the first m are computed,
+// its tokens, and how many of them the table's columns hold.
+struct Request {
+    int first, n, m;
+    long long len;
+    int keys;
+};
+__device__ __forceinline__ Request request(const AttnArgs& a, int b) {
+    Request r;
+    r.first = cu_at(a, b);
+    r.n = max(0, cu_at(a, b + 1) - r.first);
+    r.m = min(r.n, a.max_q);
+    r.len = max(0, a.lens[b]);
+    r.keys = (int)min(r.len, (long long)a.W * a.c.page);
+    return r;
+}
+// Keys that the query at place i of its request sees.
+__device__ __forceinline__ int seen_by(const AttnArgs& a, const Request& r, int i) {
+    return a.causal ? (int)max(0LL, min((long long)r.keys, r.len - r.n + i + 1)) : r.keys;
+}
+
+// Whether a scale byte may stand for an infinite or NaN value in element type T.
 template <class T>
-__global__ void __launch_bounds__(64) attn_rows_kernel(const AttnArgs a) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float qs[128], ps[64];
-    __shared__ long long code_s[64], scale_s[64];
-    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int D = a.c.D, hk = h / (a.Hq / a.c.Hkv);
-    int b = -1, first = 0, n = 0;
-    for (int i = 0; i < a.B; ++i) {
-        const int lo = cu_at(a, i), hi = cu_at(a, i + 1);
-        if (row >= lo && row < hi && b < 0) {
-            b = i;
-            first = lo;
-            n = hi - lo;
-        }
-    }
-    if (b < 0 || row - first >= a.max_q) return;
-    const long long len = max(0, a.lens[b]);
-    const long long seen = a.causal ? len - n + (row - first) + 1 : len;
-    const T* q = (const T*)a.q + row * a.qt + h * a.qh;
-    for (int d = lane; d < D; d += 64) qs[d] = (float)q[d];
-    __syncthreads();
+constexpr unsigned kScaleLimit = __is_same(T, f16) ? 141u : 253u;
+
+// One query row over the keys t0 .. t1 - 1 of its request, by one wave: 64 keys at a
+// time, a score per lane, then a pair of dims per lane. Keys the row does not see are
+// not touched at all, so that what they hold cannot reach it. Writes the output row,
+// or (wo) unnormalised O and (m, l).
+template <int D, class T>
+__device__ __attribute__((noinline)) void attend_row(const AttnArgs& a, const T* q, int hk, int b,
+                                                     int t0, int t1, T* o, float* wo, float* ml) {
+    const int lane = threadIdx.x & 63;
     float m = kNoMax, l = 0.f, o0 = 0.f, o1 = 0.f;
-    const long long cols = min(seen, (long long)a.W * a.c.page);
-    for (long long j0 = 0; j0 < cols; j0 += 64) {
-        const long long j = j0 + lane;
-        const int page = a.table[b * a.table_stride + j0 / a.c.page];
+    for (int j0 = t0; j0 < t1; j0 += 64) {
+        const int page = a.table[b * a.table_stride + j0 / a.c.page], j = j0 + lane;
         if (page < 0 || page >= a.c.pages) continue;
-        const int tok = (int)(j % a.c.page);
-        const long long ca = code_at(a.c, page, hk, tok), sa = scale_at(a.c, page, hk, tok);
         float s = -INFINITY;
-        if (j < seen) {
+        if (j < t1) {
+            const long long ca = code_at(a.c, page, hk, j % a.c.page);
+            const long long sa = scale_at(a.c, page, hk, j % a.c.page);
             s = 0.f;
-            for (int i = 0; i < D / 8; ++i) {
-                const unsigned w = *reinterpret_cast<const unsigned*>(a.c.kc + ca + 4 * i);
-                const float e = e8m0(a.c.ks[sa + 4 * (i / 4)]);
-                const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, e, 0);
-                const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, e, 1);
-                const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, e, 2);
-                const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, e, 3);
-                s += qs[8 * i] * p0[0] + qs[8 * i + 1] * p0[1] + qs[8 * i + 2] * p1[0] +
-                     qs[8 * i + 3] * p1[1] + qs[8 * i + 4] * p2[0] + qs[8 * i + 5] * p2[1] +
-                     qs[8 * i + 6] * p3[0] + qs[8 * i + 7] * p3[1];
+            for (int i = 0; i < D / 2; ++i) {
+                const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
+                    (unsigned)a.c.kc[ca + i], e8m0(a.c.ks[sa + 4 * (i / 16)]), 0);
+                s = fmaf((float)q[2 * i], x[0], s);
+                s = fmaf((float)q[2 * i + 1], x[1], s);
             }
-            s *= a.scale * kLog2e;
+            s *= a.scale * a.qsign;
         }
-        const float mn = fmaxf(m, wave_max(s)), w = exp2f(m - mn), p = exp2f(s - mn);
+        const float mn = max2(m, wave_max(s)), w = exp2f(m - mn), p = exp2f(s - mn);
         l = l * w + wave_sum(p);
         o0 *= w;
         o1 *= w;
         m = mn;
-        ps[lane] = p;
-        code_s[lane] = ca;
-        scale_s[lane] = sa;
-        __syncthreads();
-        if (2 * lane < D)
-            for (int i = 0; i < 64 && j0 + i < seen; ++i) {
-                const unsigned c = a.c.vc[code_s[i] + lane];
+        for (int i = 0; i < 64 && j0 + i < t1; ++i) {
+            const float pi = __shfl(p, i);
+            if (2 * lane < D) {
+                const int t = (j0 + i) % a.c.page;
                 const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
-                    c, e8m0(a.c.vs[scale_s[i] + 4 * (lane / 16)]), 0);
-                o0 += ps[i] * x[0];
-                o1 += ps[i] * x[1];
+                    (unsigned)a.c.vc[code_at(a.c, page, hk, t) + lane],
+                    e8m0(a.c.vs[scale_at(a.c, page, hk, t) + 4 * (lane / 16)]), 0);
+                o0 = fmaf(pi, x[0], o0);
+                o1 = fmaf(pi, x[1], o1);
             }
+        }
+    }
+    if (wo) {
+        if (2 * lane < D) *reinterpret_cast<f32x2*>(wo + 2 * lane) = f32x2{o0, o1};
+        if (lane == 0) *reinterpret_cast<f32x2*>(ml) = f32x2{m, l};
+    } else if (2 * lane < D) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        *reinterpret_cast<typename Elem<T>::x2*>(o + 2 * lane) = Elem<T>::cvt2(o0 * inv, o1 * inv);
+    }
+}
+
+// A lane's part of 16 cache rows: 32 (D = 128) or 16 dims of row l%16, D/32 dwords.
+template <int D>
+struct Codes {
+    unsigned w[D / 32];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (D == 128) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+            w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
+        } else {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+            w[0] = x[0], w[1] = x[1];
+        }
+    }
+};
+template <class T>
+__device__ __forceinline__ typename Elem<T>::x8 expand(unsigned w, float s) {
+    typename Elem<T>::x2 p[4];
+    if constexpr (__is_same(T, f16)) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
+    }
+    auto u = [](typename Elem<T>::x2 x) { return __builtin_bit_cast(unsigned, x); };
+    return __builtin_bit_cast(typename Elem<T>::x8, u32x4{u(p[0]), u(p[1]), u(p[2]), u(p[3])});
+}
+#endif
+
+// Attention of requests with few query rows (single tokens, drafts), bound by the
+// bytes of the cache.
+//
+// Work is counted in units of 64 tokens of one kv head of one request (and of one tile
+// of 16 NB query rows: a token's G heads share the keys). The lengths lie on the GPU, so
+// every workgroup adds up all requests' units and takes an equal run of them, which may
+// end inside a head and span several: a ragged batch fills the GPU as an even one does.
+// Within a run the four waves take every fourth unit of a head, each with its own
+// running max and sums, and are merged through LDS. A head that lies in one run is
+// finished there; of others each run writes unnormalised O and (m, l) to a slot of the
+// workspace (2 w + 1 of workgroup w for the run that begins the head, 2 w for the
+// others), which few_combine_kernel merges.
+//
+// A wave reads 16 keys as 16 bytes a lane: lane group g has dims g D/4 .. of key l%16 (at
+// D = 128 one scale block), converts them in registers, and they are the matrix operand
+// as they stand: the dims of a step are split over the lane groups alike for K and
+// Q, whatever their order. V goes through LDS in the element type (8 KB a wave), as the
+// second product sums over keys. The next unit's codes are loaded while one is computed.
+template <int D, class T, int NB>
+__global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using W = Tile<D, T, NB>;
+    using x8 = typename W::x8;
+    constexpr int R = 16 * NB, DW = D / 32;
+    __shared__ __attribute__((aligned(1024))) char stage[4][W::BYTES];
+    __shared__ float ml_s[4][R][2];
+    __shared__ long long run0[257];
+    __shared__ int found, redo_s;
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+
+    // Units of a request.
+    struct Units {
+        int chunks, tiles;
+    };
+    auto units_of = [&](const Request& r) {
+        const int rows = (int)min((long long)r.m * a.G, 1LL << 30);
+        Units u{0, 0};
+        if (rows > 0 && rows <= a.few_rows) {
+            u.chunks = (r.keys + 63) / 64;
+            u.tiles = (rows + R - 1) / R;
+        }
+        return u;
+    };
+    auto count = [&](const Units& u) { return (long long)u.chunks * u.tiles * a.c.Hkv; };
+    const int per_run = (a.B + 255) / 256;
+    {
+        long long n = 0;
+        for (int b = tid * per_run; b < min(a.B, (tid + 1) * per_run); ++b)
+            n += count(units_of(request(a, b)));
+        long long sum = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const long long x = __shfl_up(sum, o);
+            if (lane >= o) sum += x;
+        }
+        if (lane == 63) run0[wave] = sum;
+        __syncthreads();
+        long long before = 0;
+        for (int w = 0; w < wave; ++w) before += run0[w];
+        __syncthreads();
+        run0[tid + 1] = before + sum;
+        if (tid == 0) run0[0] = 0;
+        if (tid == 0) redo_s = 0;
         __syncthreads();
     }
-    T* o = (T*)a.o + row * a.ot + h * a.oh;
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    if (2 * lane < D) {
-        o[2 * lane] = (T)(o0 * inv);
-        o[2 * lane + 1] = (T)(o1 * inv);
+    const long long all = run0[256];
+    const long long per = max((long long)a.min_units, (all + a.groups - 1) / a.groups);
+    if (blockIdx.x == 0) {
+        long long n = run0[tid];
+        for (int b = tid * per_run; b < min(a.B, (tid + 1) * per_run); ++b) {
+            a.starts[b] = n;
+            n += count(units_of(request(a, b)));
+        }
+        if (tid == 0) a.starts[a.B] = per;
+    }
+    const long long lo = blockIdx.x * per, hi = min(all, lo + per);
+    if (lo >= hi) return;
+    if (run0[tid] <= lo && lo < run0[tid + 1]) found = tid;
+    __syncthreads();
+    int b = uni(found) * per_run;
+    long long start = run0[uni(found)], u0 = lo;
+
+    while (u0 < hi) {
+        Request req = request(a, b);
+        Units un = units_of(req);
+        while (start + count(un) <= u0) {
+            start += count(un);
+            req = request(a, ++b);
+            un = units_of(req);
+        }
+        const int chunks = uni(un.chunks), tiles = uni(un.tiles);
+        const int s = uni((int)((u0 - start) / chunks));
+        const int c0 = uni((int)(u0 - start - (long long)s * chunks));
+        const int c1 = uni((int)min((long long)chunks, c0 + (hi - u0)));
+        const int hk = uni(s / tiles), rt = s - hk * tiles;
+        const bool whole = c0 == 0 && c1 == chunks;
+        const long long slot = 2LL * blockIdx.x + (c0 == 0 ? 1 : 0);
+        u0 += c1 - c0;
+
+        // This lane's query rows (16 nb + i of the tile): Q fragments and keys seen.
+        W w;
+        w.init(lane);
+        int lim[NB];
+        const int rows = req.m * a.G;
+        const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = rt * R + 16 * nb + i, tok = r / a.G, h = hk * a.G + r - tok * a.G;
+            const bool ok = r < rows;
+            lim[nb] = ok ? seen_by(a, req, tok) : 0;
+            const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh + g * (D / 4);
+#pragma unroll
+            for (int n = 0; n < DW; ++n) {
+                u32x4 x = {};
+                if (ok) x = *reinterpret_cast<const u32x4*>(q + 8 * n);
+                w.qf[nb][n] = __builtin_bit_cast(x8, x ^ neg);
+            }
+        }
+        // Keys every row of the tile sees.
+        const int all_see = uni(seen_by(a, req, rt * R / a.G));
+
+        const auto table = (const __attribute__((address_space(4))) int*)(a.table +
+                                                                          b * a.table_stride);
+        const int shift = a.c.page == 64 ? 0 : a.c.page == 128 ? 1 : 2;
+        Codes<D> kc[4], vc[4];
+        unsigned ks = 0, vs = 0;
+        auto page_of = [&](int c) { return c < c1 ? table[c >> shift] : -1; };
+        auto fetch = [&](int c, int page) __attribute__((always_inline)) {
+            if ((unsigned)page >= (unsigned)a.c.pages) return;
+            const int tok = (c & ((1 << shift) - 1)) * 64;
+            const long long row = ((long long)page * a.c.Hkv + hk) * a.c.page + tok;
+            const long long at = row * (D / 2) + i * (D / 2) + g * (D / 8);
+            const long long sc = (row / 4 + i) * (D / 8) + (D == 128 ? g : g >> 1) * 4;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) kc[t].load(a.c.kc + at + t * 8 * D);
+            ks = *reinterpret_cast<const unsigned*>(a.c.ks + sc);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) vc[t].load(a.c.vc + at + t * 8 * D);
+            vs = *reinterpret_cast<const unsigned*>(a.c.vs + sc);
+        };
+        bool redo = false;
+        int c = c0 + wave, page = page_of(c), next = page_of(c + 4);
+        fetch(c, page);
+        for (; c < c1; c += 4) {
+            Codes<D> k[4], v[4];
+            unsigned kscale = ks, vscale = vs;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) k[t] = kc[t], v[t] = vc[t];
+            const bool ok = (unsigned)page < (unsigned)a.c.pages;
+            page = next;
+            next = page_of(c + 8);
+            fetch(c + 4, page);
+            if (!ok) continue;
+            const int key0 = c * 64;
+            const bool hidden = key0 + 64 > all_see;
+            if (hidden) {
+                // Values behind the last token are nothing; a value that some row does not
+                // see must be finite (its weight of 0 would not keep it out of the sums).
+                bool bad = false;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const bool none = key0 + 16 * t + i >= req.keys;
+                    const unsigned byte = vscale >> (8 * t) & 255;
+                    if (none) {
+                        vscale = (vscale & ~(255u << (8 * t))) | 127u << (8 * t);
+#pragma unroll
+                        for (int n = 0; n < DW; ++n) v[t].w[n] = 0;
+                    }
+                    bad |= !none && byte >= kScaleLimit<T>;
+                }
+                redo |= __any(bad);
+            }
+            char* const st = stage[wave];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4 S[2][NB];
+                x8 P[NB];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float vsc = e8m0(vscale >> (8 * (2 * half + t)) & 255);
+                    const int row = 16 * t + i;
+#pragma unroll
+                    for (int n = 0; n < DW; ++n)
+                        *reinterpret_cast<GFX906_LDS x8*>(
+                            (GFX906_LDS char*)st + row * W::RB +
+                            ((g * DW + n) ^ vswz<W::NU>(row)) * 16) =
+                            expand<T>(v[2 * half + t].w[n], vsc);
+                    const float ksc = e8m0(kscale >> (8 * (2 * half + t)) & 255);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) S[t][nb] = f32x4{};
+#pragma unroll
+                    for (int n = 0; n < DW; ++n) {
+                        const x8 kf = expand<T>(k[2 * half + t].w[n], ksc);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            S[t][nb] = Elem<T>::mma16(kf, w.qf[nb][n], S[t][nb]);
+                    }
+                }
+                if (hidden) w.mask(S, key0 + 32 * half, lim, g);
+                w.softmax(S, P, a.scale);
+                __builtin_amdgcn_wave_barrier();
+                w.pv(st, P);
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+
+        // Merge the waves: a common max, then sums of 16 rows at a time through LDS.
+        if (redo) redo_s = 1;
+        float l[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            l[nb] = quad_sum(w.lacc[nb][0]);
+            if (g == 0) {
+                ml_s[wave][16 * nb + i][0] = w.m[nb];
+                ml_s[wave][16 * nb + i][1] = l[nb];
+            }
+        }
+        __syncthreads();
+        const bool again = redo_s != 0;
+        if (__builtin_expect(again, 0)) {
+            const AttnArgs& ka = *(const AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+            for (int r = wave; r < R && rt * R + r < rows; r += 4) {
+                const int tok = (rt * R + r) / a.G, h = hk * a.G + rt * R + r - tok * a.G;
+                const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh;
+                T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh;
+                attend_row<D, T>(ka, q, hk, b, c0 * 64, min(c1 * 64, seen_by(a, req, tok)), o,
+                                 whole ? nullptr : a.ws_o + (slot * R + r) * D,
+                                 a.ws_ml + (slot * R + r) * 2);
+            }
+            __syncthreads();
+            if (tid == 0) redo_s = 0;
+            __syncthreads();
+            continue;
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            float mx = kNoMax;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mx = max2(mx, ml_s[x][16 * nb + i][0]);
+            const float f = __builtin_amdgcn_exp2f(w.m[nb] - mx);
+            auto* const buf = (GFX906_LDS float*)(GFX906_LDS char*)stage[wave];
+#pragma unroll
+            for (int ob = 0; ob < W::NO; ++ob)
+                *reinterpret_cast<GFX906_LDS f32x4*>(buf + i * D + ((16 * ob + 4 * g) ^ (4 * i & (D - 4)))) =
+                    w.oacc[ob][nb] * f;
+            __syncthreads();
+            for (int e = tid; e < 4 * D; e += 256) {  // 16 rows x D/4 quads
+                const int r = e / (D / 4), d = (e - r * (D / 4)) * 4, x = d ^ (4 * r & (D - 4));
+                f32x4 acc = {};
+                float mr = kNoMax, lr = 0.f;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) mr = max2(mr, ml_s[y][16 * nb + r][0]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    lr += ml_s[y][16 * nb + r][1] * __builtin_amdgcn_exp2f(ml_s[y][16 * nb + r][0] - mr);
+                    acc += *reinterpret_cast<const GFX906_LDS f32x4*>(
+                        (const GFX906_LDS float*)(const GFX906_LDS char*)stage[y] + r * D + x);
+                }
+                const int row = rt * R + 16 * nb + r;
+                if (row >= rows) continue;
+                if (whole) {
+                    const int tok = row / a.G, h = hk * a.G + row - tok * a.G;
+                    T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh + d;
+                    acc *= lr != 0.f ? 1.f / lr : 0.f;
+                    const auto x0 = Elem<T>::cvt2(acc[0], acc[1]), x1 = Elem<T>::cvt2(acc[2], acc[3]);
+                    *reinterpret_cast<u32x2*>(o) =
+                        u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
+                } else {
+                    *reinterpret_cast<f32x4*>(a.ws_o + (slot * R + 16 * nb + r) * D + d) = acc;
+                    if (d == 0)
+                        *reinterpret_cast<f32x2*>(a.ws_ml + (slot * R + 16 * nb + r) * 2) =
+                            f32x2{mr, lr};
+                }
+            }
+            __syncthreads();
+        }
+    }
+#endif
+}
+
+// Merges the slots of heads that lie in several runs, and writes the zeros of requests
+// without tokens. One workgroup per request, kv head and query row of it.
+template <int D, class T, int NB>
+__global__ void __launch_bounds__(256) few_combine_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int R = 16 * NB, DQ = D / 4, NG = 256 / DQ;
+    __shared__ f32x4 acc_s[NG][DQ];
+    __shared__ float ml_s[NG][2];
+    const int b = blockIdx.x / a.c.Hkv, hk = blockIdx.x - b * a.c.Hkv, row = blockIdx.y;
+    const Request req = request(a, b);
+    const long long rows = (long long)req.m * a.G;
+    if (rows > a.few_rows || row >= rows) return;
+    const int tok = row / a.G, h = hk * a.G + row - tok * a.G;
+    const int grp = threadIdx.x / DQ, d = (threadIdx.x - grp * DQ) * 4;
+    T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh + d;
+    const int chunks = (req.keys + 63) / 64, tiles = (int)((rows + R - 1) / R), rt = row / R;
+    if (chunks == 0) {
+        if (grp == 0) *reinterpret_cast<u32x2*>(o) = u32x2{};
+        return;
+    }
+    const long long per = a.starts[a.B];
+    const long long s = a.starts[b] + ((long long)hk * tiles + rt) * chunks;
+    const int w0 = (int)(s / per), w1 = (int)((s + chunks - 1) / per);
+    if (w0 == w1) return;
+    float m = kNoMax, l = 0.f;
+    f32x4 acc = {};
+    constexpr int U = 4;
+    for (int x = w0 + grp; x <= w1; x += NG * U) {
+        f32x2 ml[U];
+        f32x4 p[U];
+#pragma unroll
+        for (int n = 0; n < U; ++n) {
+            const int y = x + n * NG;
+            ml[n] = f32x2{kNoMax, 0.f};
+            p[n] = f32x4{};
+            if (y <= w1) {
+                const long long at = (2LL * y + (y == w0 ? 1 : 0)) * R + (row - rt * R);
+                ml[n] = *reinterpret_cast<const f32x2*>(a.ws_ml + at * 2);
+                p[n] = *reinterpret_cast<const f32x4*>(a.ws_o + at * D + d);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < U; ++n) {
+            const float mn = max2(m, ml[n][0]);
+            const float f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(ml[n][0] - mn);
+            acc = acc * f + p[n] * e;
+            l = l * f + ml[n][1] * e;
+            m = mn;
+        }
+    }
+    acc_s[grp][d / 4] = acc;
+    if (d == 0) {
+        ml_s[grp][0] = m;
+        ml_s[grp][1] = l;
+    }
+    __syncthreads();
+    if (grp) return;
+    float mx = kNoMax;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) mx = max2(mx, ml_s[n][0]);
+    acc = f32x4{};
+    l = 0.f;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+        const float f = __builtin_amdgcn_exp2f(ml_s[n][0] - mx);
+        acc += acc_s[n][d / 4] * f;
+        l += ml_s[n][1] * f;
+    }
+    acc *= l != 0.f ? 1.f / l : 0.f;
+    const auto x0 = Elem<T>::cvt2(acc[0], acc[1]), x1 = Elem<T>::cvt2(acc[2], acc[3]);
+    *reinterpret_cast<u32x2*>(o) =
+        u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
+#endif
+}
+
+// Requests of more than few_rows query rows: one wave per query row and head.
+template <int D, class T>
+__global__ void __launch_bounds__(64) attn_rows_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int row = blockIdx.x, h = blockIdx.y;
+    for (int b = 0; b < a.B; ++b) {
+        const Request r = request(a, b);
+        const int i = row - r.first;
+        if (i < 0 || i >= r.m || (long long)r.m * a.G <= a.few_rows) continue;
+        attend_row<D, T>(a, (const T*)a.q + row * a.qt + h * a.qh, h / a.G, b, 0, seen_by(a, r, i),
+                         (T*)a.o + row * a.ot + h * a.oh, nullptr, nullptr);
     }
 #endif
 }
@@ -355,6 +766,27 @@ int check_cache(int Hkv, int D, int pages, int page, const void* kc, const void*
     if (!aligned(kc, 16) || !aligned(vc, 16) || !aligned(ks, 4) || !aligned(vs, 4))
         return g_err.fail("%s: codes must be 16-byte and scales 4-byte aligned", who);
     return 0;
+}
+
+// How attn_few_kernel is launched. Workgroups: two a CU, or as few as the table's
+// columns can keep busy with kMinUnits units each (a unit a wave).
+constexpr int kFewRows = 64, kGroups = 512, kMinUnits = 4;
+struct FewPlan {
+    int nb, groups;
+    size_t o_off, ml_off, bytes;  // of the workspace
+};
+FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len) {
+    FewPlan p;
+    const long long rows = std::min<long long>((long long)max_q * G, kFewRows);
+    p.nb = rows > 16 ? 2 : 1;
+    const long long units = (long long)B * Hkv * ((std::max(max_len, 1) + 63LL) / 64) *
+                            ((rows + 16 * p.nb - 1) / (16 * p.nb));
+    p.groups = (int)std::max(1LL, std::min<long long>(kGroups, (units + kMinUnits - 1) / kMinUnits));
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    p.o_off = up((size_t)(B + 1) * sizeof(long long));
+    p.ml_off = p.o_off + (size_t)2 * p.groups * 16 * p.nb * D * sizeof(float);
+    p.bytes = p.ml_off + (size_t)2 * p.groups * 16 * p.nb * 2 * sizeof(float);
+    return p;
 }
 
 }  // namespace
@@ -450,8 +882,8 @@ extern "C" int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, cons
 
 extern "C" size_t kv4_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q,
                                            int max_len) {
-    (void)T, (void)B, (void)Hq, (void)Hkv, (void)D, (void)max_q, (void)max_len;
-    return 0;
+    if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0 || max_q <= 0) return 0;
+    return few_plan(B, Hq / Hkv, Hkv, D, std::min(max_q, T), max_len).bytes;
 }
 
 extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
@@ -483,7 +915,10 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     const long long oe[2] = {T, Hq};
     if (!rows_apart(o_strides, oe, 2, D)) return g_err.fail("kv4_attn: o's rows overlap");
     if (!(scale > -INFINITY && scale < INFINITY)) return g_err.fail("kv4_attn: scale must be finite");
-    (void)workspace, (void)workspace_bytes;
+    const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page);
+    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
+        return g_err.fail("kv4_attn: workspace misaligned or smaller than "
+                          "kv4_attn_workspace_bytes()");
     AttnArgs a{};
     a.q = q;
     a.o = o;
@@ -501,12 +936,39 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     a.T = T;
     a.B = B;
     a.Hq = Hq;
-    a.max_q = cu_q ? max_q : 1;
+    a.G = Hq / Hkv;
+    a.max_q = cu_q ? std::min(max_q, T) : 1;
     a.causal = causal;
-    a.scale = scale;
+    a.scale = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+    a.qsign = scale < 0.f ? -1.f : 1.f;
+    a.few_rows = kFewRows;
+    a.groups = plan.groups;
+    a.min_units = kMinUnits;
+    a.starts = (long long*)workspace;
+    a.ws_o = (float*)((char*)workspace + plan.o_off);
+    a.ws_ml = (float*)((char*)workspace + plan.ml_off);
+    const long long rows = (long long)a.max_q * a.G;
+    const dim3 cgrid((unsigned)(B * Hkv), (unsigned)std::min<long long>(rows, kFewRows));
+    if ((long long)B * Hkv >= (1LL << 31)) return g_err.fail("kv4_attn: too many heads");
+    auto few = [&](auto kernel, auto combine) {
+        hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(combine, cgrid, dim3(256), 0, stream, a);
+    };
+    auto go = [&](auto d, auto t) {
+        constexpr int kD = decltype(d)::value;
+        using E = decltype(t);
+        if (plan.nb == 1)
+            few(attn_few_kernel<kD, E, 1>, few_combine_kernel<kD, E, 1>);
+        else
+            few(attn_few_kernel<kD, E, 2>, few_combine_kernel<kD, E, 2>);
+        if (rows > kFewRows)
+            hipLaunchKernelGGL((attn_rows_kernel<kD, E>), dim3(T, Hq), dim3(64), 0, stream, a);
+    };
     if (dtype == KV4_DTYPE_F16)
-        hipLaunchKernelGGL(attn_rows_kernel<f16>, dim3(T, Hq), dim3(64), 0, stream, a);
+        D == 64 ? go(std::integral_constant<int, 64>{}, f16{})
+                : go(std::integral_constant<int, 128>{}, f16{});
     else
-        hipLaunchKernelGGL(attn_rows_kernel<bf16>, dim3(T, Hq), dim3(64), 0, stream, a);
+        D == 64 ? go(std::integral_constant<int, 64>{}, bf16{})
+                : go(std::integral_constant<int, 128>{}, bf16{});
     return g_err.launched("kv4_attn", hipGetLastError());
 }

@@ -1,5 +1,5 @@
-// One wave's work on blocks of 32 keys, for 32 query rows and head dims of 64 or
-// 128: the matrix products, the softmax and the tile layout in LDS that the sparse
+// One wave's work on blocks of 32 keys, for 16 or 32 query rows and head dims of 64
+// or 128: the matrix products, the softmax and the tile layout in LDS that the sparse
 // and the 4-bit cache's prompt kernels share. The scheme is that of attn_fwd_pipe
 // (attn_kernel.hip):
 //
@@ -82,28 +82,35 @@ __device__ __forceinline__ int vswz(int r) { return NU >= 16 ? 2 * (r & 7) : 2 *
 // Whether some element of P (non-negative) exceeds kPLimit or is NaN, in any lane.
 // bf16 goes through the same packed fp16 maxima: patterns of non-negative values
 // order alike, and kPLimit's bf16 pattern read as fp16 is 7.0.
-template <class T>
-__device__ __forceinline__ bool p_above(const typename Elem<T>::x8 (&P)[2]) {
-    const u32x4 a = __builtin_bit_cast(u32x4, P[0]), b = __builtin_bit_cast(u32x4, P[1]);
+template <class T, int NB>
+__device__ __forceinline__ bool p_above(const typename Elem<T>::x8 (&P)[NB]) {
     auto h = [](unsigned u) { return __builtin_bit_cast(f16x2, u); };
     auto mx = [](f16x2 x, f16x2 y) { return __builtin_elementwise_maximum(x, y); };
-    const f16x2 x = mx(mx(h(a[0]), h(a[1])), h(a[2])), y = mx(mx(h(a[3]), h(b[0])), h(b[1]));
-    const f16x2 r = mx(y, mx(mx(h(b[2]), h(b[3])), x));
+    const u32x4 a = __builtin_bit_cast(u32x4, P[0]);
+    f16x2 r;
+    if constexpr (NB == 2) {
+        const u32x4 b = __builtin_bit_cast(u32x4, P[1]);
+        const f16x2 x = mx(mx(h(a[0]), h(a[1])), h(a[2])), y = mx(mx(h(a[3]), h(b[0])), h(b[1]));
+        r = mx(y, mx(mx(h(b[2]), h(b[3])), x));
+    } else {
+        r = mx(mx(mx(h(a[0]), h(a[1])), h(a[2])), h(a[3]));
+    }
     const f16 lim = __is_same(T, f16) ? (f16)kPLimit : __builtin_bit_cast(f16, (bf16)kPLimit);
     return __any(!(r[0] <= lim) || !(r[1] <= lim));
 }
 
-template <int D, class T>
+// NB: column blocks of 16 query rows.
+template <int D, class T, int NB = 2>
 struct Tile {
     using E = Elem<T>;
     using x8 = typename E::x8;
     static constexpr int NU = D / 8, RB = 2 * D, BYTES = 32 * RB;  // one tile
     static constexpr int NQ = D / 32, NO = D / 16;
 
-    x8 qf[2][NQ];  // query 16 nb + l%16, dims 32 s + 8 (l/16)..+7
-    f32x4 oacc[NO][2];
-    f32x4 lacc[2];
-    float m[2];  // running max in log2 units
+    x8 qf[NB][NQ];  // query 16 nb + l%16, dims 32 s + 8 (l/16)..+7
+    f32x4 oacc[NO][NB];
+    f32x4 lacc[NB];
+    float m[NB];  // running max in log2 units
     bool far;    // (wave-uniform) some |m| is past 2^16: exact maxima from there on
     x8 one;
     int kaddr[NQ], vaddr[NO];
@@ -111,7 +118,7 @@ struct Tile {
     __device__ __forceinline__ void init(int lane) {
         const int i = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int ob = 0; ob < NO; ++ob) oacc[ob][nb] = f32x4{};
             lacc[nb] = f32x4{};
@@ -128,55 +135,55 @@ struct Tile {
     }
 
     // S of the K tile kt.
-    __device__ __forceinline__ void qk(const char* kt, f32x4 (&S)[2][2]) const {
+    __device__ __forceinline__ void qk(const char* kt, f32x4 (&S)[2][NB]) const {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) S[kb][nb] = f32x4{};
+            for (int nb = 0; nb < NB; ++nb) S[kb][nb] = f32x4{};
 #pragma unroll
         for (int s = 0; s < NQ; ++s)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const x8 kf = lds_read16<T>(kt, kaddr[s] + 16 * kb * RB);
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb) S[kb][nb] = E::mma16(kf, qf[nb][s], S[kb][nb]);
+                for (int nb = 0; nb < NB; ++nb) S[kb][nb] = E::mma16(kf, qf[nb][s], S[kb][nb]);
             }
         // K reads a few fragments ahead of the products (as attn_fwd_pipe's order).
         constexpr int A = D == 64 ? 3 : 2;
         __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
 #pragma unroll
         for (int n = 0; n < 2 * NQ - A; ++n) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * A, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, NB * A, 0);
     }
 
     // O^T += V^T P^T of the V tile vt.
-    __device__ __forceinline__ void pv(const char* vt, const x8 (&P)[2]) {
+    __device__ __forceinline__ void pv(const char* vt, const x8 (&P)[NB]) {
 #pragma unroll
         for (int ob = 0; ob < NO; ++ob) {
             const x8 vf = lds_read_tr2<T>(vt, vaddr[ob], vaddr[ob] + 16 * RB);
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) oacc[ob][nb] = E::mma16(vf, P[nb], oacc[ob][nb]);
+            for (int nb = 0; nb < NB; ++nb) oacc[ob][nb] = E::mma16(vf, P[nb], oacc[ob][nb]);
         }
         constexpr int A = D == 128 ? 4 : 3;
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * A, 0);
 #pragma unroll
         for (int n = 0; n < NO - A; ++n) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * A, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, NB * A, 0);
     }
 
     // Scores of keys key0 + 0..31 at or past lim[nb] to -inf.
-    __device__ __forceinline__ void mask(f32x4 (&S)[2][2], int key0, const int (&lim)[2],
+    __device__ __forceinline__ void mask(f32x4 (&S)[2][NB], int key0, const int (&lim)[NB],
                                          int g) const {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (key0 + 16 * kb + 4 * g + r >= lim[nb]) S[kb][nb][r] = -INFINITY;
@@ -188,7 +195,7 @@ struct Tile {
     // within what an fp32 sum of that size may be off by; at 2^33 it would be 2^9 and
     // overflow.
     template <bool FAR>
-    __device__ __forceinline__ void weights(const f32x4 (&S)[2][2], x8 (&P)[2], float c,
+    __device__ __forceinline__ void weights(const f32x4 (&S)[2][NB], x8 (&P)[NB], float c,
                                             int nb) const {
 #pragma clang fp contract(off)
         auto p = [&](float s) __attribute__((always_inline)) {
@@ -205,16 +212,16 @@ struct Tile {
         }
     }
 
-    __device__ __forceinline__ void softmax(const f32x4 (&S)[2][2], x8 (&P)[2], float c) {
+    __device__ __forceinline__ void softmax(const f32x4 (&S)[2][NB], x8 (&P)[NB], float c) {
         bool exact = far;
         if (__builtin_expect(!far, 1)) {
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) weights<false>(S, P, c, nb);
-            exact = p_above<T>(P);
+            for (int nb = 0; nb < NB; ++nb) weights<false>(S, P, c, nb);
+            exact = p_above<T, NB>(P);
         }
         if (__builtin_expect(exact, 0)) {
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) {
+            for (int nb = 0; nb < NB; ++nb) {
                 const float a = max3(S[0][nb][0], S[0][nb][1], S[0][nb][2]);
                 const float b = max3(S[0][nb][3], S[1][nb][0], S[1][nb][1]);
                 const float mx = max3(a, b, max2(S[1][nb][2], S[1][nb][3]));
@@ -227,10 +234,10 @@ struct Tile {
                 weights<true>(S, P, c, nb);
             }
             auto big = [](float x) { return fabsf(x) > 65536.f && x != kNoMax; };
-            far = __any(big(m[0]) || big(m[1]));
+            far = __any(big(m[0]) || big(m[NB - 1]));
         }
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) lacc[nb] = E::mma16(one, P[nb], lacc[nb]);
+        for (int nb = 0; nb < NB; ++nb) lacc[nb] = E::mma16(one, P[nb], lacc[nb]);
     }
 };
 
