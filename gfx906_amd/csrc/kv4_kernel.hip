@@ -298,11 +298,9 @@ constexpr unsigned kScaleLimit = __is_same(T, f16) ? 141u : 253u;
 
 // One query row over the keys t0 .. t1 - 1 of its request, by one wave: 64 keys at a
 // time, a score per lane, then a pair of dims per lane. Keys the row does not see are
-// not touched at all, so that what they hold cannot reach it. Writes the output row,
-// or (wo) unnormalised O and (m, l).
+// not touched at all, so that what they hold cannot reach it.
 template <int D, class T>
-__device__ __attribute__((noinline)) void attend_row(const AttnArgs& a, const T* q, int hk, int b,
-                                                     int t0, int t1, T* o, float* wo, float* ml) {
+__device__ void attend_row(const AttnArgs& a, const T* q, int hk, int b, int t0, int t1, T* o) {
     const int lane = threadIdx.x & 63;
     float m = kNoMax, l = 0.f, o0 = 0.f, o1 = 0.f;
     for (int j0 = t0; j0 < t1; j0 += 64) {
@@ -338,10 +336,7 @@ __device__ __attribute__((noinline)) void attend_row(const AttnArgs& a, const T*
             }
         }
     }
-    if (wo) {
-        if (2 * lane < D) *reinterpret_cast<f32x2*>(wo + 2 * lane) = f32x2{o0, o1};
-        if (lane == 0) *reinterpret_cast<f32x2*>(ml) = f32x2{m, l};
-    } else if (2 * lane < D) {
+    if (2 * lane < D) {
         const float inv = l != 0.f ? 1.f / l : 0.f;
         *reinterpret_cast<typename Elem<T>::x2*>(o + 2 * lane) = Elem<T>::cvt2(o0 * inv, o1 * inv);
     }
@@ -397,9 +392,10 @@ __device__ __forceinline__ typename Elem<T>::x8 expand(unsigned w, float s) {
 // D = 128 one scale block), converts them in registers, and they are the matrix operand
 // as they stand: the dims of a step are split over the lane groups alike for K and
 // Q, whatever their order. V goes through LDS in the element type (8 KB a wave), as the
-// second product sums over keys. The next unit's codes are loaded while one is computed.
+// second product sums over keys. The next unit's K codes are loaded once the scores of
+// one are done, its V codes at the end, so that neither needs registers twice.
 template <int D, class T, int NB>
-__global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using W = Tile<D, T, NB>;
     using x8 = typename W::x8;
@@ -407,7 +403,7 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) char stage[4][W::BYTES];
     __shared__ float ml_s[4][R][2];
     __shared__ long long run0[257];
-    __shared__ int found, redo_s;
+    __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
@@ -444,7 +440,6 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
         __syncthreads();
         run0[tid + 1] = before + sum;
         if (tid == 0) run0[0] = 0;
-        if (tid == 0) redo_s = 0;
         __syncthreads();
     }
     const long long all = run0[256];
@@ -509,87 +504,93 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
         Codes<D> kc[4], vc[4];
         unsigned ks = 0, vs = 0;
         auto page_of = [&](int c) { return c < c1 ? table[c >> shift] : -1; };
-        auto fetch = [&](int c, int page) __attribute__((always_inline)) {
-            if ((unsigned)page >= (unsigned)a.c.pages) return;
-            const int tok = (c & ((1 << shift) - 1)) * 64;
-            const long long row = ((long long)page * a.c.Hkv + hk) * a.c.page + tok;
-            const long long at = row * (D / 2) + i * (D / 2) + g * (D / 8);
-            const long long sc = (row / 4 + i) * (D / 8) + (D == 128 ? g : g >> 1) * 4;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) kc[t].load(a.c.kc + at + t * 8 * D);
-            ks = *reinterpret_cast<const unsigned*>(a.c.ks + sc);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) vc[t].load(a.c.vc + at + t * 8 * D);
-            vs = *reinterpret_cast<const unsigned*>(a.c.vs + sc);
+        const int off = i * (D / 2) + g * (D / 8);
+        const int soff = i * (D / 8) + (D == 128 ? g : g >> 1) * 4;
+        auto rows_at = [&](int c, int page) {
+            return ((long long)page * a.c.Hkv + hk) * a.c.page + (c & ((1 << shift) - 1)) * 64;
         };
-        bool redo = false;
-        int c = c0 + wave, page = page_of(c), next = page_of(c + 4);
-        fetch(c, page);
-        for (; c < c1; c += 4) {
-            Codes<D> k[4], v[4];
-            unsigned kscale = ks, vscale = vs;
+        auto fetch_k = [&](int c, int page) __attribute__((always_inline)) {
+            if ((unsigned)page >= (unsigned)a.c.pages) return;
+            const long long row = rows_at(c, page);
+            const uint8_t* p = a.c.kc + row * (D / 2);
+            ks = *reinterpret_cast<const unsigned*>(a.c.ks + row / 4 * (D / 8) + soff);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) k[t] = kc[t], v[t] = vc[t];
+            for (int t = 0; t < 4; ++t) kc[t].load(p + (off + t * 8 * D));
+        };
+        auto fetch_v = [&](int c, int page) __attribute__((always_inline)) {
+            if ((unsigned)page >= (unsigned)a.c.pages) return;
+            const long long row = rows_at(c, page);
+            const uint8_t* p = a.c.vc + row * (D / 2);
+            vs = *reinterpret_cast<const unsigned*>(a.c.vs + row / 4 * (D / 8) + soff);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) vc[t].load(p + (off + t * 8 * D));
+        };
+        char* const st = stage[wave];
+        int c = c0 + wave, page = page_of(c), next = page_of(c + 4);
+        fetch_k(c, page);
+        fetch_v(c, page);
+        for (; c < c1; c += 4) {
             const bool ok = (unsigned)page < (unsigned)a.c.pages;
             page = next;
             next = page_of(c + 8);
-            fetch(c + 4, page);
-            if (!ok) continue;
-            const int key0 = c * 64;
-            const bool hidden = key0 + 64 > all_see;
-            if (hidden) {
-                // Values behind the last token are nothing; a value that some row does not
-                // see must be finite (its weight of 0 would not keep it out of the sums).
-                bool bad = false;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const bool none = key0 + 16 * t + i >= req.keys;
-                    const unsigned byte = vscale >> (8 * t) & 255;
-                    if (none) {
-                        vscale = (vscale & ~(255u << (8 * t))) | 127u << (8 * t);
-#pragma unroll
-                        for (int n = 0; n < DW; ++n) v[t].w[n] = 0;
-                    }
-                    bad |= !none && byte >= kScaleLimit<T>;
-                }
-                redo |= __any(bad);
+            if (!ok) {
+                fetch_k(c + 4, page);
+                fetch_v(c + 4, page);
+                continue;
             }
-            char* const st = stage[wave];
+            f32x4 S[2][2][NB];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float sc = e8m0(ks >> (8 * t) & 255);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) S[t / 2][t % 2][nb] = f32x4{};
+#pragma unroll
+                for (int n = 0; n < DW; ++n) {
+                    const x8 kf = expand<T>(kc[t].w[n], sc);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                        S[t / 2][t % 2][nb] = Elem<T>::mma16(kf, w.qf[nb][n], S[t / 2][t % 2][nb]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_k(c + 4, page);
+            const int key0 = c * 64;
+            if (key0 + 64 > all_see) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) w.mask(S[half], key0 + 32 * half, lim, g);
+                // Values behind the last token are nothing.
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (key0 + 16 * t + i >= req.keys) {
+                        vs = (vs & ~(255u << (8 * t))) | 127u << (8 * t);
+#pragma unroll
+                        for (int n = 0; n < DW; ++n) vc[t].w[n] = 0;
+                    }
+            }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                f32x4 S[2][NB];
                 x8 P[NB];
+                w.softmax(S[half], P, a.scale);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const float vsc = e8m0(vscale >> (8 * (2 * half + t)) & 255);
+                    const float sc = e8m0(vs >> (8 * (2 * half + t)) & 255);
                     const int row = 16 * t + i;
 #pragma unroll
                     for (int n = 0; n < DW; ++n)
                         *reinterpret_cast<GFX906_LDS x8*>(
                             (GFX906_LDS char*)st + row * W::RB +
                             ((g * DW + n) ^ vswz<W::NU>(row)) * 16) =
-                            expand<T>(v[2 * half + t].w[n], vsc);
-                    const float ksc = e8m0(kscale >> (8 * (2 * half + t)) & 255);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) S[t][nb] = f32x4{};
-#pragma unroll
-                    for (int n = 0; n < DW; ++n) {
-                        const x8 kf = expand<T>(k[2 * half + t].w[n], ksc);
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-                            S[t][nb] = Elem<T>::mma16(kf, w.qf[nb][n], S[t][nb]);
-                    }
+                            expand<T>(vc[2 * half + t].w[n], sc);
                 }
-                if (hidden) w.mask(S, key0 + 32 * half, lim, g);
-                w.softmax(S, P, a.scale);
                 __builtin_amdgcn_wave_barrier();
                 w.pv(st, P);
                 __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_sched_barrier(0);
             }
+            fetch_v(c + 4, page);
         }
 
         // Merge the waves: a common max, then sums of 16 rows at a time through LDS.
-        if (redo) redo_s = 1;
         float l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -600,22 +601,6 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
             }
         }
         __syncthreads();
-        const bool again = redo_s != 0;
-        if (__builtin_expect(again, 0)) {
-            const AttnArgs& ka = *(const AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-            for (int r = wave; r < R && rt * R + r < rows; r += 4) {
-                const int tok = (rt * R + r) / a.G, h = hk * a.G + rt * R + r - tok * a.G;
-                const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh;
-                T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh;
-                attend_row<D, T>(ka, q, hk, b, c0 * 64, min(c1 * 64, seen_by(a, req, tok)), o,
-                                 whole ? nullptr : a.ws_o + (slot * R + r) * D,
-                                 a.ws_ml + (slot * R + r) * 2);
-            }
-            __syncthreads();
-            if (tid == 0) redo_s = 0;
-            __syncthreads();
-            continue;
-        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float mx = kNoMax;
@@ -662,8 +647,8 @@ __global__ void __launch_bounds__(256, 2) attn_few_kernel(const AttnArgs a) {
 #endif
 }
 
-// Merges the slots of heads that lie in several runs, and writes the zeros of requests
-// without tokens. One workgroup per request, kv head and query row of it.
+// Merges the slots of heads that lie in several runs, writes the zeros of requests
+// without tokens, and does rows again that a value they do not see may have spoilt. One workgroup per request, kv head and query row of it.
 template <int D, class T, int NB>
 __global__ void __launch_bounds__(256) few_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -681,6 +666,24 @@ __global__ void __launch_bounds__(256) few_combine_kernel(const AttnArgs a) {
     if (chunks == 0) {
         if (grp == 0) *reinterpret_cast<u32x2*>(o) = u32x2{};
         return;
+    }
+    // A weight of 0 does not keep an infinite or NaN value out of a sum: where a token that
+    // this row does not see may hold one, the row is done again without it.
+    const int seen = seen_by(a, req, tok);
+    if (seen < req.keys) {
+        bool bad = false;
+        for (int e = threadIdx.x; e < (req.keys - seen) * (D / 32); e += 256) {
+            const int t = seen + e / (D / 32), page = a.table[b * a.table_stride + t / a.c.page];
+            if ((unsigned)page < (unsigned)a.c.pages)
+                bad |= a.c.vs[scale_at(a.c, page, hk, t % a.c.page) + e % (D / 32) * 4] >=
+                       kScaleLimit<T>;
+        }
+        if (__syncthreads_or(bad)) {
+            if (threadIdx.x < 64)
+                attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0,
+                                 seen, o - d);
+            return;
+        }
     }
     const long long per = a.starts[a.B];
     const long long s = a.starts[b] + ((long long)hk * tiles + rt) * chunks;
@@ -747,7 +750,7 @@ __global__ void __launch_bounds__(64) attn_rows_kernel(const AttnArgs a) {
         const int i = row - r.first;
         if (i < 0 || i >= r.m || (long long)r.m * a.G <= a.few_rows) continue;
         attend_row<D, T>(a, (const T*)a.q + row * a.qt + h * a.qh, h / a.G, b, 0, seen_by(a, r, i),
-                         (T*)a.o + row * a.ot + h * a.oh, nullptr, nullptr);
+                         (T*)a.o + row * a.ot + h * a.oh);
     }
 #endif
 }
