@@ -258,17 +258,20 @@ struct AttnArgs {
     const int* cu;  // NULL: one query a request
     int W, T, B, Hq, G, max_q, causal;
     float scale, qsign;  // |scale| log2(e), at least 1e-30; a negative scale negates q
-    int few_rows;  // requests of at most so many query rows a kv head go to attn_few_kernel
+    int few_rows, tiles;  // requests of at most so many query rows a kv head go to attn_few_kernel
     // attn_few_kernel's partial results: two slots a workgroup (below).
     int groups, min_units;
-    long long* starts;  // [B + 1]: first unit of every request; units a workgroup
+    int* starts;  // [B + 1]: first unit of every request; units a workgroup
     float* ws_o;        // [slot][row][D]
     float* ws_ml;       // [slot][row][2]
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
+// Loads of arrays that no kernel of a call writes, through the scalar cache where the
+// index is uniform.
+typedef const __attribute__((address_space(4))) int* ConstInts;
 __device__ __forceinline__ int cu_at(const AttnArgs& a, int b) {
-    return a.cu ? min(max(a.cu[b], 0), a.T) : b;
+    return a.cu ? min(max(((ConstInts)a.cu)[b], 0), a.T) : b;
 }
 
 // A request: its query rows first .. first + n - 1 of which the first m are computed,
@@ -283,7 +286,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
     r.first = cu_at(a, b);
     r.n = max(0, cu_at(a, b + 1) - r.first);
     r.m = min(r.n, a.max_q);
-    r.len = max(0, a.lens[b]);
+    r.len = max(0, ((ConstInts)a.lens)[b]);
     r.keys = (int)min(r.len, (long long)a.W * a.c.page);
     return r;
 }
@@ -342,6 +345,21 @@ __device__ void attend_row(const AttnArgs& a, const T* q, int hk, int b, int t0,
     }
 }
 
+// Whether a token that query `tok` of its request does not see may hold an infinite or
+// NaN value: a weight of 0 would not keep that out of a sum. For a wave.
+template <int D, class T>
+__device__ __forceinline__ bool may_spoil(const AttnArgs& a, const Request& r, int b, int hk,
+                                          int tok) {
+    const int seen = seen_by(a, r, tok);
+    bool bad = false;
+    for (int e = threadIdx.x & 63; e < (r.keys - seen) * (D / 32); e += 64) {
+        const int t = seen + e / (D / 32), page = a.table[b * a.table_stride + t / a.c.page];
+        if ((unsigned)page < (unsigned)a.c.pages)
+            bad |= a.c.vs[scale_at(a.c, page, hk, t % a.c.page) + e % (D / 32) * 4] >= kScaleLimit<T>;
+    }
+    return __any(bad);
+}
+
 // A lane's part of 16 cache rows: 32 (D = 128) or 16 dims of row l%16, D/32 dwords.
 template <int D>
 struct Codes {
@@ -394,21 +412,24 @@ __device__ __forceinline__ typename Elem<T>::x8 expand(unsigned w, float s) {
 // Q, whatever their order. V goes through LDS in the element type (8 KB a wave), as the
 // second product sums over keys. The next unit's K codes are loaded once the scores of
 // one are done, its V codes at the end, so that neither needs registers twice.
-template <int D, class T, int NB>
-__global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const AttnArgs a) {
+//
+// DIRECT: short tables. One workgroup a head, no runs, no slots and no second kernel.
+template <int D, class T, int NB, int NW, bool DIRECT>
+__global__ void __launch_bounds__(64 * NW, NB == 2 ? 2 : D == 128 ? 3 : 4)
+attn_few_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using W = Tile<D, T, NB>;
     using x8 = typename W::x8;
-    constexpr int R = 16 * NB, DW = D / 32;
-    __shared__ __attribute__((aligned(1024))) char stage[4][W::BYTES];
-    __shared__ float ml_s[4][R][2];
-    __shared__ long long run0[257];
+    constexpr int R = 16 * NB, DW = D / 32, NT = 64 * NW;
+    __shared__ __attribute__((aligned(1024))) char stage[NW][W::BYTES];
+    __shared__ float ml_s[NW][R][2];
+    __shared__ int run0[NT + 1];
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
-    // Units of a request.
+    // Units of a request (the host has checked that all of them fit an int).
     struct Units {
         int chunks, tiles;
     };
@@ -421,60 +442,81 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
         }
         return u;
     };
-    auto count = [&](const Units& u) { return (long long)u.chunks * u.tiles * a.c.Hkv; };
-    const int per_run = (a.B + 255) / 256;
-    {
-        long long n = 0;
-        for (int b = tid * per_run; b < min(a.B, (tid + 1) * per_run); ++b)
-            n += count(units_of(request(a, b)));
-        long long sum = n;
+    auto count = [&](const Units& u) { return u.chunks * u.tiles * a.c.Hkv; };
+    int b = 0, start = 0, u0 = 0, hi = 1;
+    if constexpr (!DIRECT) {
+        const int per_run = (a.B + NT - 1) / NT;
+        int n = 0;
+        for (int x = tid * per_run; x < min(a.B, (tid + 1) * per_run); ++x)
+            n += count(units_of(request(a, x)));
+        int sum = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const long long x = __shfl_up(sum, o);
+            const int x = __shfl_up(sum, o);
             if (lane >= o) sum += x;
         }
-        if (lane == 63) run0[wave] = sum;
+        if (lane == 63) ml_s[wave][0][0] = __int_as_float(sum);
         __syncthreads();
-        long long before = 0;
-        for (int w = 0; w < wave; ++w) before += run0[w];
-        __syncthreads();
-        run0[tid + 1] = before + sum;
+        for (int w = 0; w < wave; ++w) sum += __float_as_int(ml_s[w][0][0]);
+        run0[tid + 1] = sum;
         if (tid == 0) run0[0] = 0;
         __syncthreads();
-    }
-    const long long all = run0[256];
-    const long long per = max((long long)a.min_units, (all + a.groups - 1) / a.groups);
-    if (blockIdx.x == 0) {
-        long long n = run0[tid];
-        for (int b = tid * per_run; b < min(a.B, (tid + 1) * per_run); ++b) {
-            a.starts[b] = n;
-            n += count(units_of(request(a, b)));
+        const int all = run0[NT];
+        const int per = max(a.min_units, uni((int)((unsigned)(all + a.groups - 1) / (unsigned)a.groups)));
+        if (blockIdx.x == 0) {
+            n = run0[tid];
+            for (int x = tid * per_run; x < min(a.B, (tid + 1) * per_run); ++x) {
+                a.starts[x] = n;
+                n += count(units_of(request(a, x)));
+            }
+            if (tid == 0) a.starts[a.B] = per;
         }
-        if (tid == 0) a.starts[a.B] = per;
+        // (the last run may end past 2^31 before it is cut)
+        const long long lo = (long long)blockIdx.x * per;
+        if (lo >= all) return;
+        u0 = (int)lo;
+        hi = (int)min((long long)all, lo + per);
+        if (run0[tid] <= u0 && u0 < run0[tid + 1]) found = tid;
+        __syncthreads();
+        b = uni(found) * per_run;
+        start = uni(run0[uni(found)]);
     }
-    const long long lo = blockIdx.x * per, hi = min(all, lo + per);
-    if (lo >= hi) return;
-    if (run0[tid] <= lo && lo < run0[tid + 1]) found = tid;
-    __syncthreads();
-    int b = uni(found) * per_run;
-    long long start = run0[uni(found)], u0 = lo;
 
     while (u0 < hi) {
-        Request req = request(a, b);
-        Units un = units_of(req);
-        while (start + count(un) <= u0) {
-            start += count(un);
-            req = request(a, ++b);
-            un = units_of(req);
+        Request req;
+        int chunks, c0, c1, hk, rt;
+        bool whole;
+        long long slot = 0;
+        if constexpr (DIRECT) {  // grid: requests x kv heads x row tiles
+            const int seg = uni(blockIdx.x / a.tiles);
+            rt = blockIdx.x - seg * a.tiles;
+            b = uni(seg / a.c.Hkv);
+            hk = seg - b * a.c.Hkv;
+            req = request(a, b);
+            if (rt * R >= (long long)req.m * a.G || (long long)req.m * a.G > a.few_rows) return;
+            chunks = (req.keys + 63) / 64;
+            c0 = 0;
+            c1 = chunks;
+            whole = true;
+            u0 = hi;
+        } else {
+            req = request(a, b);
+            Units un = units_of(req);
+            while (start + count(un) <= u0) {
+                start += count(un);
+                req = request(a, ++b);
+                un = units_of(req);
+            }
+            chunks = un.chunks;
+            const int s = uni((int)((unsigned)(u0 - start) / (unsigned)chunks));
+            c0 = u0 - start - s * chunks;
+            c1 = min(chunks, c0 + (hi - u0));
+            hk = uni((int)((unsigned)s / (unsigned)un.tiles));
+            rt = s - hk * un.tiles;
+            whole = c0 == 0 && c1 == chunks;
+            slot = 2LL * blockIdx.x + (c0 == 0 ? 1 : 0);
+            u0 += c1 - c0;
         }
-        const int chunks = uni(un.chunks), tiles = uni(un.tiles);
-        const int s = uni((int)((u0 - start) / chunks));
-        const int c0 = uni((int)(u0 - start - (long long)s * chunks));
-        const int c1 = uni((int)min((long long)chunks, c0 + (hi - u0)));
-        const int hk = uni(s / tiles), rt = s - hk * tiles;
-        const bool whole = c0 == 0 && c1 == chunks;
-        const long long slot = 2LL * blockIdx.x + (c0 == 0 ? 1 : 0);
-        u0 += c1 - c0;
 
         // This lane's query rows (16 nb + i of the tile): Q fragments and keys seen.
         W w;
@@ -498,8 +540,7 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
         // Keys every row of the tile sees.
         const int all_see = uni(seen_by(a, req, rt * R / a.G));
 
-        const auto table = (const __attribute__((address_space(4))) int*)(a.table +
-                                                                          b * a.table_stride);
+        const ConstInts table = (ConstInts)(a.table + b * a.table_stride);
         const int shift = a.c.page == 64 ? 0 : a.c.page == 128 ? 1 : 2;
         Codes<D> kc[4], vc[4];
         unsigned ks = 0, vs = 0;
@@ -526,16 +567,16 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
             for (int t = 0; t < 4; ++t) vc[t].load(p + (off + t * 8 * D));
         };
         char* const st = stage[wave];
-        int c = c0 + wave, page = page_of(c), next = page_of(c + 4);
+        int c = c0 + wave, page = page_of(c), next = page_of(c + NW);
         fetch_k(c, page);
         fetch_v(c, page);
-        for (; c < c1; c += 4) {
+        for (; c < c1; c += NW) {
             const bool ok = (unsigned)page < (unsigned)a.c.pages;
             page = next;
-            next = page_of(c + 8);
+            next = page_of(c + 2 * NW);
             if (!ok) {
-                fetch_k(c + 4, page);
-                fetch_v(c + 4, page);
+                fetch_k(c + NW, page);
+                fetch_v(c + NW, page);
                 continue;
             }
             f32x4 S[2][2][NB];
@@ -553,7 +594,7 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            fetch_k(c + 4, page);
+            fetch_k(c + NW, page);
             const int key0 = c * 64;
             if (key0 + 64 > all_see) {
 #pragma unroll
@@ -587,7 +628,7 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_sched_barrier(0);
             }
-            fetch_v(c + 4, page);
+            fetch_v(c + NW, page);
         }
 
         // Merge the waves: a common max, then sums of 16 rows at a time through LDS.
@@ -605,7 +646,7 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
         for (int nb = 0; nb < NB; ++nb) {
             float mx = kNoMax;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) mx = max2(mx, ml_s[x][16 * nb + i][0]);
+            for (int x = 0; x < NW; ++x) mx = max2(mx, ml_s[x][16 * nb + i][0]);
             const float f = __builtin_amdgcn_exp2f(w.m[nb] - mx);
             auto* const buf = (GFX906_LDS float*)(GFX906_LDS char*)stage[wave];
 #pragma unroll
@@ -613,14 +654,14 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
                 *reinterpret_cast<GFX906_LDS f32x4*>(buf + i * D + ((16 * ob + 4 * g) ^ (4 * i & (D - 4)))) =
                     w.oacc[ob][nb] * f;
             __syncthreads();
-            for (int e = tid; e < 4 * D; e += 256) {  // 16 rows x D/4 quads
+            for (int e = tid; e < 4 * D; e += NT) {  // 16 rows x D/4 quads
                 const int r = e / (D / 4), d = (e - r * (D / 4)) * 4, x = d ^ (4 * r & (D - 4));
                 f32x4 acc = {};
                 float mr = kNoMax, lr = 0.f;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) mr = max2(mr, ml_s[y][16 * nb + r][0]);
+                for (int y = 0; y < NW; ++y) mr = max2(mr, ml_s[y][16 * nb + r][0]);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < NW; ++y) {
                     lr += ml_s[y][16 * nb + r][1] * __builtin_amdgcn_exp2f(ml_s[y][16 * nb + r][0] - mr);
                     acc += *reinterpret_cast<const GFX906_LDS f32x4*>(
                         (const GFX906_LDS float*)(const GFX906_LDS char*)stage[y] + r * D + x);
@@ -643,16 +684,24 @@ __global__ void __launch_bounds__(256, NB == 1 ? 3 : 2) attn_few_kernel(const At
             }
             __syncthreads();
         }
+        if constexpr (DIRECT) {
+            for (int r = wave; r < R && rt * R + r < rows; r += NW) {
+                const int tok = (rt * R + r) / a.G, h = hk * a.G + rt * R + r - tok * a.G;
+                if (may_spoil<D, T>(a, req, b, hk, tok))
+                    attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0,
+                                     seen_by(a, req, tok), (T*)a.o + (req.first + tok) * a.ot + h * a.oh);
+            }
+        }
     }
 #endif
 }
 
 // Merges the slots of heads that lie in several runs, writes the zeros of requests
 // without tokens, and does rows again that a value they do not see may have spoilt. One workgroup per request, kv head and query row of it.
-template <int D, class T, int NB>
-__global__ void __launch_bounds__(256) few_combine_kernel(const AttnArgs a) {
+template <int D, class T, int NB, int NT>
+__global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int R = 16 * NB, DQ = D / 4, NG = 256 / DQ;
+    constexpr int R = 16 * NB, DQ = D / 4, NG = NT / DQ;
     __shared__ f32x4 acc_s[NG][DQ];
     __shared__ float ml_s[NG][2];
     const int b = blockIdx.x / a.c.Hkv, hk = blockIdx.x - b * a.c.Hkv, row = blockIdx.y;
@@ -667,27 +716,16 @@ __global__ void __launch_bounds__(256) few_combine_kernel(const AttnArgs a) {
         if (grp == 0) *reinterpret_cast<u32x2*>(o) = u32x2{};
         return;
     }
-    // A weight of 0 does not keep an infinite or NaN value out of a sum: where a token that
-    // this row does not see may hold one, the row is done again without it.
-    const int seen = seen_by(a, req, tok);
-    if (seen < req.keys) {
-        bool bad = false;
-        for (int e = threadIdx.x; e < (req.keys - seen) * (D / 32); e += 256) {
-            const int t = seen + e / (D / 32), page = a.table[b * a.table_stride + t / a.c.page];
-            if ((unsigned)page < (unsigned)a.c.pages)
-                bad |= a.c.vs[scale_at(a.c, page, hk, t % a.c.page) + e % (D / 32) * 4] >=
-                       kScaleLimit<T>;
-        }
-        if (__syncthreads_or(bad)) {
-            if (threadIdx.x < 64)
-                attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0,
-                                 seen, o - d);
-            return;
-        }
+    if (may_spoil<D, T>(a, req, b, hk, tok)) {  // (the same for every wave)
+        if (threadIdx.x < 64)
+            attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0,
+                             seen_by(a, req, tok), o - d);
+        return;
     }
-    const long long per = a.starts[a.B];
-    const long long s = a.starts[b] + ((long long)hk * tiles + rt) * chunks;
-    const int w0 = (int)(s / per), w1 = (int)((s + chunks - 1) / per);
+    const int per = a.starts[a.B];
+    const int s = a.starts[b] + (hk * tiles + rt) * chunks;
+    const int w0 = (int)((unsigned)s / (unsigned)per);
+    const int w1 = (int)((unsigned)(s + chunks - 1) / (unsigned)per);
     if (w0 == w1) return;
     float m = kNoMax, l = 0.f;
     f32x4 acc = {};
@@ -771,22 +809,31 @@ int check_cache(int Hkv, int D, int pages, int page, const void* kc, const void*
     return 0;
 }
 
-// How attn_few_kernel is launched. Workgroups: two a CU, or as few as the table's
-// columns can keep busy with kMinUnits units each (a unit a wave).
-constexpr int kFewRows = 64, kGroups = 512, kMinUnits = 4;
+// How attn_few_kernel is launched.
+constexpr int kFewRows = 64, kMinUnits = 4;
+// Tables of up to so many tokens go to the DIRECT form.
+constexpr int kDirectTokens = 2048;
 struct FewPlan {
-    int nb, groups;
+    int nb, tiles, groups;
+    bool direct, many;  // many: heads lie in 32 runs or more, if all requests are as long
+    long long units;
     size_t o_off, ml_off, bytes;  // of the workspace
 };
 FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len) {
-    FewPlan p;
+    FewPlan p{};
     const long long rows = std::min<long long>((long long)max_q * G, kFewRows);
     p.nb = rows > 16 ? 2 : 1;
-    const long long units = (long long)B * Hkv * ((std::max(max_len, 1) + 63LL) / 64) *
-                            ((rows + 16 * p.nb - 1) / (16 * p.nb));
-    p.groups = (int)std::max(1LL, std::min<long long>(kGroups, (units + kMinUnits - 1) / kMinUnits));
+    p.tiles = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
+    const long long segs = (long long)B * Hkv * p.tiles;
+    p.units = segs * ((std::max(max_len, 1) + 63LL) / 64);
+    p.direct = max_len <= kDirectTokens && segs < (1LL << 31);
+    if (p.direct) return p;
+    // As many workgroups as the GPU holds at once, with a unit a wave at least.
+    const int most = p.nb == 2 ? 256 : D == 128 ? 768 : 1024;
+    p.groups = (int)std::max(1LL, std::min<long long>(most, (p.units + kMinUnits - 1) / kMinUnits));
+    p.many = p.groups / segs >= 32;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    p.o_off = up((size_t)(B + 1) * sizeof(long long));
+    p.o_off = up((size_t)(B + 1) * sizeof(int));
     p.ml_off = p.o_off + (size_t)2 * p.groups * 16 * p.nb * D * sizeof(float);
     p.bytes = p.ml_off + (size_t)2 * p.groups * 16 * p.nb * 2 * sizeof(float);
     return p;
@@ -919,7 +966,8 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     if (!rows_apart(o_strides, oe, 2, D)) return g_err.fail("kv4_attn: o's rows overlap");
     if (!(scale > -INFINITY && scale < INFINITY)) return g_err.fail("kv4_attn: scale must be finite");
     const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page);
-    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16))
+    if (plan.units >= (1LL << 31) - 1) return g_err.fail("kv4_attn: table too wide for so many heads");
+    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
         return g_err.fail("kv4_attn: workspace misaligned or smaller than "
                           "kv4_attn_workspace_bytes()");
     AttnArgs a{};
@@ -947,23 +995,36 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     a.few_rows = kFewRows;
     a.groups = plan.groups;
     a.min_units = kMinUnits;
-    a.starts = (long long*)workspace;
+    a.tiles = plan.tiles;
+    a.starts = (int*)workspace;
     a.ws_o = (float*)((char*)workspace + plan.o_off);
     a.ws_ml = (float*)((char*)workspace + plan.ml_off);
     const long long rows = (long long)a.max_q * a.G;
     const dim3 cgrid((unsigned)(B * Hkv), (unsigned)std::min<long long>(rows, kFewRows));
     if ((long long)B * Hkv >= (1LL << 31)) return g_err.fail("kv4_attn: too many heads");
-    auto few = [&](auto kernel, auto combine) {
-        hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(256), 0, stream, a);
-        hipLaunchKernelGGL(combine, cgrid, dim3(256), 0, stream, a);
-    };
     auto go = [&](auto d, auto t) {
         constexpr int kD = decltype(d)::value;
         using E = decltype(t);
-        if (plan.nb == 1)
-            few(attn_few_kernel<kD, E, 1>, few_combine_kernel<kD, E, 1>);
+        auto direct = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(B * Hkv * plan.tiles)), dim3(512), 0, stream, a);
+        };
+        auto runs = [&](auto kernel, int threads, auto combine, auto combine_many) {
+            hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(threads), 0, stream, a);
+            if (plan.many)
+                hipLaunchKernelGGL(combine_many, cgrid, dim3(1024), 0, stream, a);
+            else
+                hipLaunchKernelGGL(combine, cgrid, dim3(256), 0, stream, a);
+        };
+        if (plan.direct && plan.nb == 1)
+            direct(attn_few_kernel<kD, E, 1, 8, true>);
+        else if (plan.direct)
+            direct(attn_few_kernel<kD, E, 2, 8, true>);
+        else if (plan.nb == 1)
+            runs(attn_few_kernel<kD, E, 1, 4, false>, 256, few_combine_kernel<kD, E, 1, 256>,
+                 few_combine_kernel<kD, E, 1, 1024>);
         else
-            few(attn_few_kernel<kD, E, 2>, few_combine_kernel<kD, E, 2>);
+            runs(attn_few_kernel<kD, E, 2, 8, false>, 512, few_combine_kernel<kD, E, 2, 256>,
+                 few_combine_kernel<kD, E, 2, 1024>);
         if (rows > kFewRows)
             hipLaunchKernelGGL((attn_rows_kernel<kD, E>), dim3(T, Hq), dim3(64), 0, stream, a);
     };
