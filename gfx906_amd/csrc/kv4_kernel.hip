@@ -260,7 +260,7 @@ struct AttnArgs {
     float scale, qsign;  // |scale| log2(e), at least 1e-30; a negative scale negates q
     int few_rows, tiles;  // requests of at most so many query rows a kv head go to attn_few_kernel
     // attn_few_kernel's partial results: two slots a workgroup (below).
-    int groups, min_units;
+    int groups, min_units, start_units;
     int* starts;  // [B + 1]: first unit of every request; units a workgroup
     float* ws_o;        // [slot][row][D]
     float* ws_ml;       // [slot][row][2]
@@ -287,7 +287,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
     r.n = max(0, cu_at(a, b + 1) - r.first);
     r.m = min(r.n, a.max_q);
     r.len = max(0, ((ConstInts)a.lens)[b]);
-    r.keys = (int)min(r.len, (long long)a.W * a.c.page);
+    r.keys = a.c.pages ? (int)min(r.len, (long long)a.W * a.c.page) : 0;
     return r;
 }
 // Keys that the query at place i of its request sees.
@@ -442,7 +442,10 @@ attn_few_kernel(const AttnArgs a) {
         }
         return u;
     };
-    auto count = [&](const Units& u) { return u.chunks * u.tiles * a.c.Hkv; };
+    // (a head's start and merge cost as much as a.start_units units)
+    auto count = [&](const Units& u) {
+        return u.chunks ? (u.chunks + a.start_units) * u.tiles * a.c.Hkv : 0;
+    };
     int b = 0, start = 0, u0 = 0, hi = 1;
     if constexpr (!DIRECT) {
         const int per_run = (a.B + NT - 1) / NT;
@@ -508,14 +511,17 @@ attn_few_kernel(const AttnArgs a) {
                 un = units_of(req);
             }
             chunks = un.chunks;
-            const int s = uni((int)((unsigned)(u0 - start) / (unsigned)chunks));
-            c0 = u0 - start - s * chunks;
-            c1 = min(chunks, c0 + (hi - u0));
+            const int each = chunks + a.start_units;
+            const int s = uni((int)((unsigned)(u0 - start) / (unsigned)each));
+            const int p0 = u0 - start - s * each, p1 = min(each, p0 + (hi - u0));
+            u0 += p1 - p0;
+            c0 = max(0, p0 - a.start_units);
+            c1 = p1 - a.start_units;
+            if (c1 <= 0) continue;  // (the run ends before the head's first unit)
             hk = uni((int)((unsigned)s / (unsigned)un.tiles));
             rt = s - hk * un.tiles;
             whole = c0 == 0 && c1 == chunks;
             slot = 2LL * blockIdx.x + (c0 == 0 ? 1 : 0);
-            u0 += c1 - c0;
         }
 
         // This lane's query rows (16 nb + i of the tile): Q fragments and keys seen.
@@ -544,14 +550,17 @@ attn_few_kernel(const AttnArgs a) {
         const int shift = a.c.page == 64 ? 0 : a.c.page == 128 ? 1 : 2;
         Codes<D> kc[4], vc[4];
         unsigned ks = 0, vs = 0;
-        auto page_of = [&](int c) { return c < c1 ? table[c >> shift] : -1; };
+        // (past the run: its last unit's page, read again and not used)
+        auto page_of = [&](int c) { return table[min(c, c1 - 1) >> shift]; };
         const int off = i * (D / 2) + g * (D / 8);
         const int soff = i * (D / 8) + (D == 128 ? g : g >> 1) * 4;
+        // The loads are unconditional, so that the compiler waits for them where they are
+        // used: a page outside the cache reads page 0, and the unit's keys are masked.
         auto rows_at = [&](int c, int page) {
-            return ((long long)page * a.c.Hkv + hk) * a.c.page + (c & ((1 << shift) - 1)) * 64;
+            const unsigned p = (unsigned)page < (unsigned)a.c.pages ? page : 0;
+            return ((long long)p * a.c.Hkv + hk) * a.c.page + (c & ((1 << shift) - 1)) * 64;
         };
         auto fetch_k = [&](int c, int page) __attribute__((always_inline)) {
-            if ((unsigned)page >= (unsigned)a.c.pages) return;
             const long long row = rows_at(c, page);
             const uint8_t* p = a.c.kc + row * (D / 2);
             ks = *reinterpret_cast<const unsigned*>(a.c.ks + row / 4 * (D / 8) + soff);
@@ -559,7 +568,6 @@ attn_few_kernel(const AttnArgs a) {
             for (int t = 0; t < 4; ++t) kc[t].load(p + (off + t * 8 * D));
         };
         auto fetch_v = [&](int c, int page) __attribute__((always_inline)) {
-            if ((unsigned)page >= (unsigned)a.c.pages) return;
             const long long row = rows_at(c, page);
             const uint8_t* p = a.c.vc + row * (D / 2);
             vs = *reinterpret_cast<const unsigned*>(a.c.vs + row / 4 * (D / 8) + soff);
@@ -568,41 +576,44 @@ attn_few_kernel(const AttnArgs a) {
         };
         char* const st = stage[wave];
         int c = c0 + wave, page = page_of(c), next = page_of(c + NW);
-        fetch_k(c, page);
-        fetch_v(c, page);
+        if (c < c1) {
+            fetch_k(c, page);
+            fetch_v(c, page);
+        }
         for (; c < c1; c += NW) {
             const bool ok = (unsigned)page < (unsigned)a.c.pages;
             page = next;
             next = page_of(c + 2 * NW);
-            if (!ok) {
-                fetch_k(c + NW, page);
-                fetch_v(c + NW, page);
-                continue;
-            }
             f32x4 S[2][2][NB];
+            float sc[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const float sc = e8m0(ks >> (8 * t) & 255);
+                sc[t] = e8m0(ks >> (8 * t) & 255);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) S[t / 2][t % 2][nb] = f32x4{};
+            }
 #pragma unroll
-                for (int n = 0; n < DW; ++n) {
-                    const x8 kf = expand<T>(kc[t].w[n], sc);
+            for (int n = 0; n < DW; ++n)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const x8 kf = expand<T>(kc[t].w[n], sc[t]);
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                         S[t / 2][t % 2][nb] = Elem<T>::mma16(kf, w.qf[nb][n], S[t / 2][t % 2][nb]);
                 }
-            }
             __builtin_amdgcn_sched_barrier(0);
             fetch_k(c + NW, page);
             const int key0 = c * 64;
-            if (key0 + 64 > all_see) {
+            if (key0 + 64 > all_see || !ok) {
+                int lim2[NB];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) w.mask(S[half], key0 + 32 * half, lim, g);
+                for (int nb = 0; nb < NB; ++nb) lim2[nb] = ok ? lim[nb] : 0;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) w.mask(S[half], key0 + 32 * half, lim2, g);
                 // Values behind the last token are nothing.
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
-                    if (key0 + 16 * t + i >= req.keys) {
+                    if (!ok || key0 + 16 * t + i >= req.keys) {
                         vs = (vs & ~(255u << (8 * t))) | 127u << (8 * t);
 #pragma unroll
                         for (int n = 0; n < DW; ++n) vc[t].w[n] = 0;
@@ -723,7 +734,7 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
         return;
     }
     const int per = a.starts[a.B];
-    const int s = a.starts[b] + (hk * tiles + rt) * chunks;
+    const int s = a.starts[b] + (hk * tiles + rt) * (chunks + a.start_units) + a.start_units;
     const int w0 = (int)((unsigned)s / (unsigned)per);
     const int w1 = (int)((unsigned)(s + chunks - 1) / (unsigned)per);
     if (w0 == w1) return;
@@ -810,7 +821,7 @@ int check_cache(int Hkv, int D, int pages, int page, const void* kc, const void*
 }
 
 // How attn_few_kernel is launched.
-constexpr int kFewRows = 64, kMinUnits = 4;
+constexpr int kFewRows = 64, kMinUnits = 4, kStartUnits = 8;
 // Tables of up to so many tokens go to the DIRECT form.
 constexpr int kDirectTokens = 2048;
 struct FewPlan {
@@ -825,12 +836,12 @@ FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len) {
     p.nb = rows > 16 ? 2 : 1;
     p.tiles = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
     const long long segs = (long long)B * Hkv * p.tiles;
-    p.units = segs * ((std::max(max_len, 1) + 63LL) / 64);
+    p.units = segs * ((std::max(max_len, 1) + 63LL) / 64 + kStartUnits);
     p.direct = max_len <= kDirectTokens && segs < (1LL << 31);
     if (p.direct) return p;
     // As many workgroups as the GPU holds at once, with a unit a wave at least.
     const int most = p.nb == 2 ? 256 : D == 128 ? 768 : 1024;
-    p.groups = (int)std::max(1LL, std::min<long long>(most, (p.units + kMinUnits - 1) / kMinUnits));
+    p.groups = (int)std::max(1LL, std::min<long long>(most, p.units / (kMinUnits + kStartUnits) + 1));
     p.many = p.groups / segs >= 32;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.o_off = up((size_t)(B + 1) * sizeof(int));
@@ -994,7 +1005,8 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     a.qsign = scale < 0.f ? -1.f : 1.f;
     a.few_rows = kFewRows;
     a.groups = plan.groups;
-    a.min_units = kMinUnits;
+    a.min_units = kMinUnits + kStartUnits;
+    a.start_units = kStartUnits;
     a.tiles = plan.tiles;
     a.starts = (int*)workspace;
     a.ws_o = (float*)((char*)workspace + plan.o_off);
