@@ -264,6 +264,12 @@ struct AttnArgs {
     int* starts;  // [B + 1]: first unit of every request; units a workgroup
     float* ws_o;        // [slot][row][D]
     float* ws_ml;       // [slot][row][2]
+    // The same of attn_prompt_kernel, and its plan.
+    int p_groups, p_tiles;  // p_tiles: room for so many tiles
+    int* p_first;         // [B + 1]: first tile of every request
+    long long* p_cost;    // [tiles + 1]: units before a tile, of one kv head
+    float* p_o;
+    float* p_ml;
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -345,14 +351,13 @@ __device__ void attend_row(const AttnArgs& a, const T* q, int hk, int b, int t0,
     }
 }
 
-// Whether a token that query `tok` of its request does not see may hold an infinite or
-// NaN value: a weight of 0 would not keep that out of a sum. For a wave.
+// Whether one of the tokens seen .. end - 1 of request b may hold an infinite or NaN
+// value: a weight of 0 would not keep that out of the sum of a row that does not see it. For a
+// wave.
 template <int D, class T>
-__device__ __forceinline__ bool may_spoil(const AttnArgs& a, const Request& r, int b, int hk,
-                                          int tok) {
-    const int seen = seen_by(a, r, tok);
+__device__ __forceinline__ bool may_spoil(const AttnArgs& a, int b, int hk, int seen, int end) {
     bool bad = false;
-    for (int e = threadIdx.x & 63; e < (r.keys - seen) * (D / 32); e += 64) {
+    for (int e = threadIdx.x & 63; e < (end - seen) * (D / 32); e += 64) {
         const int t = seen + e / (D / 32), page = a.table[b * a.table_stride + t / a.c.page];
         if ((unsigned)page < (unsigned)a.c.pages)
             bad |= a.c.vs[scale_at(a.c, page, hk, t % a.c.page) + e % (D / 32) * 4] >= kScaleLimit<T>;
@@ -698,7 +703,7 @@ attn_few_kernel(const AttnArgs a) {
         if constexpr (DIRECT) {
             for (int r = wave; r < R && rt * R + r < rows; r += NW) {
                 const int tok = (rt * R + r) / a.G, h = hk * a.G + rt * R + r - tok * a.G;
-                if (may_spoil<D, T>(a, req, b, hk, tok))
+                if (may_spoil<D, T>(a, b, hk, seen_by(a, req, tok), req.keys))
                     attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0,
                                      seen_by(a, req, tok), (T*)a.o + (req.first + tok) * a.ot + h * a.oh);
             }
@@ -727,7 +732,7 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
         if (grp == 0) *reinterpret_cast<u32x2*>(o) = u32x2{};
         return;
     }
-    if (may_spoil<D, T>(a, req, b, hk, tok)) {  // (the same for every wave)
+    if (may_spoil<D, T>(a, b, hk, seen_by(a, req, tok), req.keys)) {  // (the same for every wave)
         if (threadIdx.x < 64)
             attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0,
                              seen_by(a, req, tok), o - d);
@@ -789,17 +794,396 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 #endif
 }
 
-// Requests of more than few_rows query rows: one wave per query row and head.
-template <int D, class T>
-__global__ void __launch_bounds__(64) attn_rows_kernel(const AttnArgs a) {
+// -- prompts: requests of more than few_rows query rows a kv head -----------------------
+
+constexpr int kTileRows = 128, kPromptStart = 4;
+
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int row = blockIdx.x, h = blockIdx.y;
-    for (int b = 0; b < a.B; ++b) {
-        const Request r = request(a, b);
-        const int i = row - r.first;
-        if (i < 0 || i >= r.m || (long long)r.m * a.G <= a.few_rows) continue;
-        attend_row<D, T>(a, (const T*)a.q + row * a.qt + h * a.qh, h / a.G, b, 0, seen_by(a, r, i),
-                         (T*)a.o + row * a.ot + h * a.oh);
+// Row tiles of a request, and the 64-key chunks that tile rt reads.
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Request& r) {
+    const long long rows = (long long)r.m * a.G;
+    return rows > a.few_rows ? (int)((rows + kTileRows - 1) / kTileRows) : 0;
+}
+__device__ __forceinline__ int tile_end(const AttnArgs& a, const Request& r, int rt) {
+    const long long last = min((long long)r.m * a.G, (rt + 1LL) * kTileRows) - 1;
+    return seen_by(a, r, (int)(last / a.G));
+}
+__device__ __forceinline__ int tile_chunks(const AttnArgs& a, const Request& r, int rt) {
+    return (tile_end(a, r, rt) + 63) / 64;
+}
+#endif
+
+// Tiles of all requests and their units (chunks, and kPromptStart for the start and the
+// merge of a tile that has any), summed up. One workgroup.
+__global__ void __launch_bounds__(1024) prompt_plan_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ int first[kMaxRequests + 1];
+    __shared__ long long part[1024];
+    const int t = threadIdx.x;
+    auto scan = [&](long long x) {  // inclusive, over the workgroup
+        part[t] = x;
+        __syncthreads();
+        for (int o = 1; o < 1024; o <<= 1) {
+            const long long y = t >= o ? part[t - o] : 0;
+            __syncthreads();
+            part[t] += y;
+            __syncthreads();
+        }
+        return part[t];
+    };
+    const int per = (a.B + 1023) / 1024, b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
+    // (requests whose rows overlap could have more tiles than there is room for)
+    auto cap = [&](long long x) { return (int)min(x, (long long)a.p_tiles); };
+    long long n = 0;
+    for (int b = b0; b < b1; ++b) n += tiles_of(a, request(a, b));
+    n = scan(n) - n;
+    for (int b = b0; b < b1; ++b) {
+        first[b] = a.p_first[b] = cap(n);
+        n += tiles_of(a, request(a, b));
+    }
+    __syncthreads();
+    const int all = cap(part[1023]);
+    if (t == 0) first[a.B] = a.p_first[a.B] = all;
+    __syncthreads();
+
+    const int run = (all + 1023) / 1024, i0 = min(all, t * run), i1 = min(all, i0 + run);
+    int b = 0;
+    for (int hi = a.B - 1; b < hi;) {  // the last request that starts at or before tile i0
+        const int mid = (b + hi + 1) / 2;
+        if (first[mid] <= i0)
+            b = mid;
+        else
+            hi = mid - 1;
+    }
+    for (int pass = 0; pass < 2; ++pass) {
+        long long sum = pass ? part[t] : 0;
+        int x = b;
+        Request r = request(a, x);
+        for (int i = i0; i < i1; ++i) {
+            while (i >= first[x + 1]) r = request(a, ++x);
+            if (pass) a.p_cost[i] = sum;
+            const int c = tile_chunks(a, r, i - first[x]);
+            sum += c ? c + kPromptStart : 0;
+        }
+        if (!pass) {
+            __syncthreads();
+            const long long before = scan(sum) - sum;
+            if (t == 1023) a.p_cost[all] = before + sum;
+            __syncthreads();
+            part[t] = before;
+        }
+    }
+#endif
+}
+
+// Attention of requests with many query rows, bound by the matrix rate.
+//
+// A tile is 128 query rows of a kv head (a token's G heads beside each other), 32 a wave;
+// its keys come in chunks of 64. As in attn_few_kernel the tiles' chunks are laid end to
+// end and every workgroup takes an equal run, since causal tiles differ in length and a
+// chunk of a long context has too few tiles for the GPU; prompt_combine_kernel merges tiles
+// that lie in several runs.
+//
+// A chunk's codes are loaded by all threads (32 values each of K and of V at D = 128),
+// two chunks ahead, expanded to the element type on the way to LDS, and then used as
+// attn_tile_kernel uses its tiles: the second product of one block of 32 keys and the first
+// product of the next but one around the softmax of the block between, one barrier a chunk.
+// K and V have two buffers each: after the barrier of chunk w those of K(w) and V(w-1) are
+// free for K(w+2) and V(w+1).
+template <int D, class T>
+__global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using W = Tile<D, T>;
+    using x8 = typename W::x8;
+    constexpr int RB = W::RB, NU = W::NU, BYTES = 64 * RB, NB32 = D / 32;
+    __shared__ __attribute__((aligned(1024))) char ka[BYTES];
+    __shared__ __attribute__((aligned(1024))) char kb[BYTES];
+    __shared__ __attribute__((aligned(1024))) char va[BYTES];
+    __shared__ __attribute__((aligned(1024))) char vb[BYTES];
+    __shared__ int found;
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+
+    const int ntile = uni(a.p_first[a.B]);
+    const long long all = a.p_cost[ntile] * a.c.Hkv;
+    const long long per = max(4LL + kPromptStart, (all + a.p_groups - 1) / a.p_groups);
+    const int wg = (gridDim.x & 7) == 0 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)
+                                        : blockIdx.x;  // (consecutive runs on one XCD)
+    long long u0 = wg * per;
+    const long long hi = min(all, u0 + per);
+    if (u0 >= hi) return;
+    // The request, kv head and tile of unit u0.
+    for (int x = tid; x < a.B; x += 256)
+        if (a.p_cost[a.p_first[x]] * a.c.Hkv <= u0 && u0 < a.p_cost[a.p_first[x + 1]] * a.c.Hkv)
+            found = x;
+    __syncthreads();
+    int b = uni(found);
+    int t0 = uni(a.p_first[b]), t1 = uni(a.p_first[b + 1]);
+    long long base = a.p_cost[t0], each = a.p_cost[t1] - base;
+    int hk = uni((int)((u0 - base * a.c.Hkv) / each));
+    {
+        const long long at = u0 - base * a.c.Hkv - hk * each;
+        __syncthreads();
+        for (int x = t0 + tid; x < t1; x += 256)
+            if (a.p_cost[x] - base <= at && at < a.p_cost[x + 1] - base) found = x;
+        __syncthreads();
+    }
+    int tile = uni(found);
+
+    // Where this thread's values of a chunk lie: 16 bytes of codes and their scale.
+    const bool d64v = D == 64 && tid >= 128;  // D = 64: half of the threads have K, half V
+    const int part = D == 64 ? tid & 127 : tid;
+    const int crow = part / NB32, cblk = part % NB32;
+    const int coff = crow * (D / 2) + cblk * 16;
+    const int csoff = (crow & 15) * (D / 8) + cblk * 4 + (crow >> 4);
+    int kst[4], vst[4];  // their places in LDS
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        kst[n] = crow * RB + ((cblk * 4 + n) ^ kswz<NU>(crow & 31)) * 16;
+        vst[n] = crow * RB + ((cblk * 4 + n) ^ vswz<NU>(crow & 31)) * 16;
+    }
+
+    while (u0 < hi) {
+        while (u0 >= (base + 0) * a.c.Hkv + hk * each + (a.p_cost[tile + 1] - base)) {
+            if (++tile < t1) continue;  // (tiles without keys have no units)
+            tile = t0;
+            if (++hk < a.c.Hkv) continue;
+            do {
+                ++b;
+                t0 = t1;
+                t1 = uni(a.p_first[b + 1]);
+            } while (t0 == t1 || a.p_cost[t1] == a.p_cost[t0]);
+            base = a.p_cost[t0];
+            each = a.p_cost[t1] - base;
+            hk = 0;
+            tile = t0;
+        }
+        const Request req = request(a, b);
+        const int rt = tile - t0;
+        const int end = uni(tile_end(a, req, rt)), chunks = (end + 63) / 64;
+        const long long s = base * a.c.Hkv + hk * each + (a.p_cost[tile] - base);
+        const int p0 = uni((int)(u0 - s)), p1 = uni((int)min((long long)chunks + kPromptStart, hi - s));
+        u0 = s + p1;
+        const int c0 = max(0, p0 - kPromptStart), c1 = p1 - kPromptStart;
+        if (c1 <= 0) continue;
+        const bool whole = c0 == 0 && c1 == chunks;
+        const long long slot = 2LL * wg + (c0 == 0 ? 1 : 0);
+
+        W w;
+        w.init(lane);
+        int lim[2];
+        const long long rows = (long long)req.m * a.G;
+        const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
+        const long long row0 = (long long)rt * kTileRows + wave * 32;
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+            const long long r = row0 + 16 * nb + i;
+            const int tok = (int)(r / a.G), h = hk * a.G + (int)(r - (long long)tok * a.G);
+            lim[nb] = r < rows ? seen_by(a, req, tok) : 0;
+            const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh + 8 * g;
+#pragma unroll
+            for (int n = 0; n < W::NQ; ++n) {
+                u32x4 x = {};
+                if (r < rows) x = *reinterpret_cast<const u32x4*>(q + 32 * n);
+                w.qf[nb][n] = __builtin_bit_cast(x8, x ^ neg);
+            }
+        }
+        const bool active = row0 < rows;  // (wave-uniform)
+        const int all_see = active ? uni(seen_by(a, req, (int)(row0 / a.G))) : 0;
+
+        const ConstInts table = (ConstInts)(a.table + b * a.table_stride);
+        const int shift = a.c.page == 64 ? 0 : a.c.page == 128 ? 1 : 2;
+        auto page_of = [&](int c) { return table[min(c, c1 - 1) >> shift]; };
+        auto good = [&](int c, int page) { return c < c1 && (unsigned)page < (unsigned)a.c.pages; };
+        auto row_of = [&](int c, int page) {
+            const unsigned p = (unsigned)page < (unsigned)a.c.pages ? page : 0;
+            return ((long long)p * a.c.Hkv + hk) * a.c.page + (min(c, c1 - 1) & ((1 << shift) - 1)) * 64;
+        };
+        // Codes of chunks kc (K) and vc (V), on their way to LDS.
+        u32x4 kw, vw;
+        unsigned ke, ve;
+        auto load = [&](int kc, int kpage, int vc, int vpage) __attribute__((always_inline)) {
+            const long long kr = row_of(kc, kpage), vr = row_of(vc, vpage);
+            if constexpr (D == 128) {
+                kw = *reinterpret_cast<const u32x4*>(a.c.kc + kr * (D / 2) + coff);
+                ke = a.c.ks[kr / 4 * (D / 8) + csoff];
+                vw = *reinterpret_cast<const u32x4*>(a.c.vc + vr * (D / 2) + coff);
+                ve = a.c.vs[vr / 4 * (D / 8) + csoff];
+            } else {
+                const long long r = d64v ? vr : kr;
+                kw = *reinterpret_cast<const u32x4*>((d64v ? a.c.vc : a.c.kc) + r * (D / 2) + coff);
+                ke = (d64v ? a.c.vs : a.c.ks)[r / 4 * (D / 8) + csoff];
+            }
+        };
+        auto put = [&](char* dst, const int (&at)[4], u32x4 x, unsigned e)
+            __attribute__((always_inline)) {
+            const float sc = e8m0(e);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                *reinterpret_cast<GFX906_LDS x8*>((GFX906_LDS char*)dst + at[n]) = expand<T>(x[n], sc);
+        };
+        // V of chunk c is nothing behind the last key that the tile sees.
+        auto clear = [&](u32x4& x, unsigned& e, int c, int page) __attribute__((always_inline)) {
+            if (!good(c, page) || c * 64 + crow >= end) {
+                x = u32x4{};
+                e = 127;
+            }
+        };
+        auto store = [&](char* kd, char* vd, int vc, int vpage) __attribute__((always_inline)) {
+            if constexpr (D == 128) {
+                put(kd, kst, kw, ke);
+                clear(vw, ve, vc, vpage);
+                put(vd, vst, vw, ve);
+            } else if (!d64v) {
+                put(kd, kst, kw, ke);
+            } else {
+                clear(kw, ke, vc, vpage);
+                put(vd, vst, kw, ke);
+            }
+        };
+        auto mask = [&](f32x4 (&S)[2][2], int c, int page, int half) __attribute__((always_inline)) {
+            const int key0 = c * 64 + 32 * half;
+            const bool ok = good(c, page);
+            if (key0 + 32 <= all_see && ok) return;
+            int lim2[2];
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) lim2[nb] = ok ? lim[nb] : 0;
+            w.mask(S, key0, lim2, g);
+        };
+
+        f32x4 Sa[2][2], Sb[2][2];
+        x8 Pa[2], Pb[2];
+        Pb[0] = x8{};
+        Pb[1] = x8{};
+        int g0 = page_of(c0), g1 = page_of(c0 + 1), g2 = page_of(c0 + 2), g3 = page_of(c0 + 3);
+        __syncthreads();  // (the tile before: every wave is done with LDS)
+        load(c0, g0, c0, g0);
+        store(ka, va, c0, g0);
+        load(c0 + 1, g1, c0, g0);
+        if (D == 128 || !d64v) put(kb, kst, kw, ke);
+        load(c0 + 2, g2, c0 + 1, g1);
+        for (int z = tid; z < BYTES / 16; z += 256) *reinterpret_cast<u32x4*>(vb + 16 * z) = u32x4{};
+        __syncthreads();
+        if (active) w.qk(ka, Sa);
+
+        auto step = [&](int c, const char* vp, char* kc, char* vc, const char* kn)
+            __attribute__((always_inline)) {
+            if (active) {
+                mask(Sa, c, g0, 0);
+                w.pv(vp + 32 * RB, Pb);
+                w.qk(kc + 32 * RB, Sb);
+                w.softmax(Sa, Pa, a.scale);
+            }
+            lds_barrier();
+            // V(c+1) goes where V(c-1) was, K(c+2) where K(c) was.
+            store(kc, const_cast<char*>(vp), c + 1, g1);
+            load(c + 3, g3, c + 2, g2);
+            if (active) {
+                mask(Sb, c, g0, 1);
+                w.pv(vc, Pa);
+                w.qk(kn, Sa);
+                w.softmax(Sb, Pb, a.scale);
+            }
+            g0 = g1;
+            g1 = g2;
+            g2 = g3;
+            g3 = page_of(c + 4);
+        };
+        int c = c0;
+        for (; c < c1; c += 2) {
+            step(c, vb, ka, va, kb);
+            step(c + 1, va, kb, vb, ka);
+        }
+        if (active) w.pv(vb + 32 * RB, Pb);
+
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+            const long long r = row0 + 16 * nb + i;
+            const float l = quad_sum(w.lacc[nb][0]);
+            if (r >= rows) continue;
+            const long long at = slot * kTileRows + wave * 32 + 16 * nb + i;
+            if (!whole) {
+#pragma unroll
+                for (int ob = 0; ob < W::NO; ++ob)
+                    *reinterpret_cast<f32x4*>(a.p_o + at * D + 16 * ob + 4 * g) = w.oacc[ob][nb];
+                if (g == 0) *reinterpret_cast<f32x2*>(a.p_ml + at * 2) = f32x2{w.m[nb], l};
+                continue;
+            }
+            const int tok = (int)(r / a.G), h = hk * a.G + (int)(r - (long long)tok * a.G);
+            T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh + 4 * g;
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int ob = 0; ob < W::NO; ++ob) {
+                const f32x4 x = w.oacc[ob][nb] * inv;
+                const auto x0 = Elem<T>::cvt2(x[0], x[1]), x1 = Elem<T>::cvt2(x[2], x[3]);
+                *reinterpret_cast<u32x2*>(o + 16 * ob) =
+                    u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
+            }
+        }
+    }
+#endif
+}
+
+// Merges the runs of a tile, writes the zeros of tiles that see no key, and does rows
+// again that a value they do not see may have spoilt. One workgroup per tile and kv head.
+template <int D, class T>
+__global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ int found;
+    const int tile = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
+    if (tile >= a.p_first[a.B]) return;
+    for (int x = tid; x < a.B; x += 256)
+        if (a.p_first[x] <= tile && tile < a.p_first[x + 1]) found = x;
+    __syncthreads();
+    const int b = found, t0 = a.p_first[b], t1 = a.p_first[b + 1], rt = tile - t0;
+    const Request req = request(a, b);
+    const long long rows = min((long long)kTileRows, (long long)req.m * a.G - (long long)rt * kTileRows);
+    auto tok_of = [&](int r) { return (int)(((long long)rt * kTileRows + r) / a.G); };
+    auto head_of = [&](int r, int tok) {
+        return hk * a.G + (int)((long long)rt * kTileRows + r - (long long)tok * a.G);
+    };
+    const int end = tile_end(a, req, rt), chunks = (end + 63) / 64;
+    int w0 = 0, w1 = 0;
+    if (chunks) {
+        const long long all = a.p_cost[a.p_first[a.B]] * a.c.Hkv;
+        const long long per = max(4LL + kPromptStart, (all + a.p_groups - 1) / a.p_groups);
+        const long long base = a.p_cost[t0], each = a.p_cost[t1] - base;
+        const long long s = base * a.c.Hkv + hk * each + (a.p_cost[tile] - base) + kPromptStart;
+        w0 = (int)(s / per);
+        w1 = (int)((s + chunks - 1) / per);
+    }
+    if (!chunks || w0 != w1) {
+        for (int e = tid; e < rows * (D / 4); e += 256) {
+            const int r = e / (D / 4), d = (e - r * (D / 4)) * 4, tok = tok_of(r);
+            float m = kNoMax, l = 0.f;
+            f32x4 acc = {};
+            for (int y = w0; chunks && y <= w1; ++y) {
+                const long long at = (2LL * y + (y == w0 ? 1 : 0)) * kTileRows + r;
+                const f32x2 ml = *reinterpret_cast<const f32x2*>(a.p_ml + at * 2);
+                const f32x4 p = *reinterpret_cast<const f32x4*>(a.p_o + at * D + d);
+                const float mn = max2(m, ml[0]);
+                const float f = __builtin_amdgcn_exp2f(m - mn), x = __builtin_amdgcn_exp2f(ml[0] - mn);
+                acc = acc * f + p * x;
+                l = l * f + ml[1] * x;
+                m = mn;
+            }
+            acc *= l != 0.f ? 1.f / l : 0.f;
+            T* o = (T*)a.o + (req.first + tok) * a.ot + head_of(r, tok) * a.oh + d;
+            const auto x0 = Elem<T>::cvt2(acc[0], acc[1]), x1 = Elem<T>::cvt2(acc[2], acc[3]);
+            *reinterpret_cast<u32x2*>(o) =
+                u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
+        }
+    }
+    const int see0 = seen_by(a, req, tok_of(0));
+    if (see0 < end && may_spoil<D, T>(a, b, hk, see0, end)) {  // (the same for every wave)
+        __syncthreads();
+        for (int r = tid >> 6; r < rows; r += 4) {
+            const int tok = tok_of(r), see = seen_by(a, req, tok), h = head_of(r, tok);
+            if (may_spoil<D, T>(a, b, hk, see, end))
+                attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0, see,
+                                 (T*)a.o + (req.first + tok) * a.ot + h * a.oh);
+        }
     }
 #endif
 }
@@ -847,6 +1231,27 @@ FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len) {
     p.o_off = up((size_t)(B + 1) * sizeof(int));
     p.ml_off = p.o_off + (size_t)2 * p.groups * 16 * p.nb * D * sizeof(float);
     p.bytes = p.ml_off + (size_t)2 * p.groups * 16 * p.nb * 2 * sizeof(float);
+    return p;
+}
+
+// How attn_prompt_kernel is launched, and its part of the workspace behind the few
+// rows' one. tiles: the most there can be of T queries.
+struct PromptPlan {
+    bool used;
+    int groups, tiles;
+    size_t cost_off, o_off, ml_off, bytes;
+};
+PromptPlan prompt_plan(int T, int B, int G, int D, int max_q, size_t after) {
+    PromptPlan p{};
+    p.used = (long long)max_q * G > kFewRows;
+    if (!p.used) return p;
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    p.groups = 512;  // two a CU
+    p.tiles = (int)std::min<long long>((long long)T * G / kTileRows + B, (1LL << 30));
+    p.cost_off = up(after) + up((size_t)(B + 1) * sizeof(int));
+    p.o_off = p.cost_off + up((size_t)(p.tiles + 1) * sizeof(long long));
+    p.ml_off = p.o_off + (size_t)2 * p.groups * kTileRows * D * sizeof(float);
+    p.bytes = p.ml_off + (size_t)2 * p.groups * kTileRows * 2 * sizeof(float);
     return p;
 }
 
@@ -944,7 +1349,9 @@ extern "C" int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, cons
 extern "C" size_t kv4_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q,
                                            int max_len) {
     if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0 || max_q <= 0) return 0;
-    return few_plan(B, Hq / Hkv, Hkv, D, std::min(max_q, T), max_len).bytes;
+    const size_t few = few_plan(B, Hq / Hkv, Hkv, D, std::min(max_q, T), max_len).bytes;
+    const PromptPlan p = prompt_plan(T, B, Hq / Hkv, D, std::min(max_q, T), few);
+    return p.used ? p.bytes : few;
 }
 
 extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
@@ -978,7 +1385,9 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     if (!(scale > -INFINITY && scale < INFINITY)) return g_err.fail("kv4_attn: scale must be finite");
     const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page);
     if (plan.units >= (1LL << 31) - 1) return g_err.fail("kv4_attn: table too wide for so many heads");
-    if (plan.bytes && (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
+    const PromptPlan pp = prompt_plan(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);
+    const size_t need = pp.used ? pp.bytes : plan.bytes;
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return g_err.fail("kv4_attn: workspace misaligned or smaller than "
                           "kv4_attn_workspace_bytes()");
     AttnArgs a{};
@@ -1011,6 +1420,15 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     a.starts = (int*)workspace;
     a.ws_o = (float*)((char*)workspace + plan.o_off);
     a.ws_ml = (float*)((char*)workspace + plan.ml_off);
+    if (pp.used) {
+        char* ws = (char*)workspace;
+        a.p_groups = pp.groups;
+        a.p_tiles = pp.tiles;
+        a.p_first = (int*)(ws + ((plan.bytes + 255) & ~(size_t)255));
+        a.p_cost = (long long*)(ws + pp.cost_off);
+        a.p_o = (float*)(ws + pp.o_off);
+        a.p_ml = (float*)(ws + pp.ml_off);
+    }
     const long long rows = (long long)a.max_q * a.G;
     const dim3 cgrid((unsigned)(B * Hkv), (unsigned)std::min<long long>(rows, kFewRows));
     if ((long long)B * Hkv >= (1LL << 31)) return g_err.fail("kv4_attn: too many heads");
@@ -1037,8 +1455,12 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
         else
             runs(attn_few_kernel<kD, E, 2, 8, false>, 512, few_combine_kernel<kD, E, 2, 256>,
                  few_combine_kernel<kD, E, 2, 1024>);
-        if (rows > kFewRows)
-            hipLaunchKernelGGL((attn_rows_kernel<kD, E>), dim3(T, Hq), dim3(64), 0, stream, a);
+        if (pp.used) {
+            hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
+            hipLaunchKernelGGL((attn_prompt_kernel<kD, E>), dim3(pp.groups), dim3(256), 0, stream, a);
+            hipLaunchKernelGGL((prompt_combine_kernel<kD, E>), dim3(pp.tiles, Hkv), dim3(256), 0,
+                               stream, a);
+        }
     };
     if (dtype == KV4_DTYPE_F16)
         D == 64 ? go(std::integral_constant<int, 64>{}, f16{})
