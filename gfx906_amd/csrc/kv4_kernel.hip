@@ -1071,9 +1071,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             __attribute__((always_inline)) {
             if (active) {
                 mask(Sa, c, g0, 0);
-                w.pv(vp + 32 * RB, Pb);
-                w.qk(kc + 32 * RB, Sb);
-                w.softmax(Sa, Pa, a.scale);
+                w.turn(vp + 32 * RB, Pb, kc + 32 * RB, Sb, Sa, Pa, a.scale);
             }
             lds_barrier();
             // V(c+1) goes where V(c-1) was, K(c+2) where K(c) was.
@@ -1081,9 +1079,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             load(c + 3, g3, c + 2, g2);
             if (active) {
                 mask(Sb, c, g0, 1);
-                w.pv(vc, Pa);
-                w.qk(kn, Sa);
-                w.softmax(Sb, Pb, a.scale);
+                w.turn(vc, Pa, kn, Sa, Sb, Pb, a.scale);
             }
             g0 = g1;
             g1 = g2;
@@ -1126,19 +1122,23 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
 }
 
 // Merges the runs of a tile, writes the zeros of tiles that see no key, and does rows
-// again that a value they do not see may have spoilt. One workgroup per tile and kv head.
+// again that a value they do not see may have spoilt. One workgroup per 16 rows
+// of a tile and kv head.
 template <int D, class T>
 __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ int found;
-    const int tile = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
+    constexpr int ROWS = 16;
+    const int tile = blockIdx.x / (kTileRows / ROWS), hk = blockIdx.y, tid = threadIdx.x;
+    const int r0 = blockIdx.x % (kTileRows / ROWS) * ROWS;
     if (tile >= a.p_first[a.B]) return;
     for (int x = tid; x < a.B; x += 256)
         if (a.p_first[x] <= tile && tile < a.p_first[x + 1]) found = x;
     __syncthreads();
     const int b = found, t0 = a.p_first[b], t1 = a.p_first[b + 1], rt = tile - t0;
     const Request req = request(a, b);
-    const long long rows = min((long long)kTileRows, (long long)req.m * a.G - (long long)rt * kTileRows);
+    const int rows = (int)min(r0 + (long long)ROWS, (long long)req.m * a.G - (long long)rt * kTileRows);
+    if (r0 >= rows) return;
     auto tok_of = [&](int r) { return (int)(((long long)rt * kTileRows + r) / a.G); };
     auto head_of = [&](int r, int tok) {
         return hk * a.G + (int)((long long)rt * kTileRows + r - (long long)tok * a.G);
@@ -1154,8 +1154,8 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
         w1 = (int)((s + chunks - 1) / per);
     }
     if (!chunks || w0 != w1) {
-        for (int e = tid; e < rows * (D / 4); e += 256) {
-            const int r = e / (D / 4), d = (e - r * (D / 4)) * 4, tok = tok_of(r);
+        for (int e = tid; e < (rows - r0) * (D / 4); e += 256) {
+            const int r = r0 + e / (D / 4), d = e % (D / 4) * 4, tok = tok_of(r);
             float m = kNoMax, l = 0.f;
             f32x4 acc = {};
             for (int y = w0; chunks && y <= w1; ++y) {
@@ -1175,10 +1175,10 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
                 u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
         }
     }
-    const int see0 = seen_by(a, req, tok_of(0));
+    const int see0 = seen_by(a, req, tok_of(r0));
     if (see0 < end && may_spoil<D, T>(a, b, hk, see0, end)) {  // (the same for every wave)
         __syncthreads();
-        for (int r = tid >> 6; r < rows; r += 4) {
+        for (int r = r0 + (tid >> 6); r < rows; r += 4) {
             const int tok = tok_of(r), see = seen_by(a, req, tok), h = head_of(r, tok);
             if (may_spoil<D, T>(a, b, hk, see, end))
                 attend_row<D, T>(a, (const T*)a.q + (req.first + tok) * a.qt + h * a.qh, hk, b, 0, see,
@@ -1247,7 +1247,7 @@ PromptPlan prompt_plan(int T, int B, int G, int D, int max_q, size_t after) {
     if (!p.used) return p;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.groups = 512;  // two a CU
-    p.tiles = (int)std::min<long long>((long long)T * G / kTileRows + B, (1LL << 30));
+    p.tiles = (int)std::min<long long>((long long)T * G / kTileRows + B, (1LL << 27));
     p.cost_off = up(after) + up((size_t)(B + 1) * sizeof(int));
     p.o_off = p.cost_off + up((size_t)(p.tiles + 1) * sizeof(long long));
     p.ml_off = p.o_off + (size_t)2 * p.groups * kTileRows * D * sizeof(float);
@@ -1458,7 +1458,8 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
         if (pp.used) {
             hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
             hipLaunchKernelGGL((attn_prompt_kernel<kD, E>), dim3(pp.groups), dim3(256), 0, stream, a);
-            hipLaunchKernelGGL((prompt_combine_kernel<kD, E>), dim3(pp.tiles, Hkv), dim3(256), 0,
+            hipLaunchKernelGGL((prompt_combine_kernel<kD, E>), dim3(pp.tiles * (kTileRows / 16), Hkv),
+                               dim3(256), 0,
                                stream, a);
         }
     };

@@ -213,13 +213,72 @@ struct Tile {
     }
 
     __device__ __forceinline__ void softmax(const f32x4 (&S)[2][NB], x8 (&P)[NB], float c) {
-        bool exact = far;
-        if (__builtin_expect(!far, 1)) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) weights<false>(S, P, c, nb);
-            exact = p_above<T, NB>(P);
+        for (int nb = 0; nb < NB; ++nb) weights<false>(S, P, c, nb);
+        settle(S, P, c);
+    }
+
+    // One step of the pipeline: the second product of one block (vt, Pp), the first of
+    // another (kt, Sn), and P of the block S between them, in the order written: behind every
+    // fragment's products the read of the fragment AV (V) or AK (K) further on, and a share
+    // of the softmax, so that a wave's own instructions fill the matrix pipe's time. (The
+    // compiler's order has all products before all exponentials: 16 heads of 16384 tokens,
+    // 32 blocks of 64, 300 us and 284 this way; a 4-bit cache's prompts 218 and 201.)
+    __device__ __forceinline__ void turn(const char* vt, const x8 (&Pp)[NB], const char* kt,
+                                         f32x4 (&Sn)[2][NB], const f32x4 (&S)[2][NB], x8 (&P)[NB],
+                                         float c) {
+        constexpr int AV = D == 128 ? 4 : 3, AK = 2, NK = 2 * NQ, EPS = 8 * NB / (NO + NK);
+        x8 vf[NO], kf[NK];
+        float p[8 * NB];
+        auto vread = [&](int n) __attribute__((always_inline)) {
+            vf[n] = lds_read_tr2<T>(vt, vaddr[n], vaddr[n] + 16 * RB);
+        };
+        auto kread = [&](int n) __attribute__((always_inline)) {
+            kf[n] = lds_read16<T>(kt, kaddr[n / 2] + 16 * (n % 2) * RB);
+        };
+        auto share = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+            for (int q = slot * EPS; q < (slot + 1) * EPS; ++q) {
+                const int nb = q / 8, e = q % 8;
+                p[q] = __builtin_amdgcn_exp2f(fmaf(S[e / 4][nb][e & 3], c, -m[nb]));
+                if (e & 1) {
+                    const typename E::x2 h = E::cvt2(p[q - 1], p[q]);
+                    P[nb][e - 1] = h[0];
+                    P[nb][e] = h[1];
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int n = 0; n < AV; ++n) vread(n);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < NO; ++n) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) oacc[n][nb] = E::mma16(vf[n], Pp[nb], oacc[n][nb]);
+            if (n + AV < NO) vread(n + AV);
+            if (n >= NO - AK) kread(n - (NO - AK));
+            share(n);
         }
-        if (__builtin_expect(exact, 0)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) Sn[kb][nb] = f32x4{};
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                Sn[n % 2][nb] = E::mma16(kf[n], qf[nb][n / 2], Sn[n % 2][nb]);
+            if (n + AK < NK) kread(n + AK);
+            share(NO + n);
+        }
+        settle(S, P, c);
+    }
+
+    // Where some p passed the limit: the exact maximum of the block, and O, l and P after
+    // it. Then the row sums.
+    __device__ __forceinline__ void settle(const f32x4 (&S)[2][NB], x8 (&P)[NB], float c) {
+        if (__builtin_expect(p_above<T, NB>(P) || far, 0)) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const float a = max3(S[0][nb][0], S[0][nb][1], S[0][nb][2]);

@@ -29,12 +29,13 @@ std::array<long long, 3> strides3(const Tensor& t) {
 }
 
 // Read in place where the head dim is contiguous, the other strides are multiples of
-// 8 and the data 16-byte aligned; copied otherwise.
+// 8, rows lie apart and the data is 16-byte aligned; copied otherwise.
 Tensor rows_of(const Tensor& t) {
     bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     const auto s = strides3(t);
     for (int d = 0; d < 3; ++d) ok = ok && s[d] >= 0 && s[d] % 8 == 0;
-    return ok && s[2] <= (1 << 22) ? t : t.clone(at::MemoryFormat::Contiguous);
+    ok = ok && s[2] <= (1 << 22) && (t.size(2) == 1 || s[2] >= t.size(3));
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }

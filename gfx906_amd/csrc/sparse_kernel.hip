@@ -10,6 +10,7 @@
 #include "longctx_tile.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gfx906_amd_sparse.h"
 
@@ -158,9 +159,10 @@ __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
 // key blocks). Scores become 64-bit integers of the same order (0: not to be taken;
 // all ones: always), and the count-th largest is found bit by bit from the top, until
 // exactly `count` lie at or above the bits so far, or their last bit is set: then
-// scores equal to it fill up in the order of their index. Everything stays in
-// registers; a step is a compare and a population count per 64 scores (and, with
-// several waves, an exchange through LDS).
+// scores equal to it fill up in the order of their index. The upper 32 bits go first, by
+// themselves; the lower ones matter only among scores whose upper bits are the bound's.
+// Everything stays in registers; a step is a compare and a population count per 64 scores
+// (and, with several waves, an exchange through LDS).
 template <int WAVES, int K>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -174,16 +176,18 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(c
     const double* score = a.score + row * a.nk;
     int* out = a.index + row * a.count;
     const int base = wave * 64 * K + lane;
-    u64 key[K];
+    unsigned hi[K], lo[K];
 #pragma unroll
     for (int n = 0; n < K; ++n) {
         const int j = base + 64 * n;
-        key[n] = 0;
+        u64 key = 0;
         if (j < r.seen) {
             const double s = score[j] + 0.0;  // -0 becomes +0
             const u64 bits = (u64)__double_as_longlong(s != s ? INFINITY : s);
-            key[n] = j >= r.own ? ~0ull : bits >> 63 ? ~bits : bits | 1ull << 63;
+            key = j >= r.own ? ~0ull : bits >> 63 ? ~bits : bits | 1ull << 63;
         }
+        hi[n] = (unsigned)(key >> 32);
+        lo[n] = (unsigned)key;
     }
     int turn = 0;
     auto popc = [](u64 x) { return (int)__popcll(x); };  // (unsigned, else)
@@ -206,45 +210,64 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(c
         if (before) *before = pre;
         return sum;
     };
-    auto at_least = [&](u64 x) {
+    // (every key that may be taken is at least 2^51: its upper half is not 0)
+    auto upper = [&](unsigned x) {
         int n = 0;
 #pragma unroll
-        for (int m = 0; m < K; ++m) n += popc(__ballot(key[m] >= x));
+        for (int m = 0; m < K; ++m) n += popc(__ballot(hi[m] >= x));
         return total(n, nullptr);
     };
-    // All scores above `bar`, and `ties` of those equal to it.
-    u64 bar = 0;
+    unsigned bar_hi = 0, bar_lo = 0;  // the bound: all above it, and `ties` of those equal to it
+    auto lower = [&](unsigned x) {
+        int n = 0;
+#pragma unroll
+        for (int m = 0; m < K; ++m) n += popc(__ballot(hi[m] == bar_hi && lo[m] >= x));
+        return total(n, nullptr);
+    };
     int ties = 0;
-    if (at_least(1) > a.count) {
-        u64 top = 0;
+    if (upper(1) > a.count) {
         bool done = false;
-        for (int bit = 63; bit >= 0 && !done; --bit) {
-            const u64 x = top | 1ull << bit;
-            const int n = at_least(x);
-            if (n >= a.count) top = x;
+        for (int bit = 31; bit >= 0 && !done; --bit) {
+            const unsigned x = bar_hi | 1u << bit;
+            const int n = upper(x);
+            if (n >= a.count) bar_hi = x;
             done = n == a.count;
         }
-        bar = done ? top - 1 : top;
-        if (!done) ties = a.count - (top == ~0ull ? 0 : at_least(top + 1));
+        if (done) {  // all whose upper half is at least bar_hi
+            bar_hi -= 1;
+            bar_lo = ~0u;
+        } else {
+            const int need = a.count - (bar_hi == ~0u ? 0 : upper(bar_hi + 1));
+            for (int bit = 31; bit >= 0 && !done; --bit) {
+                const unsigned x = bar_lo | 1u << bit;
+                const int n = lower(x);
+                if (n >= need) bar_lo = x;
+                done = n == need;
+            }
+            if (done)
+                bar_lo -= 1;
+            else
+                ties = need - (bar_lo == ~0u ? 0 : lower(bar_lo + 1));
+        }
     }
+    auto over = [&](int n) { return hi[n] > bar_hi || (hi[n] == bar_hi && lo[n] > bar_lo); };
+    auto even = [&](int n) { return ties > 0 && hi[n] == bar_hi && lo[n] == bar_lo; };
     int above = 0, equal = 0;
 #pragma unroll
     for (int n = 0; n < K; ++n) {
-        above += popc(__ballot(key[n] > bar));
-        equal += popc(__ballot(bar && key[n] == bar));
+        above += popc(__ballot(over(n)));
+        equal += popc(__ballot(even(n)));
     }
     int ties_before;
     total(equal, &ties_before);
-    const int mine = above + min(equal, max(0, ties - ties_before));
-    int at;
-    const int all = total(mine, &at);
-    const u64 below = (1ull << lane) - 1;
     int ties_left = max(0, ties - ties_before);
+    int at;
+    const int all = total(above + min(equal, ties_left), &at);
+    const u64 below = (1ull << lane) - 1;
 #pragma unroll
     for (int n = 0; n < K; ++n) {
-        const u64 eq = __ballot(bar && key[n] == bar);
-        const bool take = key[n] > bar ||
-                          (bar && key[n] == bar && popc(eq & below) < ties_left);
+        const u64 eq = __ballot(even(n));
+        const bool take = over(n) || (even(n) && popc(eq & below) < ties_left);
         const u64 mk = __ballot(take);
         if (take) out[at + popc(mk & below)] = base + 64 * n;
         at += popc(mk);
@@ -291,19 +314,19 @@ __device__ __forceinline__ void store_pair(const AttnArgs& a, T* orow, long long
     }
 }
 
-// One row over the blocks list[e0..e1), by one wave: 64 keys at a time, a score per
+// One row over the blocks whose first keys are list[e0..e1), by one wave: 64 keys at a time, a score per
 // lane, then a pair of dims per lane. Keys the row does not see are not touched at
 // all, so that what they hold cannot reach it.
 template <int D, class T>
 __device__ __attribute__((noinline)) void attend_row(const AttnArgs& a, const T* q, const T* k,
                                                      const T* v, T* orow, long long wrow,
-                                                     const uint16_t* list, int e0, int e1,
+                                                     const int* list, int e0, int e1,
                                                      int seen) {
     const int lane = threadIdx.x & 63;
     float m = kNoMax, l = 0.f, o0 = 0.f, o1 = 0.f;
     for (int e = e0; e < e1; ++e)
         for (int u = 0; u < a.block; u += 64) {
-            const int j0 = list[e] * a.block + u, j = j0 + lane;
+            const int j0 = list[e] + u, j = j0 + lane;
             float s = -INFINITY;
             if (j < seen) {
                 s = 0.f;
@@ -338,19 +361,24 @@ __device__ __forceinline__ int xcd_order(int w, int n) {
 
 // Attention of one query block (128 rows, 32 a wave) over its listed key blocks.
 //
-// The list is read first and its valid entries gathered in LDS. Then the waves walk
-// the listed keys in tiles of 32, software-pipelined as attn_fwd_pipe: the step of
-// tile j issues the PV products of tile j-1 and the QK products of tile j+1 around
-// the softmax of tile j. K and V tiles come by loads to LDS into rings of four, K
-// three and V two steps ahead, whose waits are counted: one barrier a step. Tiles of
-// 32 (16 KB of K and V at D = 128) instead of attn_fwd_pipe's 64 let two
-// workgroups of four waves share a CU's LDS, for lists of 128 rows instead of 256.
+// The list is read first and the first keys of its valid entries gathered in LDS. Then the
+// waves walk the listed keys in tiles of 32, software-pipelined as attn_fwd_pipe: the step
+// of tile j issues the PV products of tile j-1 and the QK products of tile j+1 around
+// the softmax of tile j. K and V tiles come by loads to LDS into rings of four, K three
+// and V two steps ahead, whose waits are counted: one barrier a step. Tiles of 32 (16 KB of
+// K and V at D = 128) instead of attn_fwd_pipe's 64 let two workgroups of four waves share
+// a CU's LDS, for lists of 128 rows instead of 256.
 //
-// Tiles past the list load zeros (empty range) and are masked, so that loads and
-// waits stay static. A tile with masked keys is checked for infinite and NaN values
-// of V (which a weight of 0 would not keep out of the sums); where there are any
-// the wave does its rows again by attend_row.
-template <int D, class T>
+// Steps go four to a round, a whole number of blocks, so that which entry of the list a
+// tile belongs to is known when the kernel is compiled; entries are read a round ahead.
+// Tiles past the list load zeros (their offset is past the descriptor's range) and are
+// masked, so that loads and waits stay static. One descriptor serves a head's K (or V) of
+// less than 2^31 bytes; with FAR it is made anew for every tile.
+//
+// A tile with masked keys is checked for infinite and NaN values of V (which a weight of 0
+// would not keep out of the sums); where there are any the wave does its rows again by
+// attend_row.
+template <int D, class T, int TPB, bool FAR>
 __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using W = Tile<D, T>;
@@ -358,6 +386,8 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
     constexpr int NU = W::NU, RB = W::RB, BYTES = W::BYTES;
     constexpr int LPT = BYTES / 1024 / 4;  // loads a wave and tile
     constexpr int kWait = 0x0F70 | ((4 * LPT) & 15) | (((4 * LPT) >> 4) << 14);
+    constexpr int EPR = 4 / TPB;           // entries a round
+    constexpr int kNoKey = 0x7fffff00;     // the key of tiles past the list
     __shared__ __attribute__((aligned(1024))) char k0[BYTES];
     __shared__ __attribute__((aligned(1024))) char k1[BYTES];
     __shared__ __attribute__((aligned(1024))) char k2[BYTES];
@@ -366,7 +396,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
     __shared__ __attribute__((aligned(1024))) char v1[BYTES];
     __shared__ __attribute__((aligned(1024))) char v2[BYTES];
     __shared__ __attribute__((aligned(1024))) char v3[BYTES];
-    __shared__ uint16_t list[SPARSE_MAX_COUNT];
+    __shared__ int list[SPARSE_MAX_COUNT];
     __shared__ int n_list;
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -427,7 +457,7 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
             before = max(last, lane ? before : -1);
             const bool take = in && x > before && x < reach;
             const unsigned long long mk = __ballot(take);
-            if (take) list[n + (int)__popcll(mk & ((1ull << lane) - 1))] = (uint16_t)x;
+            if (take) list[n + (int)__popcll(mk & ((1ull << lane) - 1))] = x * (TPB * 32);
             n += (int)__popcll(mk);
             last = max(last, __shfl(top, 63));
         }
@@ -435,37 +465,61 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
     }
     for (int z = tid; z < BYTES / 16; z += 256) *reinterpret_cast<u32x4*>(v3 + 16 * z) = u32x4{};
     __syncthreads();
-    const int n_all = __builtin_amdgcn_readfirstlane(n_list);
+    const int n_all = uni(n_list);
     // (at most 2048 entries and 512 ranges)
     const int e0 = uni(n_all * range / a.nsplit), e1 = uni(n_all * (range + 1) / a.nsplit);
-    const int bshift = a.block == 64 ? 1 : 2;  // log2 of the tiles in a block
-    const int ntiles = (e1 - e0) << bshift;
+    const int ntiles = (e1 - e0) * TPB;
 
-    // First key of tile t (past the list: past every key).
-    auto key_of = [&](int t) __attribute__((always_inline)) {
-        const int e = min(e0 + (t >> bshift), SPARSE_MAX_COUNT - 1);
-        const int k = (int)list[e] * a.block + (t & ((1 << bshift) - 1)) * 32;
-        return __builtin_amdgcn_readfirstlane(t < ntiles ? k : 0x7fffff00);
-    };
-    int koff[LPT], voff[LPT];
+    const unsigned kss = (unsigned)(a.sk.s * 2), vss = (unsigned)(a.sv.s * 2);
+    unsigned koff[LPT], voff[LPT];
 #pragma unroll
     for (int n = 0; n < LPT; ++n) {
         const int u = (wave + 4 * n) * 64 + lane, r = u / NU, s = u % NU;
-        koff[n] = (int)(r * a.sk.s + (s ^ kswz<NU>(r)) * 8) * 2;
-        voff[n] = (int)(r * a.sv.s + (s ^ vswz<NU>(r)) * 8) * 2;
+        koff[n] = r * kss + (s ^ kswz<NU>(r)) * 16;
+        voff[n] = r * vss + (s ^ vswz<NU>(r)) * 16;
     }
-    auto issue = [&](const T* X, long long ss, int key, char* dst, const int (&off)[LPT])
-        __attribute__((always_inline)) {
-        const int rows = min(a.Skv - key, 32);
-        const int bytes =
-            __builtin_amdgcn_readfirstlane(rows > 0 ? (int)(((rows - 1) * ss + D) * 2) : 0);
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(X + (rows > 0 ? key : 0) * ss), 0, bytes, 0x00020000);
+    auto span = [&](int rows, unsigned ss) {  // bytes of the first rows
+        return rows > 0 ? (int)((rows - 1) * ss + 2 * D) : 0;
+    };
+    const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)K, 0, FAR ? 0 : uni(span(a.Skv, kss)), 0x00020000);
+    const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)V, 0, FAR ? 0 : uni(span(a.Skv, vss)), 0x00020000);
+    // First key of a list entry, and the offsets of its rows in K and V.
+    struct Entry {
+        int key;
+        unsigned k, v;
+    };
+    auto entry = [&](int e, int key) __attribute__((always_inline)) {
+        Entry x;
+        x.key = e < e1 ? uni(key) : kNoKey;
+        x.k = e < e1 ? x.key * kss : kOutOfRange;
+        x.v = e < e1 ? x.key * vss : kOutOfRange;
+        return x;
+    };
+    auto listed = [&](int e) { return list[min(e, SPARSE_MAX_COUNT - 1)]; };
+    // Loads a tile of K or V: tile `sub` of entry x.
+    auto issue = [&](auto is_v, const Entry& x, int sub, char* dst) __attribute__((always_inline)) {
+        constexpr bool kV = decltype(is_v)::value;
+        const unsigned ss = kV ? vss : kss;
+        __amdgpu_buffer_rsrc_t r = kV ? vrs : krs;
+        unsigned at = (kV ? x.v : x.k) + 32 * sub * ss;
+        if constexpr (FAR) {
+            const int key = x.key + 32 * sub;
+            const int rows = min(a.Skv - key, 32);
+            r = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)((kV ? V : K) + (rows > 0 ? key : 0) * (kV ? a.sv.s : a.sk.s)), 0,
+                uni(span(rows, ss)), 0x00020000);
+            at = 0;
+        }
 #pragma unroll
         for (int n = 0; n < LPT; ++n)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (GFX906_LDS void*)(dst + (wave + 4 * n) * 1024), 16, off[n], 0, 0, 0);
+                r, (GFX906_LDS void*)(dst + (wave + 4 * n) * 1024), 16, (kV ? voff : koff)[n] + at, 0,
+                0, 0);
     };
+    using IsK = std::false_type;
+    using IsV = std::true_type;
 
     bool redo = false;
     if (ntiles > 0) {
@@ -473,51 +527,61 @@ __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
         x8 Pa[2], Pb[2];
         Pb[0] = x8{};
         Pb[1] = x8{};
-        // Keys of tiles j .. j+4 and of V's tiles; shifted every step.
-        int q0 = key_of(0), q1 = key_of(1), q2 = key_of(2), q3 = key_of(3), q4 = key_of(4);
+        // Entries of tiles j .. j+8, j the round's first tile.
+        constexpr int NE = 8 / TPB + 1;
+        Entry q[NE];
+#pragma unroll
+        for (int n = 0; n < NE; ++n) q[n] = entry(e0 + n, listed(e0 + n));
+        int ahead[EPR], enext = e0 + NE;  // entries of the next round, read and not yet taken
+#pragma unroll
+        for (int n = 0; n < EPR; ++n) ahead[n] = listed(enext + n);
         bool hidden = false;  // tile j-1 had masked keys
-        issue(K, a.sk.s, q0, k0, koff);
-        issue(K, a.sk.s, q1, k1, koff);
-        issue(K, a.sk.s, q2, k2, koff);
-        issue(V, a.sv.s, q0, v0, voff);
-        issue(K, a.sk.s, q3, k3, koff);
-        issue(V, a.sv.s, q1, v1, voff);
+        issue(IsK{}, q[0], 0, k0);
+        issue(IsK{}, q[1 / TPB], 1 % TPB, k1);
+        issue(IsK{}, q[2 / TPB], 2 % TPB, k2);
+        issue(IsV{}, q[0], 0, v0);
+        issue(IsK{}, q[3 / TPB], 3 % TPB, k3);
+        issue(IsV{}, q[1 / TPB], 1 % TPB, v1);
         __builtin_amdgcn_s_waitcnt(kWait);
         lds_barrier();
         if (active) w.qk(k0, Sa);
         lds_barrier();
-        issue(K, a.sk.s, q4, k0, koff);
-        issue(V, a.sv.s, q2, v2, voff);
+        issue(IsK{}, q[4 / TPB], 4 % TPB, k0);
+        issue(IsV{}, q[2 / TPB], 2 % TPB, v2);
 
-        // Tile j: V of tile j-1 in vp, K of tile j+1 in kn; tile j+5 of K and j+3 of V
-        // go where those were.
-        auto step = [&](int j, const char* vp, const char* kn, char* kfree, char* vfree,
+        // Tile n of the round: V of the tile before in vp, K of the next in kn; K of the
+        // fifth and V of the third after it go where those were.
+        auto step = [&](auto nth, const char* vp, const char* kn, char* kfree, char* vfree,
                         f32x4 (&S)[2][2], f32x4 (&Sn)[2][2], const x8 (&Pp)[2], x8 (&P)[2])
             __attribute__((always_inline)) {
-            const int q5 = key_of(j + 5);
+            constexpr int n = decltype(nth)::value;
             if (active) {
                 if (__builtin_expect(hidden, 0)) redo |= not_finite<D, T>(vp, lane);
-                hidden = q0 + 32 > all_see;
-                if (hidden) w.mask(S, q0, lim, g);
-                w.pv(vp, Pp);
-                w.qk(kn, Sn);
-                w.softmax(S, P, a.c);
+                const int key = q[n / TPB].key + 32 * (n % TPB);
+                hidden = key + 32 > all_see;
+                if (__builtin_expect(hidden, 0)) w.mask(S, key, lim, g);
+                w.turn(vp, Pp, kn, Sn, S, P, a.c);
             }
             __builtin_amdgcn_s_waitcnt(kWait);
             lds_barrier();
-            issue(K, a.sk.s, q5, kfree, koff);
-            issue(V, a.sv.s, q3, vfree, voff);
-            q0 = q1;
-            q1 = q2;
-            q2 = q3;
-            q3 = q4;
-            q4 = q5;
+            issue(IsK{}, q[(n + 5) / TPB], (n + 5) % TPB, kfree);
+            issue(IsV{}, q[(n + 3) / TPB], (n + 3) % TPB, vfree);
         };
+        using N0 = std::integral_constant<int, 0>;
+        using N1 = std::integral_constant<int, 1>;
+        using N2 = std::integral_constant<int, 2>;
+        using N3 = std::integral_constant<int, 3>;
         for (int j = 0; j < ntiles; j += 4) {
-            step(j + 0, v3, k1, k1, v3, Sa, Sb, Pb, Pa);
-            step(j + 1, v0, k2, k2, v0, Sb, Sa, Pa, Pb);
-            step(j + 2, v1, k3, k3, v1, Sa, Sb, Pb, Pa);
-            step(j + 3, v2, k0, k0, v2, Sb, Sa, Pa, Pb);
+            step(N0{}, v3, k1, k1, v3, Sa, Sb, Pb, Pa);
+            step(N1{}, v0, k2, k2, v0, Sb, Sa, Pa, Pb);
+            step(N2{}, v1, k3, k3, v1, Sa, Sb, Pb, Pa);
+            step(N3{}, v2, k0, k0, v2, Sb, Sa, Pa, Pb);
+#pragma unroll
+            for (int n = 0; n < NE; ++n)
+                q[n] = n + EPR < NE ? q[n + EPR] : entry(enext + n + EPR - NE, ahead[n + EPR - NE]);
+            enext += EPR;
+#pragma unroll
+            for (int n = 0; n < EPR; ++n) ahead[n] = listed(enext + n);
         }
         if (active) {
             if (hidden) redo |= not_finite<D, T>(v3, lane);
@@ -572,15 +636,28 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a) {
     const long long row = id / dq;
     const int d = (int)(id - row * dq) * 4;
     if (row >= a.rows) return;
-    float mx = kNoMax;
-    for (int s = 0; s < a.nsplit; ++s) mx = max2(mx, a.ws_ml[2 * (s * a.rows + row)]);
+    // (eight ranges' loads at a time: one after another they took 6 us for 8 ranges)
+    constexpr int U = 8;
+    float m = kNoMax, l = 0.f;
     f32x4 acc = {};
-    float l = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const long long r = s * a.rows + row;
-        const float w = __builtin_amdgcn_exp2f(a.ws_ml[2 * r] - mx);
-        acc += w * *reinterpret_cast<const f32x4*>(a.ws_o + r * a.D + d);
-        l += w * a.ws_ml[2 * r + 1];
+    for (int s = 0; s < a.nsplit; s += U) {
+        f32x2 ml[U];
+        f32x4 p[U];
+#pragma unroll
+        for (int n = 0; n < U; ++n) {
+            const long long r = min(s + n, a.nsplit - 1) * a.rows + row;
+            ml[n] = *reinterpret_cast<const f32x2*>(a.ws_ml + 2 * r);
+            p[n] = *reinterpret_cast<const f32x4*>(a.ws_o + r * a.D + d);
+        }
+#pragma unroll
+        for (int n = 0; n < U; ++n) {
+            if (s + n >= a.nsplit) continue;
+            const float mn = max2(m, ml[n][0]);
+            const float f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(ml[n][0] - mn);
+            acc = acc * f + p[n] * e;
+            l = l * f + ml[n][1] * e;
+            m = mn;
+        }
     }
     acc *= l != 0.f ? 1.f / l : 0.f;
     const int bh = (int)(row / a.Sq), r = (int)(row - (long long)bh * a.Sq), b = bh / a.Hq;
@@ -695,6 +772,8 @@ extern "C" int sparse_select(const float* q_means, const float* k_means, int B, 
     const dim3 quads((unsigned)((a.rows + 3) / 4)), singles((unsigned)a.rows);
     if (a.nk <= 256)
         hipLaunchKernelGGL((select_kernel<1, 4>), quads, dim3(256), 0, stream, a);
+    else if (a.nk <= 512)
+        hipLaunchKernelGGL((select_kernel<1, 8>), quads, dim3(256), 0, stream, a);
     else if (a.nk <= 1024)
         hipLaunchKernelGGL((select_kernel<1, 16>), quads, dim3(256), 0, stream, a);
     else if (a.nk <= 16384)
@@ -742,6 +821,8 @@ extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
         return 1;
     if (k_strides[2] > (1 << 22) || v_strides[2] > (1 << 22))
         return g_err.fail("sparse_attn: k/v sequence stride above 2^22 elements");
+    if (Skv > 1 && (k_strides[2] < D || v_strides[2] < D))
+        return g_err.fail("sparse_attn: k/v rows overlap");
     const long long oe[3] = {B, Hq, Sq};
     if (!rows_apart(o_strides, oe, 3, D)) return g_err.fail("sparse_attn: o's rows overlap");
     const size_t need = sparse_attn_workspace_bytes(B, Hq, Sq, Skv, D, block, count);
@@ -766,12 +847,23 @@ extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
             hipLaunchKernelGGL(combine, dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256),
                                0, stream, a);
     };
-    if (dtype == SPARSE_DTYPE_F16) {
-        if (D == 64) go(attn_tile_kernel<64, f16>, combine_kernel<f16>);
-        else go(attn_tile_kernel<128, f16>, combine_kernel<f16>);
-    } else {
-        if (D == 64) go(attn_tile_kernel<64, bf16>, combine_kernel<bf16>);
-        else go(attn_tile_kernel<128, bf16>, combine_kernel<bf16>);
-    }
+    // Whether a head's K or V takes 2^31 bytes or more.
+    const bool far = std::max(a.sk.s, a.sv.s) * 2 * Skv >= (1LL << 31);
+    auto pick = [&](auto d, auto t) {
+        constexpr int kD = decltype(d)::value;
+        using E = decltype(t);
+        if (block == 64)
+            far ? go(attn_tile_kernel<kD, E, 2, true>, combine_kernel<E>)
+                : go(attn_tile_kernel<kD, E, 2, false>, combine_kernel<E>);
+        else
+            far ? go(attn_tile_kernel<kD, E, 4, true>, combine_kernel<E>)
+                : go(attn_tile_kernel<kD, E, 4, false>, combine_kernel<E>);
+    };
+    if (dtype == SPARSE_DTYPE_F16)
+        D == 64 ? pick(std::integral_constant<int, 64>{}, f16{})
+                : pick(std::integral_constant<int, 128>{}, f16{});
+    else
+        D == 64 ? pick(std::integral_constant<int, 64>{}, bf16{})
+                : pick(std::integral_constant<int, 128>{}, bf16{});
     return g_err.launched("sparse_attn", hipGetLastError());
 }

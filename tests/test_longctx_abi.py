@@ -128,7 +128,7 @@ def sparse_attn(lib, **kw):
     (dict(index=None), b"null"), (dict(k=None), b"null"), (dict(q=FAKE + 8), b"aligned"),
     (dict(ks=strides(1 << 20, 1 << 16, 100)), b"multiples of 8"),
     (dict(ks=strides(0, 0, 1 << 23)), b"2^22"), (dict(os=strides(0, 1 << 16, 128)), b"overlap"),
-    (dict(B=300, Hq=300), b"65535")])
+    (dict(vs=strides(1 << 20, 1 << 16, 64)), b"rows overlap"), (dict(B=300, Hq=300), b"65535")])
 def test_sparse_attention_refuses(lib, bad, word):
     assert sparse_attn(lib, **bad) == 1 and word in lib.sparse_last_error()
 
