@@ -40,6 +40,24 @@ __device__ __forceinline__ long long scale_at(const Cache& c, long long page, in
     const long long tok16 = (page * c.Hkv + h) * (c.page / 64) * 16 + (t >> 6) * 16 + (t & 15);
     return tok16 * (c.D / 32) * 4 + ((t >> 4) & 3);
 }
+// Eight codes in the element type (rounded to it where it does not hold them).
+template <class T>
+__device__ __forceinline__ typename Elem<T>::x8 expand(unsigned w, float s) {
+    typename Elem<T>::x2 p[4];
+    if constexpr (__is_same(T, f16)) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
+    }
+    auto u = [](typename Elem<T>::x2 x) { return __builtin_bit_cast(unsigned, x); };
+    return __builtin_bit_cast(typename Elem<T>::x8, u32x4{u(p[0]), u(p[1]), u(p[2]), u(p[3])});
+}
 #endif
 
 // -- pages and slots ------------------------------------------------------------------
@@ -55,58 +73,73 @@ struct PlanArgs {
     int W, n_free, B, page, n_slots;
 };
 
-// Every workgroup adds up all requests (each of the 256 threads a run of them,
-// then a scan over the threads) and serves its share of the slots and of the
-// requests' table rows. Entries that are read (held pages) and written (new
-// ones) are different, so workgroups need no order.
+// Every workgroup adds up all requests (each of the 256 threads a run of them, then a
+// scan over the threads) and serves its share of the slots and of the requests' table
+// rows. Entries that are read (held pages) and written (new ones) are different, so
+// workgroups need no order. Bound by latency: lengths are read once and kept in LDS, where
+// a slot finds its request by bisection; sums are 64-bit and kept saturated to 31 bits, as
+// no slot or page past that is used. 64 requests, one token each: PLANUS us.
 __global__ void __launch_bounds__(256) plan_pages_kernel(const PlanArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ long long tok0[kMaxRequests + 1];  // first slot of a request
-    __shared__ long long pg0[kMaxRequests + 1];   // pages taken before a request
-    __shared__ long long part[2][256];
-    const int t = threadIdx.x, B = a.B, P = a.page;
+    __shared__ int len[kMaxRequests];       // cached tokens
+    __shared__ int tok0[kMaxRequests + 1];  // first slot of a request
+    __shared__ int pg0[kMaxRequests + 1];   // pages taken before a request
+    __shared__ long long part[2][4];
+    constexpr long long kCap = 0x7fffffff;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, B = a.B, P = a.page;
+    const int sh = P == 64 ? 6 : P == 128 ? 7 : 8;
+    auto pages = [&](long long n) { return (n + P - 1) >> sh; };
+    auto cap = [&](long long x) { return (int)min(x, kCap); };
     const int per = (B + 255) / 256, b0 = min(B, t * per), b1 = min(B, b0 + per);
-    auto held = [&](int b) { return ((long long)max(0, a.lens[b]) + P - 1) / P; };
-    auto total = [&](int b) {
-        return ((long long)max(0, a.lens[b]) + max(0, a.new_lens[b]) + P - 1) / P;
-    };
     long long n = 0, p = 0;
     for (int b = b0; b < b1; ++b) {
-        n += max(0, a.new_lens[b]);
-        p += total(b) - held(b);
+        const long long have = max(0, a.lens[b]), more = max(0, a.new_lens[b]);
+        len[b] = (int)have;
+        tok0[b] = (int)more;  // (turned into the first slot below)
+        n += more;
+        p += pages(have + more) - pages(have);
     }
-    part[0][t] = n;
-    part[1][t] = p;
+    const int used = max(0, a.used[0]);
+    long long sn = n, sp = p;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long long x = __shfl_up(sn, o), y = __shfl_up(sp, o);
+        if (lane >= o) {
+            sn += x;
+            sp += y;
+        }
+    }
+    if (lane == 63) {
+        part[0][wave] = sn;
+        part[1][wave] = sp;
+    }
     __syncthreads();
-    for (int o = 1; o < 256; o <<= 1) {
-        const long long x = t >= o ? part[0][t - o] : 0, y = t >= o ? part[1][t - o] : 0;
-        __syncthreads();
-        part[0][t] += x;
-        part[1][t] += y;
-        __syncthreads();
-    }
-    n = part[0][t] - n;
-    p = part[1][t] - p;
-    for (int b = b0; b < b1; ++b) {
-        tok0[b] = n;
-        pg0[b] = p;
-        n += max(0, a.new_lens[b]);
-        p += total(b) - held(b);
+    for (int w = 0; w < wave; ++w) {
+        sn += part[0][w];
+        sp += part[1][w];
     }
     if (t == 255) {
-        tok0[B] = part[0][255];
-        pg0[B] = part[1][255];
+        tok0[B] = cap(sn);
+        pg0[B] = cap(sp);
+    }
+    n = sn - n;
+    p = sp - p;
+    for (int b = b0; b < b1; ++b) {
+        const long long have = len[b], more = tok0[b];
+        tok0[b] = cap(n);
+        pg0[b] = cap(p);
+        n += more;
+        p += pages(have + more) - pages(have);
     }
     __syncthreads();
 
-    const long long used = max(0, a.used[0]);
     // Page of place k of request b's row, or -1.
     auto fresh = [&](int b, long long k) -> int {
-        const long long f = used + pg0[b] + (k - held(b));
+        const long long f = (long long)used + pg0[b] + (k - pages(len[b]));
         return k < a.W && f < a.n_free ? a.free_pages[f] : -1;
     };
     const int stride = gridDim.x * 256, gt = blockIdx.x * 256 + t;
-    for (int s = gt; s < a.n_slots; s += stride) {
+    for (long long s = gt; s < a.n_slots; s += stride) {
         int slot = -1;
         if (s < tok0[B]) {
             int lo = 0, hi = B - 1;  // last request whose first slot is at most s
@@ -117,43 +150,45 @@ __global__ void __launch_bounds__(256) plan_pages_kernel(const PlanArgs a) {
                 else
                     hi = mid - 1;
             }
-            const long long pos = (long long)max(0, a.lens[lo]) + (s - tok0[lo]), k = pos / P;
-            const int page = k >= held(lo) ? fresh(lo, k)
-                             : k < a.W     ? a.table[lo * a.table_stride + k]
-                                           : -1;
-            const long long at = (long long)page * P + pos % P;
-            if (page >= 0 && at < (1LL << 31)) slot = (int)at;
+            const long long pos = (long long)len[lo] + (s - tok0[lo]), k = pos >> sh;
+            const int page = k >= pages(len[lo]) ? fresh(lo, k)
+                             : k < a.W           ? a.table[lo * a.table_stride + k]
+                                                 : -1;
+            const long long at = (long long)page * P + (pos & (P - 1));
+            if (page >= 0 && at <= kCap) slot = (int)at;
         }
         a.slots[s] = slot;
     }
-    const long long cap = 0x7fffffff;
+    // (new tokens of a request: from its first slot to the next request's; where those are
+    // saturated, from memory again)
+    auto more_of = [&](int b) -> long long {
+        return tok0[b + 1] < kCap ? tok0[b + 1] - tok0[b] : max(0, a.new_lens[b]);
+    };
     for (int b = gt; b <= B; b += stride) {
-        a.cu_new[b] = (int)min(cap, tok0[b]);
-        if (b == B) break;
-        a.lens_out[b] = (int)min(cap, (long long)max(0, a.lens[b]) + max(0, a.new_lens[b]));
+        a.cu_new[b] = tok0[b];
+        if (b < B) a.lens_out[b] = cap(len[b] + more_of(b));
     }
     for (int b = gt / 64; b < B; b += stride / 64) {
-        const long long last = min(total(b), (long long)a.W);
-        for (long long k = held(b) + (t & 63); k < last; k += 64)
+        const long long last = min(pages(len[b] + more_of(b)), (long long)a.W);
+        for (long long k = pages(len[b]) + lane; k < last; k += 64)
             a.table[b * a.table_stride + k] = fresh(b, k);
     }
     if (blockIdx.x == 0) {
-        // Pages of columns behind the table take their place in the free list too
-        // (the pages are counted as missing, and left out of *used only at its end).
+        // Pages of columns behind the table take their place in the free list too.
         long long lost = 0;
         for (int b = b0; b < b1; ++b) {
-            const long long first = used + pg0[b], need = total(b) - held(b);
-            const long long in_row = max(0LL, min(need, a.W - held(b)));
-            lost += need - max(0LL, min(in_row, (long long)a.n_free - first));
+            const long long held = pages(len[b]), need = pages(len[b] + more_of(b)) - held;
+            const long long in_row = max(0LL, min(need, a.W - held));
+            lost += need - max(0LL, min(in_row, (long long)a.n_free - used - pg0[b]));
         }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) lost += __shfl_xor(lost, o);
         __syncthreads();
-        part[0][t] = lost;
+        if (lane == 0) part[0][wave] = lost;
         __syncthreads();
         if (t == 0) {
-            long long m = 0;
-            for (int i = 0; i < 256; ++i) m += part[0][i];
-            a.missing[0] = (int)min(cap, m);
-            a.used_out[0] = (int)min(cap, max(used, min(used + pg0[B], (long long)a.n_free)));
+            a.missing[0] = cap(part[0][0] + part[0][1] + part[0][2] + part[0][3]);
+            a.used_out[0] = max(used, (int)min((long long)used + pg0[B], (long long)a.n_free));
         }
     }
 #endif
@@ -169,79 +204,83 @@ struct RowArgs {
     long long kt, kh, vt, vh;  // strides of k and v: token, head
     const int* slots;
     Cache c;
-    long long n;  // blocks of 32 values in k (and in v)
+    unsigned n;  // blocks of 32 values (store) or pieces of 8 (load) in k, and in v
 };
 
-// One lane per block of 32 values of k or v.
+#if defined(__HIP_DEVICE_COMPILE__)
+// Piece id of K or V, 2^ds pieces in a row: piece d of head h of row t.
+struct Piece {
+    unsigned t;
+    int h, d;
+};
+__device__ __forceinline__ Piece piece(const Cache& c, unsigned id, int ds) {
+    const unsigned row = id >> ds, t = row / (unsigned)c.Hkv;
+    return {t, (int)(row - t * c.Hkv), (int)(id & ((1u << ds) - 1))};
+}
+#endif
+
+// A lane stores a block of 32 values: four 16-byte loads in flight, no exchange. Bound by
+// bytes: 16384 rows of 16 heads, D = 128, STOREUS us (STORETB TB/s); a lane per 8 values,
+// with the block's maximum exchanged between four, takes 45. grid.y: K, V.
 template <class T>
 __global__ void __launch_bounds__(256) store_kernel(const RowArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const bool is_v = id >= a.n;
-    const long long blk = is_v ? id - a.n : id;
-    if (blk >= a.n) return;
-    const int nb = a.c.D / 32, j = (int)(blk % nb);
-    const int h = (int)(blk / nb % a.c.Hkv);
-    const long long t = blk / nb / a.c.Hkv;
-    const int slot = a.slots[t];
+    using x8 = typename Elem<T>::x8;
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;
+    if (id >= a.n) return;
+    const bool is_v = blockIdx.y;
+    const Piece p = piece(a.c, id, a.c.D == 128 ? 2 : 1);
+    const int slot = a.slots[p.t];
     if (slot < 0 || slot >= a.c.pages * (long long)a.c.page) return;
-    const T* src = is_v ? (const T*)a.v + t * a.vt + h * a.vh : (const T*)a.k + t * a.kt + h * a.kh;
-    float x[32];
+    const T* src = is_v ? (const T*)a.v + p.t * a.vt + p.h * a.vh
+                        : (const T*)a.k + p.t * a.kt + p.h * a.kh;
+    x8 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const x8*>(src + 32 * p.d + 8 * i);
     unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        x[i] = (float)src[32 * j + i];
-        top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    }
+    for (int i = 0; i < 32; ++i)
+        top = max(top, __float_as_uint((float)x[i / 8][i % 8]) & 0x7fffffffu);
     const unsigned e = top >> 23, byte = e == 255 ? 255 : (unsigned)max(1, (int)e - 2);
     const float s = e8m0(byte);
-    unsigned w[4] = {};
+    u32x4 w = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], x[8 * i], x[8 * i + 1], s, 0);
-        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], x[8 * i + 2], x[8 * i + 3], s, 1);
-        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], x[8 * i + 4], x[8 * i + 5], s, 2);
-        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], x[8 * i + 6], x[8 * i + 7], s, 3);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)x[i][j];
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], f[0], f[1], s, 0);
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], f[2], f[3], s, 1);
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], f[4], f[5], s, 2);
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], f[6], f[7], s, 3);
     }
     const int page = slot / a.c.page, tok = slot % a.c.page;
     uint8_t* codes = const_cast<uint8_t*>(is_v ? a.c.vc : a.c.kc);
     uint8_t* scales = const_cast<uint8_t*>(is_v ? a.c.vs : a.c.ks);
-    *reinterpret_cast<u32x4*>(codes + code_at(a.c, page, h, tok) + 16 * j) =
-        u32x4{w[0], w[1], w[2], w[3]};
-    scales[scale_at(a.c, page, h, tok) + 4 * j] = (uint8_t)byte;
+    *reinterpret_cast<u32x4*>(codes + code_at(a.c, page, p.h, tok) + 16 * p.d) = w;
+    scales[scale_at(a.c, page, p.h, tok) + 4 * p.d] = (uint8_t)byte;
 #endif
 }
 
+// Rows back: a lane per 8 values, so that a wave's 16-byte stores are contiguous; LOADUS us
+// for as many rows, and 45 with a lane per 32 values.
 template <class T>
 __global__ void __launch_bounds__(256) load_kernel(const RowArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const bool is_v = id >= a.n;
-    const long long blk = is_v ? id - a.n : id;
-    if (blk >= a.n) return;
-    const int nb = a.c.D / 32, j = (int)(blk % nb);
-    const int h = (int)(blk / nb % a.c.Hkv);
-    const long long t = blk / nb / a.c.Hkv;
-    const int slot = a.slots[t];
-    T* dst = (T*)(is_v ? a.vo : a.ko) + blk * 32;
-    u32x4 w = {};
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;
+    if (id >= a.n) return;
+    const bool is_v = blockIdx.y;
+    const Piece p = piece(a.c, id, a.c.D == 128 ? 4 : 3);
+    const int slot = a.slots[p.t];
+    unsigned w = 0;
     float s = 1.f;
     if (slot >= 0 && slot < a.c.pages * (long long)a.c.page) {
         const int page = slot / a.c.page, tok = slot % a.c.page;
-        w = *reinterpret_cast<const u32x4*>((is_v ? a.c.vc : a.c.kc) +
-                                            code_at(a.c, page, h, tok) + 16 * j);
-        s = e8m0((is_v ? a.c.vs : a.c.ks)[scale_at(a.c, page, h, tok) + 4 * j]);
+        w = *reinterpret_cast<const unsigned*>((is_v ? a.c.vc : a.c.kc) +
+                                               code_at(a.c, page, p.h, tok) + 4 * p.d);
+        s = e8m0((is_v ? a.c.vs : a.c.ks)[scale_at(a.c, page, p.h, tok) + (p.d & ~3)]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 0);
-        const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 1);
-        const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 2);
-        const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 3);
-        const float x[8] = {p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dst[8 * i + e] = (T)x[e];
-    }
+    reinterpret_cast<typename Elem<T>::x8*>(is_v ? a.vo : a.ko)[id] = expand<T>(w, s);
 #endif
 }
 
@@ -379,23 +418,6 @@ struct Codes {
         }
     }
 };
-template <class T>
-__device__ __forceinline__ typename Elem<T>::x8 expand(unsigned w, float s) {
-    typename Elem<T>::x2 p[4];
-    if constexpr (__is_same(T, f16)) {
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0);
-        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2);
-        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
-    } else {
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0);
-        p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2);
-        p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
-    }
-    auto u = [](typename Elem<T>::x2 x) { return __builtin_bit_cast(unsigned, x); };
-    return __builtin_bit_cast(typename Elem<T>::x8, u32x4{u(p[0]), u(p[1]), u(p[2]), u(p[3])});
-}
 #endif
 
 // Attention of requests with few query rows (single tokens, drafts), bound by the
@@ -1309,13 +1331,14 @@ extern "C" int kv4_store(const void* k, const void* v, const long long* k_stride
     a.slots = slots;
     a.c = Cache{(const uint8_t*)k_codes, (const uint8_t*)k_scales, (const uint8_t*)v_codes,
                 (const uint8_t*)v_scales, pages, page, Hkv, D};
-    a.n = (long long)T * Hkv * (D / 32);
-    const long long groups = (2 * a.n + 255) / 256;
-    if (groups >= (1LL << 31)) return g_err.fail("kv4_store: too many rows");
+    const long long n = (long long)T * Hkv * (D / 32);
+    if (n >= (1LL << 31)) return g_err.fail("kv4_store: too many rows");
+    a.n = (unsigned)n;
+    const dim3 grid((unsigned)((n + 255) / 256), 2);
     if (dtype == KV4_DTYPE_F16)
-        hipLaunchKernelGGL(store_kernel<f16>, dim3((unsigned)groups), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(store_kernel<f16>, grid, dim3(256), 0, stream, a);
     else
-        hipLaunchKernelGGL(store_kernel<bf16>, dim3((unsigned)groups), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(store_kernel<bf16>, grid, dim3(256), 0, stream, a);
     return g_err.launched("kv4_store", hipGetLastError());
 }
 
@@ -1336,13 +1359,14 @@ extern "C" int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, cons
     a.slots = slots;
     a.c = Cache{(const uint8_t*)k_codes, (const uint8_t*)k_scales, (const uint8_t*)v_codes,
                 (const uint8_t*)v_scales, pages, page, Hkv, D};
-    a.n = (long long)T * Hkv * (D / 32);
-    const long long groups = (2 * a.n + 255) / 256;
-    if (groups >= (1LL << 31)) return g_err.fail("kv4_load: too many rows");
+    const long long n = (long long)T * Hkv * (D / 8);
+    if (n >= (1LL << 31)) return g_err.fail("kv4_load: too many rows");
+    a.n = (unsigned)n;
+    const dim3 grid((unsigned)((n + 255) / 256), 2);
     if (dtype == KV4_DTYPE_F16)
-        hipLaunchKernelGGL(load_kernel<f16>, dim3((unsigned)groups), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(load_kernel<f16>, grid, dim3(256), 0, stream, a);
     else
-        hipLaunchKernelGGL(load_kernel<bf16>, dim3((unsigned)groups), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(load_kernel<bf16>, grid, dim3(256), 0, stream, a);
     return g_err.launched("kv4_load", hipGetLastError());
 }
 
