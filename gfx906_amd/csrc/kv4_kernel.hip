@@ -662,11 +662,14 @@ attn_few_kernel(const AttnArgs a) {
                             expand<T>(vc[2 * half + t].w[n], sc);
                 }
                 __builtin_amdgcn_wave_barrier();
+                if (half) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch_v(c + NW, page);
+                }
                 w.pv(st, P);
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_sched_barrier(0);
             }
-            fetch_v(c + NW, page);
         }
 
         // Merge the waves: a common max, then sums of 16 rows at a time through LDS.
