@@ -177,7 +177,9 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
     if (q.numel() == 0 || B == 0) return o;
     const c10::DeviceGuard guard(dev);
     if (max_q < 0 || max_q > T) max_q = T;
-    const Tensor qr = rows_of(q);
+    // (rows may be done a second time, from q: it is copied where out is q)
+    const bool in_place = o.data_ptr() == q.data_ptr();
+    const Tensor qr = in_place ? q.clone(at::MemoryFormat::Contiguous) : rows_of(q);
     const auto sq = strides2(qr), so = strides2(o);
     const int W = (int)table.size(1);
     const size_t bytes = kv4_attn_workspace_bytes((int)T, (int)B, (int)Hq, c.Hkv, c.D, (int)max_q,

@@ -57,5 +57,7 @@ def attn(q, k, v, scale, count, block=64, causal=False, k_means=None, out=None):
         raise ValueError("sparse.attn: scale must be positive")
     if k_means is None:
         k_means = block_means(k, block)
+    elif k_means.shape[:2] != k.shape[:2]:
+        raise ValueError("sparse.attn: k_means must have k's batches and heads")
     index = select(block_means(q, Q_BLOCK), k_means, count, q.shape[2], k.shape[2], block, causal)
     return attn_blocks(q, k, v, scale, index, block, causal, out), index

@@ -75,12 +75,13 @@ int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, const int* slot
  * requests: rows cu_q[b] .. cu_q[b+1] belong to request b (cu_q NULL: row b, T = B),
  * whose lens[b] tokens lie in pages table[b][...]. Query head h reads kv head
  * h / (Hq / Hkv). With causal != 0 the n queries of a request are its last n tokens
- * and see no later one; otherwise they see all of its tokens. A row that sees no key
- * is 0. Keys in pages outside [0, pages) or behind the table's last column weigh
+ * and see no later one; otherwise they see all of its tokens. A row that sees no key, or
+ * only such of score -inf, is 0; a token that a row does not see adds nothing to it, whatever
+ * it holds. Keys in pages outside [0, pages) or behind the table's last column weigh
  * nothing; cu_q is taken as clamped to 0 .. T. Rows outside every request, and queries
  * past the first max_q of one, are left as they were. q and o: strides {token, head} in
- * elements, head dim contiguous, q's rows 16-byte and o's 8-byte aligned; o may
- * be q. workspace: 16-byte aligned, kv4_attn_workspace_bytes() bytes, with max_len
+ * elements, head dim contiguous, q's rows 16-byte and o's 8-byte aligned; o's must
+ * not overlap each other, q or the cache. workspace: 16-byte aligned, kv4_attn_workspace_bytes() bytes, with max_len
  * = W * page; its content is neither read before it is written nor kept. */
 size_t kv4_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q, int max_len);
 int kv4_attn(const void* q, void* o, const long long* q_strides, const long long* o_strides,

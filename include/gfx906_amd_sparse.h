@@ -45,8 +45,9 @@ int sparse_select(const float* q_means, const float* k_means, int B, int Hq, int
 /* o = softmax(scale q k^T) v over the keys of the blocks in index (as
  * sparse_select writes it, [B, Hq, ceil(Sq/128), count]; read on the GPU and not
  * checked by the host: an entry outside 0 .. ceil(Skv/block)-1, or not above every
- * valid entry before it, is passed over). causal as above. A row that sees no key is
- * 0. q, k, v: rows 16-byte aligned (k's and v's
+ * valid entry before it, is passed over). causal as above. A row that sees no key,
+ * or only such of score -inf, is 0; a key that a row does not see adds nothing to it, whatever
+ * it holds. q, k, v: rows 16-byte aligned (k's and v's
  * apart, their strides at most 2^22); o: 8-byte, rows that do not overlap; o may be q.
  * workspace: 16-byte aligned, sparse_attn_workspace_bytes() bytes (may be 0). */
 size_t sparse_attn_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block, int count);

@@ -62,6 +62,13 @@ def test_plan_pages_with_a_short_slot_list():
     assert plan.slots.tolist() == list(range(256, 266)) and plan.cu_new.tolist() == [0, 70, 73]
 
 
+def test_plan_pages_of_no_requests():
+    none = i32([])
+    plan = kv4.plan_pages(none, none, i32([]).view(0, 3), i32([1, 2]), i32([1]), 64, 3)
+    assert plan.slots.tolist() == [-1] * 3 and plan.cu_new.tolist() == [0]
+    assert plan.lens.numel() == 0 and plan.used.item() == 1 and plan.missing.item() == 0
+
+
 def test_plan_pages_refuses():
     a = dict(lens=i32([1]), new_lens=i32([1]), table=i32([[0]]), free_pages=i32([1]), used=i32([0]),
              page=64, tokens=1)
@@ -240,6 +247,42 @@ def test_chunks(case, heads, dtype, causal):
     check(out, oc.cache_attn(q, host, page, table, lens, D ** -0.5, cu, causal=causal), before)
 
 
+LONG = [  # lens, queries of each request, heads: runs that end inside a head or a tile
+    ([5000], [4], (16, 2)), ([3000, 70, 2600], [1, 1, 1], (6, 2)), ([4100], [200], (4, 2)),
+    ([2500, 3000, 64], [300, 1, 64], (4, 1)), ([2300], [1], (96, 1)), ([300, 20], [3, 1], (96, 1)),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_long_contexts(case, dtype, causal):
+    lens, news, (Hq, Hkv) = LONG[case]
+    D = (128, 64)[case % 2]
+    print(f"long {case} {dtype} causal {causal}", flush=True)
+    cache, host, table = filled(lens, 64, Hkv, D, dtype, seed=case)
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    q = torch.randn(cu[-1], Hq, D, generator=torch.Generator().manual_seed(case)).to(dtype)
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), D ** -0.5, cu_q=i32(cu),
+                   max_q=max(news), causal=causal)
+    check(out, oc.cache_attn(q, host, 64, table, lens, D ** -0.5, cu, causal=causal))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_requests(wide):
+    """A thousand requests, some without tokens; with a wide table too (runs of units)."""
+    g = torch.Generator().manual_seed(12)
+    lens = [int(n) for n in torch.randint(0, 90, (1000,), generator=g)]
+    cache, host, table = filled(lens, 64, 1, 64, torch.float16, seed=12)
+    if wide:
+        table = torch.cat((table, torch.full((1000, 60), -1, dtype=torch.int32)), 1)
+    q = torch.randn(1000, 2, 64, generator=g).half()
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.125)
+    check(out, oc.cache_attn(q, host, 64, table, lens, 0.125))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
 def test_scales(scale):
     lens = [200, 3]
@@ -313,6 +356,32 @@ def test_infinite_and_nan_blocks():
         assert nan[2:5, :, dims].all() and not nan[:2].any() and not nan[5:].any()
         if where == "v":
             assert not nan[:, :, :32].any()
+
+
+@pytest.mark.parametrize("n,news,Hq", [(70, 5, 2), (2600, 6, 4), (300, 150, 2), (2600, 150, 2)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_hidden_tokens_may_hold_anything(n, news, Hq, dtype):
+    """Tokens that hold NaN or infinities, late enough that some rows do not see them: single
+    and several query rows, tables narrow and wide, prompts in one run and in several."""
+    D = 128
+    for where in ("k", "v"):
+        cache, host, table = filled([n], 64, 1, D, dtype, seed=8)
+        bad = torch.randn(2, 1, D, generator=torch.Generator().manual_seed(3)).to(dtype)
+        bad[0, 0, 40], bad[1, 0, 100] = math.nan, -math.inf
+        ok = torch.randn(2, 1, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+        late = [n - 2, n - 4]
+        slots = i32([table[0, t // 64].item() * 64 + t % 64 for t in late])
+        kv4.store(cache, (bad if where == "k" else ok).to(DEV), (bad if where == "v" else ok).to(DEV),
+                  slots)
+        host = [t.cpu() for t in cache]
+        q = torch.randn(news, Hq, D, generator=torch.Generator().manual_seed(5)).to(dtype)
+        wide = torch.cat((table, torch.full((1, 40), -1, dtype=torch.int32)), 1)
+        for t in (table, wide):
+            out = kv4.attn(q.to(DEV), cache, t.to(DEV), i32([n]), 0.1, cu_q=i32([0, news]),
+                           max_q=news)
+            rows = oc.cache_attn(q, host, 64, t, [n], 0.1, [0, news])
+            assert not out[:news - 4].isnan().any() and out[news - 1].isnan().any()
+            check(out, rows)
 
 
 def test_strided_queries_and_outputs():
@@ -432,6 +501,32 @@ def test_captured_step_replays():
         assert torch.equal(out, got), f"replay {i}"
         lens.copy_(plan.lens)
         used.copy_(plan.used)
+        torch.cuda.synchronize()
+
+
+def test_captured_prompts_replay():
+    """A batch of prompts and single tokens, captured and replayed with new queries."""
+    lens, cu = [2500, 40, 700], [0, 150, 151, 300]
+    cache, _, table = filled(lens, 64, 2, 128, torch.bfloat16, seed=4)
+    table, n, cu = table.to(DEV), i32(lens), i32(cu)
+    q = torch.randn(300, 8, 128, device=DEV).bfloat16()
+    out = torch.zeros_like(q)
+    call = lambda o=None: kv4.attn(q, cache, table, n, 0.1, cu_q=cu, max_q=150, out=o)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call(out)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device=DEV).bfloat16())
+        out.zero_()
+        graph.replay()
+        torch.randn(1 << 18, device=DEV).sum().item()
+        assert torch.equal(out, call()), f"replay {i}"
         torch.cuda.synchronize()
 
 

@@ -43,7 +43,7 @@ def strides(*s):
 
 
 def kv4_attn(lib, **kw):
-    a = dict(q=FAKE, o=FAKE, qs=strides(1024, 128), os=strides(1024, 128), dtype=0, T=4, B=4, Hq=8,
+    a = dict(q=FAKE, o=2 * FAKE, qs=strides(1024, 128), os=strides(1024, 128), dtype=0, T=4, B=4, Hq=8,
              Hkv=2, D=128, kc=FAKE, ks=FAKE, vc=FAKE, vs=FAKE, pages=9, page=64, table=FAKE,
              stride=3, W=3, lens=FAKE, cu=None, max_q=1, scale=0.1, causal=1, ws=FAKE, n=1 << 40,
              stream=None) | kw
@@ -57,7 +57,7 @@ def kv4_attn(lib, **kw):
     (dict(B=5000, T=5000), b"requests"), (dict(T=5), b"one query"), (dict(q=None), b"null"),
     (dict(lens=None), b"null"), (dict(kc=None), b"null cache"), (dict(kc=FAKE + 8), b"aligned"),
     (dict(pages=1 << 25), b"2^31"), (dict(W=1 << 26), b"too wide"), (dict(q=FAKE + 2), b"aligned"),
-    (dict(qs=strides(1024, 100)), b"multiples of 8"), (dict(os=strides(-4, 128)), b"non-negative"),
+    (dict(o=FAKE), b"must not be q"), (dict(W=1 << 24, stride=1 << 24, Hq=64, Hkv=64), b"too wide"), (dict(qs=strides(1024, 100)), b"multiples of 8"), (dict(os=strides(-4, 128)), b"non-negative"),
     (dict(os=strides(128, 128)), b"overlap"), (dict(scale=float("nan")), b"finite"),
     (dict(stride=-3), b"negative stride"), (dict(max_q=-1), b"negative")])
 def test_cache_attention_refuses(lib, bad, word):

@@ -235,6 +235,43 @@ def test_strided_tensors_and_outputs():
     assert torch.equal(q2, want)
 
 
+@pytest.mark.parametrize("D,block", [(64, 64), (128, 128)])
+@pytest.mark.parametrize("Sq", [1, 300])
+def test_heads_of_more_than_2_gib(D, block, Sq):
+    """Keys and values of [B, S, H, D] buffers whose heads span 2^31 bytes and more, against
+    copies of the same rows."""
+    S, row = 1100, 1 << 20
+    buf = torch.zeros(S * row + 4 * D, dtype=torch.float16, device=DEV)
+    k = buf.as_strided((1, 2, S, D), (0, D, row, 1))
+    v = buf.as_strided((1, 2, S, D), (0, D, row, 1), 2 * D)
+    k.copy_(rand(1, 2, S, D, seed=1).to(DEV))
+    v.copy_(rand(1, 2, S, D, seed=2).to(DEV))
+    q = rand(1, 4, Sq, D, seed=3).to(DEV)
+    index = random_index(1, 4, -(-Sq // 128), -(-S // block), 6, 7).to(DEV)
+    for causal in (False, True):
+        got = sparse.attn_blocks(q, k, v, 0.1, index, block, causal)
+        want = sparse.attn_blocks(q, k.contiguous(), v.contiguous(), 0.1, index, block, causal)
+        assert torch.equal(got, want)
+
+
+def test_overlapping_rows_are_copied():
+    buf = rand(1, 1, 1, 9000, seed=1).to(DEV).view(-1)
+    k = buf.as_strided((1, 2, 200, 64), (0, 4096, 8, 1))     # rows 8 elements apart
+    q = rand(1, 2, 200, 64, seed=2).to(DEV)
+    index = random_index(1, 2, 2, 4, 2, 7).to(DEV)
+    want = sparse.attn_blocks(q, k.contiguous(), k.contiguous(), 0.1, index)
+    assert torch.equal(sparse.attn_blocks(q, k, k, 0.1, index), want)
+
+
+def test_means_kept_for_other_heads_are_refused():
+    q, k = rand(1, 4, 9, 64).to(DEV), rand(1, 2, 300, 64).to(DEV)
+    means = sparse.block_means(k.repeat_interleave(2, 1), 64)
+    with pytest.raises(ValueError):
+        sparse.attn(q, k, k, 0.1, 3, k_means=means)
+    with pytest.raises(RuntimeError):
+        sparse.attn(q, k, k, 0.1, 3, block=128, k_means=sparse.block_means(k, 64))
+
+
 def test_attention_refuses():
     q, k = torch.zeros(1, 4, 130, 64, device=DEV).half(), torch.zeros(1, 2, 70, 64, device=DEV).half()
     ix = torch.zeros(1, 4, 2, 2, dtype=torch.int32, device=DEV)
