@@ -28,6 +28,8 @@ torch::Tensor kv4_attn_op(torch::Tensor q, torch::Tensor kc, torch::Tensor ks, t
 torch::Tensor sparse_block_means_op(torch::Tensor x, int64_t block);
 torch::Tensor sparse_select_op(torch::Tensor qm, torch::Tensor km, int64_t count, int64_t q_len,
                                int64_t k_len, int64_t block, bool causal);
+torch::Tensor sparse_choose_op(torch::Tensor q, torch::Tensor km, int64_t count, int64_t k_len,
+                               int64_t block, bool causal);
 torch::Tensor sparse_attn_op(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale,
                              torch::Tensor index, int64_t block, bool causal,
                              c10::optional<torch::Tensor> out);

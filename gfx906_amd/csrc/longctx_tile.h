@@ -96,7 +96,7 @@ __device__ __forceinline__ bool p_above(const typename Elem<T>::x8 (&P)[NB]) {
         r = mx(mx(mx(h(a[0]), h(a[1])), h(a[2])), h(a[3]));
     }
     const f16 lim = __is_same(T, f16) ? (f16)kPLimit : __builtin_bit_cast(f16, (bf16)kPLimit);
-    return __any(!(r[0] <= lim) || !(r[1] <= lim));
+    return __builtin_amdgcn_ballot_w64(!(r[0] <= lim) || !(r[1] <= lim)) != 0;
 }
 
 // NB: column blocks of 16 query rows.
@@ -227,7 +227,7 @@ struct Tile {
     __device__ __forceinline__ void turn(const char* vt, const x8 (&Pp)[NB], const char* kt,
                                          f32x4 (&Sn)[2][NB], const f32x4 (&S)[2][NB], x8 (&P)[NB],
                                          float c) {
-        constexpr int AV = D == 128 ? 4 : 3, AK = 2, NK = 2 * NQ, EPS = 8 * NB / (NO + NK);
+        constexpr int AV = 2, AK = 2, NK = 2 * NQ, EPS = 8 * NB / (NO + NK);
         x8 vf[NO], kf[NK];
         float p[8 * NB];
         auto vread = [&](int n) __attribute__((always_inline)) {
@@ -293,7 +293,7 @@ struct Tile {
                 weights<true>(S, P, c, nb);
             }
             auto big = [](float x) { return fabsf(x) > 65536.f && x != kNoMax; };
-            far = __any(big(m[0]) || big(m[NB - 1]));
+            far = __builtin_amdgcn_ballot_w64(big(m[0]) || big(m[NB - 1])) != 0;
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) lacc[nb] = E::mma16(one, P[nb], lacc[nb]);

@@ -17,5 +17,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("kv4_attn", &kv4_attn_op, "attention over the 4-bit cache");
     m.def("sparse_block_means", &sparse_block_means_op, "means of row blocks");
     m.def("sparse_select", &sparse_select_op, "key blocks of every query block");
+    m.def("sparse_choose", &sparse_choose_op, "key blocks of every query block, from its rows");
     m.def("sparse_attn", &sparse_attn_op, "attention over selected key blocks");
 }

@@ -1,5 +1,5 @@
 // PyTorch binding of sparse attention (gfx906_amd_sparse.h): sparse_block_means,
-// sparse_select and sparse_attn. The Python layer (gfx906_amd.sparse) documents the
+// sparse_select, sparse_choose and sparse_attn. The Python layer (gfx906_amd.sparse) documents the
 // arguments. Every op runs on the current HIP stream of its tensors' device without
 // synchronising; what cannot be run raises RuntimeError.
 #include <ATen/MemoryOverlap.h>
@@ -101,6 +101,34 @@ Tensor sparse_select_op(Tensor qm, Tensor km, int64_t count, int64_t q_len, int6
     check_rc(sparse_select(qc.data_ptr<float>(), kc.data_ptr<float>(), B, Hq, Hkv, (int)q_len,
                            (int)k_len, D, (int)block, (int)count, causal, index.data_ptr<int>(),
                            bytes ? ws.data_ptr() : nullptr, bytes, stream()));
+    return index;
+}
+
+Tensor sparse_choose_op(Tensor q, Tensor km, int64_t count, int64_t k_len, int64_t block,
+                        bool causal) {
+    const char* who = "choose";
+    const int dt = dtype_of(q, who);
+    check_block(block, who);
+    check_count(count, who);
+    TORCH_CHECK(km.device() == q.device() && km.dtype() == torch::kFloat && km.dim() == 4 &&
+                    k_len >= 0 && k_len < (1 << 30) && km.size(0) == q.size(0) &&
+                    km.size(3) == q.size(3) && km.size(2) == blocks(k_len, block) &&
+                    km.size(1) < (1LL << 30),
+                who, ": means must be fp32 [B, heads, ceil(k_len/block), D] on q's device");
+    const c10::DeviceGuard guard(q.device());
+    const int B = (int)q.size(0), Hq = (int)q.size(1), Sq = (int)q.size(2), D = (int)q.size(3);
+    Tensor index =
+        torch::empty({B, Hq, blocks(Sq, SPARSE_Q_BLOCK), count}, q.options().dtype(torch::kInt));
+    if (index.numel() == 0) return index;
+    const Tensor qr = rows_of(q), kc = km.contiguous();
+    const auto st = strides3(qr);
+    const size_t bytes =
+        sparse_choose_workspace_bytes(B, Hq, Sq, (int)k_len, D, (int)block);
+    Tensor ws;
+    if (bytes) ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kByte));
+    check_rc(sparse_choose(qr.data_ptr(), st.data(), dt, kc.data_ptr<float>(), B, Hq,
+                           (int)km.size(1), Sq, (int)k_len, D, (int)block, (int)count, causal,
+                           index.data_ptr<int>(), bytes ? ws.data_ptr() : nullptr, bytes, stream()));
     return index;
 }
 

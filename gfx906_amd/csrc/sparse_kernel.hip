@@ -88,6 +88,8 @@ struct SelectArgs {
     int* index;
     int Hq, Hkv, Sq, Skv, D, block, nq, nk, count, causal;
     long long rows;  // query blocks of all heads
+    const void* q;   // choose_one_kernel: the query rows, and their strides
+    long long qb, qh, qs;
 };
 
 // Key blocks a query block may take (the first `seen`), and the first of those that
@@ -163,18 +165,12 @@ __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
 // themselves; the lower ones matter only among scores whose upper bits are the bound's.
 // Everything stays in registers; a step is a compare and a population count per 64 scores
 // (and, with several waves, an exchange through LDS).
-template <int WAVES, int K>
-__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
+template <int WAVES, int K, class Score>
+__device__ __forceinline__ void choose(const SelectArgs& a, const Reach& r, Score score, int* out,
+                                       int (*part)[WAVES]) {
     typedef unsigned long long u64;
-    __shared__ int part[2][WAVES];
     const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
-    const long long row = WAVES == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-    if (row >= a.rows) return;  // (a whole wave; with several, never)
-    const int i = (int)(row % a.nq);
-    const Reach r = reach(i, a.Sq, a.Skv, a.block, a.nk, a.causal);
-    const double* score = a.score + row * a.nk;
-    int* out = a.index + row * a.count;
     const int base = wave * 64 * K + lane;
     unsigned hi[K], lo[K];
 #pragma unroll
@@ -182,7 +178,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(c
         const int j = base + 64 * n;
         u64 key = 0;
         if (j < r.seen) {
-            const double s = score[j] + 0.0;  // -0 becomes +0
+            const double s = score(j) + 0.0;  // -0 becomes +0
             const u64 bits = (u64)__double_as_longlong(s != s ? INFINITY : s);
             key = j >= r.own ? ~0ull : bits >> 63 ? ~bits : bits | 1ull << 63;
         }
@@ -275,6 +271,111 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(c
     }
     for (int e = all + (WAVES == 1 ? lane : (int)threadIdx.x); e < a.count; e += 64 * WAVES)
         out[e] = -1;
+}
+#endif
+
+template <int WAVES, int K>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ int part[2][WAVES];
+    const long long row = WAVES == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= a.rows) return;  // (a whole wave; with several, never)
+    const Reach r = reach((int)(row % a.nq), a.Sq, a.Skv, a.block, a.nk, a.causal);
+    const double* score = a.score + row * a.nk;
+    choose<WAVES, K>(a, r, [&](int j) { return score[j]; }, a.index + row * a.count, part);
+#endif
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// Adds up N = 8 or 16 neighbouring lanes (DPP moves within rows of 16: a swap of
+// neighbours, of pairs, and mirrors of what is then equal in halves).
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double x) {
+    const long long b = __double_as_longlong(x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xf, 0xf, true);
+    return x + __longlong_as_double((long long)((unsigned long long)(unsigned)hi << 32 | (unsigned)lo));
+}
+template <int N>
+__device__ __forceinline__ double lanes_sum(double x) {
+    x = dpp_add<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+    x = dpp_add<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+    x = dpp_add<0x141>(x);  // row_half_mirror
+    if constexpr (N == 16) x = dpp_add<0x140>(x);  // row_mirror
+    return x;
+}
+#endif
+
+// The choice for one query block of every head straight from its rows (single tokens): mean,
+// scores and choice in one workgroup, of up to 4096 key blocks, instead of three kernels
+// whose launches outweigh the work. D/8 lanes take a row (of q or of the means) and add up
+// their parts. 64 heads of one query, 512 blocks: ONEUS us, and 19 in three kernels.
+template <int D, class T>
+__global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LPR = D / 8, ROWS = 512 / LPR;  // lanes a row, rows at a time
+    __shared__ double score[4096];
+    __shared__ double part_q[8][D];
+    __shared__ float qs[D];
+    __shared__ int part[2][8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x, b = row / a.Hq, h = row - b * a.Hq;
+    const int kvh = b * a.Hkv + h / (a.Hq / a.Hkv);
+    const int c = tid % LPR, r0 = tid / LPR;
+    double sum[8] = {};
+    const T* q = (const T*)a.q + b * a.qb + h * a.qh + c * 8;
+    for (int r = r0; r < a.Sq; r += ROWS) {
+        const typename Elem<T>::x8 x = *reinterpret_cast<const typename Elem<T>::x8*>(q + r * a.qs);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += (double)(float)x[e];
+    }
+#pragma unroll
+    for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], o);
+    if (lane < LPR)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part_q[wave][8 * c + e] = sum[e];
+    __syncthreads();
+    if (tid < D) {
+        double s = 0.0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += part_q[w][tid];
+        qs[tid] = (float)(s / a.Sq);
+    }
+    __syncthreads();
+    double qd[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qd[e] = qs[8 * c + e];
+    const Reach r = reach(0, a.Sq, a.Skv, a.block, a.nk, a.causal);
+    const float* km = a.km + (long long)kvh * a.nk * D + c * 8;
+    constexpr int U = 8;
+    for (int j0 = r0; j0 < r.seen; j0 += U * ROWS) {
+        f32x4 x[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float* p = km + (long long)min(j0 + u * ROWS, r.seen - 1) * D;
+            x[u][0] = *reinterpret_cast<const f32x4*>(p);
+            x[u][1] = *reinterpret_cast<const f32x4*>(p + 4);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            double s = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fma(qd[e], (double)x[u][e / 4][e % 4], s);
+            s = lanes_sum<LPR>(s);
+            const int j = j0 + u * ROWS;
+            if (c == 0 && j < r.seen) score[j] = s;
+        }
+    }
+    __syncthreads();
+    int* out = a.index + (long long)row * a.count;
+    auto at = [&](int j) { return score[j]; };
+    if (a.nk <= 512) {  // one wave: no exchange between waves in a step
+        if (wave == 0) choose<1, 8>(a, r, at, out, (int(*)[1])part);
+    } else {
+        choose<8, 8>(a, r, at, out, part);
+    }
 #endif
 }
 
@@ -729,37 +830,72 @@ extern "C" size_t sparse_select_workspace_bytes(int B, int Hq, int Sq, int Skv, 
     return (size_t)B * Hq * blocks_of(Sq, kQBlock) * blocks_of(Skv, block) * sizeof(double);
 }
 
+namespace {
+
+// Checks that sparse_select and sparse_choose share; `who` names the caller.
+int check_choice(const void* q, const float* k_means, int B, int Hq, int Hkv, int Sq, int Skv, int D,
+                 int block, int count, int causal, const int* index, const char* who) {
+    if (check_sizes(B, Hq, Sq, D, block, who) || check_sizes(B, Hkv, Skv, D, block, who)) return 1;
+    if (Hq > 0 && (Hkv <= 0 || Hq % Hkv))
+        return g_err.fail("%s: query heads must be a multiple of kv heads", who);
+    if (blocks_of(Skv, block) > SPARSE_MAX_BLOCKS)
+        return g_err.fail("%s: at most %d key blocks", who, SPARSE_MAX_BLOCKS);
+    if (count < 1 || count > SPARSE_MAX_COUNT)
+        return g_err.fail("%s: count must be 1 .. %d", who, SPARSE_MAX_COUNT);
+    if (B == 0 || Hq == 0 || Sq == 0) return 0;
+    if (!q || !index || (Skv > 0 && !k_means)) return g_err.fail("%s: null argument", who);
+    if (!aligned(k_means, 16)) return g_err.fail("%s: means must be 16-byte aligned", who);
+    // Blocks that hold the positions of a query block: the most over all of them.
+    const int own = (std::min(Sq, kQBlock) + block - 2) / block + 1;
+    if (causal && count < own)
+        return g_err.fail("%s: count must be at least %d, the blocks that hold a query block's own "
+                          "positions", who, own);
+    if ((long long)B * Hq * blocks_of(Sq, kQBlock) >= (1LL << 31))
+        return g_err.fail("%s: too many query blocks", who);
+    return 0;
+}
+
+SelectArgs select_args(const float* q_means, const float* k_means, int B, int Hq, int Hkv, int Sq,
+                       int Skv, int D, int block, int count, int causal, int* index, void* scores) {
+    SelectArgs a{};
+    a.qm = q_means;
+    a.km = k_means;
+    a.score = (double*)scores;
+    a.index = index;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.Sq = Sq;
+    a.Skv = Skv;
+    a.D = D;
+    a.block = block;
+    a.nq = blocks_of(Sq, kQBlock);
+    a.nk = blocks_of(Skv, block);
+    a.count = count;
+    a.causal = causal;
+    a.rows = (long long)B * Hq * a.nq;
+    return a;
+}
+
+}  // namespace
+
 extern "C" int sparse_select(const float* q_means, const float* k_means, int B, int Hq, int Hkv,
                              int Sq, int Skv, int D, int block, int count, int causal, int* index,
                              void* workspace, size_t workspace_bytes, hipStream_t stream) {
     g_err.text[0] = 0;
-    if (check_sizes(B, Hq, Sq, D, block, "sparse_select") ||
-        check_sizes(B, Hkv, Skv, D, block, "sparse_select"))
+    if (check_choice(q_means, k_means, B, Hq, Hkv, Sq, Skv, D, block, count, causal, index,
+                     "sparse_select"))
         return 1;
-    if (Hq > 0 && (Hkv <= 0 || Hq % Hkv))
-        return g_err.fail("sparse_select: query heads must be a multiple of kv heads");
-    if (blocks_of(Skv, block) > SPARSE_MAX_BLOCKS)
-        return g_err.fail("sparse_select: at most %d key blocks", SPARSE_MAX_BLOCKS);
-    if (count < 1 || count > SPARSE_MAX_COUNT)
-        return g_err.fail("sparse_select: count must be 1 .. %d", SPARSE_MAX_COUNT);
     if (B == 0 || Hq == 0 || Sq == 0) return 0;
-    if (!q_means || !index || (Skv > 0 && !k_means))
-        return g_err.fail("sparse_select: null argument");
-    // Blocks that hold the positions of a query block: the most over all of them.
-    const int own = (std::min(Sq, kQBlock) + block - 2) / block + 1;
-    if (causal && count < own)
-        return g_err.fail("sparse_select: count must be at least %d, the blocks that hold a query "
-                          "block's own positions", own);
+    if (!aligned(q_means, 16)) return g_err.fail("sparse_select: means must be 16-byte aligned");
     const size_t need = sparse_select_workspace_bytes(B, Hq, Sq, Skv, block);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return g_err.fail("sparse_select: workspace misaligned or smaller than "
                           "sparse_select_workspace_bytes()");
-    SelectArgs a{q_means, k_means, (double*)workspace, index, Hq, Hkv, Sq, Skv, D, block,
-                 blocks_of(Sq, kQBlock), blocks_of(Skv, block), count, causal, 0};
-    a.rows = (long long)B * Hq * a.nq;
-    if (a.rows >= (1LL << 31)) return g_err.fail("sparse_select: too many query blocks");
+    const SelectArgs a = select_args(q_means, k_means, B, Hq, Hkv, Sq, Skv, D, block, count, causal,
+                                     index, workspace);
     if (a.nk > 0) {
-        const int x = (Hq / Hkv * a.nq + 15) / 16, y = B * Hkv, tiles = (a.nk + 15) / 16;
+        const int x = (int)(((long long)Hq / Hkv * a.nq + 15) / 16), y = B * Hkv;
+        const int tiles = (a.nk + 15) / 16;
         // Shares of the key tiles: enough workgroups for the GPU, a tile a wave at least.
         const int z = (int)std::max<long long>(
             1, std::min<long long>((tiles + 3) / 4, 1024 / std::max(1LL, (long long)x * y)));
@@ -781,6 +917,61 @@ extern "C" int sparse_select(const float* q_means, const float* k_means, int B, 
     else
         hipLaunchKernelGGL((select_kernel<16, 32>), singles, dim3(1024), 0, stream, a);
     return g_err.launched("sparse_select", hipGetLastError());
+}
+
+namespace {
+// Whether a choice is choose_one_kernel's.
+bool one_block(int Sq, int Skv, int block) { return Sq <= kQBlock && blocks_of(Skv, block) <= 4096; }
+size_t means_bytes(int B, int Hq, int Sq, int D) {
+    return ((size_t)B * Hq * blocks_of(Sq, kQBlock) * D * sizeof(float) + 255) & ~(size_t)255;
+}
+}  // namespace
+
+extern "C" size_t sparse_choose_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block) {
+    if (B <= 0 || Hq <= 0 || Sq <= 0 || D <= 0 || block <= 0 || one_block(Sq, Skv, block)) return 0;
+    return means_bytes(B, Hq, Sq, D) + sparse_select_workspace_bytes(B, Hq, Sq, Skv, block);
+}
+
+extern "C" int sparse_choose(const void* q, const long long* q_strides, int dtype,
+                             const float* k_means, int B, int Hq, int Hkv, int Sq, int Skv, int D,
+                             int block, int count, int causal, int* index, void* workspace,
+                             size_t workspace_bytes, hipStream_t stream) {
+    g_err.text[0] = 0;
+    if (check_choice(q, k_means, B, Hq, Hkv, Sq, Skv, D, block, count, causal, index,
+                     "sparse_choose"))
+        return 1;
+    if (dtype != SPARSE_DTYPE_F16 && dtype != SPARSE_DTYPE_BF16)
+        return g_err.fail("sparse_choose: bad dtype");
+    if (B == 0 || Hq == 0 || Sq == 0) return 0;
+    if (!q_strides) return g_err.fail("sparse_choose: null argument");
+    if (check_strides(q_strides, q, 16, 8, "sparse_choose")) return 1;
+    const size_t need = sparse_choose_workspace_bytes(B, Hq, Sq, Skv, D, block);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return g_err.fail("sparse_choose: workspace misaligned or smaller than "
+                          "sparse_choose_workspace_bytes()");
+    if (!one_block(Sq, Skv, block)) {
+        float* means = (float*)workspace;
+        const size_t used = means_bytes(B, Hq, Sq, D);
+        const int rc =
+            sparse_block_means(q, q_strides, dtype, B, Hq, Sq, D, kQBlock, means, stream);
+        return rc ? rc
+                  : sparse_select(means, k_means, B, Hq, Hkv, Sq, Skv, D, block, count, causal,
+                                  index, (char*)workspace + used, workspace_bytes - used, stream);
+    }
+    SelectArgs a = select_args(nullptr, k_means, B, Hq, Hkv, Sq, Skv, D, block, count, causal, index,
+                               nullptr);
+    a.q = q;
+    a.qb = q_strides[0];
+    a.qh = q_strides[1];
+    a.qs = q_strides[2];
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(B * Hq), dim3(512), 0, stream, a);
+    };
+    if (dtype == SPARSE_DTYPE_F16)
+        D == 64 ? go(choose_one_kernel<64, f16>) : go(choose_one_kernel<128, f16>);
+    else
+        D == 64 ? go(choose_one_kernel<64, bf16>) : go(choose_one_kernel<128, bf16>);
+    return g_err.launched("sparse_choose", hipGetLastError());
 }
 
 extern "C" size_t sparse_attn_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block,

@@ -3,8 +3,7 @@
 ``attn`` does all of it; its parts serve programs that keep some of the results:
 
     k_means = sparse.block_means(k, 64)             # a decoder keeps them beside its keys
-    index = sparse.select(sparse.block_means(q, sparse.Q_BLOCK), k_means, 32,
-                          q.shape[2], k.shape[2])
+    index = sparse.choose(q, k_means, 32, k.shape[2])
     out = sparse.attn_blocks(q, k, v, scale, index)
 
 A block's score is the product of the query block's mean and the key block's mean,
@@ -40,6 +39,12 @@ def select(q_means, k_means, count, q_len, k_len, block=64, causal=False):
     return extension().sparse_select(q_means, k_means, count, q_len, k_len, block, causal)
 
 
+def choose(q, k_means, count, k_len, block=64, causal=False):
+    """``select`` for the query rows themselves, whose block means are taken on the way (up
+    to 128 rows and 4096 key blocks in one kernel)."""
+    return extension().sparse_choose(q, k_means, count, k_len, block, causal)
+
+
 def attn_blocks(q, k, v, scale, index, block=64, causal=False, out=None):
     """softmax(scale * q k^T) v over the keys of the blocks in ``index``
     (``[B, Hq, ceil(Sq/128), count]``, as ``select`` returns it), in a new tensor or
@@ -59,5 +64,5 @@ def attn(q, k, v, scale, count, block=64, causal=False, k_means=None, out=None):
         k_means = block_means(k, block)
     elif k_means.shape[:2] != k.shape[:2]:
         raise ValueError("sparse.attn: k_means must have k's batches and heads")
-    index = select(block_means(q, Q_BLOCK), k_means, count, q.shape[2], k.shape[2], block, causal)
+    index = choose(q, k_means, count, k.shape[2], block, causal)
     return attn_blocks(q, k, v, scale, index, block, causal, out), index

@@ -33,7 +33,7 @@ int sparse_block_means(const void* x, const long long* strides, int dtype, int B
  * the last. Taken are those with the largest product of q_means[b][h][i] and
  * k_means[b][h / (Hq/Hkv)][j] (fp64; NaN counts as largest, equal products by the
  * lower index). Means are packed fp32 [B, Hq, ceil(Sq/128), D] and
- * [B, Hkv, ceil(Skv/block), D]. With causal != 0 query row r stands at key position
+ * [B, Hkv, ceil(Skv/block), D], 16-byte aligned. With causal != 0 query row r stands at key position
  * r + Skv - Sq; blocks past the query block's last position are never taken, and
  * those that hold its own positions always (count must be at least 128/block + 1,
  * or their number where Sq < 128). workspace: sparse_select_workspace_bytes() bytes. */
@@ -41,6 +41,15 @@ size_t sparse_select_workspace_bytes(int B, int Hq, int Sq, int Skv, int block);
 int sparse_select(const float* q_means, const float* k_means, int B, int Hq, int Hkv, int Sq,
                   int Skv, int D, int block, int count, int causal, int* index, void* workspace,
                   size_t workspace_bytes, hipStream_t stream);
+
+/* The same from the query rows q [B, Hq, Sq, D] themselves (16-byte aligned), whose means
+ * over 128 rows are taken as sparse_block_means does. workspace:
+ * sparse_choose_workspace_bytes() bytes (0 for up to 128 rows and 4096 key blocks, which
+ * take one kernel). */
+size_t sparse_choose_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block);
+int sparse_choose(const void* q, const long long* q_strides, int dtype, const float* k_means, int B,
+                  int Hq, int Hkv, int Sq, int Skv, int D, int block, int count, int causal,
+                  int* index, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* o = softmax(scale q k^T) v over the keys of the blocks in index (as
  * sparse_select writes it, [B, Hq, ceil(Sq/128), count]; read on the GPU and not

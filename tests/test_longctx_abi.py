@@ -57,7 +57,9 @@ def kv4_attn(lib, **kw):
     (dict(B=5000, T=5000), b"requests"), (dict(T=5), b"one query"), (dict(q=None), b"null"),
     (dict(lens=None), b"null"), (dict(kc=None), b"null cache"), (dict(kc=FAKE + 8), b"aligned"),
     (dict(pages=1 << 25), b"2^31"), (dict(W=1 << 26), b"too wide"), (dict(q=FAKE + 2), b"aligned"),
-    (dict(o=FAKE), b"must not be q"), (dict(W=1 << 24, stride=1 << 24, Hq=64, Hkv=64), b"too wide"), (dict(qs=strides(1024, 100)), b"multiples of 8"), (dict(os=strides(-4, 128)), b"non-negative"),
+    (dict(o=FAKE), b"must not be q"),
+    (dict(W=1 << 24, stride=1 << 24, Hq=64, Hkv=64, os=strides(8192, 128)), b"too wide"),
+    (dict(qs=strides(1024, 100)), b"multiples of 8"), (dict(os=strides(-4, 128)), b"non-negative"),
     (dict(os=strides(128, 128)), b"overlap"), (dict(scale=float("nan")), b"finite"),
     (dict(stride=-3), b"negative stride"), (dict(max_q=-1), b"negative")])
 def test_cache_attention_refuses(lib, bad, word):
@@ -148,6 +150,18 @@ def test_select_refuses(lib, bad, word):
     a = dict(qm=FAKE, km=FAKE, B=2, Hq=4, Hkv=2, Sq=300, Skv=400, D=64, block=64, count=3, causal=0,
              index=FAKE, ws=FAKE, n=1 << 30, stream=None) | bad
     assert lib.sparse_select(*a.values()) == 1 and word in lib.sparse_last_error()
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(dtype=2), b"dtype"), (dict(qs=None), b"null"), (dict(qs=strides(9, 8, 8)), b"multiples"),
+    (dict(q=FAKE + 4), b"aligned"), (dict(km=FAKE + 8), b"aligned"), (dict(n=15), b"workspace"),
+    (dict(causal=1, count=2), b"own positions"), (dict(Hkv=3), b"multiple of kv heads")])
+def test_choose_refuses(lib, bad, word):
+    lib.sparse_choose.argtypes = [P, ctypes.POINTER(L), I, P] + [I] * 9 + [P, P, Z, P]
+    a = dict(q=FAKE, qs=strides(1 << 20, 1 << 16, 64), dtype=0, km=FAKE, B=2, Hq=4, Hkv=2, Sq=300,
+             Skv=400, D=64, block=64, count=3, causal=0, index=FAKE, ws=FAKE, n=1 << 30,
+             stream=None) | bad
+    assert lib.sparse_choose(*a.values()) == 1 and word in lib.sparse_last_error()
 
 
 def test_means_refuses(lib):

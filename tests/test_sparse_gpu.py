@@ -100,6 +100,37 @@ def test_choice_among_equal_and_special_scores(count):
     assert got[0, 0].tolist() == [list(range(count))] * 3
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Skv,D,block,count,causal", [
+    (1, 1, 1, 1, 1, 64, 64, 2, False), (2, 6, 2, 1, 30000, 128, 64, 40, True),
+    (1, 4, 1, 128, 9000, 64, 128, 5, True), (1, 2, 2, 77, 50, 128, 64, 4, True),
+    (1, 2, 1, 100, 70000, 64, 64, 300, False), (1, 1, 1, 3, 262144, 64, 64, 7, True),
+    (1, 1, 1, 3, 262145, 64, 64, 7, True), (2, 2, 1, 129, 3000, 128, 64, 9, True),
+    (1, 2, 2, 500, 0, 64, 64, 3, False), (1, 2, 2, 5, 0, 64, 64, 3, True)])
+def test_choice_from_rows(B, Hq, Hkv, Sq, Skv, D, block, count, causal, dtype):
+    """One kernel or several (above 128 rows or 4096 blocks), with equal scores among them."""
+    q = rand(B, Sq, Hq, D, seed=Sq, dtype=dtype).transpose(1, 2)
+    nk = -(-Skv // block)
+    km = torch.randn(B, Hkv, nk, D, generator=torch.Generator().manual_seed(nk))
+    if nk > 4:
+        km[0, 0, nk // 2] = km[0, 0, nk - 1] = km[0, 0, 1]
+    got = sparse.choose(q.to(DEV), km.to(DEV), count, Skv, block, causal)
+    want = oc.select(oc.block_means(q, 128), km, count, Sq, Skv, block, causal)
+    assert torch.equal(got.cpu(), want)
+    assert torch.equal(got, sparse.select(sparse.block_means(q.to(DEV), 128), km.to(DEV), count, Sq,
+                                          Skv, block, causal))
+
+
+def test_choice_from_rows_refuses():
+    q, km = rand(1, 4, 9, 64).to(DEV), torch.zeros(1, 2, 5, 64, device=DEV)
+    a = dict(q=q, k_means=km, count=4, k_len=300)
+    for kw in (dict(q=q.float()), dict(k_means=km.half()), dict(k_len=200), dict(count=0),
+               dict(k_means=km[:, :, :, :32]), dict(q=q[:, :3]), dict(block=32), dict(k_len=-1),
+               dict(k_means=km.cpu()), dict(q=q[0]), dict(causal=True, count=0)):
+        with pytest.raises(RuntimeError):
+            sparse.choose(**(a | kw))
+
+
 def test_choice_refuses():
     qm, km = torch.zeros(1, 2, 2, 64, device=DEV), torch.zeros(1, 2, 4, 64, device=DEV)
     a = dict(q_means=qm, k_means=km, count=4, q_len=200, k_len=256)
