@@ -78,7 +78,7 @@ struct PlanArgs {
 // rows. Entries that are read (held pages) and written (new ones) are different, so
 // workgroups need no order. Bound by latency: lengths are read once and kept in LDS, where
 // a slot finds its request by bisection; sums are 64-bit and kept saturated to 31 bits, as
-// no slot or page past that is used. 64 requests, one token each: PLANUS us.
+// no slot or page past that is used. 64 requests, one token each: 6.3 us.
 __global__ void __launch_bounds__(256) plan_pages_kernel(const PlanArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ int len[kMaxRequests];       // cached tokens
@@ -220,7 +220,7 @@ __device__ __forceinline__ Piece piece(const Cache& c, unsigned id, int ds) {
 #endif
 
 // A lane stores a block of 32 values: four 16-byte loads in flight, no exchange. Bound by
-// bytes: 16384 rows of 16 heads, D = 128, STOREUS us (STORETB TB/s); a lane per 8 values,
+// bytes: 16384 rows of 16 heads, D = 128, 34 us (5.0 TB/s); a lane per 8 values,
 // with the block's maximum exchanged between four, takes 45. grid.y: K, V.
 template <class T>
 __global__ void __launch_bounds__(256) store_kernel(const RowArgs a) {
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(256) store_kernel(const RowArgs a) {
 #endif
 }
 
-// Rows back: a lane per 8 values, so that a wave's 16-byte stores are contiguous; LOADUS us
+// Rows back: a lane per 8 values, so that a wave's 16-byte stores are contiguous; 35 us
 // for as many rows, and 45 with a lane per 32 values.
 template <class T>
 __global__ void __launch_bounds__(256) load_kernel(const RowArgs a) {
@@ -427,7 +427,7 @@ struct Codes {
 // of 16 NB query rows: a token's G heads share the keys). The lengths lie on the GPU, so
 // every workgroup adds up all requests' units and takes an equal run of them, which may
 // end inside a head and span several: a ragged batch fills the GPU as an even one does.
-// Within a run the four waves take every fourth unit of a head, each with its own
+// Within a run the eight waves take every eighth unit of a head, each with its own
 // running max and sums, and are merged through LDS. A head that lies in one run is
 // finished there; of others each run writes unnormalised O and (m, l) to a slot of the
 // workspace (2 w + 1 of workgroup w for the run that begins the head, 2 w for the
@@ -441,13 +441,12 @@ struct Codes {
 // one are done, its V codes at the end, so that neither needs registers twice.
 //
 // DIRECT: short tables. One workgroup a head, no runs, no slots and no second kernel.
-template <int D, class T, int NB, int NW, bool DIRECT>
-__global__ void __launch_bounds__(64 * NW, NB == 2 ? 2 : D == 128 ? 3 : 4)
-attn_few_kernel(const AttnArgs a) {
+template <int D, class T, int NB, bool DIRECT>
+__global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using W = Tile<D, T, NB>;
     using x8 = typename W::x8;
-    constexpr int R = 16 * NB, DW = D / 32, NT = 64 * NW;
+    constexpr int R = 16 * NB, DW = D / 32, NW = 8, NT = 64 * NW;
     __shared__ __attribute__((aligned(1024))) char stage[NW][W::BYTES];
     __shared__ float ml_s[NW][R][2];
     __shared__ int run0[NT + 1];
@@ -1230,11 +1229,19 @@ int check_cache(int Hkv, int D, int pages, int page, const void* kc, const void*
 }
 
 // How attn_few_kernel is launched.
-constexpr int kFewRows = 64, kMinUnits = 4, kStartUnits = 8;
-// Tables of up to so many tokens go to the DIRECT form.
-constexpr int kDirectTokens = 2048;
+// Requests of up to so many query rows a kv head go to attn_few_kernel, in tiles of 32 that
+// read the cache again, the others to the prompt kernels. One request behind 16384 tokens, 8 kv
+// heads, us here / there: 128 rows 32 / 70, 256 42 / 69, 384 53 / 71; 8 requests behind 4096,
+// 4 kv heads: 256 rows 44 / 58, 384 76 / 64.
+constexpr int kFewRows = 256, kGroups = 256, kMinUnits = 8;
+// Tables of up to so many tokens go to the DIRECT form, and twice as many where there are heads
+// enough for the GPU. One query each, 8 kv heads, us DIRECT / in runs: 1 request of 1000 tokens
+// 8.5 / 13.4, of 2000 12.0 / 13.5, of 4000 19.5 / 13.8; 32 requests of 2000 16.3 / 24.2, of 4000
+// 25.9 / 30.2, of 100 .. 4000 20.5 / 20.7.
+constexpr int kDirectTokens = 2048, kDirectHeads = 256;
 struct FewPlan {
     int nb, tiles, groups;
+    int start;          // units that a head's start counts
     bool direct, many;  // many: heads lie in 32 runs or more, if all requests are as long
     long long units;
     size_t o_off, ml_off, bytes;  // of the workspace
@@ -1245,12 +1252,16 @@ FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len) {
     p.nb = rows > 16 ? 2 : 1;
     p.tiles = (int)((rows + 16 * p.nb - 1) / (16 * p.nb));
     const long long segs = (long long)B * Hkv * p.tiles;
-    p.units = segs * ((std::max(max_len, 1) + 63LL) / 64 + kStartUnits);
-    p.direct = max_len <= kDirectTokens && segs < (1LL << 31);
+    // (a unit of 32 rows takes about as long as two of 16. 32 requests of 100 .. 16384 tokens,
+    // one query each: 36.1 us with 8 units, 28.8 with 16, 30.5 with 24; 131072 tokens with 32
+    // rows: 22.5 with 8, 24.0 with 16)
+    p.start = p.nb == 1 ? 16 : 8;
+    p.units = segs * ((std::max(max_len, 1) + 63LL) / 64 + p.start);
+    p.direct = max_len <= (segs >= kDirectHeads ? 2 : 1) * kDirectTokens && segs < (1LL << 31);
     if (p.direct) return p;
-    // As many workgroups as the GPU holds at once, with a unit a wave at least.
-    const int most = p.nb == 2 ? 256 : D == 128 ? 768 : 1024;
-    p.groups = (int)std::max(1LL, std::min<long long>(most, p.units / (kMinUnits + kStartUnits) + 1));
+    // A workgroup a CU, with a unit a wave at least. (Three of four waves, with 8 units for a
+    // start: 32 ragged requests 29.3 us and not 28.8, 32 of 4000 tokens 33.5 and not 30.)
+    p.groups = (int)std::max(1LL, std::min<long long>(kGroups, p.units / (kMinUnits + p.start) + 1));
     p.many = p.groups / segs >= 32;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.o_off = up((size_t)(B + 1) * sizeof(int));
@@ -1442,8 +1453,8 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     a.qsign = scale < 0.f ? -1.f : 1.f;
     a.few_rows = kFewRows;
     a.groups = plan.groups;
-    a.min_units = kMinUnits + kStartUnits;
-    a.start_units = kStartUnits;
+    a.min_units = kMinUnits + plan.start;
+    a.start_units = plan.start;
     a.tiles = plan.tiles;
     a.starts = (int*)workspace;
     a.ws_o = (float*)((char*)workspace + plan.o_off);
@@ -1466,22 +1477,22 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
         auto direct = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)(B * Hkv * plan.tiles)), dim3(512), 0, stream, a);
         };
-        auto runs = [&](auto kernel, int threads, auto combine, auto combine_many) {
-            hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(threads), 0, stream, a);
+        auto runs = [&](auto kernel, auto combine, auto combine_many) {
+            hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(512), 0, stream, a);
             if (plan.many)
                 hipLaunchKernelGGL(combine_many, cgrid, dim3(1024), 0, stream, a);
             else
                 hipLaunchKernelGGL(combine, cgrid, dim3(256), 0, stream, a);
         };
         if (plan.direct && plan.nb == 1)
-            direct(attn_few_kernel<kD, E, 1, 8, true>);
+            direct(attn_few_kernel<kD, E, 1, true>);
         else if (plan.direct)
-            direct(attn_few_kernel<kD, E, 2, 8, true>);
+            direct(attn_few_kernel<kD, E, 2, true>);
         else if (plan.nb == 1)
-            runs(attn_few_kernel<kD, E, 1, 4, false>, 256, few_combine_kernel<kD, E, 1, 256>,
+            runs(attn_few_kernel<kD, E, 1, false>, few_combine_kernel<kD, E, 1, 256>,
                  few_combine_kernel<kD, E, 1, 1024>);
         else
-            runs(attn_few_kernel<kD, E, 2, 8, false>, 512, few_combine_kernel<kD, E, 2, 256>,
+            runs(attn_few_kernel<kD, E, 2, false>, few_combine_kernel<kD, E, 2, 256>,
                  few_combine_kernel<kD, E, 2, 1024>);
         if (pp.used) {
             hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(1024), 0, stream, a);

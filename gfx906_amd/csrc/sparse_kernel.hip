@@ -306,10 +306,10 @@ __device__ __forceinline__ double lanes_sum(double x) {
 }
 #endif
 
-// The choice for one query block of every head straight from its rows (single tokens): mean,
-// scores and choice in one workgroup, of up to 4096 key blocks, instead of three kernels
-// whose launches outweigh the work. D/8 lanes take a row (of q or of the means) and add up
-// their parts. 64 heads of one query, 512 blocks: ONEUS us, and 19 in three kernels.
+// The choice straight from the query rows: mean, scores and choice of a query block in one
+// workgroup, of up to 4096 key blocks, where the launches of three kernels outweigh that every
+// block reads all key means (one_kernel below). D/8 lanes take a row (of q or of the means)
+// and add up their parts. 64 heads of one query, 512 blocks: 12.4 us, and 19 in three kernels.
 template <int D, class T>
 __global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -319,12 +319,13 @@ __global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
     __shared__ float qs[D];
     __shared__ int part[2][8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x, b = row / a.Hq, h = row - b * a.Hq;
+    const int bh = blockIdx.x / a.nq, i = blockIdx.x - bh * a.nq, b = bh / a.Hq, h = bh - b * a.Hq;
     const int kvh = b * a.Hkv + h / (a.Hq / a.Hkv);
     const int c = tid % LPR, r0 = tid / LPR;
+    const int rows = min(kQBlock, a.Sq - i * kQBlock);
     double sum[8] = {};
-    const T* q = (const T*)a.q + b * a.qb + h * a.qh + c * 8;
-    for (int r = r0; r < a.Sq; r += ROWS) {
+    const T* q = (const T*)a.q + b * a.qb + h * a.qh + (long long)i * kQBlock * a.qs + c * 8;
+    for (int r = r0; r < rows; r += ROWS) {
         const typename Elem<T>::x8 x = *reinterpret_cast<const typename Elem<T>::x8*>(q + r * a.qs);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += (double)(float)x[e];
@@ -341,13 +342,13 @@ __global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
         double s = 0.0;
 #pragma unroll
         for (int w = 0; w < 8; ++w) s += part_q[w][tid];
-        qs[tid] = (float)(s / a.Sq);
+        qs[tid] = (float)(s / rows);
     }
     __syncthreads();
     double qd[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) qd[e] = qs[8 * c + e];
-    const Reach r = reach(0, a.Sq, a.Skv, a.block, a.nk, a.causal);
+    const Reach r = reach(i, a.Sq, a.Skv, a.block, a.nk, a.causal);
     const float* km = a.km + (long long)kvh * a.nk * D + c * 8;
     constexpr int U = 8;
     for (int j0 = r0; j0 < r.seen; j0 += U * ROWS) {
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
         }
     }
     __syncthreads();
-    int* out = a.index + (long long)row * a.count;
+    int* out = a.index + (long long)blockIdx.x * a.count;
     auto at = [&](int j) { return score[j]; };
     if (a.nk <= 512) {  // one wave: no exchange between waves in a step
         if (wave == 0) choose<1, 8>(a, r, at, out, (int(*)[1])part);
@@ -782,12 +783,13 @@ int check_sizes(int B, int H, int S, int D, int block, const char* who) {
 
 int blocks_of(int S, int block) { return (S + block - 1) / block; }
 
-// Ranges the lists are split in: enough for two workgroups a CU, of 4 tiles or more.
+// Ranges the lists are split in: enough for two workgroups a CU, of 8 tiles or more (a tile takes
+// about 0.65 us, the merge 5).
 int split_count(int B, int Hq, int Sq, int Skv, int block, int count) {
     const long long units = (long long)B * Hq * blocks_of(Sq, kQBlock);
     const int entries = std::min(count, blocks_of(Skv, block));
     if (units >= 256 || entries <= 1) return 1;
-    const int most = std::max(1, entries * (block / 32) / 4);
+    const int most = std::max(1, entries * (block / 32) / 8);
     return (int)std::min<long long>(most, 512 / units);
 }
 
@@ -920,15 +922,23 @@ extern "C" int sparse_select(const float* q_means, const float* k_means, int B, 
 }
 
 namespace {
-// Whether a choice is choose_one_kernel's.
-bool one_block(int Sq, int Skv, int block) { return Sq <= kQBlock && blocks_of(Skv, block) <= 4096; }
+// Whether a choice is choose_one_kernel's: its workgroups together read at most so many bytes
+// of key means (640 query blocks of 79 key blocks, D = 128, 26 MB: the whole call takes 87.5 us in
+// one kernel and 87.2 in three; 2048 of 256, 268 MB: 45 against 31 for the choice alone).
+constexpr double kOneBytes = 2.0e7;
+bool one_kernel(int B, int Hq, int Sq, int Skv, int D, int block) {
+    const double nk = blocks_of(Skv, block);
+    return nk <= 4096 && (double)B * Hq * blocks_of(Sq, kQBlock) * nk * D * 4 <= kOneBytes;
+}
 size_t means_bytes(int B, int Hq, int Sq, int D) {
     return ((size_t)B * Hq * blocks_of(Sq, kQBlock) * D * sizeof(float) + 255) & ~(size_t)255;
 }
 }  // namespace
 
 extern "C" size_t sparse_choose_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block) {
-    if (B <= 0 || Hq <= 0 || Sq <= 0 || D <= 0 || block <= 0 || one_block(Sq, Skv, block)) return 0;
+    if (B <= 0 || Hq <= 0 || Sq <= 0 || D <= 0 || block <= 0 ||
+        one_kernel(B, Hq, Sq, Skv, D, block))
+        return 0;
     return means_bytes(B, Hq, Sq, D) + sparse_select_workspace_bytes(B, Hq, Sq, Skv, block);
 }
 
@@ -949,7 +959,7 @@ extern "C" int sparse_choose(const void* q, const long long* q_strides, int dtyp
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return g_err.fail("sparse_choose: workspace misaligned or smaller than "
                           "sparse_choose_workspace_bytes()");
-    if (!one_block(Sq, Skv, block)) {
+    if (!one_kernel(B, Hq, Sq, Skv, D, block)) {
         float* means = (float*)workspace;
         const size_t used = means_bytes(B, Hq, Sq, D);
         const int rc =
@@ -965,7 +975,7 @@ extern "C" int sparse_choose(const void* q, const long long* q_strides, int dtyp
     a.qh = q_strides[1];
     a.qs = q_strides[2];
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(B * Hq), dim3(512), 0, stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(512), 0, stream, a);
     };
     if (dtype == SPARSE_DTYPE_F16)
         D == 64 ? go(choose_one_kernel<64, f16>) : go(choose_one_kernel<128, f16>);

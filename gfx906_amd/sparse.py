@@ -40,8 +40,7 @@ def select(q_means, k_means, count, q_len, k_len, block=64, causal=False):
 
 
 def choose(q, k_means, count, k_len, block=64, causal=False):
-    """``select`` for the query rows themselves, whose block means are taken on the way (up
-    to 128 rows and 4096 key blocks in one kernel)."""
+    """``select`` for the query rows themselves, whose block means are taken on the way."""
     return extension().sparse_choose(q, k_means, count, k_len, block, causal)
 
 

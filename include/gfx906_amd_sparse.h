@@ -44,8 +44,7 @@ int sparse_select(const float* q_means, const float* k_means, int B, int Hq, int
 
 /* The same from the query rows q [B, Hq, Sq, D] themselves (16-byte aligned), whose means
  * over 128 rows are taken as sparse_block_means does. workspace:
- * sparse_choose_workspace_bytes() bytes (0 for up to 128 rows and 4096 key blocks, which
- * take one kernel). */
+ * sparse_choose_workspace_bytes() bytes (0 for few query blocks, which take one kernel). */
 size_t sparse_choose_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block);
 int sparse_choose(const void* q, const long long* q_strides, int dtype, const float* k_means, int B,
                   int Hq, int Hkv, int Sq, int Skv, int D, int block, int count, int causal,

@@ -154,7 +154,8 @@ def test_select_refuses(lib, bad, word):
 
 @pytest.mark.parametrize("bad,word", [
     (dict(dtype=2), b"dtype"), (dict(qs=None), b"null"), (dict(qs=strides(9, 8, 8)), b"multiples"),
-    (dict(q=FAKE + 4), b"aligned"), (dict(km=FAKE + 8), b"aligned"), (dict(n=15), b"workspace"),
+    (dict(q=FAKE + 4), b"aligned"), (dict(km=FAKE + 8), b"aligned"),
+    (dict(n=15, Sq=300000, Skv=300000), b"workspace"),
     (dict(causal=1, count=2), b"own positions"), (dict(Hkv=3), b"multiple of kv heads")])
 def test_choose_refuses(lib, bad, word):
     lib.sparse_choose.argtypes = [P, ctypes.POINTER(L), I, P] + [I] * 9 + [P, P, Z, P]

@@ -106,9 +106,10 @@ def test_choice_among_equal_and_special_scores(count):
     (1, 4, 1, 128, 9000, 64, 128, 5, True), (1, 2, 2, 77, 50, 128, 64, 4, True),
     (1, 2, 1, 100, 70000, 64, 64, 300, False), (1, 1, 1, 3, 262144, 64, 64, 7, True),
     (1, 1, 1, 3, 262145, 64, 64, 7, True), (2, 2, 1, 129, 3000, 128, 64, 9, True),
-    (1, 2, 2, 500, 0, 64, 64, 3, False), (1, 2, 2, 5, 0, 64, 64, 3, True)])
+    (1, 2, 2, 500, 0, 64, 64, 3, False), (1, 2, 2, 5, 0, 64, 64, 3, True),
+    (1, 4, 2, 6000, 6000, 64, 128, 9, True), (1, 1, 1, 40000, 70000, 128, 64, 5, False)])
 def test_choice_from_rows(B, Hq, Hkv, Sq, Skv, D, block, count, causal, dtype):
-    """One kernel or several (above 128 rows or 4096 blocks), with equal scores among them."""
+    """In one kernel and in several, with equal scores among them."""
     q = rand(B, Sq, Hq, D, seed=Sq, dtype=dtype).transpose(1, 2)
     nk = -(-Skv // block)
     km = torch.randn(B, Hkv, nk, D, generator=torch.Generator().manual_seed(nk))
