@@ -307,6 +307,7 @@ struct AttnArgs {
     int p_groups, p_tiles;  // p_tiles: room for so many tiles
     int* p_first;         // [B + 1]: first tile of every request
     long long* p_cost;    // [tiles + 1]: units before a tile, of one kv head
+    int* p_req;           // [tiles]: request of a tile
     float* p_o;
     float* p_ml;
 };
@@ -441,6 +442,11 @@ struct Codes {
 // one are done, its V codes at the end, so that neither needs registers twice.
 //
 // DIRECT: short tables. One workgroup a head, no runs, no slots and no second kernel.
+//
+// 32 requests of 100 .. 16384 tokens, 8 kv heads of 128, one query each: 23 us and 5 for the
+// merge (103 MB: 3.6 TB/s in all); 131072 tokens, 2 kv heads, 32 rows: 17 and 6 (what is left above
+// the bytes' 7 us is two units' latency a wave, and the merge); 1024 tokens, 16 heads of 64, in
+// DIRECT: 7.
 template <int D, class T, int NB, bool DIRECT>
 __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -820,7 +826,11 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 
 // -- prompts: requests of more than few_rows query rows a kv head -----------------------
 
+// A run is at least kPromptRun units: two prompts of 200 queries behind 800 tokens, 16/4 heads, 30
+// us with 5, 37 with 8, 53 with 16.
 constexpr int kTileRows = 128, kPromptStart = 4;
+constexpr long long kPromptRun = kPromptStart + 1;
+constexpr int kSelfTiles = 1024, kSelfRequests = 256;  // SELF (attn_prompt_kernel)
 
 #if defined(__HIP_DEVICE_COMPILE__)
 // Row tiles of a request, and the 64-key chunks that tile rt reads.
@@ -885,7 +895,10 @@ __global__ void __launch_bounds__(1024) prompt_plan_kernel(const AttnArgs a) {
         Request r = request(a, x);
         for (int i = i0; i < i1; ++i) {
             while (i >= first[x + 1]) r = request(a, ++x);
-            if (pass) a.p_cost[i] = sum;
+            if (pass) {
+                a.p_cost[i] = sum;
+                a.p_req[i] = x;
+            }
             const int c = tile_chunks(a, r, i - first[x]);
             sum += c ? c + kPromptStart : 0;
         }
@@ -914,7 +927,14 @@ __global__ void __launch_bounds__(1024) prompt_plan_kernel(const AttnArgs a) {
 // product of the next but one around the softmax of the block between, one barrier a chunk.
 // K and V have two buffers each: after the barrier of chunk w those of K(w) and V(w-1) are
 // free for K(w+2) and V(w+1).
-template <int D, class T>
+//
+// 3 prompts of 77 .. 2111 queries behind 300 .. 8192 tokens, 16/4 heads of 128: 203 us (173
+// GFLOP: 850 TFLOP/s; a library product of 8192 reaches 1180), bound as attn_tile_kernel is.
+// Small batches are bound by a run's start: two tiles' loads and merges, 20 us.
+//
+// SELF: few tiles. Every workgroup adds up the tiles itself, as in attn_few_kernel, instead
+// of a kernel before this one.
+template <int D, class T, bool SELF>
 __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using W = Tile<D, T>;
@@ -929,9 +949,71 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
-    const int ntile = uni(a.p_first[a.B]);
-    const long long all = a.p_cost[ntile] * a.c.Hkv;
-    const long long per = max(4LL + kPromptStart, (all + a.p_groups - 1) / a.p_groups);
+    __shared__ int first_s[SELF ? kSelfRequests + 1 : 1];
+    __shared__ long long cost_s[SELF ? kSelfTiles + 1 : 1], sum_s[4];
+    auto p_first = [&](int x) { return SELF ? first_s[x] : a.p_first[x]; };
+    auto p_cost = [&](int x) { return SELF ? cost_s[x] : a.p_cost[x]; };
+    if constexpr (SELF) {
+        auto scan = [&](long long x) {  // inclusive, over the workgroup
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const long long y = __shfl_up(x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 63) sum_s[wave] = x;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) x += sum_s[w];
+            return x;
+        };
+        const long long n = scan(tid < a.B ? tiles_of(a, request(a, tid)) : 0);
+        first_s[tid + 1] = (int)min(n, (long long)a.p_tiles);
+        if (tid == 0) first_s[0] = 0;
+        __syncthreads();
+        const int nt = first_s[a.B];
+        constexpr int PER = kSelfTiles / 256;
+        long long c[PER], sum = 0;
+        int req[PER];
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int t = tid * PER + n;
+            c[n] = req[n] = 0;
+            if (t >= nt) continue;
+            int lo = 0;
+            for (int hi = a.B - 1; lo < hi;) {
+                const int mid = (lo + hi + 1) / 2;
+                if (first_s[mid] <= t)
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            const int chunks = tile_chunks(a, request(a, lo), t - first_s[lo]);
+            req[n] = lo;
+            c[n] = chunks ? chunks + kPromptStart : 0;
+            sum += c[n];
+        }
+        long long at = scan(sum) - sum;
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int t = tid * PER + n;
+            if (t < nt) cost_s[t] = at;
+            if (blockIdx.x == 0 && t < nt) {
+                a.p_cost[t] = at;
+                a.p_req[t] = req[n];
+            }
+            at += c[n];
+        }
+        if (tid == 255) cost_s[nt] = at;
+        if (blockIdx.x == 0) {
+            if (tid <= a.B) a.p_first[tid] = first_s[tid];
+            if (tid == 0 && a.B == 256) a.p_first[256] = first_s[256];
+            if (tid == 255) a.p_cost[nt] = at;
+        }
+        __syncthreads();
+    }
+    const int ntile = uni(p_first(a.B));
+    const long long all = p_cost(ntile) * a.c.Hkv;
+    const long long per = max(kPromptRun, (all + a.p_groups - 1) / a.p_groups);
     const int wg = (gridDim.x & 7) == 0 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)
                                         : blockIdx.x;  // (consecutive runs on one XCD)
     long long u0 = wg * per;
@@ -939,18 +1021,17 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
     if (u0 >= hi) return;
     // The request, kv head and tile of unit u0.
     for (int x = tid; x < a.B; x += 256)
-        if (a.p_cost[a.p_first[x]] * a.c.Hkv <= u0 && u0 < a.p_cost[a.p_first[x + 1]] * a.c.Hkv)
-            found = x;
+        if (p_cost(p_first(x)) * a.c.Hkv <= u0 && u0 < p_cost(p_first(x + 1)) * a.c.Hkv) found = x;
     __syncthreads();
     int b = uni(found);
-    int t0 = uni(a.p_first[b]), t1 = uni(a.p_first[b + 1]);
-    long long base = a.p_cost[t0], each = a.p_cost[t1] - base;
+    int t0 = uni(p_first(b)), t1 = uni(p_first(b + 1));
+    long long base = p_cost(t0), each = p_cost(t1) - base;
     int hk = uni((int)((u0 - base * a.c.Hkv) / each));
     {
         const long long at = u0 - base * a.c.Hkv - hk * each;
         __syncthreads();
         for (int x = t0 + tid; x < t1; x += 256)
-            if (a.p_cost[x] - base <= at && at < a.p_cost[x + 1] - base) found = x;
+            if (p_cost(x) - base <= at && at < p_cost(x + 1) - base) found = x;
         __syncthreads();
     }
     int tile = uni(found);
@@ -969,24 +1050,24 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
     }
 
     while (u0 < hi) {
-        while (u0 >= (base + 0) * a.c.Hkv + hk * each + (a.p_cost[tile + 1] - base)) {
+        while (u0 >= base * a.c.Hkv + hk * each + (p_cost(tile + 1) - base)) {
             if (++tile < t1) continue;  // (tiles without keys have no units)
             tile = t0;
             if (++hk < a.c.Hkv) continue;
             do {
                 ++b;
                 t0 = t1;
-                t1 = uni(a.p_first[b + 1]);
-            } while (t0 == t1 || a.p_cost[t1] == a.p_cost[t0]);
-            base = a.p_cost[t0];
-            each = a.p_cost[t1] - base;
+                t1 = uni(p_first(b + 1));
+            } while (t0 == t1 || p_cost(t1) == p_cost(t0));
+            base = p_cost(t0);
+            each = p_cost(t1) - base;
             hk = 0;
             tile = t0;
         }
         const Request req = request(a, b);
         const int rt = tile - t0;
         const int end = uni(tile_end(a, req, rt)), chunks = (end + 63) / 64;
-        const long long s = base * a.c.Hkv + hk * each + (a.p_cost[tile] - base);
+        const long long s = base * a.c.Hkv + hk * each + (p_cost(tile) - base);
         const int p0 = uni((int)(u0 - s)), p1 = uni((int)min((long long)chunks + kPromptStart, hi - s));
         u0 = s + p1;
         const int c0 = max(0, p0 - kPromptStart), c1 = p1 - kPromptStart;
@@ -1025,20 +1106,24 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             return ((long long)p * a.c.Hkv + hk) * a.c.page + (min(c, c1 - 1) & ((1 << shift) - 1)) * 64;
         };
         // Codes of chunks kc (K) and vc (V), on their way to LDS.
-        u32x4 kw, vw;
-        unsigned ke, ve;
+        struct Raw {
+            u32x4 kw, vw;
+            unsigned ke, ve;
+        };
         auto load = [&](int kc, int kpage, int vc, int vpage) __attribute__((always_inline)) {
+            Raw r{};
             const long long kr = row_of(kc, kpage), vr = row_of(vc, vpage);
             if constexpr (D == 128) {
-                kw = *reinterpret_cast<const u32x4*>(a.c.kc + kr * (D / 2) + coff);
-                ke = a.c.ks[kr / 4 * (D / 8) + csoff];
-                vw = *reinterpret_cast<const u32x4*>(a.c.vc + vr * (D / 2) + coff);
-                ve = a.c.vs[vr / 4 * (D / 8) + csoff];
+                r.kw = *reinterpret_cast<const u32x4*>(a.c.kc + kr * (D / 2) + coff);
+                r.ke = a.c.ks[kr / 4 * (D / 8) + csoff];
+                r.vw = *reinterpret_cast<const u32x4*>(a.c.vc + vr * (D / 2) + coff);
+                r.ve = a.c.vs[vr / 4 * (D / 8) + csoff];
             } else {
-                const long long r = d64v ? vr : kr;
-                kw = *reinterpret_cast<const u32x4*>((d64v ? a.c.vc : a.c.kc) + r * (D / 2) + coff);
-                ke = (d64v ? a.c.vs : a.c.ks)[r / 4 * (D / 8) + csoff];
+                const long long row = d64v ? vr : kr;
+                r.kw = *reinterpret_cast<const u32x4*>((d64v ? a.c.vc : a.c.kc) + row * (D / 2) + coff);
+                r.ke = (d64v ? a.c.vs : a.c.ks)[row / 4 * (D / 8) + csoff];
             }
+            return r;
         };
         auto put = [&](char* dst, const int (&at)[4], u32x4 x, unsigned e)
             __attribute__((always_inline)) {
@@ -1054,16 +1139,16 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
                 e = 127;
             }
         };
-        auto store = [&](char* kd, char* vd, int vc, int vpage) __attribute__((always_inline)) {
+        auto store = [&](char* kd, char* vd, int vc, int vpage, Raw& r) __attribute__((always_inline)) {
             if constexpr (D == 128) {
-                put(kd, kst, kw, ke);
-                clear(vw, ve, vc, vpage);
-                put(vd, vst, vw, ve);
+                put(kd, kst, r.kw, r.ke);
+                clear(r.vw, r.ve, vc, vpage);
+                put(vd, vst, r.vw, r.ve);
             } else if (!d64v) {
-                put(kd, kst, kw, ke);
+                put(kd, kst, r.kw, r.ke);
             } else {
-                clear(kw, ke, vc, vpage);
-                put(vd, vst, kw, ke);
+                clear(r.kw, r.ke, vc, vpage);
+                put(vd, vst, r.kw, r.ke);
             }
         };
         auto mask = [&](f32x4 (&S)[2][2], int c, int page, int half) __attribute__((always_inline)) {
@@ -1082,11 +1167,10 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         Pb[1] = x8{};
         int g0 = page_of(c0), g1 = page_of(c0 + 1), g2 = page_of(c0 + 2), g3 = page_of(c0 + 3);
         __syncthreads();  // (the tile before: every wave is done with LDS)
-        load(c0, g0, c0, g0);
-        store(ka, va, c0, g0);
-        load(c0 + 1, g1, c0, g0);
-        if (D == 128 || !d64v) put(kb, kst, kw, ke);
-        load(c0 + 2, g2, c0 + 1, g1);
+        Raw raw0 = load(c0, g0, c0, g0), raw1 = load(c0 + 1, g1, c0, g0);
+        Raw raw = load(c0 + 2, g2, c0 + 1, g1);
+        store(ka, va, c0, g0, raw0);
+        if (D == 128 || !d64v) put(kb, kst, raw1.kw, raw1.ke);
         for (int z = tid; z < BYTES / 16; z += 256) *reinterpret_cast<u32x4*>(vb + 16 * z) = u32x4{};
         __syncthreads();
         if (active) w.qk(ka, Sa);
@@ -1099,8 +1183,8 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             }
             lds_barrier();
             // V(c+1) goes where V(c-1) was, K(c+2) where K(c) was.
-            store(kc, const_cast<char*>(vp), c + 1, g1);
-            load(c + 3, g3, c + 2, g2);
+            store(kc, const_cast<char*>(vp), c + 1, g1, raw);
+            raw = load(c + 3, g3, c + 2, g2);
             if (active) {
                 mask(Sb, c, g0, 1);
                 w.turn(vc, Pa, kn, Sa, Sb, Pb, a.scale);
@@ -1151,15 +1235,12 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
 template <int D, class T>
 __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ int found;
     constexpr int ROWS = 16;
     const int tile = blockIdx.x / (kTileRows / ROWS), hk = blockIdx.y, tid = threadIdx.x;
     const int r0 = blockIdx.x % (kTileRows / ROWS) * ROWS;
+    const int b = a.p_req[tile];
     if (tile >= a.p_first[a.B]) return;
-    for (int x = tid; x < a.B; x += 256)
-        if (a.p_first[x] <= tile && tile < a.p_first[x + 1]) found = x;
-    __syncthreads();
-    const int b = found, t0 = a.p_first[b], t1 = a.p_first[b + 1], rt = tile - t0;
+    const int t0 = a.p_first[b], t1 = a.p_first[b + 1], rt = tile - t0;
     const Request req = request(a, b);
     const int rows = (int)min(r0 + (long long)ROWS, (long long)req.m * a.G - (long long)rt * kTileRows);
     if (r0 >= rows) return;
@@ -1171,7 +1252,7 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
     int w0 = 0, w1 = 0;
     if (chunks) {
         const long long all = a.p_cost[a.p_first[a.B]] * a.c.Hkv;
-        const long long per = max(4LL + kPromptStart, (all + a.p_groups - 1) / a.p_groups);
+        const long long per = max(kPromptRun, (all + a.p_groups - 1) / a.p_groups);
         const long long base = a.p_cost[t0], each = a.p_cost[t1] - base;
         const long long s = base * a.c.Hkv + hk * each + (a.p_cost[tile] - base) + kPromptStart;
         w0 = (int)(s / per);
@@ -1182,15 +1263,27 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
             const int r = r0 + e / (D / 4), d = e % (D / 4) * 4, tok = tok_of(r);
             float m = kNoMax, l = 0.f;
             f32x4 acc = {};
-            for (int y = w0; chunks && y <= w1; ++y) {
-                const long long at = (2LL * y + (y == w0 ? 1 : 0)) * kTileRows + r;
-                const f32x2 ml = *reinterpret_cast<const f32x2*>(a.p_ml + at * 2);
-                const f32x4 p = *reinterpret_cast<const f32x4*>(a.p_o + at * D + d);
-                const float mn = max2(m, ml[0]);
-                const float f = __builtin_amdgcn_exp2f(m - mn), x = __builtin_amdgcn_exp2f(ml[0] - mn);
-                acc = acc * f + p * x;
-                l = l * f + ml[1] * x;
-                m = mn;
+            constexpr int U = 4;
+            for (int x = w0; chunks && x <= w1; x += U) {
+                f32x2 ml[U];
+                f32x4 p[U];
+#pragma unroll
+                for (int n = 0; n < U; ++n) {
+                    const int y = min(x + n, w1);
+                    const long long at = (2LL * y + (y == w0 ? 1 : 0)) * kTileRows + r;
+                    ml[n] = *reinterpret_cast<const f32x2*>(a.p_ml + at * 2);
+                    p[n] = *reinterpret_cast<const f32x4*>(a.p_o + at * D + d);
+                }
+#pragma unroll
+                for (int n = 0; n < U; ++n) {
+                    if (x + n > w1) continue;
+                    const float mn = max2(m, ml[n][0]);
+                    const float f = __builtin_amdgcn_exp2f(m - mn);
+                    const float e = __builtin_amdgcn_exp2f(ml[n][0] - mn);
+                    acc = acc * f + p[n] * e;
+                    l = l * f + ml[n][1] * e;
+                    m = mn;
+                }
             }
             acc *= l != 0.f ? 1.f / l : 0.f;
             T* o = (T*)a.o + (req.first + tok) * a.ot + head_of(r, tok) * a.oh + d;
@@ -1275,7 +1368,8 @@ FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len) {
 struct PromptPlan {
     bool used;
     int groups, tiles;
-    size_t cost_off, o_off, ml_off, bytes;
+    bool self;
+    size_t cost_off, req_off, o_off, ml_off, bytes;
 };
 PromptPlan prompt_plan(int T, int B, int G, int D, int max_q, size_t after) {
     PromptPlan p{};
@@ -1285,7 +1379,9 @@ PromptPlan prompt_plan(int T, int B, int G, int D, int max_q, size_t after) {
     p.groups = 512;  // two a CU
     p.tiles = (int)std::min<long long>((long long)T * G / kTileRows + B, (1LL << 27));
     p.cost_off = up(after) + up((size_t)(B + 1) * sizeof(int));
-    p.o_off = p.cost_off + up((size_t)(p.tiles + 1) * sizeof(long long));
+    p.self = p.tiles <= kSelfTiles && B <= kSelfRequests;
+    p.req_off = p.cost_off + up((size_t)(p.tiles + 1) * sizeof(long long));
+    p.o_off = p.req_off + up((size_t)p.tiles * sizeof(int));
     p.ml_off = p.o_off + (size_t)2 * p.groups * kTileRows * D * sizeof(float);
     p.bytes = p.ml_off + (size_t)2 * p.groups * kTileRows * 2 * sizeof(float);
     return p;
@@ -1465,6 +1561,7 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
         a.p_tiles = pp.tiles;
         a.p_first = (int*)(ws + ((plan.bytes + 255) & ~(size_t)255));
         a.p_cost = (long long*)(ws + pp.cost_off);
+        a.p_req = (int*)(ws + pp.req_off);
         a.p_o = (float*)(ws + pp.o_off);
         a.p_ml = (float*)(ws + pp.ml_off);
     }
@@ -1495,8 +1592,14 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
             runs(attn_few_kernel<kD, E, 2, false>, few_combine_kernel<kD, E, 2, 256>,
                  few_combine_kernel<kD, E, 2, 1024>);
         if (pp.used) {
-            hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
-            hipLaunchKernelGGL((attn_prompt_kernel<kD, E>), dim3(pp.groups), dim3(256), 0, stream, a);
+            if (pp.self) {
+                hipLaunchKernelGGL((attn_prompt_kernel<kD, E, true>), dim3(pp.groups), dim3(256), 0,
+                                   stream, a);
+            } else {
+                hipLaunchKernelGGL(prompt_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
+                hipLaunchKernelGGL((attn_prompt_kernel<kD, E, false>), dim3(pp.groups), dim3(256), 0,
+                                   stream, a);
+            }
             hipLaunchKernelGGL((prompt_combine_kernel<kD, E>), dim3(pp.tiles * (kTileRows / 16), Hkv),
                                dim3(256), 0,
                                stream, a);

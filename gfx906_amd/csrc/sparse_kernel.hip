@@ -34,7 +34,8 @@ struct MeansArgs {
 
 // One wave per block of rows: a lane reads 16 bytes (8 dims) of a row, so that a load
 // takes 4 (D = 128) or 8 (D = 64) whole rows, 16 loads in flight; the lanes that hold
-// the same dims add up at the end. Bound by the bytes of x.
+// the same dims add up at the end. Bound by the bytes of x: 16 heads of 16384, D = 128, 14.5
+// us (4.6 TB/s).
 template <int D, class T>
 __global__ void __launch_bounds__(256) means_kernel(const MeansArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -112,6 +113,8 @@ __host__ __device__ inline Reach reach(int i, int Sq, int Skv, int block, int nk
 // through tiles of 16 key blocks. In step s of a tile lane group g supplies dim
 // g D/4 + s, so that a lane reads D/4 consecutive floats of its row.
 //
+// 8 heads, 1024 x 1024 blocks, D = 64: 35 us, for 67 MB of scores; 16 heads, 128 x 256, 9.5.
+//
 // grid: row tiles, kv heads of all batches, shares of the key tiles; 4 waves.
 template <int D>
 __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
@@ -164,7 +167,8 @@ __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
 // scores equal to it fill up in the order of their index. The upper 32 bits go first, by
 // themselves; the lower ones matter only among scores whose upper bits are the bound's.
 // Everything stays in registers; a step is a compare and a population count per 64 scores
-// (and, with several waves, an exchange through LDS).
+// (and, with several waves, an exchange through LDS). 8192 rows of 1024 scores: 41 us; 2048 of
+// 256: 7.5.
 #if defined(__HIP_DEVICE_COMPILE__)
 template <int WAVES, int K, class Score>
 __device__ __forceinline__ void choose(const SelectArgs& a, const Reach& r, Score score, int* out,
@@ -480,6 +484,12 @@ __device__ __forceinline__ int xcd_order(int w, int n) {
 // A tile with masked keys is checked for infinite and NaN values of V (which a weight of 0
 // would not keep out of the sums); where there are any the wave does its rows again by
 // attend_row.
+//
+// 16 heads of 16384 tokens, 32 blocks of 64, D = 128: 280 us (980 TFLOP/s; 311 and 885 once the
+// card has slowed down under load, where a library product of 8192 reaches 1130); 8 heads of
+// 131072, 64 blocks of 128, D = 64: 2.3 ms (955). Reads of LDS take 1024 of the matrix pipe's
+// 1088 clocks a pair of steps, as a fragment serves 32 rows, and loads into it 256 more: that and
+// the card's power bound it. Single queries are bound by the blocks' bytes (138 MB in 22 us).
 template <int D, class T, int TPB, bool FAR>
 __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)

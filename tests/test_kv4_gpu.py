@@ -283,6 +283,38 @@ def test_many_requests(wide):
     check(out, oc.cache_attn(q, host, 64, table, lens, 0.125))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_among_many_requests(dtype):
+    """Three hundred requests, four of them prompts (their tiles are summed up by a kernel of
+    its own), and the prompts by themselves."""
+    g = torch.Generator().manual_seed(2)
+    lens = [int(n) for n in torch.randint(0, 70, (300,), generator=g)]
+    news = [min(1, n) for n in lens]
+    for b, n in ((5, 400), (6, 130), (170, 700), (299, 257)):
+        lens[b], news[b] = n, max(129, n - 100)
+    cache, host, table = filled(lens, 64, 1, 64, dtype, seed=2)
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    q = torch.randn(cu[-1], 2, 64, generator=g).to(dtype)
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.125, cu_q=i32(cu),
+                   max_q=max(news))
+    check(out, oc.cache_attn(q, host, 64, table, lens, 0.125, cu))
+    rows = oc.cache_attn(q, host, 64, table, lens, 0.125, cu)
+    b = 170
+    alone = kv4.attn(q[cu[b]:cu[b + 1]].to(DEV), cache, table[b:b + 1].to(DEV), i32(lens[b:b + 1]),
+                     0.125, cu_q=i32([0, news[b]]), max_q=news[b])
+    check(alone, {r - cu[b]: rows[r] for r in range(cu[b], cu[b + 1])})
+
+
+@pytest.mark.parametrize("n", [255, 256, 257])
+def test_row_counts_around_the_prompt_kernels(n):
+    cache, host, table = filled([700], 64, 1, 128, torch.float16, seed=n)
+    q = torch.randn(n, 1, 128, generator=torch.Generator().manual_seed(n)).half()
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32([700]), 0.1, cu_q=i32([0, n]), max_q=n)
+    check(out, oc.cache_attn(q, host, 64, table, [700], 0.1, [0, n]))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
 def test_scales(scale):
     lens = [200, 3]
