@@ -39,9 +39,9 @@ struct Parts {
                         who, ": the cache must be contiguous uint8 tensors on one device");
         TORCH_CHECK(v.sizes() == k.sizes() && vs.sizes() == ks.sizes(), who,
                     ": key and value parts of the cache differ in shape");
-        TORCH_CHECK(k.size(0) < (1LL << 31) && k.size(1) < 65536 && k.size(2) <= 256 &&
-                        k.size(3) <= 256,
-                    who, ": cache too large");
+        TORCH_CHECK(k.size(0) < (1LL << 31) && k.size(1) > 0 && k.size(1) < 65536 &&
+                        k.size(2) > 0 && k.size(2) <= 256 && k.size(3) <= 256,
+                    who, ": cache too large, or without heads or tokens");
         pages = (int)k.size(0);
         Hkv = (int)k.size(1);
         page = (int)k.size(2);
@@ -85,8 +85,8 @@ std::vector<Tensor> kv4_plan_pages_op(Tensor lens, Tensor new_lens, Tensor table
                     table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) &&
                     (B <= 1 || table.stride(0) >= table.size(1)),
                 who, ": table must be int32 [B, W] with contiguous rows that do not overlap");
-    TORCH_CHECK(B <= KV4_MAX_REQUESTS && tokens >= 0 && tokens < (1LL << 31) &&
-                    table.size(1) < (1LL << 31) && free_pages.size(0) < (1LL << 31),
+    TORCH_CHECK(B <= KV4_MAX_REQUESTS && tokens >= 0 && tokens < (1LL << 31) && page > 0 &&
+                    page <= 256 && table.size(1) < (1LL << 31) && free_pages.size(0) < (1LL << 31),
                 who, ": sizes out of range");
     for (const Tensor* t : {&lens, &new_lens, &free_pages, &used}) at::assert_no_overlap(table, *t);
     const c10::DeviceGuard guard(dev);
@@ -160,8 +160,8 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
         TORCH_CHECK(T == B, who, ": without cu_q, one query a request");
     TORCH_CHECK(table.device() == dev && table.dtype() == torch::kInt && table.dim() == 2 &&
                     table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) &&
-                    (B <= 1 || table.stride(0) >= 0) && table.size(1) < (1LL << 31),
-                who, ": table must be int32 [B, W] with contiguous rows");
+                    (B <= 1 || table.stride(0) >= 0) && table.size(1) * c.page < (1LL << 31),
+                who, ": table must be int32 [B, W] with contiguous rows of fewer than 2^31 tokens");
     Tensor o;
     if (out.has_value()) {
         o = *out;

@@ -607,8 +607,10 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
             for (int t = 0; t < 4; ++t) vc[t].load(p + (off + t * 8 * D));
         };
         char* const st = stage[wave];
-        int c = c0 + wave, page = page_of(c), next = page_of(c + NW);
-        if (c < c1) {
+        int c = c0 + wave, page = -1, next = -1;
+        if (c < c1) {  // (a request without keys may have no table)
+            page = page_of(c);
+            next = page_of(c + NW);
             fetch_k(c, page);
             fetch_v(c, page);
         }
@@ -1321,7 +1323,6 @@ int check_cache(int Hkv, int D, int pages, int page, const void* kc, const void*
     return 0;
 }
 
-// How attn_few_kernel is launched.
 // Requests of up to so many query rows a kv head go to attn_few_kernel, in tiles of 32 that
 // read the cache again, the others to the prompt kernels. One request behind 16384 tokens, 8 kv
 // heads, us here / there: 128 rows 32 / 70, 256 42 / 69, 384 53 / 71; 8 requests behind 4096,
@@ -1332,6 +1333,7 @@ constexpr int kFewRows = 256, kGroups = 256, kMinUnits = 8;
 // 8.5 / 13.4, of 2000 12.0 / 13.5, of 4000 19.5 / 13.8; 32 requests of 2000 16.3 / 24.2, of 4000
 // 25.9 / 30.2, of 100 .. 4000 20.5 / 20.7.
 constexpr int kDirectTokens = 2048, kDirectHeads = 256;
+// How attn_few_kernel is launched.
 struct FewPlan {
     int nb, tiles, groups;
     int start;          // units that a head's start counts
@@ -1522,6 +1524,11 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     if (plan.units >= (1LL << 30)) return g_err.fail("kv4_attn: table too wide for so many heads");
     const PromptPlan pp = prompt_plan(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);
     const size_t need = pp.used ? pp.bytes : plan.bytes;
+    const long long heads = (long long)B * Hkv;
+    if (!(plan.direct ? launchable(heads * plan.tiles, 512)
+                      : launchable(heads, plan.many ? 1024 : 256)) ||
+        (pp.used && !launchable(pp.tiles * (long long)(kTileRows / 16), 256)))
+        return g_err.fail("kv4_attn: too many requests, heads or query rows for one call");
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return g_err.fail("kv4_attn: workspace misaligned or smaller than "
                           "kv4_attn_workspace_bytes()");
@@ -1566,13 +1573,12 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
         a.p_ml = (float*)(ws + pp.ml_off);
     }
     const long long rows = (long long)a.max_q * a.G;
-    const dim3 cgrid((unsigned)(B * Hkv), (unsigned)std::min<long long>(rows, kFewRows));
-    if ((long long)B * Hkv >= (1LL << 31)) return g_err.fail("kv4_attn: too many heads");
+    const dim3 cgrid((unsigned)heads, (unsigned)std::min<long long>(rows, kFewRows));
     auto go = [&](auto d, auto t) {
         constexpr int kD = decltype(d)::value;
         using E = decltype(t);
         auto direct = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(B * Hkv * plan.tiles)), dim3(512), 0, stream, a);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(heads * plan.tiles)), dim3(512), 0, stream, a);
         };
         auto runs = [&](auto kernel, auto combine, auto combine_many) {
             hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(512), 0, stream, a);

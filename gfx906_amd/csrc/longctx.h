@@ -90,6 +90,9 @@ struct LastError {
     const char* get() const { return text[0] ? text : nullptr; }
 };
 
+// Whether HIP launches so many workgroups (fewer than 2^32 threads in x).
+inline bool launchable(long long groups, int threads) { return groups < (1LL << 32) / threads; }
+
 inline bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
 // Whether rows of D elements at the strides s[0..n) over sizes e[0..n) lie apart:

@@ -827,7 +827,7 @@ extern "C" int sparse_block_means(const void* x, const long long* strides, int d
     const int nb = blocks_of(S, block);
     const long long blocks = (long long)B * H * nb;
     const MeansArgs a{x, strides[0], strides[1], strides[2], means, H, S, block, nb, blocks};
-    if ((blocks + 3) / 4 >= (1LL << 31)) return g_err.fail("sparse_block_means: too many blocks");
+    if (!launchable((blocks + 3) / 4, 256)) return g_err.fail("sparse_block_means: too many blocks");
     const dim3 grid((unsigned)((blocks + 3) / 4));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
     if (dtype == SPARSE_DTYPE_F16)
@@ -862,7 +862,7 @@ int check_choice(const void* q, const float* k_means, int B, int Hq, int Hkv, in
     if (causal && count < own)
         return g_err.fail("%s: count must be at least %d, the blocks that hold a query block's own "
                           "positions", who, own);
-    if ((long long)B * Hq * blocks_of(Sq, kQBlock) >= (1LL << 31))
+    if (!launchable((long long)B * Hq * blocks_of(Sq, kQBlock), 1024))
         return g_err.fail("%s: too many query blocks", who);
     return 0;
 }
@@ -1051,7 +1051,7 @@ extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
         a.ws_ml = a.ws_o + (size_t)a.nsplit * a.rows * D;
     }
     const long long grid = (long long)a.nq * B * Hq * a.nsplit;
-    if (grid >= (1LL << 31)) return g_err.fail("sparse_attn: too many query blocks");
+    if (!launchable(grid, 256)) return g_err.fail("sparse_attn: too many query blocks");
     auto go = [&](auto kernel, auto combine) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
         if (a.nsplit > 1)

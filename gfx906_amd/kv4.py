@@ -96,7 +96,8 @@ def attn(q, cache, table, lens, scale, cu_q=None, max_q=None, causal=True, out=N
     the request's last tokens and see none behind themselves. ``max_q``: at least the
     most queries of a request (queries past it are not computed); without it T is
     taken, and a decoding step pays for what it does not need. Rows outside
-    every request are left as they were (in a new tensor: unset). Rows that see no
+    every request are left as they were (in a new tensor: unset). ``out`` may be ``q``
+    itself and must not overlap the other arguments otherwise. Rows that see no
     key are 0; keys without a page weigh nothing."""
     if max_q is None:
         max_q = 1 if cu_q is None else q.shape[0]

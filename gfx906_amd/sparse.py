@@ -47,8 +47,9 @@ def choose(q, k_means, count, k_len, block=64, causal=False):
 def attn_blocks(q, k, v, scale, index, block=64, causal=False, out=None):
     """softmax(scale * q k^T) v over the keys of the blocks in ``index``
     (``[B, Hq, ceil(Sq/128), count]``, as ``select`` returns it), in a new tensor or
-    in ``out``. An entry that names no block, or is not above the valid entries before
-    it, is passed over; a row that sees no key is 0."""
+    in ``out`` (which may be ``q`` itself, and must not overlap ``k`` or ``v``). An entry
+    that names no block, or is not above the valid entries before it, is passed over; a
+    row that sees no key is 0."""
     return extension().sparse_attn(q, k, v, float(scale), index, block, causal, out)
 
 

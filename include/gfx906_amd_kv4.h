@@ -81,8 +81,9 @@ int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, const int* slot
  * nothing; cu_q is taken as clamped to 0 .. T. Rows outside every request, and queries
  * past the first max_q of one, are left as they were. q and o: strides {token, head} in
  * elements, head dim contiguous, q's rows 16-byte and o's 8-byte aligned; o's must
- * not overlap each other, q or the cache. workspace: 16-byte aligned, kv4_attn_workspace_bytes() bytes, with max_len
- * = W * page; its content is neither read before it is written nor kept. */
+ * not overlap each other, q or the cache. workspace: 16-byte aligned,
+ * kv4_attn_workspace_bytes() bytes, with max_len = W * page (and max_q = 1 where cu_q is
+ * NULL); its content is neither read before it is written nor kept. */
 size_t kv4_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q, int max_len);
 int kv4_attn(const void* q, void* o, const long long* q_strides, const long long* o_strides,
              int dtype, int T, int B, int Hq, int Hkv, int D, const void* k_codes,

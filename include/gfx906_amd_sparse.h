@@ -56,7 +56,8 @@ int sparse_choose(const void* q, const long long* q_strides, int dtype, const fl
  * valid entry before it, is passed over). causal as above. A row that sees no key,
  * or only such of score -inf, is 0; a key that a row does not see adds nothing to it, whatever
  * it holds. q, k, v: rows 16-byte aligned (k's and v's
- * apart, their strides at most 2^22); o: 8-byte, rows that do not overlap; o may be q.
+ * apart, their strides at most 2^22); o: 8-byte, rows that do not overlap each other, k, v or
+ * index; o may be q (the same rows).
  * workspace: 16-byte aligned, sparse_attn_workspace_bytes() bytes (may be 0). */
 size_t sparse_attn_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block, int count);
 int sparse_attn(const void* q, const void* k, const void* v, void* o, const long long* q_strides,

@@ -451,6 +451,33 @@ def test_attention_refuses():
         kv4.attn(x[:1], cache, table, n, 0.1, out=x.view(-1)[64:320].view(1, 4, 64))
 
 
+def test_caches_without_heads_and_sizes_past_an_int_are_refused():
+    q, n, table = torch.zeros(1, 4, 64, device=DEV).half(), i32([1]), i32([[0]])
+    none = kv4.new_cache(2, 64, 0, 64)
+    for call in (lambda: kv4.attn(q, none, table, n, 0.1), lambda: kv4.load(none, n),
+                 lambda: kv4.store(none, q[:, :0], q[:, :0], n),
+                 lambda: kv4.plan_pages(n, n, table, n, n, 2 ** 32 + 64, 1)):
+        with pytest.raises(RuntimeError):
+            call()
+    cache = kv4.new_cache(2, 64, 1, 64)
+    wide = torch.zeros(1, 2 ** 25, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError):
+        kv4.attn(q, cache, wide, n, 0.1)
+
+
+@pytest.mark.parametrize("news", [1, 20])
+@pytest.mark.parametrize("D", [64, 128])
+def test_requests_without_keys_read_no_table(D, news):
+    """No tokens, no columns in the table, or no pages: rows of zeros."""
+    cache = kv4.new_cache(2, 64, 2, D)
+    q = torch.randn(2 * news, 8, D, device=DEV).half()
+    kw = dict(cu_q=i32([0, news, 2 * news]), max_q=news)
+    for c, table, lens in ((cache, torch.empty(2, 0, dtype=torch.int32, device=DEV), [0, 90]),
+                           (cache, i32([[1], [-1]]), [0, 9]),
+                           (kv4.new_cache(0, 64, 2, D), i32([[1], [0]]), [70, 64])):
+        assert kv4.attn(q, c, table, i32(lens), 0.1, **kw).eq(0).all()
+
+
 def test_no_queries_and_an_empty_cache():
     cache = kv4.new_cache(0, 64, 2, 64)
     table = torch.empty(2, 0, dtype=torch.int32, device=DEV)

@@ -175,6 +175,21 @@ def test_means_refuses(lib):
         assert lib.sparse_block_means(*args) == 1, (at, val)
 
 
+def test_grids_past_what_a_launch_takes_are_refused(lib):
+    """Sizes whose grid would have 2^32 threads or more: refused before the first launch."""
+    many = dict(B=4096, T=4096, Hq=4096, Hkv=4096, W=1, stride=1, os=strides(4096 * 128, 128))
+    assert kv4_attn(lib, **many) == 1 and b"too many" in lib.kv4_last_error()
+    rows = dict(T=1 << 25, Hq=64, Hkv=8, cu=FAKE, max_q=1 << 25, os=strides(8192, 128))
+    assert kv4_attn(lib, **rows) == 1 and b"too many" in lib.kv4_last_error()
+    far = strides(0, 1 << 40, 128)
+    assert sparse_attn(lib, B=1, Hq=4, Sq=1 << 29, os=far) == 1
+    assert b"too many" in lib.sparse_last_error()
+    a = (FAKE, FAKE, 1, 1, 1, 1 << 29, 400, 64, 64, 3, 0, FAKE, FAKE, 1 << 50, None)
+    assert lib.sparse_select(*a) == 1 and b"too many" in lib.sparse_last_error()
+    assert lib.sparse_block_means(FAKE, far, 0, 1, 8, 1 << 29, 128, 64, FAKE, None) == 1
+    assert b"too many" in lib.sparse_last_error()
+
+
 def test_python_layer_refuses_on_the_cpu(lib):
     with pytest.raises(ValueError):
         kv4.new_cache(4, 32, 2, 128, device="cpu")
