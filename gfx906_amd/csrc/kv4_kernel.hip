@@ -19,6 +19,11 @@ using namespace gfx906_amd::longctx;
 thread_local LastError g_err;
 
 constexpr int kMaxRequests = KV4_MAX_REQUESTS;
+// Requests of up to so many query rows a kv head go to attn_few_kernel, in tiles of 32 that
+// read the cache again, the others to the prompt kernels. One request behind 16384 tokens, 8 kv
+// heads, us here / there: 128 rows 32 / 70, 256 42 / 69, 384 53 / 71; 8 requests behind 4096,
+// 4 kv heads: 256 rows 44 / 58, 384 76 / 64.
+constexpr int kFewRows = 256;
 
 // The cache as kernels see it. Offsets of rows are 64-bit: a cache may hold more
 // than 2^32 bytes.
@@ -744,15 +749,15 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
 #endif
 }
 
-// Merges the slots of heads that lie in several runs, writes the zeros of requests
-// without tokens, and does rows again that a value they do not see may have spoilt. One workgroup per request, kv head and query row of it.
-template <int D, class T, int NB, int NT>
-__global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
+// Merges the slots of a head that lies in several runs, writes the zeros of a request
+// without tokens, and does a row again that a value it does not see may have spoilt: query row
+// `row` of kv head hk of request b, by a workgroup of NT threads.
+template <int D, class T, int NB, int NT>
+__device__ __forceinline__ void few_combine(const AttnArgs& a, int b, int hk, int row) {
     constexpr int R = 16 * NB, DQ = D / 4, NG = NT / DQ;
     __shared__ f32x4 acc_s[NG][DQ];
     __shared__ float ml_s[NG][2];
-    const int b = blockIdx.x / a.c.Hkv, hk = blockIdx.x - b * a.c.Hkv, row = blockIdx.y;
     const Request req = request(a, b);
     const long long rows = (long long)req.m * a.G;
     if (rows > a.few_rows || row >= rows) return;
@@ -823,13 +828,22 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
     const auto x0 = Elem<T>::cvt2(acc[0], acc[1]), x1 = Elem<T>::cvt2(acc[2], acc[3]);
     *reinterpret_cast<u32x2*>(o) =
         u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
+}
+#endif
+
+// grid: requests x kv heads, query rows.
+template <int D, class T, int NB, int NT>
+__global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int b = blockIdx.x / a.c.Hkv;
+    few_combine<D, T, NB, NT>(a, b, blockIdx.x - b * a.c.Hkv, blockIdx.y);
 #endif
 }
 
 // -- prompts: requests of more than few_rows query rows a kv head -----------------------
 
 // A run is at least kPromptRun units: two prompts of 200 queries behind 800 tokens, 16/4 heads, 30
-// us with 5, 37 with 8, 53 with 16.
+// us in the prompt kernels with 5, 37 with 8, 53 with 16.
 constexpr int kTileRows = 128, kPromptStart = 4;
 constexpr long long kPromptRun = kPromptStart + 1;
 constexpr int kSelfTiles = 1024, kSelfRequests = 256;  // SELF (attn_prompt_kernel)
@@ -1233,12 +1247,19 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
 
 // Merges the runs of a tile, writes the zeros of tiles that see no key, and does rows
 // again that a value they do not see may have spoilt. One workgroup per 16 rows
-// of a tile and kv head.
+// of a tile and kv head; behind these one per request and query row of attn_few_kernel's. (4 requests
+// of 1 .. 70 queries in 1000 .. 20000 tokens, 32/8 heads: 87 us, and 96 with two merges one after the
+// other; 16 of 1 .. 300 in 300 .. 4000, 16/4 heads: 86 and 90.)
 template <int D, class T>
 __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int ROWS = 16;
     const int tile = blockIdx.x / (kTileRows / ROWS), hk = blockIdx.y, tid = threadIdx.x;
+    if (tile >= a.p_tiles) {
+        const int e = blockIdx.x - a.p_tiles * (kTileRows / ROWS), few = e / kFewRows;
+        few_combine<D, T, 2, 256>(a, few, hk, e - few * kFewRows);
+        return;
+    }
     const int r0 = blockIdx.x % (kTileRows / ROWS) * ROWS;
     const int b = a.p_req[tile];
     if (tile >= a.p_first[a.B]) return;
@@ -1323,11 +1344,7 @@ int check_cache(int Hkv, int D, int pages, int page, const void* kc, const void*
     return 0;
 }
 
-// Requests of up to so many query rows a kv head go to attn_few_kernel, in tiles of 32 that
-// read the cache again, the others to the prompt kernels. One request behind 16384 tokens, 8 kv
-// heads, us here / there: 128 rows 32 / 70, 256 42 / 69, 384 53 / 71; 8 requests behind 4096,
-// 4 kv heads: 256 rows 44 / 58, 384 76 / 64.
-constexpr int kFewRows = 256, kGroups = 256, kMinUnits = 8;
+constexpr int kGroups = 256, kMinUnits = 8;
 // Tables of up to so many tokens go to the DIRECT form, and twice as many where there are heads
 // enough for the GPU. One query each, 8 kv heads, us DIRECT / in runs: 1 request of 1000 tokens
 // 8.5 / 13.4, of 2000 12.0 / 13.5, of 4000 19.5 / 13.8; 32 requests of 2000 16.3 / 24.2, of 4000
@@ -1525,9 +1542,11 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     const PromptPlan pp = prompt_plan(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);
     const size_t need = pp.used ? pp.bytes : plan.bytes;
     const long long heads = (long long)B * Hkv;
+    const long long combines = pp.tiles * (long long)(kTileRows / 16) +
+                               (plan.direct ? 0 : (long long)B * kFewRows);
     if (!(plan.direct ? launchable(heads * plan.tiles, 512)
                       : launchable(heads, plan.many ? 1024 : 256)) ||
-        (pp.used && !launchable(pp.tiles * (long long)(kTileRows / 16), 256)))
+        (pp.used && !launchable(combines, 256)))
         return g_err.fail("kv4_attn: too many requests, heads or query rows for one call");
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return g_err.fail("kv4_attn: workspace misaligned or smaller than "
@@ -1582,6 +1601,7 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
         };
         auto runs = [&](auto kernel, auto combine, auto combine_many) {
             hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(512), 0, stream, a);
+            if (pp.used) return;  // (prompt_combine_kernel merges)
             if (plan.many)
                 hipLaunchKernelGGL(combine_many, cgrid, dim3(1024), 0, stream, a);
             else
@@ -1606,9 +1626,8 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
                 hipLaunchKernelGGL((attn_prompt_kernel<kD, E, false>), dim3(pp.groups), dim3(256), 0,
                                    stream, a);
             }
-            hipLaunchKernelGGL((prompt_combine_kernel<kD, E>), dim3(pp.tiles * (kTileRows / 16), Hkv),
-                               dim3(256), 0,
-                               stream, a);
+            hipLaunchKernelGGL((prompt_combine_kernel<kD, E>), dim3((unsigned)combines, Hkv),
+                               dim3(256), 0, stream, a);
         }
     };
     if (dtype == KV4_DTYPE_F16)
