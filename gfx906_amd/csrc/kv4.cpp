@@ -91,10 +91,18 @@ std::vector<Tensor> kv4_plan_pages_op(Tensor lens, Tensor new_lens, Tensor table
     for (const Tensor* t : {&lens, &new_lens, &free_pages, &used}) at::assert_no_overlap(table, *t);
     const c10::DeviceGuard guard(dev);
     // One buffer for every result: slots, cu_new, lens, used, missing.
-    const Tensor buf = torch::empty({tokens + 2 * B + 3}, lens.options());
-    const Tensor slots = buf.narrow(0, 0, tokens), cu = buf.narrow(0, tokens, B + 1),
-                 out = buf.narrow(0, tokens + B + 1, B), u = buf.narrow(0, tokens + 2 * B + 1, 1),
-                 miss = buf.narrow(0, tokens + 2 * B + 2, 1);
+    const Tensor buf = at::empty({tokens + 2 * B + 3}, lens.options());
+    // (made by hand: five views through the dispatcher take 2 us of the call's 7)
+    int64_t at = 0;
+    auto next = [&](int64_t n) {
+        Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()),
+                                                            buf.key_set(), buf.dtype());
+        t.unsafeGetTensorImpl()->set_storage_offset(at);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(n);
+        at += n;
+        return t;
+    };
+    const Tensor slots = next(tokens), cu = next(B + 1), out = next(B), u = next(1), miss = next(1);
     check_rc(kv4_plan_pages(lens.data_ptr<int>(), new_lens.data_ptr<int>(), table.data_ptr<int>(),
                             B <= 1 ? table.size(1) : table.stride(0), (int)table.size(1),
                             free_pages.data_ptr<int>(), (int)free_pages.size(0),
@@ -132,7 +140,7 @@ std::vector<Tensor> kv4_load_op(Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tens
     TORCH_CHECK(slots.size(0) < (1LL << 31), who, ": too many rows");
     const c10::DeviceGuard guard(kc.device());
     const int64_t T = slots.size(0);
-    Tensor k = torch::empty({T, c.Hkv, c.D}, kc.options().dtype(dtype)), v = torch::empty_like(k);
+    Tensor k = at::empty({T, c.Hkv, c.D}, kc.options().dtype(dtype)), v = at::empty_like(k);
     if (k.numel())
         check_rc(kv4_load(k.data_ptr(), v.data_ptr(), dt, (int)T, c.Hkv, c.D,
                           slots.data_ptr<int>(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(),
@@ -172,7 +180,7 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
         for (const Tensor* t : {&kc, &ks, &vc, &vs, &table, &lens}) at::assert_no_overlap(o, *t);
         if (cu_q.has_value()) at::assert_no_overlap(o, *cu_q);
     } else {
-        o = torch::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+        o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     }
     if (q.numel() == 0 || B == 0) return o;
     const c10::DeviceGuard guard(dev);
@@ -185,7 +193,7 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
     const size_t bytes = kv4_attn_workspace_bytes((int)T, (int)B, (int)Hq, c.Hkv, c.D, (int)max_q,
                                                   W * c.page);
     Tensor ws;
-    if (bytes) ws = torch::empty({(int64_t)bytes}, kc.options());
+    if (bytes) ws = at::empty({(int64_t)bytes}, kc.options());
     check_rc(kv4_attn(qr.data_ptr(), o.data_ptr(), sq.data(), so.data(), dt, (int)T, (int)B,
                       (int)Hq, c.Hkv, c.D, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(),
                       vs.data_ptr(), c.pages, c.page, table.data_ptr<int>(),

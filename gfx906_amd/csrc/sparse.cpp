@@ -62,7 +62,7 @@ Tensor sparse_block_means_op(Tensor x, int64_t block) {
     check_block(block, who);
     const c10::DeviceGuard guard(x.device());
     const int64_t B = x.size(0), H = x.size(1), S = x.size(2), D = x.size(3);
-    Tensor m = torch::empty({B, H, blocks(S, block), D}, x.options().dtype(torch::kFloat));
+    Tensor m = at::empty({B, H, blocks(S, block), D}, x.options().dtype(torch::kFloat));
     if (m.numel() == 0) return m;
     const Tensor r = rows_of(x);
     const auto st = strides3(r);
@@ -91,13 +91,13 @@ Tensor sparse_select_op(Tensor qm, Tensor km, int64_t count, int64_t q_len, int6
     const c10::DeviceGuard guard(qm.device());
     const int B = (int)qm.size(0), Hq = (int)qm.size(1), Hkv = (int)km.size(1),
               D = (int)qm.size(3);
-    Tensor index = torch::empty({B, Hq, qm.size(2), count}, qm.options().dtype(torch::kInt));
+    Tensor index = at::empty({B, Hq, qm.size(2), count}, qm.options().dtype(torch::kInt));
     if (index.numel() == 0) return index;
     const Tensor qc = qm.contiguous(), kc = km.contiguous();
     const size_t bytes =
         sparse_select_workspace_bytes(B, Hq, (int)q_len, (int)k_len, (int)block);
     Tensor ws;
-    if (bytes) ws = torch::empty({(int64_t)bytes}, qm.options().dtype(torch::kByte));
+    if (bytes) ws = at::empty({(int64_t)bytes}, qm.options().dtype(torch::kByte));
     check_rc(sparse_select(qc.data_ptr<float>(), kc.data_ptr<float>(), B, Hq, Hkv, (int)q_len,
                            (int)k_len, D, (int)block, (int)count, causal, index.data_ptr<int>(),
                            bytes ? ws.data_ptr() : nullptr, bytes, stream()));
@@ -118,14 +118,14 @@ Tensor sparse_choose_op(Tensor q, Tensor km, int64_t count, int64_t k_len, int64
     const c10::DeviceGuard guard(q.device());
     const int B = (int)q.size(0), Hq = (int)q.size(1), Sq = (int)q.size(2), D = (int)q.size(3);
     Tensor index =
-        torch::empty({B, Hq, blocks(Sq, SPARSE_Q_BLOCK), count}, q.options().dtype(torch::kInt));
+        at::empty({B, Hq, blocks(Sq, SPARSE_Q_BLOCK), count}, q.options().dtype(torch::kInt));
     if (index.numel() == 0) return index;
     const Tensor qr = rows_of(q), kc = km.contiguous();
     const auto st = strides3(qr);
     const size_t bytes =
         sparse_choose_workspace_bytes(B, Hq, Sq, (int)k_len, D, (int)block);
     Tensor ws;
-    if (bytes) ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kByte));
+    if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(torch::kByte));
     check_rc(sparse_choose(qr.data_ptr(), st.data(), dt, kc.data_ptr<float>(), B, Hq,
                            (int)km.size(1), Sq, (int)k_len, D, (int)block, (int)count, causal,
                            index.data_ptr<int>(), bytes ? ws.data_ptr() : nullptr, bytes, stream()));
@@ -163,7 +163,7 @@ Tensor sparse_attn_op(Tensor q, Tensor k, Tensor v, double scale, Tensor index, 
         at::assert_no_overlap(o, v);
         at::assert_no_overlap(o, index);
     } else {
-        o = torch::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+        o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     }
     if (q.numel() == 0) return o;
     const c10::DeviceGuard guard(q.device());
@@ -173,7 +173,7 @@ Tensor sparse_attn_op(Tensor q, Tensor k, Tensor v, double scale, Tensor index, 
     const size_t bytes = sparse_attn_workspace_bytes((int)B, (int)Hq, (int)Sq, (int)Skv, (int)D,
                                                      (int)block, count);
     Tensor ws;
-    if (bytes) ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kByte));
+    if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(torch::kByte));
     check_rc(sparse_attn(qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(), sq.data(),
                          sk.data(), sv.data(), so.data(), dt, (int)B, (int)Hq, (int)Hkv, (int)Sq,
                          (int)Skv, (int)D, (float)scale, ix.data_ptr<int>(), (int)block, count,
