@@ -62,6 +62,28 @@ def test_plan_pages_with_a_short_slot_list():
     assert plan.slots.tolist() == list(range(256, 266)) and plan.cu_new.tolist() == [0, 70, 73]
 
 
+def test_plan_pages_with_counts_up_to_an_int():
+    """Sums past 31 bits saturate; what comes before them is as ever."""
+    top = 2 ** 31 - 1
+    table = i32([[3, 4, 5], [6, 7, 9], [9, 9, 9]])
+    plan = kv4.plan_pages(i32([top, 100, 0]), i32([top, top, 5]), table, i32([11, 12, 13, 14]),
+                          i32([0]), 64, 70)
+    assert plan.slots.tolist() == [-1] * 70      # all of request 0, behind its row's three pages
+    assert plan.cu_new.tolist() == [0, top, top, top] and plan.lens.tolist() == [top, top, 5]
+    # 2^26 - 2^25 pages lacked, ceil((2^31 + 99) / 64) - 2 = 2^25, and 1: none is left for the others
+    assert plan.used.item() == 4 and plan.missing.item() == 2 ** 26 + 1
+    assert table.tolist() == [[3, 4, 5], [6, 7, -1], [-1, 9, 9]]
+
+    table = i32([[-1, -1], [9, -1]])
+    plan = kv4.plan_pages(i32([0, 5]), i32([3, top]), table, i32([7, 8]), i32([0]), 64, 200)
+    want = [448, 449, 450] + [9 * 64 + p for p in range(5, 64)] + [512 + p for p in range(64)]
+    assert plan.slots.tolist() == want + [-1] * (200 - len(want))
+    assert plan.cu_new.tolist() == [0, 3, top] and plan.lens.tolist() == [3, top]
+    # request 1 lacks ceil((2^31 + 4) / 64) - 1 = 2^25 pages and gets one
+    assert plan.used.item() == 2 and plan.missing.item() == 2 ** 25 - 1
+    assert table.tolist() == [[7, -1], [9, 8]]
+
+
 def test_plan_pages_of_no_requests():
     none = i32([])
     plan = kv4.plan_pages(none, none, i32([]).view(0, 3), i32([1, 2]), i32([1]), 64, 3)
