@@ -1,4 +1,4 @@
-// PyTorch binding of the 4-bit key/value cache (gfx906_amd_kv4.h): kv4_plan_pages,
+// PyTorch binding of the 4-bit key/value cache (gfx906_amd_attn.h): kv4_plan_pages,
 // kv4_store, kv4_load and kv4_attn. The Python layer (gfx906_amd.kv4) documents the
 // arguments. Every op runs on the current HIP stream of its tensors' device without
 // synchronising; what cannot be run raises RuntimeError.
@@ -7,7 +7,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include "bindings.h"
-#include "gfx906_amd_kv4.h"
+#include "gfx906_amd_attn.h"
 
 namespace {
 

@@ -1,6 +1,6 @@
 // Key/value cache in 4 bits for AMD MI355X (gfx950): pages and slots from
 // request lengths, storing and reading rows, attention over the cache. The
-// format and the entry points are described in gfx906_amd_kv4.h.
+// format and the entry points are described in gfx906_amd_attn.h.
 //
 // gfx950 converts between E2M1 pairs with an E8M0 scale and fp16, bf16 or fp32
 // in one instruction (v_cvt_scalef32_*), rounding to nearest even and
@@ -10,7 +10,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gfx906_amd_kv4.h"
+#include "gfx906_amd_attn.h"
 
 namespace {
 

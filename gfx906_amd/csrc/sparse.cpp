@@ -1,4 +1,4 @@
-// PyTorch binding of sparse attention (gfx906_amd_sparse.h): sparse_block_means,
+// PyTorch binding of sparse attention (gfx906_amd_attn.h): sparse_block_means,
 // sparse_select, sparse_choose and sparse_attn. The Python layer (gfx906_amd.sparse) documents the
 // arguments. Every op runs on the current HIP stream of its tensors' device without
 // synchronising; what cannot be run raises RuntimeError.
@@ -7,7 +7,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include "bindings.h"
-#include "gfx906_amd_sparse.h"
+#include "gfx906_amd_attn.h"
 
 namespace {
 

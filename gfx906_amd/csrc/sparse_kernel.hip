@@ -1,6 +1,6 @@
 // Sparse attention for AMD MI355X (gfx950): means of row blocks, the choice of key
 // blocks by the product of means, and attention over the chosen blocks. The entry
-// points are described in gfx906_amd_sparse.h.
+// points are described in gfx906_amd_attn.h.
 //
 // The choice is an output (and decides what is read), so it must not hang on the
 // order of a sum: block sums are taken in fp64, where sums of 128 fp16 values are
@@ -12,7 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gfx906_amd_sparse.h"
+#include "gfx906_amd_attn.h"
 
 namespace {
 

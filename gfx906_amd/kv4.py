@@ -10,7 +10,7 @@ which gfx950 converts in hardware. A serving step goes
 
 with every length, table and slot on the GPU: no call synchronises, and all of
 them may be captured into a HIP graph. The layout and what happens to values out
-of range is described in ``include/gfx906_amd_kv4.h``. All calls run on the
+of range is described in ``include/gfx906_amd_attn.h``. All calls run on the
 current stream, raise ``RuntimeError`` for what they do not accept, and have no
 fallback. The reference has no counterpart.
 """

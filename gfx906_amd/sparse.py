@@ -8,7 +8,7 @@
 
 A block's score is the product of the query block's mean and the key block's mean,
 computed so that the choice does not hang on the order of a sum (see
-``include/gfx906_amd_sparse.h``). q is ``[B, Hq, Sq, D]``, k and v
+``include/gfx906_amd_attn.h``). q is ``[B, Hq, Sq, D]``, k and v
 ``[B, Hkv, Skv, D]``, fp16 or bf16, D 64 or 128, Hq a multiple of Hkv; strided views
 with a contiguous head dim are read in place. All calls run on the current stream
 without synchronising, raise ``RuntimeError`` for what they do not accept, and have

@@ -1,4 +1,5 @@
-/* C ABI of the MI355X (gfx950) flash-attention forward.
+/* C ABI of the MI355X (gfx950) flash-attention forward, and at the end of two
+ * forms of it for long contexts: a 4-bit key/value cache and sparse attention.
  *
  * All pointers are device pointers. For launch() and attn_fwd() the tensors
  * are contiguous fp16:
@@ -145,6 +146,155 @@ size_t attn_split_scratch_capacity(void);
  * the last call succeeded. No counterpart in the reference, whose launch()
  * (attn_kernel.hip:710-742) never reports errors. */
 const char* attn_last_error(void);
+
+/* -- A key/value cache held in 4 bits: pages and slots from request lengths,
+ * storing and reading rows, and attention over the cache. No counterpart in the reference, whose attention reads fp16 tensors.
+ *
+ * Cache. Keys and values are E2M1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) with one E8M0 scale (2^(byte - 127); 255 is NaN) per 32 head dims
+ * of a token (the OCP MX format MXFP4), in pages of `page` tokens (64, 128 or
+ * 256), for head dims of 64 or 128:
+ *   codes  [pages, Hkv, page, D/2] bytes; dim 2i in the low, 2i+1 in the high
+ *          nibble of byte i
+ *   scales [pages, Hkv, page/64, 16, D/32, 4] bytes; the scale of dims
+ *          32j..32j+31 of a page's token 64a + 16c + b at [a, b, j, c], so that a
+ *          lane reads the scales of four 16-token tiles as one dword
+ * A block of 32 values x is stored with scale byte E - 2, E the biased fp32
+ * exponent of max |x| (at least 1; 255, a block of NaN, where some x is infinite
+ * or NaN), as the nearest codes, ties to even, saturating at 6 scales. fp16
+ * rows hold 16384 <= max |x| <= 65504 as well; a cache of bf16 rows read as fp16
+ * gives infinities for values past 65504.
+ *
+ * Lengths, slots, tables and other int arguments named here as device arrays
+ * are read on the GPU and not checked by the host; any value is safe (see each).
+ * All pointers are device pointers; calls are asynchronous on `stream`, return
+ * 0, 1 for a rejected argument (nothing launched) or 2 for a HIP error, and set
+ * kv4_last_error() for the calling thread.
+ */
+
+#define KV4_DTYPE_F16 0
+#define KV4_DTYPE_BF16 1
+#define KV4_MAX_REQUESTS 4096
+
+/* Pages and slots for new tokens. Request b holds lens[b] tokens, in pages
+ * table[b][0 .. ceil(lens[b] / page)), and gets new_lens[b] more (negative counts are
+ * taken as 0). Requests take the pages they lack from free_pages[*used ..), in
+ * request order; written are
+ *   table[b][...]   the new pages (rows table_stride apart; W columns)
+ *   slots[0..n_slots)  page * `page` + place of every new token, requests one after
+ *                   another; -1 for a token without a page (the free list or the
+ *                   table's row ended, or a held page is negative) and behind the last
+ *   cu_new[0..B]    first slot of every request, and their number (int32; saturates)
+ *   lens_out[b]     lens[b] + new_lens[b]
+ *   used_out        *used + the pages lacked, at most n_free
+ *   missing         pages that could not be taken: the free list ended (table
+ *                   entry -1), or the table's row did (its place in the free list is
+ *                   passed over)
+ * The arrays written must not overlap those read, except table. */
+int kv4_plan_pages(const int* lens, const int* new_lens, int* table, long long table_stride, int W,
+                   const int* free_pages, int n_free, const int* used, int B, int page,
+                   int n_slots, int* slots, int* cu_new, int* lens_out, int* used_out,
+                   int* missing, hipStream_t stream);
+
+/* Stores rows t of k and v ([T, Hkv, D], fp16 or bf16; strides {token, head} in
+ * elements, head dim contiguous, 16-byte aligned rows) at slots[t]; a slot outside
+ * [0, pages * page) stores nothing. Slots of stored rows must differ: two rows with
+ * one slot leave some mix of both there. */
+int kv4_store(const void* k, const void* v, const long long* k_strides, const long long* v_strides,
+              int dtype, int T, int Hkv, int D, const int* slots, void* k_codes, void* k_scales,
+              void* v_codes, void* v_scales, int pages, int page, hipStream_t stream);
+
+/* Reads rows slots[t] of the cache into contiguous k and v [T, Hkv, D]; a slot
+ * outside the cache reads as zeros. */
+int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, const int* slots,
+             const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+             int pages, int page, hipStream_t stream);
+
+/* o = softmax(scale q k^T) v over the cache, for T query rows q [T, Hq, D] of B
+ * requests: rows cu_q[b] .. cu_q[b+1] belong to request b (cu_q NULL: row b, T = B),
+ * whose lens[b] tokens lie in pages table[b][...]. Query head h reads kv head
+ * h / (Hq / Hkv). With causal != 0 the n queries of a request are its last n tokens
+ * and see no later one; otherwise they see all of its tokens. A row that sees no key, or
+ * only such of score -inf, is 0; a token that a row does not see adds nothing to it, whatever
+ * it holds. Keys in pages outside [0, pages) or behind the table's last column weigh
+ * nothing; cu_q is taken as clamped to 0 .. T. Rows outside every request, and queries
+ * past the first max_q of one, are left as they were. q and o: strides {token, head} in
+ * elements, head dim contiguous, q's rows 16-byte and o's 8-byte aligned; o's must
+ * not overlap each other, q or the cache. workspace: 16-byte aligned,
+ * kv4_attn_workspace_bytes() bytes, with max_len = W * page (and max_q = 1 where cu_q is
+ * NULL); its content is neither read before it is written nor kept. */
+size_t kv4_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q, int max_len);
+int kv4_attn(const void* q, void* o, const long long* q_strides, const long long* o_strides,
+             int dtype, int T, int B, int Hq, int Hkv, int D, const void* k_codes,
+             const void* k_scales, const void* v_codes, const void* v_scales, int pages, int page,
+             const int* table, long long table_stride, int W, const int* lens, const int* cu_q,
+             int max_q, float scale, int causal, void* workspace, size_t workspace_bytes,
+             hipStream_t stream);
+
+/* Message for the last failed call on the calling thread, or NULL. */
+const char* kv4_last_error(void);
+
+/* -- Sparse attention: every block of 128 query rows
+ * reads a few blocks of keys, which a score of block means selects. No counterpart
+ * in the reference, whose attention reads every key.
+ *
+ * Calls are asynchronous on `stream`, return 0, 1 for a rejected argument (nothing
+ * launched) or 2 for a HIP error, and set sparse_last_error() for the calling
+ * thread. Pointers are device pointers, strides in elements {batch, head,
+ * sequence}, head dims contiguous, D 64 or 128, key blocks of 64 or 128 rows.
+ */
+
+#define SPARSE_DTYPE_F16 0
+#define SPARSE_DTYPE_BF16 1
+#define SPARSE_Q_BLOCK 128
+#define SPARSE_MAX_BLOCKS 32768 /* key blocks of a head */
+#define SPARSE_MAX_COUNT 2048   /* blocks chosen for a query block */
+
+/* means[b][h][j][:] = mean of rows j*block .. of x [B, H, S, D] (the last block
+ * may be short), summed in fp64 and rounded once to fp32; packed. x's rows are
+ * 16-byte aligned. */
+int sparse_block_means(const void* x, const long long* strides, int dtype, int B, int H, int S,
+                       int D, int block, float* means, hipStream_t stream);
+
+/* index[b][h][i][0..count): the key blocks of query block i, ascending, -1 behind
+ * the last. Taken are those with the largest product of q_means[b][h][i] and
+ * k_means[b][h / (Hq/Hkv)][j] (fp64; NaN counts as largest, equal products by the
+ * lower index). Means are packed fp32 [B, Hq, ceil(Sq/128), D] and
+ * [B, Hkv, ceil(Skv/block), D], 16-byte aligned. With causal != 0 query row r stands at key position
+ * r + Skv - Sq; blocks past the query block's last position are never taken, and
+ * those that hold its own positions always (count must be at least 128/block + 1,
+ * or their number where Sq < 128). workspace: sparse_select_workspace_bytes() bytes. */
+size_t sparse_select_workspace_bytes(int B, int Hq, int Sq, int Skv, int block);
+int sparse_select(const float* q_means, const float* k_means, int B, int Hq, int Hkv, int Sq,
+                  int Skv, int D, int block, int count, int causal, int* index, void* workspace,
+                  size_t workspace_bytes, hipStream_t stream);
+
+/* The same from the query rows q [B, Hq, Sq, D] themselves (16-byte aligned), whose means
+ * over 128 rows are taken as sparse_block_means does. workspace:
+ * sparse_choose_workspace_bytes() bytes (0 for few query blocks, which take one kernel). */
+size_t sparse_choose_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block);
+int sparse_choose(const void* q, const long long* q_strides, int dtype, const float* k_means, int B,
+                  int Hq, int Hkv, int Sq, int Skv, int D, int block, int count, int causal,
+                  int* index, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* o = softmax(scale q k^T) v over the keys of the blocks in index (as
+ * sparse_select writes it, [B, Hq, ceil(Sq/128), count]; read on the GPU and not
+ * checked by the host: an entry outside 0 .. ceil(Skv/block)-1, or not above every
+ * valid entry before it, is passed over). causal as above. A row that sees no key,
+ * or only such of score -inf, is 0; a key that a row does not see adds nothing to it, whatever
+ * it holds. q, k, v: rows 16-byte aligned (k's and v's
+ * apart, their strides at most 2^22); o: 8-byte, rows that do not overlap each other, k, v or
+ * index; o may be q (the same rows).
+ * workspace: 16-byte aligned, sparse_attn_workspace_bytes() bytes (may be 0). */
+size_t sparse_attn_workspace_bytes(int B, int Hq, int Sq, int Skv, int D, int block, int count);
+int sparse_attn(const void* q, const void* k, const void* v, void* o, const long long* q_strides,
+                const long long* k_strides, const long long* v_strides,
+                const long long* o_strides, int dtype, int B, int Hq, int Hkv, int Sq, int Skv,
+                int D, float scale, const int* index, int block, int count, int causal,
+                void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Message for the last failed call on the calling thread, or NULL. */
+const char* sparse_last_error(void);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,6 @@
 """CPU oracle of the 4-bit cache and of sparse attention (test infrastructure only).
 
-Plain loops in 64 bits over the definitions in ``include/gfx906_amd_kv4.h`` and
-``include/gfx906_amd_sparse.h``; nothing here comes from the kernels.
+Plain loops in 64 bits over the definitions in ``include/gfx906_amd_attn.h``; nothing here comes from the kernels.
 """
 
 from __future__ import annotations
