@@ -446,7 +446,8 @@ struct Codes {
 // as they stand: the dims of a step are split over the lane groups alike for K and
 // Q, whatever their order. V goes through LDS in the element type (8 KB a wave), as the
 // second product sums over keys. The next unit's K codes are loaded once the scores of
-// one are done, its V codes at the end, so that neither needs registers twice.
+// one are done, its V codes at the end, so that neither needs registers twice (two units ahead,
+// in twice the registers, measured 31.3 us a call and not 28.6 on the batch below).
 //
 // DIRECT: short tables. One workgroup a head, no runs, no slots and no second kernel.
 //
