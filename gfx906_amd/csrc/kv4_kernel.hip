@@ -758,9 +758,9 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
 // `row` of kv head hk of request b, by a workgroup of NT threads.
 template <int D, class T, int NB, int NT>
 __device__ __forceinline__ void few_combine(const AttnArgs& a, int b, int hk, int row) {
-    constexpr int R = 16 * NB, DQ = D / 4, NG = NT / DQ;
-    __shared__ f32x4 acc_s[NG][DQ];
-    __shared__ float ml_s[NG][2];
+    constexpr int R = 16 * NB, DQ = D / 4, NG = NT / DQ, NW = NT / 64;
+    __shared__ f32x4 acc_s[NW][DQ];
+    __shared__ float ml_s[NW][2];
     const Request req = request(a, b);
     const long long rows = (long long)req.m * a.G;
     if (rows > a.few_rows || row >= rows) return;
@@ -809,20 +809,34 @@ __device__ __forceinline__ void few_combine(const AttnArgs& a, int b, int hk, in
             m = mn;
         }
     }
-    acc_s[grp][d / 4] = acc;
-    if (d == 0) {
-        ml_s[grp][0] = m;
-        ml_s[grp][1] = l;
+    // The groups of a wave, then the waves. (All groups through LDS: 100000 tokens, one kv head of 64,
+    // 16.3 us a call and not 14.0; 131072, 2 of 128, 32 rows, 22.5 and 22.1.)
+#pragma unroll
+    for (int step = DQ; step < 64; step <<= 1) {
+        const float mo = __shfl_xor(m, step), lo = __shfl_xor(l, step), mn = max2(m, mo);
+        const float f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(mo - mn);
+        l = l * f + lo * e;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[n] = acc[n] * f + __shfl_xor(acc[n], step) * e;
+        m = mn;
+    }
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) < DQ) {
+        acc_s[wave][d / 4] = acc;
+        if (d == 0) {
+            ml_s[wave][0] = m;
+            ml_s[wave][1] = l;
+        }
     }
     __syncthreads();
     if (grp) return;
     float mx = kNoMax;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) mx = max2(mx, ml_s[n][0]);
+    for (int n = 0; n < NW; ++n) mx = max2(mx, ml_s[n][0]);
     acc = f32x4{};
     l = 0.f;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
+    for (int n = 0; n < NW; ++n) {
         const float f = __builtin_amdgcn_exp2f(ml_s[n][0] - mx);
         acc += acc_s[n][d / 4] * f;
         l += ml_s[n][1] * f;
