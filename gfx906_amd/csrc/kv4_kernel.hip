@@ -63,6 +63,14 @@ __device__ __forceinline__ typename Elem<T>::x8 expand(unsigned w, float s) {
     auto u = [](typename Elem<T>::x2 x) { return __builtin_bit_cast(unsigned, x); };
     return __builtin_bit_cast(typename Elem<T>::x8, u32x4{u(p[0]), u(p[1]), u(p[2]), u(p[3])});
 }
+// The two codes of a byte, rounded to the element type as expand() does.
+template <class T>
+__device__ __forceinline__ f32x2 expand_pair(unsigned byte, float s) {
+    if constexpr (__is_same(T, f16))
+        return __builtin_convertvector(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(byte, s, 0), f32x2);
+    else
+        return __builtin_convertvector(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(byte, s, 0), f32x2);
+}
 #endif
 
 // -- pages and slots ------------------------------------------------------------------
@@ -354,7 +362,9 @@ constexpr unsigned kScaleLimit = __is_same(T, f16) ? 141u : 253u;
 
 // One query row over the keys t0 .. t1 - 1 of its request, by one wave: 64 keys at a
 // time, a score per lane, then a pair of dims per lane. Keys the row does not see are
-// not touched at all, so that what they hold cannot reach it.
+// not touched at all, so that what they hold cannot reach it. Keys and values are those of the
+// matrix kernels, rounded to the element type: whether a row is done here depends on tokens
+// that it does not see, and a value past fp16's range must be the same infinity either way.
 template <int D, class T>
 __device__ void attend_row(const AttnArgs& a, const T* q, int hk, int b, int t0, int t1, T* o) {
     const int lane = threadIdx.x & 63;
@@ -368,8 +378,8 @@ __device__ void attend_row(const AttnArgs& a, const T* q, int hk, int b, int t0,
             const long long sa = scale_at(a.c, page, hk, j % a.c.page);
             s = 0.f;
             for (int i = 0; i < D / 2; ++i) {
-                const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
-                    (unsigned)a.c.kc[ca + i], e8m0(a.c.ks[sa + 4 * (i / 16)]), 0);
+                const f32x2 x =
+                    expand_pair<T>((unsigned)a.c.kc[ca + i], e8m0(a.c.ks[sa + 4 * (i / 16)]));
                 s = fmaf((float)q[2 * i], x[0], s);
                 s = fmaf((float)q[2 * i + 1], x[1], s);
             }
@@ -384,9 +394,9 @@ __device__ void attend_row(const AttnArgs& a, const T* q, int hk, int b, int t0,
             const float pi = __shfl(p, i);
             if (2 * lane < D) {
                 const int t = (j0 + i) % a.c.page;
-                const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
-                    (unsigned)a.c.vc[code_at(a.c, page, hk, t) + lane],
-                    e8m0(a.c.vs[scale_at(a.c, page, hk, t) + 4 * (lane / 16)]), 0);
+                const f32x2 x =
+                    expand_pair<T>((unsigned)a.c.vc[code_at(a.c, page, hk, t) + lane],
+                                   e8m0(a.c.vs[scale_at(a.c, page, hk, t) + 4 * (lane / 16)]));
                 o0 = fmaf(pi, x[0], o0);
                 o1 = fmaf(pi, x[1], o1);
             }

@@ -648,3 +648,62 @@ def test_offsets_past_32_bits():
         far = kv4.attn(x, cache, table, i32([300]), 0.1, cu_q=cu, max_q=m)
         near = kv4.attn(x, small, i32([[0, 1]]), i32([300]), 0.1, cu_q=cu, max_q=m)
         assert torch.equal(far, near)
+
+
+def as_fp16(q, host, page, table, n, scale):
+    """{row: (o, tolerance)} of one request's last tokens, its values as fp16 holds them:
+    infinities past 65504, multiples of 2^-24 below the smallest normal number."""
+    T, Hq, D = q.shape
+    at = [(table[0, t // page].item(), t % page) for t in range(n)]
+    k, v = (torch.stack([oc.dequantise(*oc.read_cache(*host[i:i + 2], p, t)) for p, t in at])
+            .half().double() for i in (0, 2))
+    G = Hq // k.shape[1]
+    hide = torch.arange(n)[None] > torch.arange(T)[:, None] + n - T
+    got = [oc.softmax_rows(q[:, h], k[:, h // G], v[:, h // G], scale, hide) for h in range(Hq)]
+    vmax = v.nan_to_num(0.0, 0.0, 0.0).abs().max().item()
+    tols = [oc.tolerance(o, s.nan_to_num(0.0, 0.0, 0.0), z, q.dtype, D, n, vmax) for o, s, z in got]
+    return {r: (torch.stack([g[0][r] for g in got]), torch.stack([t[r] for t in tols]))
+            for r in range(T)}
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("n,news", [(90, 6), (2600, 6), (300, 200), (2600, 150)])
+@pytest.mark.parametrize("what", ["large values", "small keys"])
+def test_hidden_tokens_leave_bf16_rows_read_as_fp16(what, n, news, wide):
+    """fp16 queries over a cache of bf16 rows that fp16 does not hold: a row's result is that of
+    the rounded values, whether a token it does not see holds NaN or not."""
+    D, Hq, page = 128, 4, 64
+    print(f"{what} n {n} news {news} wide {wide}", flush=True)
+    g = torch.Generator().manual_seed(n + news)
+    k = torch.randn(n, 1, D, generator=g)
+    v = torch.randn(n, 1, D, generator=g)
+    q = torch.randn(news, Hq, D, generator=g).half()
+    scale = 0.1
+    if what == "large values":
+        v[7, 0, 3] = 1e5        # the nearest code stands for 98304
+    else:
+        k, q, scale = k * 2.0 ** -26, q * 10000, 1500.0   # scores of some units
+    pages = -(-n // page)
+    perm = torch.randperm(pages, generator=g).int()
+    table = perm[None]
+    if wide:
+        table = torch.cat((table, torch.full((1, 40), -1, dtype=torch.int32)), 1)
+    t = torch.arange(n)
+    slots = (perm[t // page] * page + t % page).int()
+    outs = []
+    for hidden in (1.0, math.nan):
+        v[n - 1, 0, 64:] = hidden
+        cache = kv4.new_cache(pages, page, 1, D)
+        kv4.store(cache, k.bfloat16().to(DEV), v.bfloat16().to(DEV), slots.to(DEV))
+        out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32([n]), scale, cu_q=i32([0, news]),
+                       max_q=news).cpu()
+        rows = as_fp16(q, [x.cpu() for x in cache], page, table, n, scale)
+        for r in range(news - 1):     # (the last row sees the token)
+            o, tol = rows[r]
+            inf = o.isinf()
+            assert torch.equal(out[r].double()[inf], o[inf]), (r, hidden)
+            err = ((out[r].double() - o).abs() / tol)[~inf].max().item()
+            assert err <= 1.0, (r, hidden, err)
+        assert rows[0][0].isinf().any() == (what == "large values")
+        outs.append(out[:-1])
+    assert torch.equal(outs[0].isfinite(), outs[1].isfinite())
