@@ -185,6 +185,7 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
     if (q.numel() == 0 || B == 0) return o;
     const c10::DeviceGuard guard(dev);
     if (max_q < 0 || max_q > T) max_q = T;
+    if (!cu_q.has_value()) max_q = std::min<int64_t>(max_q, 1);  // (as the library plans it)
     // (rows may be done a second time, from q: it is copied where out is q)
     const bool in_place = o.data_ptr() == q.data_ptr();
     const Tensor qr = in_place ? q.clone(at::MemoryFormat::Contiguous) : rows_of(q);

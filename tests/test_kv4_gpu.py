@@ -707,3 +707,19 @@ def test_hidden_tokens_leave_bf16_rows_read_as_fp16(what, n, news, wide):
         assert rows[0][0].isinf().any() == (what == "large values")
         outs.append(out[:-1])
     assert torch.equal(outs[0].isfinite(), outs[1].isfinite())
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,W", [(32, 16, 4, 64), (64, 2, 2, 64), (32, 16, 4, 33), (40, 64, 1, 40)])
+def test_single_tokens_with_room_for_more(B, Hq, Hkv, W):
+    """Without cu_q a request has one query, whatever max_q allows for: tables on either side
+    of the short form's limits."""
+    g = torch.Generator().manual_seed(B + W)
+    lens = [int(n) for n in torch.randint(1, 300, (B,), generator=g)]
+    cache, host, table = filled(lens, 64, Hkv, 64, torch.float16, seed=B)
+    table = torch.cat((table, torch.full((B, W), -1, dtype=torch.int32)), 1)[:, :W].contiguous()
+    q = torch.randn(B, Hq, 64, generator=g).half()
+    want = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.125)
+    check(want, oc.cache_attn(q, host, 64, table, lens, 0.125))
+    for max_q in (2, 17, B, 1000, -1):
+        got = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.125, max_q=max_q)
+        assert torch.equal(got, want), max_q

@@ -211,3 +211,16 @@ def test_python_layer_refuses_on_the_cpu(lib):
     for scale in (0.0, -1.0, float("nan")):
         with pytest.raises(ValueError):
             sparse.attn(x, x, x, scale, 4)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,W", [(32, 16, 4, 64), (64, 2, 2, 64), (40, 64, 1, 40)])
+def test_without_cu_q_a_request_has_one_query(lib, B, Hq, Hkv, W):
+    """The workspace of max_q = 1 is the one that is asked for, whatever max_q is: a larger
+    one would have these tables in the form that needs none, or in the prompts'."""
+    need = lib.kv4_attn_workspace_bytes(B, B, Hq, Hkv, 128, 1, 64 * W)
+    assert need > 0
+    assert lib.kv4_attn_workspace_bytes(B, B, Hq, Hkv, 128, B, 64 * W) != need
+    for max_q in (1, 2, B, 1000):
+        kw = dict(T=B, B=B, Hq=Hq, Hkv=Hkv, W=W, stride=W, max_q=max_q, os=strides(128 * Hq, 128))
+        assert kv4_attn(lib, **kw, n=need - 1) == 1
+        assert b"workspace" in lib.kv4_last_error()
