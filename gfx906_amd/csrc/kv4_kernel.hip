@@ -311,7 +311,7 @@ struct AttnArgs {
     const int* lens;
     const int* cu;  // NULL: one query a request
     int W, T, B, Hq, G, max_q, causal;
-    float scale, qsign;  // |scale| log2(e), at least 1e-30; a negative scale negates q
+    float scale, qsign;  // log2_scale(); a negative scale negates q
     int few_rows, tiles;  // requests of at most so many query rows a kv head go to attn_few_kernel
     // attn_few_kernel's partial results: two slots a workgroup (below).
     int groups, min_units, start_units;
@@ -1598,7 +1598,7 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     a.G = Hq / Hkv;
     a.max_q = cu_q ? std::min(max_q, T) : 1;
     a.causal = causal;
-    a.scale = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+    a.scale = log2_scale(scale);
     a.qsign = scale < 0.f ? -1.f : 1.f;
     a.few_rows = kFewRows;
     a.groups = plan.groups;

@@ -90,6 +90,11 @@ struct LastError {
     const char* get() const { return text[0] ? text : nullptr; }
 };
 
+// |scale| in log2 units, as the kernels multiply scores by it. Never 0, so that a masked score
+// stays -inf and not NaN; the smallest fp32 number, as scores of bf16 rows reach 3e38: times it
+// they are below 1e-6 and weigh alike. (Kernels are built with fp32 denormals.)
+inline float log2_scale(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1.4e-45f); }
+
 // Whether HIP launches so many workgroups (fewer than 2^32 threads in x).
 inline bool launchable(long long groups, int threads) { return groups < (1LL << 32) / threads; }
 

@@ -398,7 +398,7 @@ struct AttnArgs {
     Strides sq, sk, sv, so;
     const int* index;
     int Hq, Hkv, Sq, Skv, D, block, nq, nk, count, causal;
-    float c, qsign;  // |scale| log2(e), at least 1e-30; a negative scale negates q
+    float c, qsign;  // log2_scale(); a negative scale negates q
     // Lists are split in nsplit ranges of a query block's entries; a range writes its
     // unnormalised O (fp32) and (m, l) to the workspace, at row range * rows + row of
     // all heads' rows, and combine_kernel merges them.
@@ -1043,7 +1043,7 @@ extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
     auto st = [](const long long* s) { return Strides{s[0], s[1], s[2]}; };
     AttnArgs a{q, k, v, o, st(q_strides), st(k_strides), st(v_strides), st(o_strides), index,
                Hq, Hkv, Sq, Skv, D, block, blocks_of(Sq, kQBlock), blocks_of(Skv, block), count,
-               causal, fmaxf(fabsf(scale) * kLog2e, 1e-30f), scale < 0.f ? -1.f : 1.f,
+               causal, log2_scale(scale), scale < 0.f ? -1.f : 1.f,
                Skv > 0 ? split_count(B, Hq, Sq, Skv, block, count) : 1, (long long)B * Hq * Sq,
                nullptr, nullptr};
     if (a.nsplit > 1) {

@@ -723,3 +723,15 @@ def test_single_tokens_with_room_for_more(B, Hq, Hkv, W):
     for max_q in (2, 17, B, 1000, -1):
         got = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.125, max_q=max_q)
         assert torch.equal(got, want), max_q
+
+
+@pytest.mark.parametrize("n,news", [(200, 1), (2300, 2), (300, 200)])
+@pytest.mark.parametrize("scale", [0.0, 1e-37, -1e-37])
+def test_small_scales_of_large_bf16_scores(scale, n, news):
+    """Products up to 1e38: a scale of 0 weighs every key alike, one of 1e-37 gives scores of
+    some units."""
+    cache, host, table = filled([n], 64, 1, 64, torch.bfloat16, seed=n, gain=2.0 ** 60)
+    q = torch.randn(news, 2, 64, generator=torch.Generator().manual_seed(n))
+    q = (q * 2.0 ** 60).bfloat16()
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32([n]), scale, cu_q=i32([0, news]), max_q=news)
+    check(out, oc.cache_attn(q, host, 64, table, [n], scale, [0, news]))

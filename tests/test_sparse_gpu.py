@@ -413,3 +413,15 @@ def test_offsets_past_32_bits():
     want = sparse.attn_blocks(q[:, H - 1:], near, near, 0.3, small, block=128)
     # (the lists may be split differently: two fp32 sums of the same weights)
     assert torch.allclose(got[:, H - 1:].float(), want.float(), atol=1e-6, rtol=2 ** -9)
+
+
+@pytest.mark.parametrize("Sq", [1, 200])
+@pytest.mark.parametrize("scale", [0.0, 1e-37, -1e-37])
+def test_small_scales_of_large_bf16_scores(scale, Sq):
+    """Products up to 1e38: a scale of 0 weighs every key alike, one of 1e-37 gives scores of
+    some units."""
+    q, k, v = (rand(1, h, S, 64, seed=h + S, dtype=torch.bfloat16) for h, S in ((2, Sq), (1, 300), (2, 300)))
+    q, k, v = q * 2.0 ** 60, k * 2.0 ** 60, v[:, :1]
+    index = random_index(1, 2, -(-Sq // 128), 5, 4, 1)
+    out = sparse.attn_blocks(q.to(DEV), k.to(DEV), v.to(DEV), scale, index.to(DEV), 64)
+    check(out, *oc.sparse_attn(q, k, v, scale, index, 64, False))
