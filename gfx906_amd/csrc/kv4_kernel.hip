@@ -1563,7 +1563,7 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
     if (q == o) return g_err.fail("kv4_attn: o must not be q");
     const long long oe[2] = {T, Hq};
     if (!rows_apart(o_strides, oe, 2, D)) return g_err.fail("kv4_attn: o's rows overlap");
-    if (!(scale > -INFINITY && scale < INFINITY)) return g_err.fail("kv4_attn: scale must be finite");
+    if (!good_scale(scale)) return g_err.fail("kv4_attn: scale must be finite, and below 2.3e38");
     const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page);
     if (plan.units >= (1LL << 30)) return g_err.fail("kv4_attn: table too wide for so many heads");
     const PromptPlan pp = prompt_plan(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);

@@ -94,6 +94,8 @@ struct LastError {
 // stays -inf and not NaN; the smallest fp32 number, as scores of bf16 rows reach 3e38: times it
 // they are below 1e-6 and weigh alike. (Kernels are built with fp32 denormals.)
 inline float log2_scale(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1.4e-45f); }
+// Whether a scale is a number and finite in these units (a score of 0 would be NaN, else).
+inline bool good_scale(float scale) { return scale == scale && log2_scale(scale) < INFINITY; }
 
 // Whether HIP launches so many workgroups (fewer than 2^32 threads in x).
 inline bool launchable(long long groups, int threads) { return groups < (1LL << 32) / threads; }

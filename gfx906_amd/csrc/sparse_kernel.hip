@@ -1019,8 +1019,8 @@ extern "C" int sparse_attn(const void* q, const void* k, const void* v, void* o,
         return g_err.fail("sparse_attn: at most %d key blocks", SPARSE_MAX_BLOCKS);
     if (count < 1 || count > SPARSE_MAX_COUNT)
         return g_err.fail("sparse_attn: count must be 1 .. %d", SPARSE_MAX_COUNT);
-    if (!(scale > -INFINITY && scale < INFINITY))
-        return g_err.fail("sparse_attn: scale must be finite");
+    if (!good_scale(scale))
+        return g_err.fail("sparse_attn: scale must be finite, and below 2.3e38");
     if (B == 0 || Hq == 0 || Sq == 0) return 0;
     if (!q || !o || !index || (Skv > 0 && (!k || !v)) || !q_strides || !k_strides || !v_strides ||
         !o_strides)

@@ -224,3 +224,10 @@ def test_without_cu_q_a_request_has_one_query(lib, B, Hq, Hkv, W):
         kw = dict(T=B, B=B, Hq=Hq, Hkv=Hkv, W=W, stride=W, max_q=max_q, os=strides(128 * Hq, 128))
         assert kv4_attn(lib, **kw, n=need - 1) == 1
         assert b"workspace" in lib.kv4_last_error()
+
+
+@pytest.mark.parametrize("scale", [2.5e38, -3e38, float("inf"), float("-inf"), float("nan")])
+def test_scales_past_fp32_in_log2_units_are_refused(lib, scale):
+    """Scores are multiplied by scale * log2(e), which must not be infinite."""
+    assert kv4_attn(lib, scale=scale) == 1 and b"finite" in lib.kv4_last_error()
+    assert sparse_attn(lib, scale=scale) == 1 and b"finite" in lib.sparse_last_error()
