@@ -2,11 +2,12 @@
 // blocks by the product of means, and attention over the chosen blocks. The entry
 // points are described in gfx906_amd_attn.h.
 //
-// The choice is an output (and decides what is read), so it must not hang on the
-// order of a sum: block sums are taken in fp64, where sums of 128 fp16 values are
-// exact, and rounded once to fp32; products of two fp32 are exact in fp64 and add
-// up there. Scores of different blocks closer than 1e-15 relative are as good as
-// never seen; equal ones go by the index.
+// The choice is an output (and decides what is read), so it must be the same by whichever
+// kernel it is made. Block sums are taken in fp64, exact for fp16 rows (and for bf16 rows
+// unless the values of a dim lie more than 38 octaves apart), by block_sum() alone, and rounded
+// once to fp32. Products of two such means are exact in fp64; both kernels that add them up do
+// it in one order (kChain): blocks whose scores differ by less than its error, 2^-48 sum |q k|,
+// may change places against exact sums, but alike in every call. Equal sums go by the index.
 #include "longctx_tile.h"
 
 #include <algorithm>
@@ -32,40 +33,52 @@ struct MeansArgs {
     long long blocks;  // of all heads
 };
 
-// One wave per block of rows: a lane reads 16 bytes (8 dims) of a row, so that a load
-// takes 4 (D = 128) or 8 (D = 64) whole rows, 16 loads in flight; the lanes that hold
-// the same dims add up at the end. Bound by the bytes of x: 16 heads of 16384, D = 128, 14.5
-// us (4.6 TB/s).
+#if defined(__HIP_DEVICE_COMPILE__)
+// Column sums of `rows` rows, V dims a lane, N loads in flight: D/8 lanes beside each other
+// take a row, a wave 512/D rows at a time, and the lanes that hold the same dims add up at the
+// end (all of them have the sum). A dim's sum is added up in the same order whatever V and N.
+// x: the lane's dims of the first row.
+template <int D, int V, int N, class T>
+__device__ __forceinline__ void block_sum(const T* x, long long stride, int rows, double (&sum)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    constexpr int LPR = D / 8, RPL = 64 / LPR;
+    const int r = (threadIdx.x & 63) / LPR;
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = 0.0;
+    for (int t = 0; t < rows; t += N * RPL) {
+        vec v[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int row = t + n * RPL + r;
+            v[n] = vec{};
+            if (row < rows) v[n] = *reinterpret_cast<const vec*>(x + row * stride);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[e] += (double)(float)v[n][e];
+    }
+#pragma unroll
+    for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += __shfl_xor(sum[e], o);
+}
+#endif
+
+// One wave per block of rows, 16 bytes a lane: a load takes 4 (D = 128) or 8 (D = 64) whole rows.
+// Bound by the bytes of x: 16 heads of 16384, D = 128, 14.5 us (4.6 TB/s).
 template <int D, class T>
 __global__ void __launch_bounds__(256) means_kernel(const MeansArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using x8 = typename Elem<T>::x8;
-    constexpr int LPR = D / 8, RPL = 64 / LPR, N = 16;
+    constexpr int LPR = D / 8;
     const int lane = threadIdx.x & 63;
     const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= a.blocks) return;
     const int j = (int)(id % a.nb), bh = (int)(id / a.nb), b = bh / a.H, h = bh - b * a.H;
     const int r0 = j * a.block, rows = min(a.block, a.S - r0);
     const int c = lane % LPR, r = lane / LPR;
-    const T* x = (const T*)a.x + b * a.sb + h * a.sh + r0 * a.ss + c * 8;
-    double sum[8] = {};
-    for (int t = 0; t < rows; t += N * RPL) {
-        x8 v[N];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int row = t + n * RPL + r;
-            v[n] = x8{};
-            if (row < rows) v[n] = *reinterpret_cast<const x8*>(x + row * a.ss);
-        }
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += (double)(float)v[n][e];
-    }
-#pragma unroll
-    for (int o = LPR; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], o);
+    double sum[8];
+    block_sum<D, 8, 16>((const T*)a.x + b * a.sb + h * a.sh + r0 * a.ss + c * 8, a.ss, rows, sum);
     if (r == 0) {
         float* m = a.means + id * D + c * 8;
         f32x4 lo, hi;
@@ -113,9 +126,15 @@ __host__ __device__ inline Reach reach(int i, int Sq, int Skv, int block, int nk
 // through tiles of 16 key blocks. In step s of a tile lane group g supplies dim
 // g D/4 + s, so that a lane reads D/4 consecutive floats of its row.
 //
+// Order of a score's sum (here and in choose_one_kernel): v_mfma_f64_16x16x4 adds its four
+// products to the accumulator one after another, each rounded once, as four fmas do. kChain
+// steps make a chain of 4 kChain dims that starts at 0, and chains are added pairwise, neighbours
+// first.
+//
 // 8 heads, 1024 x 1024 blocks, D = 64: 35 us, for 67 MB of scores; 16 heads, 128 x 256, 9.5.
 //
 // grid: row tiles, kv heads of all batches, shares of the key tiles; 4 waves.
+constexpr int kChain = 4;
 template <int D>
 __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -146,15 +165,24 @@ __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
         f32x4 k[N / 4];
 #pragma unroll
         for (int s = 0; s < N / 4; ++s) k[s] = *reinterpret_cast<const f32x4*>(p + 4 * s);
-        f64x4 c = {};
+        f64x4 sum[N / kChain];
 #pragma unroll
-        for (int s = 0; s < N; ++s)
-            c = __builtin_amdgcn_mfma_f64_16x16x4f64(q[s], (double)k[s / 4][s % 4], c, 0, 0, 0);
+        for (int x = 0; x < N / kChain; ++x) {
+            f64x4 c = {};
+#pragma unroll
+            for (int s = x * kChain; s < (x + 1) * kChain; ++s)
+                c = __builtin_amdgcn_mfma_f64_16x16x4f64(q[s], (double)k[s / 4][s % 4], c, 0, 0, 0);
+            sum[x] = c;
+        }
+#pragma unroll
+        for (int o = 1; o < N / kChain; o *= 2)
+#pragma unroll
+            for (int x = 0; x < N / kChain; x += 2 * o) sum[x] += sum[x + o];
         // (accumulator element e: row 4 e + l/16, column l%16)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int r = r0 + 4 * e + g, j = 16 * t + i;
-            if (r < rows && j < a.nk) a.score[row_of(r) * a.nk + j] = c[e];
+            if (r < rows && j < a.nk) a.score[row_of(r) * a.nk + j] = sum[0][e];
         }
     }
 #endif
@@ -291,8 +319,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) select_kernel(c
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// Adds up N = 8 or 16 neighbouring lanes (DPP moves within rows of 16: a swap of
-// neighbours, of pairs, and mirrors of what is then equal in halves).
+// Adds up N = 4 or 8 neighbouring lanes, pairwise (DPP moves within rows of 16: a swap of
+// neighbours, of pairs, and a mirror of what is then equal in halves).
 template <int CTRL>
 __device__ __forceinline__ double dpp_add(double x) {
     const long long b = __double_as_longlong(x);
@@ -304,75 +332,74 @@ template <int N>
 __device__ __forceinline__ double lanes_sum(double x) {
     x = dpp_add<0xB1>(x);   // quad_perm [1, 0, 3, 2]
     x = dpp_add<0x4E>(x);   // quad_perm [2, 3, 0, 1]
-    x = dpp_add<0x141>(x);  // row_half_mirror
-    if constexpr (N == 16) x = dpp_add<0x140>(x);  // row_mirror
+    if constexpr (N == 8) x = dpp_add<0x141>(x);  // row_half_mirror
     return x;
 }
 #endif
 
 // The choice straight from the query rows: mean, scores and choice of a query block in one
 // workgroup, of up to 4096 key blocks, where the launches of three kernels outweigh that every
-// block reads all key means (one_kernel below). D/8 lanes take a row (of q or of the means)
-// and add up their parts. 64 heads of one query, 512 blocks: 12.4 us, and 19 in three kernels.
+// block reads all key means (one_kernel below). Four waves take the mean; then
+// D/16 lanes take a row of the key means, a chain of score_kernel's order each. 64 heads of
+// one query, 512 blocks: 12.4 us, and 19 in three kernels.
 template <int D, class T>
 __global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int LPR = D / 8, ROWS = 512 / LPR;  // lanes a row, rows at a time
+    // dims of a lane group in score_kernel; lanes a row, rows at a time
+    constexpr int N = D / 4, LPR = N / kChain, ROWS = 512 / LPR;
+    static_assert(kChain == 4, "a chain is a 16-byte load of every group");
     __shared__ double score[4096];
-    __shared__ double part_q[8][D];
-    __shared__ float qs[D];
+    __shared__ __attribute__((aligned(16))) float qs[D];
     __shared__ int part[2][8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, wave = tid >> 6;
     const int bh = blockIdx.x / a.nq, i = blockIdx.x - bh * a.nq, b = bh / a.Hq, h = bh - b * a.Hq;
     const int kvh = b * a.Hkv + h / (a.Hq / a.Hkv);
+    if (wave < 4) {  // D/4 dims a wave
+        const int rows = min(kQBlock, a.Sq - i * kQBlock), d = 2 * (wave * (D / 8) + tid % (D / 8));
+        double sum[2];
+        block_sum<D, 2, kQBlock * D / 512>(
+            (const T*)a.q + b * a.qb + h * a.qh + (long long)i * kQBlock * a.qs + d, a.qs, rows, sum);
+        if (tid % 64 < D / 8) *reinterpret_cast<f32x2*>(qs + d) =
+            f32x2{(float)(sum[0] / rows), (float)(sum[1] / rows)};
+    }
+    __syncthreads();
     const int c = tid % LPR, r0 = tid / LPR;
-    const int rows = min(kQBlock, a.Sq - i * kQBlock);
-    double sum[8] = {};
-    const T* q = (const T*)a.q + b * a.qb + h * a.qh + (long long)i * kQBlock * a.qs + c * 8;
-    for (int r = r0; r < rows; r += ROWS) {
-        const typename Elem<T>::x8 x = *reinterpret_cast<const typename Elem<T>::x8*>(q + r * a.qs);
+    double qd[4][4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += (double)(float)x[e];
-    }
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-    for (int o = LPR; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], o);
-    if (lane < LPR)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) part_q[wave][8 * c + e] = sum[e];
-    __syncthreads();
-    if (tid < D) {
-        double s = 0.0;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) s += part_q[w][tid];
-        qs[tid] = (float)(s / rows);
-    }
-    __syncthreads();
-    double qd[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) qd[e] = qs[8 * c + e];
+        for (int e = 0; e < 4; ++e) qd[g][e] = qs[g * N + c * 4 + e];
     const Reach r = reach(i, a.Sq, a.Skv, a.block, a.nk, a.causal);
-    const float* km = a.km + (long long)kvh * a.nk * D + c * 8;
-    constexpr int U = 8;
-    for (int j0 = r0; j0 < r.seen; j0 += U * ROWS) {
-        f32x4 x[U][2];
+    const float* km = a.km + (long long)kvh * a.nk * D + c * 4;
+    // U rows a lane at a time: 512 in all, or 128 of a short sequence (512 queries of 32 heads, 64
+    // blocks, D = 128: 8.8 us a call, and 10.6 with 512).
+    auto rows_by = [&](auto per) __attribute__((always_inline)) {
+        constexpr int U = decltype(per)::value;
+        for (int j0 = r0; j0 < r.seen; j0 += U * ROWS) {
+            f32x4 x[U][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float* p = km + (long long)min(j0 + u * ROWS, r.seen - 1) * D;
-            x[u][0] = *reinterpret_cast<const f32x4*>(p);
-            x[u][1] = *reinterpret_cast<const f32x4*>(p + 4);
+            for (int u = 0; u < U; ++u) {
+                const float* p = km + (long long)min(j0 + u * ROWS, r.seen - 1) * D;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) x[u][g] = *reinterpret_cast<const f32x4*>(p + g * N);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                double s = 0.0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) s = fma(qd[g][e], (double)x[u][g][e], s);
+                s = lanes_sum<LPR>(s);
+                const int j = j0 + u * ROWS;
+                if (c == 0 && j < r.seen) score[j] = s;
+            }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            double s = 0.0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s = fma(qd[e], (double)x[u][e / 4][e % 4], s);
-            s = lanes_sum<LPR>(s);
-            const int j = j0 + u * ROWS;
-            if (c == 0 && j < r.seen) score[j] = s;
-        }
-    }
+    };
+    if (r.seen <= 128)
+        rows_by(std::integral_constant<int, 128 / ROWS>{});
+    else
+        rows_by(std::integral_constant<int, 512 / ROWS>{});
     __syncthreads();
     int* out = a.index + (long long)blockIdx.x * a.count;
     auto at = [&](int j) { return score[j]; };

@@ -7,7 +7,8 @@
     out = sparse.attn_blocks(q, k, v, scale, index)
 
 A block's score is the product of the query block's mean and the key block's mean,
-computed so that the choice does not hang on the order of a sum (see
+added up in 64 bits in one order, so that the choice is the same whichever of these
+calls makes it, and for a query alone or in a batch (see
 ``include/gfx906_amd_attn.h``). q is ``[B, Hq, Sq, D]``, k and v
 ``[B, Hkv, Skv, D]``, fp16 or bf16, D 64 or 128, Hq a multiple of Hkv; strided views
 with a contiguous head dim are read in place. All calls run on the current stream

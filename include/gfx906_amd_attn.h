@@ -258,8 +258,9 @@ int sparse_block_means(const void* x, const long long* strides, int dtype, int B
 
 /* index[b][h][i][0..count): the key blocks of query block i, ascending, -1 behind
  * the last. Taken are those with the largest product of q_means[b][h][i] and
- * k_means[b][h / (Hq/Hkv)][j] (fp64; NaN counts as largest, equal products by the
- * lower index). Means are packed fp32 [B, Hq, ceil(Sq/128), D] and
+ * k_means[b][h / (Hq/Hkv)][j] (NaN counts as largest, equal products by the lower index).
+ * A product is added up in fp64, within 2^-48 sum |q k| of the exact one and always in the
+ * same order: sizes and the entry point do not change a choice. Means are packed fp32 [B, Hq, ceil(Sq/128), D] and
  * [B, Hkv, ceil(Skv/block), D], 16-byte aligned. With causal != 0 query row r stands at key position
  * r + Skv - Sq; blocks past the query block's last position are never taken, and
  * those that hold its own positions always (count must be at least 128/block + 1,

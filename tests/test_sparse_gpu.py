@@ -425,3 +425,42 @@ def test_small_scales_of_large_bf16_scores(scale, Sq):
     index = random_index(1, 2, -(-Sq // 128), 5, 4, 1)
     out = sparse.attn_blocks(q.to(DEV), k.to(DEV), v.to(DEV), scale, index.to(DEV), 64)
     check(out, *oc.sparse_attn(q, k, v, scale, index, 64, False))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_choice_is_the_same_by_every_way(D, dtype):
+    """Scores whose sums nearly cancel, and differ in the last bits by the order in which they
+    are added: choose, select, and a query alone or in a batch take the same blocks."""
+    g = torch.Generator().manual_seed(D)
+    nk, count = 500, 40
+    # Permutations of one set of terms over 50 octaves: equal sums, in no order alike in fp64.
+    terms = torch.randn(D // 2, generator=g)
+    terms *= torch.exp2(torch.randint(-50, 1, terms.shape, generator=g).float())
+    terms = torch.cat((terms, -terms * (1 + 2.0 ** -20)))
+    km = torch.stack([terms[torch.randperm(D, generator=g)] for _ in range(nk)])[None, None]
+    q = torch.ones(1, 1, 1, D, dtype=dtype)
+    alone = sparse.choose(q.to(DEV), km.to(DEV), count, nk * 64)
+    picked = sparse.select(sparse.block_means(q.to(DEV), 128), km.to(DEV), count, 1, nk * 64)
+    assert torch.equal(alone, picked)
+    # (so many heads go through three kernels)
+    many = sparse.choose(q.expand(1, 400, 1, D).contiguous().to(DEV), km.to(DEV), count, nk * 64)
+    assert torch.equal(many, alone.expand(1, 400, 1, count))
+
+
+@pytest.mark.parametrize("Sq", [1, 100, 128, 300])
+@pytest.mark.parametrize("D", [64, 128])
+def test_means_of_wide_bf16_rows_are_the_same_by_every_way(D, Sq):
+    """bf16 rows over 80 octaves, most of which cancel: fp64 sums depend on their order, and the
+    choice from the rows is that from block_means all the same."""
+    g = torch.Generator().manual_seed(D + Sq)
+    x = torch.randn(2, Sq, 1, D, generator=g)
+    x *= torch.exp2(torch.randint(-40, 41, x.shape, generator=g).float())
+    x[:, Sq // 2:Sq // 2 * 2] = -x[:, :Sq // 2].flip(1)
+    q = x.transpose(1, 2).bfloat16()
+    km = torch.randn(2, 1, 300, D, generator=g).to(DEV)
+    means = sparse.block_means(q.to(DEV), 128)
+    want = sparse.select(means, km, 20, Sq, 300 * 64)
+    assert torch.equal(sparse.choose(q.to(DEV), km, 20, 300 * 64), want)
+    many = sparse.choose(q.expand(2, 200, Sq, D).contiguous().to(DEV), km, 20, 300 * 64)
+    assert torch.equal(many, want.expand(2, 200, -1, 20))
