@@ -735,3 +735,17 @@ def test_small_scales_of_large_bf16_scores(scale, n, news):
     q = (q * 2.0 ** 60).bfloat16()
     out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32([n]), scale, cu_q=i32([0, news]), max_q=news)
     check(out, oc.cache_attn(q, host, 64, table, [n], scale, [0, news]))
+
+
+def test_rows_of_two_requests_are_one_of_theirs():
+    """Bounds [0, 5, 3, 9]: rows 3 and 4 belong to requests 0 and 2, the others to one."""
+    lens, cu = [100, 70, 64], [0, 5, 3, 9]
+    cache, host, table = filled(lens, 64, 1, 64, torch.float16, seed=2)
+    q = torch.randn(9, 2, 64, generator=torch.Generator().manual_seed(1)).half()
+    out = kv4.attn(q.to(DEV), cache, table.to(DEV), i32(lens), 0.1, cu_q=i32(cu))
+    first = oc.cache_attn(q, host, 64, table[:1], lens[:1], 0.1, [0, 5])
+    last = oc.cache_attn(q, host, 64, table[2:], lens[2:], 0.1, [3, 9])
+    check(out, {r: first[r] for r in range(3)} | {r: last[r] for r in range(5, 9)})
+    for r in (3, 4):   # (four dims at a time may come from either)
+        off = [(out[r].double().cpu() - o).abs() <= tol for o, tol in (first[r], last[r])]
+        assert (off[0] | off[1]).all(), r

@@ -231,3 +231,21 @@ def test_scales_past_fp32_in_log2_units_are_refused(lib, scale):
     """Scores are multiplied by scale * log2(e), which must not be infinite."""
     assert kv4_attn(lib, scale=scale) == 1 and b"finite" in lib.kv4_last_error()
     assert sparse_attn(lib, scale=scale) == 1 and b"finite" in lib.sparse_last_error()
+
+
+def test_workspaces_that_calls_need_are_not_empty(lib):
+    """Long tables and short query lists are split, and ask for all of what the sizing calls say."""
+    need = lib.kv4_attn_workspace_bytes(4, 4, 8, 2, 128, 1, 64000)
+    assert need > 0
+    for bad in (dict(n=need - 1), dict(n=0), dict(ws=None), dict(ws=FAKE + 4, n=need)):
+        assert kv4_attn(lib, W=1000, stride=1000, **bad) == 1
+        assert b"workspace" in lib.kv4_last_error()
+    prompt = lib.kv4_attn_workspace_bytes(400, 4, 8, 2, 128, 300, 64000)
+    assert prompt > need
+    assert kv4_attn(lib, W=1000, stride=1000, T=400, cu=FAKE, max_q=300, n=prompt - 1) == 1
+    assert b"workspace" in lib.kv4_last_error()
+    need = lib.sparse_attn_workspace_bytes(2, 4, 1, 32768, 128, 64, 64)
+    assert need > 0
+    for bad in (dict(n=need - 1), dict(n=0), dict(ws=None), dict(ws=FAKE + 4, n=need)):
+        assert sparse_attn(lib, Sq=1, Skv=32768, count=64, **bad) == 1
+        assert b"workspace" in lib.sparse_last_error()
