@@ -235,8 +235,9 @@ __device__ __forceinline__ Piece piece(const Cache& c, unsigned id, int ds) {
 #endif
 
 // A lane stores a block of 32 values: four 16-byte loads in flight, no exchange. Bound by
-// bytes: 16384 rows of 16 heads, D = 128, 34 us (5.0 TB/s); a lane per 8 values,
-// with the block's maximum exchanged between four, takes 45. grid.y: K, V.
+// bytes: 16384 rows of 16 heads, D = 128, 41 us (4.1 TB/s), and 34 where the last-level cache
+// holds rows; there a lane per 8 values, with the block's maximum exchanged between four, takes 45.
+// grid.y: K, V.
 template <class T>
 __global__ void __launch_bounds__(256) store_kernel(const RowArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(256) store_kernel(const RowArgs a) {
 #endif
 }
 
-// Rows back: a lane per 8 values, so that a wave's 16-byte stores are contiguous; 35 us
+// Rows back: a lane per 8 values, so that a wave's 16-byte stores are contiguous; 34 us
 // for as many rows, and 45 with a lane per 32 values.
 template <class T>
 __global__ void __launch_bounds__(256) load_kernel(const RowArgs a) {
@@ -461,9 +462,11 @@ struct Codes {
 //
 // DIRECT: short tables. One workgroup a head, no runs, no slots and no second kernel.
 //
-// 32 requests of 100 .. 16384 tokens, 8 kv heads of 128, one query each: 23 us and 5 for the
-// merge (103 MB: 3.6 TB/s in all); 131072 tokens, 2 kv heads, 32 rows: 17 and 6 (what is left above
-// the bytes' 7 us is two units' latency a wave, and the merge); 1024 tokens, 16 heads of 64, in
+// 32 requests of 100 .. 16384 tokens, 8 kv heads of 128, one query each: 26 us and 5 for the
+// merge (103 MB: 3.3 TB/s in all); 131072 tokens, 2 kv heads, 32 rows: 17 and 6, of which the bytes
+// take 7, with two units a wave. 262144 tokens take 26 and 524288 36, 2.6 us more for every unit a
+// wave, and 16384 tokens (34 workgroups) still 15: some ten of the 17 are a run's start (the search,
+// Q, first loads) and end (eight waves' merge, partial results); 1024 tokens, 16 heads of 64, in
 // DIRECT: 7.
 template <int D, class T, int NB, bool DIRECT>
 __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kernel(const AttnArgs a) {
@@ -971,9 +974,12 @@ __global__ void __launch_bounds__(1024) prompt_plan_kernel(const AttnArgs a) {
 // K and V have two buffers each: after the barrier of chunk w those of K(w) and V(w-1) are
 // free for K(w+2) and V(w+1).
 //
-// 3 prompts of 77 .. 2111 queries behind 300 .. 8192 tokens, 16/4 heads of 128: 203 us (173
-// GFLOP: 850 TFLOP/s; a library product of 8192 reaches 1180), bound as attn_tile_kernel is.
-// Small batches are bound by a run's start: two tiles' loads and merges, 20 us.
+// 3 prompts of 77 .. 2111 queries behind 300 .. 8192 tokens, 16/4 heads of 128: 175 us (173
+// GFLOP: 990 TFLOP/s; a library product of 8192 reaches 1180), and 206 in the first calls of a
+// process. No unit is full: the matrix pipe is busy for 44 % of the clocks (at 2.25 GHz), the vector
+// unit for 42, LDS for 42, a quarter of that in bank conflicts, which the stores of expanded tiles
+// have (the same reads in attn_tile_kernel have none). Small batches are bound by a run's start:
+// two tiles' loads and merges, 20 us.
 //
 // SELF: few tiles. Every workgroup adds up the tiles itself, as in attn_few_kernel, instead
 // of a kernel before this one.

@@ -222,8 +222,8 @@ struct Tile {
     // another (kt, Sn), and P of the block S between them, in the order written: behind every
     // fragment's products the read of the fragment AV (V) or AK (K) further on, and a share
     // of the softmax, so that a wave's own instructions fill the matrix pipe's time. (The
-    // compiler's order has all products before all exponentials: 16 heads of 16384 tokens,
-    // 32 blocks of 64, 300 us and 284 this way; a 4-bit cache's prompts 218 and 201.)
+    // compiler's order has all products before all exponentials: the call of 16 heads of 16384
+    // tokens, 32 blocks of 64, 300 us and 284 this way; a 4-bit cache's prompts 218 and 201.)
     __device__ __forceinline__ void turn(const char* vt, const x8 (&Pp)[NB], const char* kt,
                                          f32x4 (&Sn)[2][NB], const f32x4 (&S)[2][NB], x8 (&P)[NB],
                                          float c) {

@@ -66,7 +66,8 @@ __device__ __forceinline__ void block_sum(const T* x, long long stride, int rows
 #endif
 
 // One wave per block of rows, 16 bytes a lane: a load takes 4 (D = 128) or 8 (D = 64) whole rows.
-// Bound by the bytes of x: 16 heads of 16384, D = 128, 14.5 us (4.6 TB/s).
+// Bound by the bytes of x: 16 heads of 16384, D = 128, 17 us
+// (4.0 TB/s), and 13 where the last-level cache holds rows.
 template <int D, class T>
 __global__ void __launch_bounds__(256) means_kernel(const MeansArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -131,7 +132,7 @@ __host__ __device__ inline Reach reach(int i, int Sq, int Skv, int block, int nk
 // steps make a chain of 4 kChain dims that starts at 0, and chains are added pairwise, neighbours
 // first.
 //
-// 8 heads, 1024 x 1024 blocks, D = 64: 35 us, for 67 MB of scores; 16 heads, 128 x 256, 9.5.
+// 8 heads, 1024 x 1024 blocks, D = 64: 33 us, for 67 MB of scores; 16 heads, 128 x 256, 8.4.
 //
 // grid: row tiles, kv heads of all batches, shares of the key tiles; 4 waves.
 constexpr int kChain = 4;
@@ -195,8 +196,8 @@ __global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
 // scores equal to it fill up in the order of their index. The upper 32 bits go first, by
 // themselves; the lower ones matter only among scores whose upper bits are the bound's.
 // Everything stays in registers; a step is a compare and a population count per 64 scores
-// (and, with several waves, an exchange through LDS). 8192 rows of 1024 scores: 41 us; 2048 of
-// 256: 7.5.
+// (and, with several waves, an exchange through LDS). 8192 rows of 1024 scores: 36 us; 2048 of
+// 256: 6.6.
 #if defined(__HIP_DEVICE_COMPILE__)
 template <int WAVES, int K, class Score>
 __device__ __forceinline__ void choose(const SelectArgs& a, const Reach& r, Score score, int* out,
@@ -341,7 +342,7 @@ __device__ __forceinline__ double lanes_sum(double x) {
 // workgroup, of up to 4096 key blocks, where the launches of three kernels outweigh that every
 // block reads all key means (one_kernel below). Four waves take the mean; then
 // D/16 lanes take a row of the key means, a chain of score_kernel's order each. 64 heads of
-// one query, 512 blocks: 12.4 us, and 19 in three kernels.
+// one query, 512 blocks: 11 to 13 us, and 19 in three kernels.
 template <int D, class T>
 __global__ void __launch_bounds__(512) choose_one_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -512,11 +513,13 @@ __device__ __forceinline__ int xcd_order(int w, int n) {
 // would not keep out of the sums); where there are any the wave does its rows again by
 // attend_row.
 //
-// 16 heads of 16384 tokens, 32 blocks of 64, D = 128: 280 us (980 TFLOP/s; 311 and 885 once the
-// card has slowed down under load, where a library product of 8192 reaches 1130); 8 heads of
-// 131072, 64 blocks of 128, D = 64: 2.3 ms (955). Reads of LDS take 1024 of the matrix pipe's
-// 1088 clocks a pair of steps, as a fragment serves 32 rows, and loads into it 256 more: that and
-// the card's power bound it. Single queries are bound by the blocks' bytes (138 MB in 22 us).
+// 16 heads of 16384 tokens, 32 blocks of 64, D = 128: 259 us (1060 TFLOP/s, where a library
+// product of 8192 reaches 1130; 293 in the first calls of a process): the matrix pipe is busy for
+// 56 % of the clocks, the vector unit for 46, LDS for 27, at 1.98 GHz. 8 heads of 131072, 64 blocks
+// of 128, D = 64: 2.25 ms (977): 60, 72 and 27 % at 1.71 GHz, with twice the exponentials a product.
+// So the matrix and the vector unit's work, which the two waves of a SIMD overlap in part, and the
+// clock that the card keeps under it (2.4 GHz at most) bound it, not LDS. Single queries are bound
+// by the blocks' bytes (138 MB in 21 us).
 template <int D, class T, int TPB, bool FAR>
 __global__ void __launch_bounds__(256, 2) attn_tile_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)

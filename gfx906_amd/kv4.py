@@ -93,9 +93,9 @@ def attn(q, cache, table, lens, scale, cu_q=None, max_q=None, causal=True, out=N
     Rows ``cu_q[b] .. cu_q[b+1]`` (int32 ``[B + 1]``) are the queries of request b,
     which holds ``lens[b]`` tokens (int32 ``[B]``) in the pages of ``table``'s row b;
     without ``cu_q`` row b is the one query of request b. With ``causal`` they are
-    the request's last tokens and see none behind themselves. ``max_q``: at least the
-    most queries of a request (queries past it are not computed); without it T is
-    taken, and a decoding step pays for what it does not need. Rows outside
+    the request's last tokens and see none behind themselves. ``max_q``, for ``cu_q``: at
+    least the most queries of a request (queries past it are not computed); without it
+    T is taken, and a decoding step pays for what it does not need. Rows outside
     every request are left as they were (in a new tensor: unset). ``out`` may be ``q``
     itself and must not overlap the other arguments otherwise. Rows that see no
     key are 0; keys without a page weigh nothing."""

@@ -57,7 +57,7 @@ def attn_blocks(q, k, v, scale, index, block=64, causal=False, out=None):
 def attn(q, k, v, scale, count, block=64, causal=False, k_means=None, out=None):
     """Attention over the ``count`` best key blocks of every query block; returns the
     output and the choice (see ``select``). ``k_means``: ``block_means(k, block)``
-    where the program holds them. ``scale`` must be positive, as the choice takes the
+    where the program holds them (copied here unless packed). ``scale`` must be positive, as the choice takes the
     largest products."""
     if not scale > 0:
         raise ValueError("sparse.attn: scale must be positive")
