@@ -216,7 +216,8 @@ int kv4_load(void* k, void* v, int dtype, int T, int Hkv, int D, const int* slot
  * h / (Hq / Hkv). With causal != 0 the n queries of a request are its last n tokens
  * and see no later one; otherwise they see all of its tokens. A row that sees no key, or
  * only such of score -inf, is 0; a token that a row does not see adds nothing to it, whatever
- * it holds. Keys in pages outside [0, pages) or behind the table's last column weigh
+ * it holds (of an infinite value that it does see, with a weight that the element type rounds
+ * to 0, comes an infinity or NaN). Keys in pages outside [0, pages) or behind the table's last column weigh
  * nothing; cu_q is taken as clamped to 0 .. T. Rows outside every request, and queries
  * past the first max_q of one, are left as they were. q and o: strides {token, head} in
  * elements, head dim contiguous, q's rows 16-byte and o's 8-byte aligned; o's must
@@ -283,7 +284,7 @@ int sparse_choose(const void* q, const long long* q_strides, int dtype, const fl
  * checked by the host: an entry outside 0 .. ceil(Skv/block)-1, or not above every
  * valid entry before it, is passed over). causal as above. A row that sees no key,
  * or only such of score -inf, is 0; a key that a row does not see adds nothing to it, whatever
- * it holds. q, k, v: rows 16-byte aligned (k's and v's
+ * it holds (infinite values that it does see: as in kv4_attn). q, k, v: rows 16-byte aligned (k's and v's
  * apart, their strides at most 2^22); o: 8-byte, rows that do not overlap each other, k, v or
  * index; o may be q (the same rows).
  * workspace: 16-byte aligned, sparse_attn_workspace_bytes() bytes (may be 0). */
