@@ -4,26 +4,18 @@
 // synchronising; what cannot be run raises RuntimeError.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 
 #include "bindings.h"
 #include "gfx906_amd_attn.h"
+#include "tensors.h"
 
 namespace {
 
-using torch::Tensor;
+using namespace gfx906_amd;
 
 int dtype_of(at::ScalarType t, const char* who) {
     TORCH_CHECK(t == torch::kHalf || t == torch::kBFloat16, who, ": fp16 or bf16 needed");
     return t == torch::kBFloat16 ? KV4_DTYPE_BF16 : KV4_DTYPE_F16;
-}
-
-void check_ints(const Tensor& t, int64_t n, const c10::Device& dev, const char* who,
-                const char* name) {
-    TORCH_CHECK(t.device() == dev && t.dtype() == torch::kInt && t.dim() == 1 &&
-                    (n < 0 || t.size(0) == n) && t.is_contiguous(),
-                who, ": ", name, " must be a contiguous int32 vector of the right length on the "
-                "other tensors' device");
 }
 
 // The four tensors of a cache, checked against each other.
@@ -52,19 +44,6 @@ struct Parts {
     }
 };
 
-// [T, H, D] rows the kernels read in place: contiguous head dim, the other strides
-// multiples of 8, 16-byte aligned. Anything else is copied.
-Tensor rows_of(const Tensor& t) {
-    const bool ok = (t.stride(2) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
-                    (t.size(0) == 1 || (t.stride(0) >= 0 && t.stride(0) % 8 == 0)) &&
-                    (t.size(1) == 1 || (t.stride(1) >= 0 && t.stride(1) % 8 == 0));
-    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-std::array<long long, 2> strides2(const Tensor& t) {
-    return {t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1)};
-}
-
-hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
 void check_rc(int rc) {
     TORCH_CHECK(rc == 0, "kernel: ", kv4_last_error() ? kv4_last_error() : "launch failed");
 }
@@ -166,10 +145,7 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
         check_ints(*cu_q, B + 1, dev, who, "cu_q");
     else
         TORCH_CHECK(T == B, who, ": without cu_q, one query a request");
-    TORCH_CHECK(table.device() == dev && table.dtype() == torch::kInt && table.dim() == 2 &&
-                    table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) &&
-                    (B <= 1 || table.stride(0) >= 0) && table.size(1) * c.page < (1LL << 31),
-                who, ": table must be int32 [B, W] with contiguous rows of fewer than 2^31 tokens");
+    check_table(table, B, c.page, dev, who);
     Tensor o;
     if (out.has_value()) {
         o = *out;
@@ -198,7 +174,7 @@ Tensor kv4_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor 
     check_rc(kv4_attn(qr.data_ptr(), o.data_ptr(), sq.data(), so.data(), dt, (int)T, (int)B,
                       (int)Hq, c.Hkv, c.D, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(),
                       vs.data_ptr(), c.pages, c.page, table.data_ptr<int>(),
-                      B <= 1 ? W : table.stride(0), W, lens.data_ptr<int>(),
+                      table_stride(table), W, lens.data_ptr<int>(),
                       cu_q.has_value() ? cu_q->data_ptr<int>() : nullptr, (int)max_q, (float)scale,
                       causal, bytes ? ws.data_ptr() : nullptr, bytes, stream()));
     return o;

@@ -6,6 +6,7 @@
 // in one instruction (v_cvt_scalef32_*), rounding to nearest even and
 // saturating, so the format costs half an instruction a value to read.
 #include "longctx_tile.h"
+#include "paged.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -329,34 +330,6 @@ struct AttnArgs {
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// Loads of arrays that no kernel of a call writes, through the scalar cache where the
-// index is uniform.
-typedef const __attribute__((address_space(4))) int* ConstInts;
-__device__ __forceinline__ int cu_at(const AttnArgs& a, int b) {
-    return a.cu ? min(max(((ConstInts)a.cu)[b], 0), a.T) : b;
-}
-
-// A request: its query rows first .. first + n - 1 of which the first m are computed,
-// its tokens, and how many of them the table's columns hold.
-struct Request {
-    int first, n, m;
-    long long len;
-    int keys;
-};
-__device__ __forceinline__ Request request(const AttnArgs& a, int b) {
-    Request r;
-    r.first = cu_at(a, b);
-    r.n = max(0, cu_at(a, b + 1) - r.first);
-    r.m = min(r.n, a.max_q);
-    r.len = max(0, ((ConstInts)a.lens)[b]);
-    r.keys = a.c.pages ? (int)min(r.len, (long long)a.W * a.c.page) : 0;
-    return r;
-}
-// Keys that the query at place i of its request sees.
-__device__ __forceinline__ int seen_by(const AttnArgs& a, const Request& r, int i) {
-    return a.causal ? (int)max(0LL, min((long long)r.keys, r.len - r.n + i + 1)) : r.keys;
-}
-
 // Whether a scale byte may stand for an infinite or NaN value in element type T.
 template <class T>
 constexpr unsigned kScaleLimit = __is_same(T, f16) ? 141u : 253u;

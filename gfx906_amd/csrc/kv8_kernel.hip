@@ -1,0 +1,837 @@
+// Key/value cache in 8 bits for AMD MI355X (gfx950): storing and reading rows, the attention
+// weights of its blocks and eviction by them. The format and the entry points are
+// described in gfx906_amd_serving.h; the attention is in kv8_attn_kernel.hip.
+//
+// gfx950 converts between pairs of E4M3 codes and fp16, bf16 or fp32 with a power-of-two
+// scale in one instruction (v_cvt_scalef32_*), rounding to nearest even.
+#include "kv8.h"
+
+#include <algorithm>
+#include <type_traits>
+
+#include "longctx_tile.h"
+#include "paged.h"
+
+namespace gfx906_amd {
+namespace kv8 {
+LastError& last_error() {
+    static thread_local LastError e;
+    return e;
+}
+}  // namespace kv8
+}  // namespace gfx906_amd
+
+namespace {
+
+using namespace gfx906_amd::kv8;
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// Exponents of scales.
+constexpr int kLow = -15, kHigh = 7;
+__device__ __forceinline__ float scale_of(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+// Exponent of the least scale for rows whose largest |x| has the bits `top` (of fp32): 448 is
+// 1.75 * 2^8, so mantissas past 0.75 take the next one.
+__device__ __forceinline__ int exponent_for(unsigned top) {
+    return min(kHigh, max(kLow, (int)((top + 0x1fffffu) >> 23) - 135));
+}
+
+// A pair of numbers as E4M3 codes in the low or high half of w.
+template <class T, bool HIGH>
+__device__ __forceinline__ unsigned pack2(unsigned w, unsigned pair, float s) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const s16x2 old = __builtin_bit_cast(s16x2, w);
+    if constexpr (__is_same(T, f16))
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(
+                                                old, __builtin_bit_cast(f16x2, pair), s, HIGH));
+    else
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(
+                                                old, __builtin_bit_cast(bf16x2, pair), s, HIGH));
+}
+template <class T>
+__device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, float s) {
+    return pack2<T, true>(pack2<T, false>(0, a, s), b, s);
+}
+// Four codes at scale `from` as codes at scale `to`: exact, but where they become subnormal.
+__device__ __forceinline__ unsigned rescale(unsigned w, float from, float to) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, from, false);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, from, true);
+    s16x2 r = {};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a[0], a[1], to, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, b[0], b[1], to, true);
+    return __builtin_bit_cast(unsigned, r);
+}
+
+// Patterns of the element type: infinity, NaN, and 57344, the largest number held.
+template <class T>
+constexpr unsigned kInf16 = __is_same(T, f16) ? 0x7c00u : 0x7f80u;
+template <class T>
+constexpr unsigned kNan16 = __is_same(T, f16) ? 0x7e00u : 0x7fc0u;
+template <class T>
+constexpr unsigned kMax16 = __is_same(T, f16) ? 0x7b00u : 0x4760u;
+
+// Larger |x| of both numbers of each dword, patterns compared as integers.
+__device__ __forceinline__ unsigned top2(unsigned m, unsigned w) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned,
+                              __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                        __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+__device__ __forceinline__ unsigned wave_top(unsigned m) {
+    m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o));
+    return m;
+}
+// Infinite and NaN numbers as NaN, others at most 57344 in size; m: the larger of m and the
+// finite ones.
+template <class T>
+__device__ __forceinline__ unsigned tame(unsigned w, unsigned& m) {
+    unsigned out = 0, mags = 0;
+#pragma unroll
+    for (int sh = 0; sh < 32; sh += 16) {
+        const unsigned x = w >> sh & 0xffffu, a = x & 0x7fffu;
+        const bool bad = a >= kInf16<T>;
+        const unsigned b = bad ? kNan16<T> : min(a, kMax16<T>);
+        out |= ((x & 0x8000u) | b) << sh;
+        mags |= (bad ? 0u : b) << sh;
+    }
+    m = top2(m, mags);
+    return out;
+}
+template <class T>
+__device__ __forceinline__ unsigned f32_bits(unsigned x16) {
+    if constexpr (__is_same(T, f16))
+        return __float_as_uint((float)__builtin_bit_cast(f16, (unsigned short)x16));
+    else
+        return x16 << 16;
+}
+#endif
+
+// -- storing and reading rows ---------------------------------------------------------
+
+struct StoreArgs {
+    const void* k;
+    const void* v;
+    long long kt, kh, vt, vh;  // strides: token, head
+    Cache c;
+    const int* table;
+    long long table_stride;
+    const int* lens;
+    const int* cu;
+    float* weights;
+    int W, T, B, max_q, causal;
+    unsigned tasks;  // blocks that may be written, of one head
+};
+
+// A wave has a block of a request that gets rows, of one kv head, of K or V: it is the only
+// one to touch it, so the block's maximum, its scale and its older codes need no exchange
+// between waves. Request b's blocks have the numbers from cu[b] / 64 + 2b on (n rows touch at
+// most n / 64 + 2 blocks), where a wave finds its request by two steps of 64.
+//
+// A lane has 8 dims of every row group's tokens (D / 8 of them): the 16 or 8 tokens whose codes lie
+// side by side in V, so that V is written in 16 or 8 bytes without an exchange. Up to four rows
+// (a decoding step) are written as they are where the scale stays, a dword of dims a lane.
+//
+// Bound by bytes.
+template <class T, int D>
+__global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int DL = D / 8, NT = D / 8;  // lanes a row; tokens a lane
+    const int lane = threadIdx.x & 63;
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const unsigned id = uni(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const bool is_v = id & 1;
+    const unsigned task = (id >> 1) / (unsigned)a.c.Hkv;
+    const int h = uni((int)((id >> 1) - task * a.c.Hkv));
+    if (task >= a.tasks) return;
+    // The last request whose first number is at most `task`.
+    auto starts = [&](int b) { return b < a.B && (unsigned)((cu_at(a, b) >> 6) + 2 * b) <= task; };
+    const int step = (a.B + 63) / 64;
+    int b = uni(max(0, __popcll(__ballot(starts(lane * step))) - 1)) * step;
+    b += uni(max(0, __popcll(__ballot(lane < step && starts(b + lane))) - 1));
+    const Request r = request(a, b);
+    const long long old = r.len - r.n;  // tokens before the new ones (negative: rows too many)
+    const long long j = max(0LL, old) / kBlock + (task - (unsigned)((cu_at(a, b) >> 6) + 2 * b));
+    const long long p0 = max(old, j * kBlock), p1 = min(r.len, (j + 1) * kBlock);
+    if (p0 < 0 || p0 >= p1 || j * kBlock >= (long long)a.W * a.c.page) return;
+    const int page = a.table[b * a.table_stride + j * kBlock / a.c.page];
+    if ((unsigned)page >= (unsigned)a.c.pages) return;
+    const int before = uni((int)(p0 - j * kBlock)), count = uni((int)(p1 - p0));
+    const long long row0 = r.first + (p0 - old) - before;  // row of the block's token 0
+    const long long blk = block_at(a.c, page, h, (int)(j % (a.c.page / kBlock)));
+    uint8_t* codes = const_cast<uint8_t*>(is_v ? a.c.vc : a.c.kc) + blk * (kBlock * D);
+    float* scale = const_cast<float*>(is_v ? a.c.vs : a.c.ks) + blk;
+    const T* src = is_v ? (const T*)a.v + h * a.vh : (const T*)a.k + h * a.kh;
+    const long long st = is_v ? a.vt : a.kt;
+    const int old_e =
+        before ? min(kHigh, max(kLow, (int)(__float_as_uint(*scale) >> 23 & 255) - 127)) : kLow;
+    if (!is_v && a.weights && before == 0 && lane == 0) a.weights[blk] = 0.f;
+
+    constexpr int FEW = 4;
+    if (count <= FEW) {
+        unsigned x[FEW], m = 0;
+#pragma unroll
+        for (int n = 0; n < FEW; ++n) {
+            x[n] = 0;
+            if (n < count && 2 * lane < D)
+                x[n] = *reinterpret_cast<const unsigned*>(src + (row0 + before + n) * st + 2 * lane);
+            m = top2(m, x[n]);
+        }
+        m = wave_top(m);
+        if (m > kMax16<T>) {
+            m = 0;
+#pragma unroll
+            for (int n = 0; n < FEW; ++n) x[n] = tame<T>(x[n], m);
+            m = wave_top(m);
+        }
+        const int e = max(old_e, exponent_for(f32_bits<T>(m)));
+        if (before == 0 || e == old_e) {
+            const float s = scale_of(e);
+            if (before == 0 && lane == 0) *scale = s;
+#pragma unroll
+            for (int n = 0; n < FEW; ++n) {
+                if (n >= count || 2 * lane >= D) continue;
+                const unsigned w = pack2<T, false>(0, x[n], s);
+                const int t = before + n;
+                if (is_v) {
+                    codes[2 * lane * kBlock + place(t)] = (uint8_t)w;
+                    codes[(2 * lane + 1) * kBlock + place(t)] = (uint8_t)(w >> 8);
+                } else {
+                    *reinterpret_cast<unsigned short*>(codes + t * D + 2 * lane) = (unsigned short)w;
+                }
+            }
+            return;
+        }
+    }
+
+    const int dl = lane % DL, sub = lane / DL;
+    auto token = [&](int n) {
+        return D == 128 ? 16 * (n >> 2) + 4 * sub + (n & 3)
+                        : 32 * (sub >> 2) + 16 * (n >> 2) + 4 * (sub & 3) + (n & 3);
+    };
+    auto is_new = [&](int t) { return t >= before && t < before + count; };
+    u32x4 x[NT];
+    unsigned m = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int t = token(n);
+        x[n] = u32x4{};
+        if (is_new(t)) x[n] = *reinterpret_cast<const u32x4*>(src + (row0 + t) * st + 8 * dl);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = top2(m, x[n][i]);
+    m = wave_top(m);
+    if (m > kMax16<T>) {
+        m = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[n][i] = tame<T>(x[n][i], m);
+        m = wave_top(m);
+    }
+    const int e = max(old_e, exponent_for(f32_bits<T>(m)));
+    const float s = scale_of(e), old_s = scale_of(old_e);
+    const bool grown = before && e > old_e;
+    if ((grown || !before) && lane == 0) *scale = s;
+    if (!is_v) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int t = token(n);
+            u32x2* dst = reinterpret_cast<u32x2*>(codes + t * D + 8 * dl);
+            if (is_new(t)) {
+                *dst = u32x2{pack4<T>(x[n][0], x[n][1], s), pack4<T>(x[n][2], x[n][3], s)};
+            } else if (grown && t < before) {
+                const u32x2 w = *dst;
+                *dst = u32x2{rescale(w[0], old_s, s), rescale(w[1], old_s, s)};
+            }
+        }
+        return;
+    }
+    unsigned mask[NT / 4];  // bytes of new tokens
+#pragma unroll
+    for (int q = 0; q < NT / 4; ++q) {
+        mask[q] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mask[q] |= is_new(token(4 * q + i)) ? 255u << (8 * i) : 0u;
+    }
+    uint8_t* row = codes + 8 * dl * kBlock + place(token(0));
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+        unsigned w[NT / 4];
+#pragma unroll
+        for (int q = 0; q < NT / 4; ++q) {
+            // dim d of four tokens, two and two
+            auto pair = [&](int n) {
+                return __builtin_amdgcn_perm(x[n + 1][d / 2], x[n][d / 2],
+                                             d & 1 ? 0x07060302u : 0x05040100u);
+            };
+            w[q] = pack4<T>(pair(4 * q), pair(4 * q + 2), s);
+        }
+        if (before) {
+#pragma unroll
+            for (int q = 0; q < NT / 4; ++q) {
+                unsigned o = *reinterpret_cast<const unsigned*>(row + d * kBlock + 4 * q);
+                if (grown) o = rescale(o, old_s, s);
+                w[q] = (o & ~mask[q]) | (w[q] & mask[q]);
+            }
+        }
+        if constexpr (NT == 16)
+            *reinterpret_cast<u32x4*>(row + d * kBlock) = u32x4{w[0], w[1], w[2], w[3]};
+        else
+            *reinterpret_cast<u32x2*>(row + d * kBlock) = u32x2{w[0], w[1]};
+    }
+#endif
+}
+
+struct LoadArgs {
+    void* k;
+    void* v;
+    const int* slots;
+    Cache c;
+    int T;
+};
+
+// 64 rows of a head a workgroup, 8 dims a lane: of V these are 8 bytes in as many lines, which
+// the rows of a block share. grid: rows / 64, heads x (K, V).
+template <class T, int D>
+__global__ void __launch_bounds__(256) load_kernel(const LoadArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int DL = D / 8, RW = 256 / DL;
+    const int h = blockIdx.y >> 1, dl = threadIdx.x % DL;
+    const bool is_v = blockIdx.y & 1;
+#pragma unroll
+    for (int n = 0; n < 64 / RW; ++n) {
+        const long long t = blockIdx.x * 64LL + n * RW + threadIdx.x / DL;
+        if (t >= a.T) continue;
+        const int slot = a.slots[t];
+        unsigned w[2] = {};
+        float s = 1.f;
+        if (slot >= 0 && slot < a.c.pages * (long long)a.c.page) {
+            const int page = slot / a.c.page, tok = slot % a.c.page;
+            const long long blk = block_at(a.c, page, h, tok / kBlock);
+            s = (is_v ? a.c.vs : a.c.ks)[blk];
+            if (is_v) {
+                const uint8_t* p = a.c.vc + blk * (kBlock * D) + 8 * dl * kBlock + place(tok % kBlock);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) w[d / 4] |= (unsigned)p[d * kBlock] << (8 * (d & 3));
+            } else {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(
+                    a.c.kc + blk * (kBlock * D) + (tok % kBlock) * D + 8 * dl);
+                w[0] = x[0], w[1] = x[1];
+            }
+        }
+        reinterpret_cast<typename Elem<T>::x8*>(is_v ? a.v : a.k)[(t * a.c.Hkv + h) * DL + dl] =
+            expand<T>(w[0], w[1], s);
+    }
+#endif
+}
+
+// -- attention weights of blocks ------------------------------------------------------
+
+struct WeighArgs {
+    float* weights;
+    const void* q;
+    const float* lse;
+    long long qt, qh;  // strides: token, head
+    Cache c;
+    const int* table;
+    long long table_stride;
+    const int* lens;
+    const int* cu;
+    int W, T, B, Hq, G, max_q, causal;
+    float scale, qsign;  // log2_scale(); a negative scale negates q
+};
+
+// Weights of a block of 64 keys: its keys stay in registers as the matrix operand, the query
+// rows (a token's G heads beside each other) go by in tiles of 16, and each lane adds up the
+// exponentials of its rows and keys. SHARE waves of a workgroup have one block and every SHARE-th
+// tile of it (prompts), or four blocks (single tokens).
+//
+// grid: blocks of the table, kv heads, requests.
+template <int D, class T, int SHARE>
+__global__ void __launch_bounds__(256) weigh_kernel(const WeighArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using x8 = typename Elem<T>::x8;
+    constexpr int NJ = D / 64;
+    __shared__ float part[4];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int wave = uni(threadIdx.x >> 6);
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const long long chunk = (long long)blockIdx.x * (4 / SHARE) + (SHARE == 1 ? wave : 0);
+    const Request req = request(a, b);
+    if (chunk * kBlock >= req.keys) return;  // (SHARE > 1: the same for all waves)
+    const int page = uni(a.table[b * a.table_stride + chunk * kBlock / a.c.page]);
+    if ((unsigned)page >= (unsigned)a.c.pages) return;
+    const int key0 = (int)chunk * kBlock;
+    const long long blk = block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock)));
+
+    // Keys 16 t + i, dims 64 j + 16 g + 8 n .. + 7.
+    x8 kf[4][NJ][2];
+    const float ks = ((ConstFloats)a.c.ks)[blk];
+    const uint8_t* kp = a.c.kc + blk * (kBlock * D) + i * D + 16 * g;
+    u32x4 raw[4][NJ];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            raw[t][j] = *reinterpret_cast<const u32x4*>(kp + t * 16 * D + 64 * j);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            kf[t][j][0] = expand<T>(raw[t][j][0], raw[t][j][1], ks);
+            kf[t][j][1] = expand<T>(raw[t][j][2], raw[t][j][3], ks);
+        }
+
+    const long long rows = (long long)req.m * a.G;
+    // The first query that sees the block's first key.
+    const long long q0 = a.causal ? max(0LL, key0 - (req.len - req.n)) : 0;
+    const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
+    float acc = 0.f;
+    for (long long r0 = (q0 * a.G & ~15LL) + (SHARE > 1 ? 16 * wave : 0); r0 < rows; r0 += 16 * SHARE) {
+        const long long r = r0 + i;
+        const int tok = (int)(r / a.G), h = hk * a.G + (int)(r - (long long)tok * a.G);
+        const bool ok = r < rows;
+        int lim = ok ? seen_by(a, req, tok) : 0;
+        const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh + 16 * g;
+        x8 qf[NJ][2];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                u32x4 x = {};
+                if (ok) x = *reinterpret_cast<const u32x4*>(q + 64 * j + 8 * n);
+                qf[j][n] = __builtin_bit_cast(x8, x ^ neg);
+            }
+        const float lse = ok ? a.lse[(long long)(req.first + tok) * a.Hq + h] : -INFINITY;
+        if (lse == -INFINITY) lim = 0;
+        const float m = lse * kLog2e;
+        f32x4 S[4] = {};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) S[t] = Elem<T>::mma16(kf[t][j][n], qf[j][n], S[t]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(S[t][e], a.scale, -m));
+                acc += key0 + 16 * t + 4 * g + e < lim ? p : 0.f;
+            }
+    }
+    acc = wave_sum(acc);
+    if constexpr (SHARE > 1) {
+        if (lane == 0) part[wave] = acc;
+        __syncthreads();
+        acc = part[0] + part[1] + part[2] + part[3];
+        if (wave) return;
+    }
+    // (once a block and call, so that its order is set; requests that share a page add in any)
+    if (lane == 0) atomicAdd(a.weights + blk, acc);
+#endif
+}
+
+// -- eviction -------------------------------------------------------------------------
+
+struct EvictArgs {
+    const float* weights;
+    int pages, Hkv, page, W, B, first, recent, n_free;
+    int* table;
+    long long table_stride;
+    const int* lens;
+    const int* keep;
+    int* free_pages;
+    const int* used;
+    int *lens_out, *used_out, *lost;
+    unsigned long long* keys;  // [B][W], for wide tables
+};
+
+constexpr int kEvictThreads = 512, kEvictLds = 4096;
+
+// A workgroup a request. How many pages every request gives back follows from lengths and
+// budgets alone, so each finds the place of its pages in the free list by adding up all of them.
+// Which ones: the `gone`-th smallest of the pages' weights, as 64-bit keys that order alike, by
+// histograms of 8 bits from the highest one in which they differ; mostly two or three
+// passes until a bin is taken whole. Then the row closes up, 512 columns at a time. Bound by
+// latency (dependent steps in one workgroup).
+//
+// LDS: whether the keys are kept there or in the workspace.
+template <bool LDS>
+__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef unsigned long long u64;
+    constexpr int NT = kEvictThreads, NW = NT / 64;
+    __shared__ u64 keys_s[LDS ? kEvictLds : 1];
+    __shared__ u64 red[NW][2];
+    __shared__ int hist[256];
+    __shared__ int wave_n[NW];
+    __shared__ int chosen[3];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x;
+    auto pages_of = [&](int x) {
+        return (int)min(((long long)max(0, a.lens[x]) + a.page - 1) / a.page, (long long)a.W);
+    };
+    auto gone_of = [&](int x) {
+        const long long n = pages_of(x);
+        return max(0LL, min(n - a.keep[x], n - a.recent - a.first));
+    };
+    // Pages given back before this request, and by all.
+    long long before = 0, all = 0;
+    for (int x = t; x < a.B; x += NT) {
+        const long long n = gone_of(x);
+        all += n;
+        before += x < b ? n : 0;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        all += __shfl_xor(all, o);
+        before += __shfl_xor(before, o);
+    }
+    if (lane == 0) {
+        red[wave][0] = (u64)before;
+        red[wave][1] = (u64)all;
+    }
+    __syncthreads();
+    before = all = 0;
+    for (int w = 0; w < NW; ++w) {
+        before += (long long)red[w][0];
+        all += (long long)red[w][1];
+    }
+    const int used = min(max(0, a.used[0]), a.n_free);
+    const int back = (int)max(0LL, used - all);
+    if (b == 0 && t == 0) {
+        a.used_out[0] = back;
+        a.lost[0] = (int)min(max(0LL, all - used), 0x7fffffffLL);
+    }
+    if (b >= a.B) return;
+    const int n = pages_of(b), gone = (int)gone_of(b);
+    if (t == 0) a.lens_out[b] = a.lens[b] - gone * a.page;
+    if (gone == 0) return;
+
+    int* const row = a.table + b * a.table_stride;
+    u64* const keys = LDS ? keys_s : a.keys + (long long)b * a.W;
+    const int c0 = a.first, c1 = n - a.recent;  // candidates
+    const int per = a.Hkv * (a.page / kBlock);
+    u64 any = 0, each = ~0ull;
+    for (int c = c0 + t; c < c1; c += NT) {
+        const int page = row[c];
+        u64 key = 0;
+        if ((unsigned)page < (unsigned)a.pages) {
+            const float* w = a.weights + (long long)page * per;
+            double sum = 0.0;
+            for (int x = 0; x < per; ++x) sum += (double)w[x];
+            const u64 u = (u64)__double_as_longlong(sum + 0.0);
+            key = sum != sum ? ~0ull : u >> 63 ? ~u : u | 1ull << 63;
+        }
+        keys[c] = key;
+        any |= key;
+        each &= key;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        any |= __shfl_xor(any, o);
+        each &= __shfl_xor(each, o);
+    }
+    __syncthreads();
+    if (lane == 0) {
+        red[wave][0] = any;
+        red[wave][1] = each;
+    }
+    __syncthreads();
+    for (int w = 0; w < NW; ++w) {
+        any |= red[w][0];
+        each &= red[w][1];
+    }
+    // Of the keys whose bits from `hi` up are those of `limit`, the least `rem` go, and all below.
+    u64 limit = each;
+    int rem = gone, hi = any == each ? 0 : 64 - __clzll((long long)(any ^ each));
+    bool whole = false;  // the keys up to `limit` go, else those below and the first `rem` equal ones
+    while (hi > 0) {
+        const int lo = max(0, hi - 8);
+        limit = hi < 64 ? limit & ~0ull << hi : 0;
+        for (int x = t; x < 256; x += NT) hist[x] = 0;
+        __syncthreads();
+        for (int c = c0 + t; c < c1; c += NT) {
+            const u64 k = keys[c];
+            if (hi == 64 || k >> hi == limit >> hi)
+                atomicAdd(&hist[(int)(k >> lo) & ((1 << (hi - lo)) - 1)], 1);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            int x[4], sum = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                x[q] = hist[4 * lane + q];
+                sum += x[q];
+            }
+            int upto = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(upto, o);
+                if (lane >= o) upto += y;
+            }
+            int at = upto - sum;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (at < rem && rem <= at + x[q]) {
+                    chosen[0] = 4 * lane + q;
+                    chosen[1] = rem - at;
+                    chosen[2] = x[q];
+                }
+                at += x[q];
+            }
+        }
+        __syncthreads();
+        const int bin = chosen[0], held = chosen[2];
+        rem = chosen[1];
+        limit |= (u64)bin << lo;
+        hi = lo;
+        __syncthreads();
+        if (rem == held) {
+            limit |= (1ull << lo) - 1;
+            whole = true;
+            break;
+        }
+    }
+
+    // The row closes up. Entries are read before the barriers behind which others are written
+    // to their places or in front of them.
+    auto scan = [&](bool x, int& total) {  // how many before this thread have x
+        const u64 m = __ballot(x);
+        __syncthreads();
+        if (lane == 0) wave_n[wave] = __popcll(m);
+        __syncthreads();
+        int at = __popcll(m & ((1ull << lane) - 1));
+        total = 0;
+        for (int w = 0; w < NW; ++w) {
+            at += w < wave ? wave_n[w] : 0;
+            total += wave_n[w];
+        }
+        return at;
+    };
+    int equal0 = 0, gone0 = 0;
+    for (int base = 0; base < n; base += NT) {
+        const int c = base + t;
+        const int page = c < n ? row[c] : -1;
+        const bool may = c >= c0 && c < c1;
+        const u64 key = may ? keys[c] : 0;
+        const bool equal = may && !whole && key == limit;
+        int total;
+        const int eq = equal0 + scan(equal, total);
+        equal0 += total;
+        const bool out = may && (whole ? key <= limit : key < limit || (equal && eq < rem));
+        const int at = gone0 + scan(out, total);
+        gone0 += total;
+        if (out) {
+            const long long f = (long long)back + before + at;
+            if (f < used) a.free_pages[f] = page;
+        } else if (c < n) {
+            row[c - at] = page;
+        }
+    }
+    __syncthreads();
+    for (int c = n - gone + t; c < n; c += NT) row[c] = -1;
+#endif
+}
+
+template <class F>
+void for_types(int dtype, int D, F go) {
+    if (dtype == KV8_DTYPE_F16)
+        D == 64 ? go(std::integral_constant<int, 64>{}, f16{})
+                : go(std::integral_constant<int, 128>{}, f16{});
+    else
+        D == 64 ? go(std::integral_constant<int, 64>{}, bf16{})
+                : go(std::integral_constant<int, 128>{}, bf16{});
+}
+
+int check_table(const int* table, long long stride, int B, int W, int page, const char* who) {
+    if (W < 0 || (B > 0 && W > 0 && !table)) return last_error().fail("%s: null table or negative width", who);
+    if ((long long)W * page >= (1LL << 31) || stride < 0)
+        return last_error().fail("%s: table too wide or a negative stride", who);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" const char* kv8_last_error(void) { return last_error().get(); }
+
+extern "C" int kv8_store(const void* k, const void* v, const long long* k_strides,
+                         const long long* v_strides, int dtype, int T, int B, int Hkv, int D,
+                         void* k_codes, float* k_scales, void* v_codes, float* v_scales, int pages,
+                         int page, const int* table, long long table_stride, int W, const int* lens,
+                         const int* cu_new, float* weights, hipStream_t stream) {
+    const char* who = "kv8_store";
+    LastError& err = last_error();
+    err.text[0] = 0;
+    if (check_cache(Hkv, D, pages, page, k_codes, k_scales, v_codes, v_scales, who)) return 1;
+    if (dtype != KV8_DTYPE_F16 && dtype != KV8_DTYPE_BF16) return err.fail("%s: bad dtype", who);
+    if (T < 0 || B < 0) return err.fail("%s: negative sizes", who);
+    if (B > kMaxRequests) return err.fail("%s: at most %d requests", who, kMaxRequests);
+    if (!cu_new && T != B) return err.fail("%s: without cu_new, one row a request", who);
+    if (check_table(table, table_stride, B, W, page, who)) return 1;
+    if (T == 0 || B == 0 || pages == 0 || W == 0) return 0;
+    if (!k || !v || !lens || !k_strides || !v_strides) return err.fail("%s: null argument", who);
+    for (int i = 0; i < 2; ++i)
+        if (k_strides[i] < 0 || v_strides[i] < 0 || k_strides[i] % 8 || v_strides[i] % 8)
+            return err.fail("%s: strides must be non-negative multiples of 8 elements", who);
+    if (!aligned(k, 16) || !aligned(v, 16))
+        return err.fail("%s: k and v must be 16-byte aligned", who);
+    StoreArgs a{};
+    a.k = k;
+    a.v = v;
+    a.kt = k_strides[0];
+    a.kh = k_strides[1];
+    a.vt = v_strides[0];
+    a.vh = v_strides[1];
+    a.c = Cache{(const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
+                pages, page, Hkv, D};
+    a.table = table;
+    a.table_stride = table_stride;
+    a.lens = lens;
+    a.cu = cu_new;
+    a.weights = weights;
+    a.W = W;
+    a.T = T;
+    a.B = B;
+    a.max_q = T;
+    a.tasks = (unsigned)(T / kBlock) + 2u * B;
+    const long long waves = (long long)a.tasks * Hkv * 2, grid = (waves + 3) / 4;
+    if (!launchable(grid, 256) || waves >= (1LL << 32))
+        return err.fail("%s: too many rows for one call", who);
+    for_types(dtype, D, [&](auto d, auto t) {
+        hipLaunchKernelGGL((store_kernel<decltype(t), decltype(d)::value>), dim3((unsigned)grid),
+                           dim3(256), 0, stream, a);
+    });
+    return err.launched(who, hipGetLastError());
+}
+
+extern "C" int kv8_load(void* k, void* v, int dtype, int T, int Hkv, int D, const int* slots,
+                        const void* k_codes, const float* k_scales, const void* v_codes,
+                        const float* v_scales, int pages, int page, hipStream_t stream) {
+    const char* who = "kv8_load";
+    LastError& err = last_error();
+    err.text[0] = 0;
+    if (check_cache(Hkv, D, pages, page, k_codes, k_scales, v_codes, v_scales, who)) return 1;
+    if (dtype != KV8_DTYPE_F16 && dtype != KV8_DTYPE_BF16) return err.fail("%s: bad dtype", who);
+    if (T < 0) return err.fail("%s: negative token count", who);
+    if (T == 0) return 0;
+    if (!k || !v || !slots) return err.fail("%s: null argument", who);
+    if (!aligned(k, 16) || !aligned(v, 16))
+        return err.fail("%s: k and v must be 16-byte aligned", who);
+    if (Hkv > 32767 || !launchable((T + 63LL) / 64 * Hkv * 2, 256))
+        return err.fail("%s: too many rows or heads for one call", who);
+    const LoadArgs a{k, v, slots,
+                     Cache{(const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
+                           pages, page, Hkv, D},
+                     T};
+    for_types(dtype, D, [&](auto d, auto t) {
+        hipLaunchKernelGGL((load_kernel<decltype(t), decltype(d)::value>),
+                           dim3((unsigned)((T + 63LL) / 64), (unsigned)Hkv * 2), dim3(256), 0, stream,
+                           a);
+    });
+    return err.launched(who, hipGetLastError());
+}
+
+extern "C" int kv8_weigh(float* weights, const void* q, const long long* q_strides, int dtype,
+                         const float* lse, int T, int B, int Hq, int Hkv, int D,
+                         const void* k_codes, const float* k_scales, int pages, int page,
+                         const int* table, long long table_stride, int W, const int* lens,
+                         const int* cu_q, int max_q, float scale, int causal, hipStream_t stream) {
+    const char* who = "kv8_weigh";
+    LastError& err = last_error();
+    err.text[0] = 0;
+    if (check_cache(Hkv, D, pages, page, k_codes, k_scales, k_codes, k_scales, who)) return 1;
+    if (dtype != KV8_DTYPE_F16 && dtype != KV8_DTYPE_BF16) return err.fail("%s: bad dtype", who);
+    if (T < 0 || B < 0 || max_q < 0) return err.fail("%s: negative sizes", who);
+    if (B > kMaxRequests) return err.fail("%s: at most %d requests", who, kMaxRequests);
+    if (Hq <= 0 || Hq % Hkv || Hq > 65535)
+        return err.fail("%s: query heads must be a multiple of kv heads", who);
+    if (!cu_q && T != B) return err.fail("%s: without cu_q, one query a request", who);
+    if (check_table(table, table_stride, B, W, page, who)) return 1;
+    if (!good_scale(scale)) return err.fail("%s: scale must be finite, and below 2.3e38", who);
+    if (T == 0 || B == 0 || max_q == 0 || pages == 0 || W == 0) return 0;
+    if (!weights || !q || !q_strides || !lse || !lens) return err.fail("%s: null argument", who);
+    for (int i = 0; i < 2; ++i)
+        if (q_strides[i] < 0 || q_strides[i] % 8)
+            return err.fail("%s: strides must be non-negative multiples of 8 elements", who);
+    if (!aligned(q, 16) || !aligned(weights, 4) || !aligned(lse, 4))
+        return err.fail("%s: q must be 16-byte, weights and lse 4-byte aligned", who);
+    WeighArgs a{};
+    a.weights = weights;
+    a.q = q;
+    a.lse = lse;
+    a.qt = q_strides[0];
+    a.qh = q_strides[1];
+    a.c = Cache{(const uint8_t*)k_codes, k_scales, nullptr, nullptr, pages, page, Hkv, D};
+    a.table = table;
+    a.table_stride = table_stride;
+    a.lens = lens;
+    a.cu = cu_q;
+    a.W = W;
+    a.T = T;
+    a.B = B;
+    a.Hq = Hq;
+    a.G = Hq / Hkv;
+    a.max_q = cu_q ? std::min(max_q, T) : 1;
+    a.causal = causal;
+    a.scale = log2_scale(scale);
+    a.qsign = scale < 0.f ? -1.f : 1.f;
+    const long long blocks = (long long)W * (page / kBlock);
+    const bool share = (long long)a.max_q * a.G > 64;
+    const long long gx = share ? blocks : (blocks + 3) / 4;
+    if (!launchable(gx * Hkv * B, 256)) return err.fail("%s: table too wide for so many heads", who);
+    for_types(dtype, D, [&](auto d, auto t) {
+        constexpr int kD = decltype(d)::value;
+        const dim3 grid((unsigned)gx, (unsigned)Hkv, (unsigned)B);
+        if (share)
+            hipLaunchKernelGGL((weigh_kernel<kD, decltype(t), 4>), grid, dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL((weigh_kernel<kD, decltype(t), 1>), grid, dim3(256), 0, stream, a);
+    });
+    return err.launched(who, hipGetLastError());
+}
+
+extern "C" size_t kv8_evict_workspace_bytes(int B, int W) {
+    return B > 0 && W > kEvictLds ? (size_t)B * W * sizeof(unsigned long long) : 0;
+}
+
+extern "C" int kv8_evict(const float* weights, int pages, int Hkv, int page, int* table,
+                         long long table_stride, int W, const int* lens, const int* keep, int B,
+                         int first, int recent, int* free_pages, int n_free, const int* used,
+                         int* lens_out, int* used_out, int* lost, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream) {
+    const char* who = "kv8_evict";
+    LastError& err = last_error();
+    err.text[0] = 0;
+    if (page != 64 && page != 128 && page != 256)
+        return err.fail("%s: pages hold 64, 128 or 256 tokens", who);
+    if (Hkv <= 0 || Hkv > 65535) return err.fail("%s: bad number of kv heads", who);
+    if (pages < 0 || (long long)pages * page >= (1LL << 31))
+        return err.fail("%s: the cache must hold fewer than 2^31 tokens", who);
+    if (B < 0 || B > kMaxRequests) return err.fail("%s: at most %d requests", who, kMaxRequests);
+    if (n_free < 0) return err.fail("%s: negative sizes", who);
+    if (first < 0 || recent < 1)
+        return err.fail("%s: first must be at least 0 and recent at least 1", who);
+    if (check_table(table, table_stride, B, W, page, who)) return 1;
+    if (B > 1 && table_stride < W) return err.fail("%s: overlapping table rows", who);
+    if (!used || !used_out || !lost || (n_free > 0 && !free_pages) ||
+        (B > 0 && (!lens || !keep || !lens_out)) || (pages > 0 && !weights))
+        return err.fail("%s: null argument", who);
+    const size_t need = kv8_evict_workspace_bytes(B, W);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
+        return err.fail("%s: workspace misaligned or smaller than kv8_evict_workspace_bytes()", who);
+    const EvictArgs a{weights, pages, Hkv,  page,       W,    B,        first,    recent,
+                      n_free,  table, table_stride, lens, keep, free_pages, used, lens_out,
+                      used_out, lost, (unsigned long long*)workspace};
+    const dim3 grid((unsigned)std::max(B, 1));
+    if (W <= kEvictLds)
+        hipLaunchKernelGGL(evict_kernel<true>, grid, dim3(kEvictThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL(evict_kernel<false>, grid, dim3(kEvictThreads), 0, stream, a);
+    return err.launched(who, hipGetLastError());
+}

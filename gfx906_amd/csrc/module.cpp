@@ -1,7 +1,7 @@
 // The torch extension module: attn (attention forward) and conv3d (implicit-GEMM
 // conv3d), the ops of the reference's two extensions (attn.cpp:21 and
-// hip_conv/conv3d.cpp:53) in one module, and the ops behind gfx906_amd.kv4 and
-// gfx906_amd.sparse, which have no counterpart there.
+// hip_conv/conv3d.cpp:53) in one module, and the ops behind gfx906_amd.kv4, kv8, qknorm and
+// sparse, which have no counterpart there.
 #include "bindings.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -19,4 +19,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sparse_select", &sparse_select_op, "key blocks of every query block");
     m.def("sparse_choose", &sparse_choose_op, "key blocks of every query block, from its rows");
     m.def("sparse_attn", &sparse_attn_op, "attention over selected key blocks");
+    m.def("norm_rotate", &norm_rotate_op, "norms of queries and keys with the position rotation");
+    m.def("kv8_store", &kv8_store_op, "rows of k and v into the 8-bit cache");
+    m.def("kv8_load", &kv8_load_op, "rows of the 8-bit cache");
+    m.def("kv8_weigh", &kv8_weigh_op, "attention weights of the 8-bit cache's blocks");
+    m.def("kv8_evict", &kv8_evict_op, "eviction of pages by their attention weights");
 }

@@ -1,0 +1,279 @@
+// Norms of queries and keys for each head with the position rotation in the same
+// pass, for AMD MI355X (gfx950). The entry point is described in
+// gfx906_amd_serving.h.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w        over the D dims of a head
+//   (y_i, y_j) <- (c y_i - s y_j, s y_i + c y_j)   for the pairs of the first R dims
+//
+// in fp32, rounded once. Bound by bytes: every row is read and written once, and a
+// token's angles are kept in registers while a wave goes over its heads.
+#include "longctx.h"
+
+#include <algorithm>
+
+#include "gfx906_amd_serving.h"
+
+namespace {
+
+using namespace gfx906_amd::longctx;
+
+thread_local LastError g_err;
+
+constexpr int kUnroll = 4;  // rows in flight a lane
+
+struct Rows {
+    const void* x;
+    void* y;
+    const void* w;
+    long long xb, xs, xh, yb, ys, yh;  // strides: batch, token, head
+    int H, chunks;                     // heads; chunks of them a wave takes
+};
+struct RotateArgs {
+    Rows part[2];  // q, k
+    const float* cos;
+    const float* sin;
+    const int* pos;
+    long long ab, pb, ps;  // strides of a row of angles, of pos: batch, token
+    unsigned B, S, N, groups;  // groups: of tokens
+    int D, R, w32, heads;  // w32: weights are fp32; heads a wave goes over
+    int tok_step, head_step, head_next;  // of a row group; from one round of a wave to the next
+    float eps;
+};
+
+// A row is 8 dims a lane in L = 2^k lanes (some idle where D is not 8 L), a wave 64 / L rows:
+// of one token's heads side by side, or of one head's tokens, whichever lie closer in memory
+// (tok_step, head_step). The wave then goes over `heads` heads with the same tokens' angles.
+//
+// NEAR: pairs are neighbours (2i, 2i+1) and lie in one lane; else halves
+// (i, i + R/2), whose other number another lane holds.
+template <class T, int L, bool NEAR>
+__global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using x8 = typename Elem<T>::x8;
+    constexpr int RG = 64 / L;
+    const int lane = threadIdx.x & 63, l = lane % L, grp = lane / L;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned task = blockIdx.x * 4 + wave;
+    const unsigned per = a.part[0].chunks + a.part[1].chunks;
+    const unsigned tg = task / per;
+    if (tg >= a.groups) return;
+    int chunk = task - tg * per;
+    const bool is_k = chunk >= a.part[0].chunks;
+    if (is_k) chunk -= a.part[0].chunks;
+    const Rows& p = a.part[is_k];
+    // token of this lane, counted over batches
+    const unsigned t = a.tok_step ? tg * RG + grp : tg;
+    const bool live = t < a.B * a.S && 8 * l < a.D;
+    const unsigned b = min(t, a.B * a.S - 1) / a.S, s = min(t, a.B * a.S - 1) - b * a.S;
+
+    float w[8], c[NEAR ? 4 : 8], n[NEAR ? 4 : 8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+    if (p.w && 8 * l < a.D) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            w[e] = a.w32 ? ((const float*)p.w)[8 * l + e] : (float)((const T*)p.w)[8 * l + e];
+    }
+    const bool turn = 8 * l < a.R;
+    const int half = a.R / 16;  // lanes between the numbers of a pair
+    if (turn) {
+        const long long at = a.pos ? a.pos[b * a.pb + s * a.ps] : (long long)s;
+        const bool ok = (unsigned long long)at < a.N;
+        const long long off = (ok ? at : 0) * a.ab + (NEAR ? 4 * l : 8 * (l < half ? l : l - half));
+        const float sign = NEAR || l >= half ? 1.f : -1.f;
+#pragma unroll
+        for (int e = 0; e < (NEAR ? 4 : 8); e += 4) {
+            const f32x4 cc = *reinterpret_cast<const f32x4*>(a.cos + off + e);
+            const f32x4 ss = *reinterpret_cast<const f32x4*>(a.sin + off + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[e + i] = ok ? cc[i] : NAN;
+                n[e + i] = ok ? sign * ss[i] : NAN;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < (NEAR ? 4 : 8); ++e) c[e] = 1.f, n[e] = 0.f;
+    }
+    const int other = grp * L + (l < half ? l + half : l - half);
+
+    const T* x = (const T*)p.x + b * p.xb + s * p.xs + 8 * l;
+    T* y = (T*)p.y + b * p.yb + s * p.ys + 8 * l;
+    const int h0 = chunk * a.heads + grp * a.head_step, h1 = min(p.H, (chunk + 1) * a.heads);
+    for (int h = h0; __any(h < h1); h += kUnroll * a.head_next) {
+        u32x4 raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            raw[u] = u32x4{};
+            const int hh = h + u * a.head_next;
+            if (live && hh < h1) raw[u] = *reinterpret_cast<const u32x4*>(x + hh * p.xh);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const x8 in = __builtin_bit_cast(x8, raw[u]);
+            float v[8], sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = (float)in[e];
+                sum = fmaf(v[e], v[e], sum);
+            }
+#pragma unroll
+            for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o);
+            float eps = a.eps;
+            if (__builtin_expect(__any(!(sum < INFINITY)), 0)) {
+                // Squares past fp32 (bf16 rows): the row times 2^-80.
+                const float f = sum < INFINITY ? 1.f : 0x1p-80f;
+                sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] *= f;
+                    sum = fmaf(v[e], v[e], sum);
+                }
+#pragma unroll
+                for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o);
+                eps *= f * f;
+            }
+            const float r = 1.0f / sqrtf(sum / (float)a.D + eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
+            if (a.R) {
+                float z[8];
+                if constexpr (NEAR) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        z[e] = v[e] * c[e / 2] - v[e + 1] * n[e / 2];
+                        z[e + 1] = v[e] * n[e / 2] + v[e + 1] * c[e / 2];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = v[e] * c[e] + __shfl(v[e], other) * n[e];
+                }
+                if (turn) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = z[e];
+                }
+            }
+            const int hh = h + u * a.head_next;
+            if (live && hh < h1) {
+                u32x4 out;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    out[e] = __builtin_bit_cast(unsigned, Elem<T>::cvt2(v[2 * e], v[2 * e + 1]));
+                *reinterpret_cast<u32x4*>(y + hh * p.yh) = out;
+            }
+        }
+    }
+#endif
+}
+
+}  // namespace
+
+extern "C" const char* qk_norm_rotate_last_error(void) { return g_err.get(); }
+
+extern "C" int qk_norm_rotate(const void* q, const void* k, void* q_out, void* k_out,
+                              const long long* q_strides, const long long* k_strides,
+                              const long long* q_out_strides, const long long* k_out_strides,
+                              int dtype, int B, int S, int Hq, int Hk, int D, const void* q_weight,
+                              const void* k_weight, int weight_f32, float eps, const float* cos,
+                              const float* sin, long long angle_stride, int N, int R,
+                              int neighbours, const int* positions, const long long* p_strides,
+                              hipStream_t stream) {
+    g_err.text[0] = 0;
+    const char* who = "qk_norm_rotate";
+    if (dtype != KV8_DTYPE_F16 && dtype != KV8_DTYPE_BF16) return g_err.fail("%s: bad dtype", who);
+    if (D <= 0 || D > 512 || D % 8)
+        return g_err.fail("%s: head dim must be a multiple of 8 up to 512", who);
+    if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq > 65535 || Hk > 65535)
+        return g_err.fail("%s: bad number of tokens or heads", who);
+    if ((long long)B * S >= (1LL << 31)) return g_err.fail("%s: too many tokens", who);
+    if (R < 0 || R > D || R % (neighbours ? 8 : 16))
+        return g_err.fail("%s: rotated dims must be a multiple of %d up to the head dim", who,
+                          neighbours ? 8 : 16);
+    if (!(eps >= 0.f) || !(eps < INFINITY))
+        return g_err.fail("%s: eps must be finite and not negative", who);
+    if (B == 0 || S == 0 || Hq + Hk == 0) return 0;
+    if ((Hq && (!q || !q_out || !q_strides || !q_out_strides)) ||
+        (Hk && (!k || !k_out || !k_strides || !k_out_strides)) || (R && (!cos || !sin)) ||
+        (positions && !p_strides))
+        return g_err.fail("%s: null argument", who);
+    if (R && (N <= 0 || angle_stride < 0 || angle_stride % 4 || !aligned(cos, 16) || !aligned(sin, 16)))
+        return g_err.fail("%s: angles need rows, 16-byte aligned ones", who);
+    if (R && !positions && N < S) return g_err.fail("%s: fewer rows of angles than tokens", who);
+    const void* ptrs[4] = {q, k, q_out, k_out};
+    const long long* strides[4] = {q_strides, k_strides, q_out_strides, k_out_strides};
+    for (int i = 0; i < 4; ++i) {
+        const int H = i % 2 ? Hk : Hq;
+        if (!H) continue;
+        if (!aligned(ptrs[i], 16)) return g_err.fail("%s: rows must be 16-byte aligned", who);
+        for (int j = 0; j < 3; ++j)
+            if (strides[i][j] < 0 || strides[i][j] % 8)
+                return g_err.fail("%s: strides must be non-negative multiples of 8 elements", who);
+        const long long e[3] = {B, S, H};
+        if (i >= 2 && !rows_apart(strides[i], e, 3, D))
+            return g_err.fail("%s: rows of the results overlap", who);
+    }
+    int L = 1;
+    while (8 * L < D) L *= 2;
+    RotateArgs a{};
+    const int rg = 64 / L;
+    // Rows of a wave are a token's heads, or a head's tokens where those lie closer and there are
+    // enough of them.
+    const long long* st = Hq ? q_strides : k_strides;
+    const bool by_token = S >= rg && st[1] < st[2];
+    a.tok_step = by_token;
+    a.head_step = by_token ? 0 : 1;
+    a.head_next = by_token ? 1 : rg;
+    const long long tokens = (long long)B * S;
+    a.groups = (unsigned)(by_token ? (tokens + rg - 1) / rg : tokens);
+    // Rounds of a wave: as many as keep 4096 waves (16 a CU) busy, kUnroll at least.
+    const int most = (std::max(Hq, Hk) + a.head_next - 1) / a.head_next;
+    const long long rounds_all = a.groups * (long long)((Hq + Hk + a.head_next - 1) / a.head_next);
+    const int rounds = (int)std::min<long long>(
+        most, rounds_all < 4096 ? 1 : std::max<long long>(kUnroll, rounds_all / 4096 / kUnroll * kUnroll));
+    a.heads = rounds * a.head_next;
+    a.part[0] = Rows{q, q_out, q_weight, 0, 0, 0, 0, 0, 0, Hq, (Hq + a.heads - 1) / a.heads};
+    a.part[1] = Rows{k, k_out, k_weight, 0, 0, 0, 0, 0, 0, Hk, (Hk + a.heads - 1) / a.heads};
+    for (int i = 0; i < 2; ++i) {
+        if (!a.part[i].H) continue;
+        a.part[i].xb = strides[i][0], a.part[i].xs = strides[i][1], a.part[i].xh = strides[i][2];
+        a.part[i].yb = strides[i + 2][0], a.part[i].ys = strides[i + 2][1];
+        a.part[i].yh = strides[i + 2][2];
+    }
+    a.cos = cos;
+    a.sin = sin;
+    a.ab = angle_stride;
+    a.pos = R ? positions : nullptr;
+    if (a.pos) a.pb = p_strides[0], a.ps = p_strides[1];
+    a.B = (unsigned)B;
+    a.S = (unsigned)S;
+    a.N = (unsigned)std::max(N, 0);
+    a.D = D;
+    a.R = R;
+    a.w32 = weight_f32;
+    a.eps = eps;
+    const long long tasks = a.groups * (long long)(a.part[0].chunks + a.part[1].chunks);
+    const long long grid = (tasks + 3) / 4;
+    if (!launchable(grid, 256)) return g_err.fail("%s: too many rows for one call", who);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
+        };
+#define GFX906_ROW(l)                                                                            \
+    case l:                                                                                      \
+        neighbours ? run(norm_rotate_kernel<T, l, true>) : run(norm_rotate_kernel<T, l, false>); \
+        break;
+        switch (L) {
+            GFX906_ROW(1)
+            GFX906_ROW(2)
+            GFX906_ROW(4)
+            GFX906_ROW(8)
+            GFX906_ROW(16)
+            GFX906_ROW(32)
+            GFX906_ROW(64)
+        }
+#undef GFX906_ROW
+    };
+    dtype == KV8_DTYPE_F16 ? go(f16{}) : go(bf16{});
+    return g_err.launched(who, hipGetLastError());
+}

@@ -1,0 +1,45 @@
+// Checks of tensors that the bindings of the caches and of the head norms share.
+#pragma once
+
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include <array>
+
+namespace gfx906_amd {
+
+using torch::Tensor;
+
+inline void check_ints(const Tensor& t, int64_t n, const c10::Device& dev, const char* who,
+                const char* name) {
+    TORCH_CHECK(t.device() == dev && t.dtype() == torch::kInt && t.dim() == 1 &&
+                    (n < 0 || t.size(0) == n) && t.is_contiguous(),
+                who, ": ", name, " must be a contiguous int32 vector of the right length on the "
+                "other tensors' device");
+}
+
+// Table of pages, a row a request, and its row stride.
+inline void check_table(const Tensor& table, int64_t B, int page, const c10::Device& dev,
+                        const char* who) {
+    TORCH_CHECK(table.device() == dev && table.dtype() == torch::kInt && table.dim() == 2 &&
+                    table.size(0) == B && (table.size(1) <= 1 || table.stride(1) == 1) &&
+                    (B <= 1 || table.stride(0) >= 0) && table.size(1) * page < (1LL << 31),
+                who, ": table must be int32 [B, W] with contiguous rows of fewer than 2^31 tokens");
+}
+inline int64_t table_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+// [T, H, D] rows the kernels read in place: contiguous head dim, the other strides
+// multiples of 8, 16-byte aligned. Anything else is copied.
+inline Tensor rows_of(const Tensor& t) {
+    const bool ok = (t.stride(2) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                    (t.size(0) == 1 || (t.stride(0) >= 0 && t.stride(0) % 8 == 0)) &&
+                    (t.size(1) == 1 || (t.stride(1) >= 0 && t.stride(1) % 8 == 0));
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+inline std::array<long long, 2> strides2(const Tensor& t) {
+    return {t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1)};
+}
+
+inline hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+}  // namespace gfx906_amd

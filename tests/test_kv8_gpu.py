@@ -1,0 +1,366 @@
+"""The 8-bit cache on the GPU against the CPU oracle in 64 bits: storing and reading, attention
+over it, weights of its blocks, eviction, and a run of them together."""
+
+import math
+
+import pytest
+import torch
+
+from gfx906_amd import kv8
+from oracle import serving as sv
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def offsets(news):
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    return cu
+
+
+def tables(lens, page, seed, spare=2, wider=1):
+    """(table as lists, pages of the cache): shuffled pages, -1 behind the last."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-max(0, n) // page) for n in lens]
+    W = max(max(need, default=0), 1) + wider
+    phys = torch.randperm(sum(need) + spare, generator=g).tolist()
+    out, at = [], 0
+    for n in need:
+        out.append(phys[at:at + n] + [-1] * (W - n))
+        at += n
+    return out, sum(need) + spare
+
+
+def dirty_cache(pages, page, H, D):
+    """A cache whose every byte is a NaN and whose scales are nonsense: nothing may read it."""
+    cache = kv8.new_cache(pages, page, H, D)
+    for t in (cache.k, cache.v):
+        t.fill_(0xff)
+    for t in (cache.k_scale, cache.v_scale):
+        t.fill_(math.nan)
+    return cache
+
+
+def same(cache, want, tables_, lens):
+    """The tokens that requests hold are exactly what the oracle says."""
+    got = [sv.decode(cache.k.cpu(), cache.k_scale.cpu(), False),
+           sv.decode(cache.v.cpu(), cache.v_scale.cpu(), True)]
+    for b, n in enumerate(lens):
+        for t in range(n):
+            page = tables_[b][t // cache.page] if t // cache.page < len(tables_[b]) else -1
+            if not 0 <= page < len(cache.k):
+                continue
+            for g, x in zip(got, want.x):
+                a, e = g[page, :, t % cache.page], x[page, :, t % cache.page]
+                assert torch.equal(a.nan_to_num(9e9), e.nan_to_num(9e9)), (b, t)
+
+
+# -- storing and reading ------------------------------------------------------------------
+
+STORES = [  # lens before, rows of each request in turn, page
+    ([0], [[1]], 64), ([0, 5, 63], [[1, 1, 1]] * 3, 64), ([0, 0], [[100, 3], [30, 130]], 128),
+    ([10, 64, 120, 0], [[200, 0, 9, 64], [1, 1, 1, 1], [5, 63, 64, 65]], 256),
+    ([7] * 70, [[1] * 70] * 2, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,D", [(1, 64), (3, 128)])
+@pytest.mark.parametrize("case", range(len(STORES)))
+def test_store(case, H, D, dtype):
+    lens, steps, page = STORES[case]
+    print(f"store {case} H{H} D{D} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(case)
+    final = [n + sum(s[b] for s in steps) for b, n in enumerate(lens)]
+    table, pages = tables(final, page, case)
+    cache, want = dirty_cache(pages, page, H, D), sv.Cache(pages, page, H, D)
+    weights = kv8.new_weights(cache)
+    steps = [lens] + steps       # the tokens that are there come in one call
+    lens = [0] * len(lens)
+    for step, news in enumerate(steps):
+        lens = [n + m for n, m in zip(lens, news)]
+        cu = offsets(news)
+        # sizes over many powers of two, so that scales grow
+        x = torch.randn(2, cu[-1], H, D, generator=g) * torch.exp2(
+            torch.randint(-14, 8, (2, cu[-1], H, 1), generator=g).float())
+        if cu[-1] > 1:
+            x[0, 0, 0, :4] = torch.tensor([math.nan, math.inf, -math.inf, 1.0])
+            x[1, -1, -1, :3] = torch.tensor([65504.0, -60000.0, 2.0 ** -24])
+            if dtype == torch.bfloat16:
+                x[1, 0, 0, 5] = -3e38
+        k, v = x.to(dtype)
+        weights.fill_(7.0)
+        want.begun[:] = False
+        one = all(m == 1 for m in news) and case % 2
+        kv8.store(cache, k.to(DEV), v.to(DEV), i32(table), i32(lens), None if one else i32(cu),
+                  weights if step else None)
+        want.store(k, v, table, lens, cu)
+        same(cache, want, table, lens)
+        if step:
+            begun = want.begun[:, None].expand(-1, H, -1)
+            assert torch.equal(weights.cpu() == 0, begun) and weights.cpu()[~begun].eq(7).all()
+    e = torch.stack(want.e)
+    for b, n in enumerate(lens):     # scales are the least that hold the tokens so far
+        for t in range(0, n, 64):
+            at = table[b][t // page], slice(None), t % page // 64
+            for scale, x in ((cache.k_scale, e[0]), (cache.v_scale, e[1])):
+                assert torch.equal(scale.cpu()[at], torch.exp2(x[at].float()))
+    slots = [table[b][t // page] * page + t % page for b, n in enumerate(lens) for t in range(n)]
+    for got, x in zip(kv8.load(cache, i32(slots + [-1, pages * page, 2 ** 31 - 1]), dtype), want.x):
+        rows = torch.stack([x[s // page, :, s % page] for s in slots])
+        assert torch.equal(got[:len(slots)].double().cpu().nan_to_num(9e9), rows.nan_to_num(9e9))
+        assert got[len(slots):].eq(0).all()
+
+
+def test_every_code_is_held_exactly_in_both_types():
+    """All codes at the ends of the scales' range, read as fp16 and bf16."""
+    cache = kv8.new_cache(2, 64, 1, 64)
+    codes = torch.arange(256, dtype=torch.uint8, device=DEV)
+    cache.k.view(-1)[:256] = codes
+    cache.v.view(-1)[:256] = codes
+    for exp in (-15, 0, 7):
+        cache.k_scale.fill_(2.0 ** exp)
+        cache.v_scale.fill_(2.0 ** exp)
+        want = (sv.decode(cache.k.cpu(), cache.k_scale.cpu(), False),
+                sv.decode(cache.v.cpu(), cache.v_scale.cpu(), True))
+        for dtype in DTYPES:
+            got = kv8.load(cache, torch.arange(64, device=DEV).int(), dtype)
+            for g, w in zip(got, want):
+                assert torch.equal(g.double().cpu()[:, 0].nan_to_num(9e9), w[0, 0].nan_to_num(9e9))
+
+
+def test_store_passes_over_rows_without_a_place():
+    """Pages that lack, tables that end, more rows than tokens, offsets past the rows."""
+    page, H, D = 64, 2, 64
+    x = torch.randn(2, 300, H, D).half()
+    table = [[0, -1, 2], [3, 99, 4], [5, 6, 7], [8, 9, 10]]
+    lens, cu = [192, 130, 5, 500], [-5, 150, 200, 210, 400]
+    cache = kv8.new_cache(11, page, H, D)
+    untouched = sv.Cache(11, page, H, D)
+    untouched.store(x[0], x[1], table, lens, cu)
+    kv8.store(cache, x[0].to(DEV), x[1].to(DEV), i32(table), i32(lens), i32(cu))
+    got = sv.decode(cache.k.cpu(), cache.k_scale.cpu(), False)
+    assert torch.equal(got, untouched.x[0])       # rows not stored left the cache as it was
+    got = sv.decode(cache.v.cpu(), cache.v_scale.cpu(), True)
+    assert torch.equal(got, untouched.x[1])
+
+
+def test_store_reads_strided_rows_and_wide_tables():
+    T, H, D, page = 70, 2, 64, 64
+    big = torch.randn(T, 3, 3, 96, device=DEV).half()
+    k, v = big[:, 0, :H, :D], big[:, 1, 1:, 3:3 + D]   # v: not 16-byte aligned, copied
+    wide = torch.full((1, 9), -7, dtype=torch.int32, device=DEV)
+    wide[0, :2] = i32([1, 0])
+    cache, want = kv8.new_cache(2, page, H, D), sv.Cache(2, page, H, D)
+    kv8.store(cache, k, v, wide[:, :2], i32([T]), i32([0, T]))
+    want.store(k.cpu(), v.cpu(), [[1, 0]], [T], [0, T])
+    same(cache, want, [[1, 0]], [T])
+    kv8.store(cache, k[:0], v[:0], wide[:, :2], i32([T]), i32([0, 0]))
+    kv8.store(cache, k[:0], v[:0], wide[:0], i32([]), i32([0]))
+    same(cache, want, [[1, 0]], [T])
+
+
+def test_shorter_again():
+    """Drafted tokens that were refused: the next ones take their places."""
+    H, D = 1, 128
+    x = torch.randn(2, 100, H, D).bfloat16()
+    x[:, 60:70] *= 30
+    cache, want, table = kv8.new_cache(3, 64, H, D), sv.Cache(3, 64, H, D), [[2, 1]]
+    for lens, a, b in ((62, 0, 62), (70, 62, 70), (64, 70, 72), (66, 72, 74), (92, 74, 100)):
+        n = b - a
+        kv8.store(cache, *x[:, a:b].to(DEV), i32(table), i32([lens]), i32([0, n]))
+        want.store(*x[:, a:b], table, [lens], [0, n])
+        same(cache, want, table, [lens])
+
+
+def test_store_and_load_refuse():
+    cache = kv8.new_cache(2, 64, 2, 64)
+    x, t, n, cu = torch.zeros(3, 2, 64, device=DEV).half(), i32([[0]]), i32([3]), i32([0, 3])
+    w = kv8.new_weights(cache)
+    ok = dict(cache=cache, k=x, v=x, table=t, lens=n, cu_new=cu, weights=w)
+    for bad in (dict(k=x.float(), v=x.float()), dict(v=x.bfloat16()), dict(v=x[:2]),
+                dict(k=x[:, :1], v=x[:, :1]), dict(k=x.cpu()), dict(cu_new=None),
+                dict(cu_new=cu.long()), dict(cu_new=i32([0])), dict(lens=i32([3, 3])),
+                dict(table=t[0]), dict(table=t.long()), dict(table=t.cpu()), dict(weights=w[:1]),
+                dict(weights=w.half()), dict(weights=w.cpu()),
+                dict(cache=cache._replace(k=cache.k.int())), dict(cache=cache._replace(v=cache.v[:1])),
+                dict(cache=cache._replace(k_scale=cache.k_scale[:, :1])),
+                dict(cache=cache._replace(v=cache.v.transpose(3, 4).contiguous().transpose(3, 4))),
+                dict(cache=kv8.Cache(*(y.cpu() for y in cache)))):
+        with pytest.raises(RuntimeError):
+            kv8.store(**(ok | bad))
+    for bad in (n.long(), n.cpu(), n[None]):
+        with pytest.raises(RuntimeError):
+            kv8.load(cache, bad)
+    with pytest.raises(RuntimeError):
+        kv8.load(cache, n, torch.float32)
+
+
+# -- weights of blocks --------------------------------------------------------------------
+
+def filled(lens, page, Hkv, D, dtype, seed, gain=2.0):
+    """(cache on the GPU, what it holds, table) of random rows; the rest holds NaN."""
+    g = torch.Generator().manual_seed(seed)
+    table, pages = tables(lens, page, seed)
+    cache, held = dirty_cache(pages, page, Hkv, D), sv.Cache(pages, page, Hkv, D)
+    cu = offsets([max(0, n) for n in lens])
+    k = (torch.randn(cu[-1], Hkv, D, generator=g) * gain).to(dtype)
+    v = torch.randn(cu[-1], Hkv, D, generator=g).to(dtype)
+    kv8.store(cache, k.to(DEV), v.to(DEV), i32(table), i32(lens), i32(cu))
+    # (as the GPU holds it: the stores have tests of their own)
+    held.x = [sv.decode(cache.k.cpu(), cache.k_scale.cpu(), False),
+              sv.decode(cache.v.cpu(), cache.v_scale.cpu(), True)]
+    return cache, held, table
+
+
+def weighed(got, want, tol, table, lens, page):
+    """Blocks that hold tokens within the bound, the others as they were."""
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    worst = ((got - want).abs() / tol)[~want.isnan()].max().item()
+    print(f"  worst {worst:.3f} of the bound", flush=True)
+    assert worst <= 1.0
+
+
+HEADS = [(1, 1), (8, 2), (5, 5), (16, 1), (24, 2), (40, 1), (6, 2)]
+WEIGHS = [  # lens, queries of each request
+    ([1], [1]), ([0, 5], [1, 1]), ([63, 64, 65], [1, 1, 1]), ([130, 77, 300], [130, 1, 45]),
+    ([500, 0, 20, 9], [3, 0, 20, 0]), ([5, 200], [9, 2]), ([700], [300]), ([1030, 4], [1, 4]),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,page", [(64, 64), (128, 128), (128, 256)])
+@pytest.mark.parametrize("case", range(len(WEIGHS)))
+def test_weigh(case, D, page, dtype, causal):
+    lens, news = WEIGHS[case]
+    Hq, Hkv = HEADS[(case + D // 64 + page // 64) % len(HEADS)]
+    print(f"weigh {case} heads {Hq}/{Hkv} D{D} page {page} {dtype} causal {causal}", flush=True)
+    cache, held, table = filled(lens, page, Hkv, D, dtype, seed=case)
+    cu = offsets(news)
+    g = torch.Generator().manual_seed(case)
+    q = torch.randn(cu[-1] + 1, Hq, D, generator=g).to(dtype)
+    # any lse will do, the call takes what it is given
+    lse = torch.randn(cu[-1] + 1, Hq, generator=g) + 8
+    lse[0, 0] = -math.inf
+    weights = torch.rand(len(cache.k), Hkv, page // 64, generator=g)
+    got = weights.to(DEV)
+    single = all(m == 1 for m in news)
+    kv8.weigh(got, (q[:-1] if single else q).to(DEV), (lse[:-1] if single else lse).to(DEV), cache,
+              i32(table), i32(lens), D ** -0.5, cu_q=None if single else i32(cu), max_q=max(news),
+              causal=causal)
+    want, tol = sv.weigh(weights, q, lse, held, table, lens, D ** -0.5, cu, causal=causal)
+    weighed(got, want, tol, table, lens, page)
+    again = weights.to(DEV)
+    kv8.weigh(again, q.to(DEV), lse.to(DEV), cache, i32(table), i32(lens), D ** -0.5, cu_q=i32(cu),
+              max_q=max(news), causal=causal)
+    assert torch.equal(got, again) or single    # the order of sums is set by sizes
+
+
+def test_weigh_with_lost_pages_negative_scale_fewer_queries_and_nan():
+    cache, held, table = filled([300, 130], 64, 2, 64, torch.float16, seed=3)
+    table[0][1], table[1][0] = -1, 99
+    q = torch.randn(20, 4, 64).half()
+    lse = torch.full((20, 4), 5.0)
+    lse[3, 1] = math.nan            # reaches every block that the row sees
+    lse[4, 2] = math.inf
+    weights = torch.rand(len(cache.k), 2, 1)
+    for cu, max_q in (([0, 2, 20], 7), ([0, 18, 20], None)):
+        got = weights.to(DEV)
+        kv8.weigh(got, q.to(DEV), lse.to(DEV), cache, i32(table), i32([300, 130]), -0.2,
+                  cu_q=i32(cu), max_q=max_q)
+        want, tol = sv.weigh(weights, q, lse, held, table, [300, 130], -0.2, cu, max_q)
+        weighed(got, want, tol, table, [300, 130], 64)
+
+
+def test_weigh_refuses():
+    cache, _, table = filled([70], 64, 2, 64, torch.float16, seed=1)
+    w, q = kv8.new_weights(cache), torch.zeros(1, 4, 64, device=DEV).half()
+    ok = dict(weights=w, q=q, lse=torch.zeros(1, 4, device=DEV), cache=cache, table=i32(table),
+              lens=i32([70]), scale=0.1)
+    for bad in (dict(weights=w[:1]), dict(weights=w.double()), dict(q=q.float()), dict(q=q[:, :3]),
+                dict(lse=torch.zeros(1, 3, device=DEV)), dict(lse=torch.zeros(1, 4)),
+                dict(lse=torch.zeros(1, 4, device=DEV).half()), dict(scale=math.inf),
+                dict(scale=math.nan), dict(lens=i32([70, 1])), dict(cu_q=i32([0])),
+                dict(table=i32(table)[0]), dict(lens=i32([70]).long())):
+        with pytest.raises(RuntimeError):
+            kv8.weigh(**(ok | bad))
+
+
+# -- eviction -----------------------------------------------------------------------------
+
+EVICTS = [  # lens, keep, page, first, recent, used less than what is held
+    ([64 * 9], [4], 64, 1, 1, 0), ([64 * 9 + 1, 30, 0, 640], [4, 1, 0, 20], 64, 1, 1, 0),
+    ([3000, 500], [2, 0], 64, 5, 3, 0), ([256 * 40, 256 * 13 - 9], [3, 5], 256, 0, 1, 0),
+    ([128 * 700], [100], 128, 1, 4, 0), ([64 * 30] * 90, list(range(90)), 64, 1, 1, 0),
+    ([640, 640], [2, 2], 64, 0, 2, 7), ([640, 640], [2, 2], 64, 0, 2, 19),
+    ([64 * 4500, 64 * 4200], [1000, 4199], 64, 1, 1, 0), ([64 * 6], [-5], 64, 4, 9, 0),
+]
+
+
+@pytest.mark.parametrize("kind", ["spread", "equal", "special"])
+@pytest.mark.parametrize("case", range(len(EVICTS)))
+def test_evict(case, kind):
+    lens, keep, page, first, recent, less = EVICTS[case]
+    print(f"evict {case} {kind}", flush=True)
+    g = torch.Generator().manual_seed(case)
+    table, pages = tables(lens, page, case, spare=3)
+    H = 1 + case % 3
+    weights = torch.exp(3 * torch.randn(pages, H, page // 64, generator=g))
+    if kind == "equal":
+        weights = (weights > 1).float()
+    if kind == "special":
+        weights[::3] = 0.0
+        weights[1::5, 0] = math.inf
+        weights[2::7, 0] = math.nan
+        weights[::9] = -weights[::9]
+        for row in table[:2]:
+            row[1] = [-1, pages, 2 ** 31 - 1, -2 ** 31][case % 4]
+    held = sum(-(-n // page) for n in lens)
+    free = list(range(1000, 1000 + held + 4))
+    used = max(0, held - less)
+    dev_table = torch.full((len(lens), len(table[0]) + 2), -7, dtype=torch.int32, device=DEV)
+    dev_table[:, :len(table[0])] = i32(table)
+    t, f = dev_table[:, :len(table[0])], i32(free)
+    got = kv8.evict(weights.to(DEV), t, i32(lens), i32(keep), f, i32([used]), first, recent)
+    want = sv.evict(weights, page, table, lens, keep, free, used, first, recent)
+    for name, a, b in zip(("table", "free", "lens", "used", "lost"), (t, f, *got),
+                          (want[0], want[1], want[2], [want[3]], [want[4]])):
+        assert a.tolist() == b, name
+    assert dev_table[:, len(table[0]):].eq(-7).all()
+
+
+def test_evict_of_nothing():
+    w = torch.zeros(4, 2, 1, device=DEV)
+    none = i32([])
+    got = kv8.evict(w, none.view(0, 3), none, none, i32([5, 6]), i32([9]))
+    assert got.lens.numel() == 0 and got.used.item() == 2 and got.lost.item() == 0
+    t = i32([[0, 1], [2, 3]])
+    got = kv8.evict(w, t, i32([100, -4]), i32([2, 0]), i32([]), i32([0]))
+    assert t.tolist() == [[0, 1], [2, 3]] and got.lens.tolist() == [100, -4]
+    # lengths past the table's row: what the row holds counts
+    got = kv8.evict(w, t, i32([2 ** 31 - 1, 64]), i32([1, 1]), i32([9, 9]), i32([2]), first=0)
+    assert t.tolist() == [[1, -1], [2, 3]] and got.lens.tolist() == [2 ** 31 - 1 - 64, 64]
+
+
+def test_evict_refuses():
+    w = torch.zeros(4, 2, 1, device=DEV)
+    ok = dict(weights=w, table=i32([[0, 1]]), lens=i32([100]), keep=i32([1]), free_pages=i32([7, 8]),
+              used=i32([1]))
+    t = i32([[0, 1]])
+    for bad in (dict(weights=w.half()), dict(weights=w.cpu()), dict(weights=w[..., None]),
+                dict(weights=torch.zeros(4, 2, 3, device=DEV)), dict(keep=i32([1, 1])), dict(first=-1),
+                dict(recent=0), dict(used=i32([1, 1])), dict(lens=i32([1, 1])),
+                dict(table=i32([0, 1])), dict(free_pages=i32([7, 8]).long()),
+                dict(table=t, free_pages=t[0]),
+                dict(lens=i32([1, 1]), keep=i32([1, 1]), table=t.expand(2, 2))):
+        with pytest.raises(RuntimeError):
+            kv8.evict(**(ok | bad))
