@@ -61,7 +61,7 @@ HIP_FLAGS = [
 
 KERNEL_SOURCES = [CSRC / "attn_kernel.hip", CSRC / "conv3d_kernel.hip", CSRC / "scratch.hip",
                   CSRC / "kv4_kernel.hip", CSRC / "sparse_kernel.hip", CSRC / "kv8_kernel.hip",
-                  CSRC / "qknorm_kernel.hip"]
+                  CSRC / "kv8_attn_kernel.hip", CSRC / "qknorm_kernel.hip"]
 # A torch-free C caller of launch() (the reference's micro3.hip pattern),
 # linked against the kernel library.
 HARNESS_SOURCE = CSRC / "launch_harness.cpp"

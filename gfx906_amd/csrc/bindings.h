@@ -46,6 +46,11 @@ void kv8_store_op(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Ten
 std::vector<torch::Tensor> kv8_load_op(torch::Tensor kc, torch::Tensor ks, torch::Tensor vc,
                                        torch::Tensor vs, torch::Tensor slots,
                                        at::ScalarType dtype);
+std::vector<torch::Tensor> kv8_attn_op(torch::Tensor q, torch::Tensor kc, torch::Tensor ks,
+                                       torch::Tensor vc, torch::Tensor vs, torch::Tensor table,
+                                       torch::Tensor lens, double scale,
+                                       c10::optional<torch::Tensor> cu_q, int64_t max_q,
+                                       bool causal, c10::optional<torch::Tensor> out, bool lse);
 void kv8_weigh_op(torch::Tensor weights, torch::Tensor q, torch::Tensor lse, torch::Tensor kc,
                   torch::Tensor ks, torch::Tensor vc, torch::Tensor vs, torch::Tensor table,
                   torch::Tensor lens, double scale, c10::optional<torch::Tensor> cu_q,

@@ -135,6 +135,47 @@ std::vector<Tensor> kv8_load_op(Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tens
     return {k, v};
 }
 
+std::vector<Tensor> kv8_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor table,
+                                Tensor lens, double scale, c10::optional<Tensor> cu_q,
+                                int64_t max_q, bool causal, c10::optional<Tensor> out, bool lse) {
+    const char* who = "attn";
+    const Parts c(kc, ks, vc, vs, who);
+    const auto dev = kc.device();
+    const Queries n(q, c, table, lens, cu_q, max_q, dev, who);
+    Tensor o;
+    if (out.has_value()) {
+        o = *out;
+        TORCH_CHECK(o.device() == dev && o.dtype() == q.dtype() && o.sizes() == q.sizes(), who,
+                    ": out must have q's shape, dtype and device");
+        TORCH_CHECK(o.stride(2) == 1, who, ": out's head dim must be contiguous");
+        at::assert_no_partial_overlap(o, q);
+        for (const Tensor* t : {&kc, &ks, &vc, &vs, &table, &lens}) at::assert_no_overlap(o, *t);
+        if (cu_q.has_value()) at::assert_no_overlap(o, *cu_q);
+    } else {
+        o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    }
+    std::vector<Tensor> result{o};
+    if (lse) result.push_back(at::empty({n.T, n.Hq}, q.options().dtype(torch::kFloat)));
+    if (q.numel() == 0 || n.B == 0) return result;
+    const c10::DeviceGuard guard(dev);
+    // (a workgroup may read rows of q after another has written theirs: q is copied where out is q)
+    const bool in_place = o.data_ptr() == q.data_ptr();
+    const Tensor qr = in_place ? q.clone(at::MemoryFormat::Contiguous) : rows_of(q);
+    const auto sq = strides2(qr), so = strides2(o);
+    const int W = (int)table.size(1);
+    const size_t bytes = kv8_attn_workspace_bytes((int)n.T, (int)n.B, (int)n.Hq, c.Hkv, c.D,
+                                                  (int)max_q, W * c.page);
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, kc.options());
+    check_rc(kv8_attn(qr.data_ptr(), o.data_ptr(), lse ? result[1].data_ptr<float>() : nullptr,
+                      sq.data(), so.data(), n.dt, (int)n.T, (int)n.B, (int)n.Hq, c.Hkv, c.D,
+                      kc.data_ptr(), ks.data_ptr<float>(), vc.data_ptr(), vs.data_ptr<float>(),
+                      c.pages, c.page, table.data_ptr<int>(), table_stride(table), W,
+                      lens.data_ptr<int>(), ints(cu_q), (int)max_q, (float)scale, causal,
+                      bytes ? ws.data_ptr() : nullptr, bytes, stream()));
+    return result;
+}
+
 void kv8_weigh_op(Tensor weights, Tensor q, Tensor lse, Tensor kc, Tensor ks, Tensor vc, Tensor vs,
                   Tensor table, Tensor lens, double scale, c10::optional<Tensor> cu_q,
                   int64_t max_q, bool causal) {

@@ -13,7 +13,9 @@
 //
 // Tiles of 32 rows lie in LDS in the element type, 16-byte units XOR-swizzled so
 // that the reads of K (16 rows x one unit) and the transposed reads of V (4 rows x
-// 2 units) are free of bank conflicts.
+// 2 units) are free of bank conflicts. Or (FRAG) operand by operand, as the lanes
+// read them: 1 KB each, K's for dims step s and 16 keys kb at 2 s + kb, V's for 16 dims ob at
+// ob, with a lane's 16 bytes at frag_slot().
 #pragma once
 
 #include "longctx.h"
@@ -99,8 +101,16 @@ __device__ __forceinline__ bool p_above(const typename Elem<T>::x8 (&P)[NB]) {
     return __builtin_amdgcn_ballot_w64(!(r[0] <= lim) || !(r[1] <= lim)) != 0;
 }
 
-// NB: column blocks of 16 query rows.
-template <int D, class T, int NB = 2>
+// Place of the 16 bytes of lane 16 g + i within an operand (odd: those of every second operand
+// that lanes with side by side data write together): reads by lanes and writes by rows of data are
+// both free of bank conflicts.
+__device__ __forceinline__ int frag_slot(int i, int g, int odd) {
+    return (4 * i + ((g + (i >> 1)) & 3)) ^ (4 * odd);
+}
+
+// NB: column blocks of 16 query rows. FRAG: order of tiles in LDS. SUM: row sums of the
+// unrounded weights are kept too.
+template <int D, class T, int NB = 2, bool FRAG = false, bool SUM = false>
 struct Tile {
     using E = Elem<T>;
     using x8 = typename E::x8;
@@ -114,6 +124,7 @@ struct Tile {
     bool far;    // (wave-uniform) some |m| is past 2^16: exact maxima from there on
     x8 one;
     int kaddr[NQ], vaddr[NO];
+    float lsum[SUM ? NB : 1], psum[SUM ? NB : 1];  // of this lane's keys; of the block at hand
 
     __device__ __forceinline__ void init(int lane) {
         const int i = lane & 15, g = lane >> 4;
@@ -123,15 +134,29 @@ struct Tile {
             for (int ob = 0; ob < NO; ++ob) oacc[ob][nb] = f32x4{};
             lacc[nb] = f32x4{};
             m[nb] = kNoMax;
+            if constexpr (SUM) lsum[nb] = 0.f;
         }
         far = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) one[e] = (T)(i == 0 ? 1.0f : 0.0f);
 #pragma unroll
-        for (int s = 0; s < NQ; ++s) kaddr[s] = i * RB + ((4 * s + g) ^ kswz<NU>(i)) * 16;
+        for (int s = 0; s < NQ; ++s)
+            kaddr[s] = FRAG ? 16 * frag_slot(i, g, s >> 1) : i * RB + ((4 * s + g) ^ kswz<NU>(i)) * 16;
         const int vrow = 4 * g + (i >> 2), vx = vswz<NU>(vrow) >> 1;
 #pragma unroll
-        for (int ob = 0; ob < NO; ++ob) vaddr[ob] = vrow * RB + (ob ^ vx) * 32 + (i & 3) * 8;
+        for (int ob = 0; ob < NO; ++ob)
+            vaddr[ob] = FRAG ? 16 * frag_slot(i, g, 0) : vrow * RB + (ob ^ vx) * 32 + (i & 3) * 8;
+    }
+
+    // Operand n = 2 s + kb of the K tile kt, and ob of the V tile vt.
+    __device__ __forceinline__ x8 kread(const char* kt, int n) const {
+        return lds_read16<T>(kt, kaddr[n / 2] + (FRAG ? n * 1024 : 16 * (n % 2) * RB));
+    }
+    __device__ __forceinline__ x8 vread(const char* vt, int ob) const {
+        if constexpr (FRAG)
+            return lds_read16<T>(vt, vaddr[ob] + ob * 1024);
+        else
+            return lds_read_tr2<T>(vt, vaddr[ob], vaddr[ob] + 16 * RB);
     }
 
     // S of the K tile kt.
@@ -144,7 +169,7 @@ struct Tile {
         for (int s = 0; s < NQ; ++s)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const x8 kf = lds_read16<T>(kt, kaddr[s] + 16 * kb * RB);
+                const x8 kf = kread(kt, 2 * s + kb);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) S[kb][nb] = E::mma16(kf, qf[nb][s], S[kb][nb]);
             }
@@ -163,16 +188,16 @@ struct Tile {
     __device__ __forceinline__ void pv(const char* vt, const x8 (&P)[NB]) {
 #pragma unroll
         for (int ob = 0; ob < NO; ++ob) {
-            const x8 vf = lds_read_tr2<T>(vt, vaddr[ob], vaddr[ob] + 16 * RB);
+            const x8 vf = vread(vt, ob);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) oacc[ob][nb] = E::mma16(vf, P[nb], oacc[ob][nb]);
         }
-        constexpr int A = D == 128 ? 4 : 3;
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * A, 0);
+        constexpr int A = D == 128 ? 4 : 3, VR = FRAG ? 1 : 2;
+        __builtin_amdgcn_sched_group_barrier(0x100, VR * A, 0);
 #pragma unroll
         for (int n = 0; n < NO - A; ++n) {
             __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, VR, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, NB * A, 0);
     }
@@ -196,20 +221,24 @@ struct Tile {
     // overflow.
     template <bool FAR>
     __device__ __forceinline__ void weights(const f32x4 (&S)[2][NB], x8 (&P)[NB], float c,
-                                            int nb) const {
+                                            int nb) {
 #pragma clang fp contract(off)
         auto p = [&](float s) __attribute__((always_inline)) {
 #pragma clang fp contract(off)
             const float sc = s * c;
             return __builtin_amdgcn_exp2f(FAR ? sc - m[nb] : fmaf(s, c, -m[nb]));
         };
+        float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
             const f32x4& s = e < 4 ? S[0][nb] : S[1][nb];
-            const typename E::x2 h = E::cvt2(p(s[e & 3]), p(s[(e & 3) + 1]));
+            const float p0 = p(s[e & 3]), p1 = p(s[(e & 3) + 1]);
+            if constexpr (SUM) sum += p0 + p1;
+            const typename E::x2 h = E::cvt2(p0, p1);
             P[nb][e] = h[0];
             P[nb][e + 1] = h[1];
         }
+        if constexpr (SUM) psum[nb] = sum;
     }
 
     __device__ __forceinline__ void softmax(const f32x4 (&S)[2][NB], x8 (&P)[NB], float c) {
@@ -230,17 +259,14 @@ struct Tile {
         constexpr int AV = 2, AK = 2, NK = 2 * NQ, EPS = 8 * NB / (NO + NK);
         x8 vf[NO], kf[NK];
         float p[8 * NB];
-        auto vread = [&](int n) __attribute__((always_inline)) {
-            vf[n] = lds_read_tr2<T>(vt, vaddr[n], vaddr[n] + 16 * RB);
-        };
-        auto kread = [&](int n) __attribute__((always_inline)) {
-            kf[n] = lds_read16<T>(kt, kaddr[n / 2] + 16 * (n % 2) * RB);
-        };
+        auto vget = [&](int n) __attribute__((always_inline)) { vf[n] = vread(vt, n); };
+        auto kget = [&](int n) __attribute__((always_inline)) { kf[n] = kread(kt, n); };
         auto share = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
             for (int q = slot * EPS; q < (slot + 1) * EPS; ++q) {
                 const int nb = q / 8, e = q % 8;
                 p[q] = __builtin_amdgcn_exp2f(fmaf(S[e / 4][nb][e & 3], c, -m[nb]));
+                if constexpr (SUM) psum[nb] = e ? psum[nb] + p[q] : p[q];
                 if (e & 1) {
                     const typename E::x2 h = E::cvt2(p[q - 1], p[q]);
                     P[nb][e - 1] = h[0];
@@ -250,14 +276,14 @@ struct Tile {
             __builtin_amdgcn_sched_barrier(0);
         };
 #pragma unroll
-        for (int n = 0; n < AV; ++n) vread(n);
+        for (int n = 0; n < AV; ++n) vget(n);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < NO; ++n) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) oacc[n][nb] = E::mma16(vf[n], Pp[nb], oacc[n][nb]);
-            if (n + AV < NO) vread(n + AV);
-            if (n >= NO - AK) kread(n - (NO - AK));
+            if (n + AV < NO) vget(n + AV);
+            if (n >= NO - AK) kget(n - (NO - AK));
             share(n);
         }
 #pragma unroll
@@ -269,7 +295,7 @@ struct Tile {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
                 Sn[n % 2][nb] = E::mma16(kf[n], qf[nb][n / 2], Sn[n % 2][nb]);
-            if (n + AK < NK) kread(n + AK);
+            if (n + AK < NK) kget(n + AK);
             share(NO + n);
         }
         settle(S, P, c);
@@ -289,6 +315,7 @@ struct Tile {
 #pragma unroll
                 for (int ob = 0; ob < NO; ++ob) oacc[ob][nb] *= w;
                 lacc[nb] *= w;
+                if constexpr (SUM) lsum[nb] *= w;
                 m[nb] = mn;
                 weights<true>(S, P, c, nb);
             }
@@ -296,7 +323,10 @@ struct Tile {
             far = __builtin_amdgcn_ballot_w64(big(m[0]) || big(m[NB - 1])) != 0;
         }
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) lacc[nb] = E::mma16(one, P[nb], lacc[nb]);
+        for (int nb = 0; nb < NB; ++nb) {
+            lacc[nb] = E::mma16(one, P[nb], lacc[nb]);
+            if constexpr (SUM) lsum[nb] += psum[nb];
+        }
     }
 };
 

@@ -22,6 +22,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("norm_rotate", &norm_rotate_op, "norms of queries and keys with the position rotation");
     m.def("kv8_store", &kv8_store_op, "rows of k and v into the 8-bit cache");
     m.def("kv8_load", &kv8_load_op, "rows of the 8-bit cache");
+    m.def("kv8_attn", &kv8_attn_op, "attention over the 8-bit cache");
     m.def("kv8_weigh", &kv8_weigh_op, "attention weights of the 8-bit cache's blocks");
     m.def("kv8_evict", &kv8_evict_op, "eviction of pages by their attention weights");
 }

@@ -88,6 +88,27 @@ def load(cache, slots, dtype=torch.float16):
     return tuple(extension().kv8_load(*cache, slots, dtype))
 
 
+def attn(q, cache, table, lens, scale, cu_q=None, max_q=None, causal=True, out=None, lse=False):
+    """softmax(scale * q k^T) v over the cache: ``q`` ``[T, Hq, D]`` (fp16 or bf16; Hq
+    a multiple of the cache's heads), the result in a new tensor or in ``out``; with ``lse`` the pair of
+    it and of the logarithms of the sums of exp(scale * q k), fp32 ``[T, Hq]``.
+
+    Rows ``cu_q[b] .. cu_q[b+1]`` (int32 ``[B + 1]``) are the queries of request b,
+    which holds ``lens[b]`` tokens (int32 ``[B]``) in the pages of ``table``'s row b;
+    without ``cu_q`` row b is the one query of request b. With ``causal`` they are
+    the request's last tokens and see none behind themselves. ``max_q``, for ``cu_q``: at
+    least the most queries of a request (queries past it are not computed); without it
+    T is taken, and a decoding step pays for what it does not need. Rows outside
+    every request are left as they were (in a new tensor: unset). ``out`` may be ``q``
+    itself and must not overlap the other arguments otherwise. Rows that see no
+    key are 0, with an lse of -inf; keys without a page weigh nothing."""
+    if max_q is None:
+        max_q = 1 if cu_q is None else q.shape[0]
+    res = extension().kv8_attn(q, *cache, table, lens, float(scale), cu_q, max_q, causal, out,
+                               bool(lse))
+    return tuple(res) if lse else res[0]
+
+
 def weigh(weights, q, lse, cache, table, lens, scale, cu_q=None, max_q=None, causal=True) -> None:
     """Adds to ``weights`` (:func:`new_weights`) the attention that every block's tokens get
     from the queries: the softmax weights summed over tokens, queries and the query heads of

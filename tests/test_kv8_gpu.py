@@ -203,8 +203,6 @@ def test_store_and_load_refuse():
         kv8.load(cache, n, torch.float32)
 
 
-# -- weights of blocks --------------------------------------------------------------------
-
 def filled(lens, page, Hkv, D, dtype, seed, gain=2.0):
     """(cache on the GPU, what it holds, table) of random rows; the rest holds NaN."""
     g = torch.Generator().manual_seed(seed)
@@ -220,6 +218,211 @@ def filled(lens, page, Hkv, D, dtype, seed, gain=2.0):
     return cache, held, table
 
 
+# -- attention ----------------------------------------------------------------------------
+
+def check(out, lse, rows, untouched=None):
+    """Computed rows within the bound, the others as they were."""
+    out = out.double().cpu()
+    lse = None if lse is None else lse.double().cpu()
+    worst = far = 0.0
+    for r in range(out.shape[0]):
+        if r not in rows:
+            if untouched is not None:
+                assert torch.equal(out[r], untouched[r].double().cpu()), f"row {r} written"
+            continue
+        o, tol, l, ltol = rows[r]
+        nan = o.isnan()
+        assert torch.equal(out[r].isnan(), nan), f"row {r}: NaN"
+        err = ((out[r] - o).abs() / tol)[~nan]
+        if err.numel():
+            worst = max(worst, err.max().item())
+            assert worst <= 1.0, f"row {r}: {worst} of the bound"
+        if lse is not None:
+            fin = torch.isfinite(l)
+            assert torch.equal(lse[r][~fin].nan_to_num(9e9, 8e9, 7e9), l[~fin].nan_to_num(9e9, 8e9, 7e9))
+            if fin.any():
+                far = max(far, ((lse[r] - l).abs() / ltol)[fin].max().item())
+                assert far <= 1.0, f"row {r}: lse {far} of the bound"
+    print(f"  worst {worst:.3f} of the bound, lse {far:.3f}", flush=True)
+
+
+HEADS = [(1, 1), (8, 2), (5, 5), (16, 1), (24, 2), (40, 1), (6, 2)]
+DECODES = [[1], [0, 5], [63, 64, 65], [0, 1, 130, 700, 33], [2050, 1, 300]]
+
+
+@pytest.mark.parametrize("lse", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,page", [(64, 64), (128, 64), (128, 128), (64, 256), (128, 256)])
+@pytest.mark.parametrize("lens", DECODES)
+def test_single_tokens(lens, D, page, dtype, lse):
+    Hq, Hkv = HEADS[(len(lens) + D // 64 + page // 64) % len(HEADS)]
+    print(f"decode lens {lens} heads {Hq}/{Hkv} D{D} page {page} {dtype}", flush=True)
+    cache, held, table = filled(lens, page, Hkv, D, dtype, seed=sum(lens))
+    q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(7)).to(dtype)
+    out = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), D ** -0.5, lse=lse)
+    check(*(out if lse else (out, None)), sv.attention(q, held, table, lens, D ** -0.5))
+
+
+CHUNKS = [  # lens, queries of each request, rows behind the last
+    ([1], [1], 0), ([64], [64], 0), ([130, 77, 300], [130, 1, 45], 5),
+    ([500, 0, 20, 9], [3, 0, 20, 0], 1), ([5, 200], [9, 2], 0),   # more queries than tokens
+    ([700], [300], 0), ([129, 1025], [2, 17], 3),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(4, 4), (6, 2), (8, 1)])
+@pytest.mark.parametrize("case", range(len(CHUNKS)))
+def test_chunks(case, heads, dtype, causal):
+    lens, news, behind = CHUNKS[case]
+    Hq, Hkv = heads
+    D, page = (64, 128)[(case + Hq // 3) % 2], (64, 128, 256)[(case + Hq) % 3]
+    print(f"chunks {case} heads {heads} D{D} page {page} {dtype} causal {causal}", flush=True)
+    cache, held, table = filled(lens, page, Hkv, D, dtype, seed=case)
+    cu = offsets(news)
+    T = cu[-1] + behind
+    q = torch.randn(T, Hq, D, generator=torch.Generator().manual_seed(case)).to(dtype)
+    out = torch.full((T, Hq, D), 3.0, dtype=dtype, device=DEV)
+    before = out.clone()
+    got, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), D ** -0.5, cu_q=i32(cu),
+                        max_q=max(news), causal=causal, out=out, lse=True)
+    assert got.data_ptr() == out.data_ptr()
+    rows = sv.attention(q, held, table, lens, D ** -0.5, cu, causal=causal)
+    check(out, lse, rows, before)
+    plain = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), D ** -0.5, cu_q=i32(cu),
+                     max_q=max(news), causal=causal)
+    keep = sorted(rows)
+    assert torch.equal(plain[keep], out[keep])     # with or without lse, the same result
+
+
+LONG = [  # lens, queries of each request, heads: runs that end inside a head or a tile
+    ([5000], [4], (16, 2)), ([3000, 70, 2600], [1, 1, 1], (6, 2)), ([4100], [200], (4, 2)),
+    ([2500, 3000, 64], [300, 1, 64], (4, 1)), ([2300], [1], (96, 1)), ([300, 20], [3, 1], (96, 1)),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_long_contexts(case, D, dtype, causal):
+    lens, news, (Hq, Hkv) = LONG[case]
+    print(f"long {case} D{D} {dtype} causal {causal}", flush=True)
+    cache, held, table = filled(lens, 64, Hkv, D, dtype, seed=case)
+    cu = offsets(news)
+    q = torch.randn(cu[-1], Hq, D, generator=torch.Generator().manual_seed(case)).to(dtype)
+    out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), D ** -0.5, cu_q=i32(cu),
+                        max_q=max(news), causal=causal, lse=True)
+    check(out, lse, sv.attention(q, held, table, lens, D ** -0.5, cu, causal=causal))
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_requests(wide):
+    """A thousand requests, some without tokens; with a wide table too (runs of units)."""
+    g = torch.Generator().manual_seed(12)
+    lens = [int(n) for n in torch.randint(0, 90, (1000,), generator=g)]
+    cache, held, table = filled(lens, 64, 1, 64, torch.float16, seed=12)
+    if wide:
+        table = [row + [-1] * 60 for row in table]
+    q = torch.randn(1000, 2, 64, generator=g).half()
+    out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), 0.125, lse=True)
+    check(out, lse, sv.attention(q, held, table, lens, 0.125))
+
+
+def test_prompts_among_many_requests():
+    """Three hundred requests, four of them prompts (their tiles are summed up by a kernel of
+    its own)."""
+    g = torch.Generator().manual_seed(2)
+    lens = [int(n) for n in torch.randint(0, 70, (300,), generator=g)]
+    news = [min(1, n) for n in lens]
+    for b, n in ((5, 400), (6, 130), (170, 700), (299, 257)):
+        lens[b], news[b] = n, max(129, n - 100)
+    cache, held, table = filled(lens, 64, 1, 64, torch.bfloat16, seed=2)
+    cu = offsets(news)
+    q = torch.randn(cu[-1], 2, 64, generator=g).bfloat16()
+    out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), 0.125, cu_q=i32(cu),
+                        max_q=max(news), lse=True)
+    check(out, lse, sv.attention(q, held, table, lens, 0.125, cu))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("news", [[5, 1], [150, 40]])
+def test_nan_reaches_only_the_rows_that_see_it(news, D, dtype):
+    """NaN and infinities among the keys and values of tokens that some rows do not see."""
+    lens, page, H = [230, 130], 64, 2
+    table, pages = tables(lens, page, 4)
+    cache, held = dirty_cache(pages, page, H, D), sv.Cache(pages, page, H, D)
+    g = torch.Generator().manual_seed(5)
+    k, v = torch.randn(2, sum(lens), H, D, generator=g).to(dtype)
+    v[lens[0] - 2, 0, 5], v[lens[0] - 3, 1, D - 1] = math.nan, math.inf
+    v[10, 0, 7] = -math.inf                       # a token that all rows see
+    v[lens[0] + 100, 1, 3] = math.nan
+    k[lens[0] - 1, 1, 0] = math.nan
+    cu = offsets(lens)
+    kv8.store(cache, k.to(DEV), v.to(DEV), i32(table), i32(lens), i32(cu))
+    held.store(k, v, table, lens, cu)
+    cu = offsets(news)
+    q = torch.randn(cu[-1], 4, D, generator=g).to(dtype)
+    for causal in (True, False):
+        out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), 0.1, cu_q=i32(cu),
+                            max_q=max(news), causal=causal, lse=True)
+        rows = sv.attention(q, held, table, lens, 0.1, cu, causal=causal)
+        assert any(r[0].isnan().any() for r in rows.values())
+        check(out, lse, rows)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wide", [0, 60])
+def test_lost_pages_and_scores_that_vanish(wide, dtype):
+    """Pages that lack, scores of -inf, far scores, and a negative scale."""
+    lens, news, page, H, D = [300, 64, 500], [4, 1, 290], 64, 2, 64
+    cache, held, table = filled(lens, page, H, D, dtype, seed=8, gain=30.0)
+    table[0][1], table[1][0], table[2][3] = -1, 99, -7
+    table = [row + [-1] * wide for row in table]
+    cu = offsets(news)
+    q = (torch.randn(cu[-1], 4, D, generator=torch.Generator().manual_seed(1)) * 5).to(dtype)
+    for scale in (0.125, -0.3, 8.0):
+        out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), scale, cu_q=i32(cu),
+                            max_q=290, lse=True)
+        check(out, lse, sv.attention(q, held, table, lens, scale, cu))
+
+
+def test_fewer_queries_than_there_are_in_place_and_strided():
+    lens, news, page, H, D = [200, 90], [150, 7], 64, 1, 128
+    cache, held, table = filled(lens, page, H, D, torch.float16, seed=6)
+    cu = offsets(news)
+    buf = torch.randn(cu[-1], 3, 2 * D, device=DEV).half()
+    q = buf[:, :2, :D]
+    rows = sv.attention(q.cpu(), held, table, lens, 0.1, cu, 9)
+    out = torch.zeros(cu[-1], 5, D, device=DEV).half()
+    kv8.attn(q, cache, i32(table), i32(lens), 0.1, cu_q=i32(cu), max_q=9, out=out[:, 1:3])
+    check(out[:, 1:3], None, rows, torch.zeros(cu[-1], 2, D))
+    assert out[:, 0].eq(0).all() and out[:, 3:].eq(0).all()
+    want = kv8.attn(q, cache, i32(table), i32(lens), 0.1, cu_q=i32(cu))
+    q = q.contiguous()
+    assert kv8.attn(q, cache, i32(table), i32(lens), 0.1, cu_q=i32(cu), out=q).data_ptr() == q.data_ptr()
+    assert torch.equal(q, want)
+
+
+def test_attn_refuses():
+    cache, _, table = filled([70], 64, 2, 64, torch.float16, seed=1)
+    q = torch.zeros(1, 4, 64, device=DEV).half()
+    ok = dict(q=q, cache=cache, table=i32(table), lens=i32([70]), scale=0.1)
+    for bad in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q.cpu()), dict(q=q[..., :32]),
+                dict(scale=math.inf), dict(scale=math.nan), dict(lens=i32([70, 1])),
+                dict(cu_q=i32([0])), dict(table=i32(table)[0]), dict(lens=i32([70]).long()),
+                dict(out=q[:, :2]), dict(out=q.float()),
+                dict(out=cache.k.view(-1)[:512].view(torch.float16).view(1, 4, 64)),
+                dict(out=torch.zeros(1, 4, 128, device=DEV).half()[..., ::2]),
+                dict(cache=cache._replace(v=cache.k))):
+        with pytest.raises(RuntimeError):
+            kv8.attn(**(ok | bad))
+
+
+# -- weights of blocks --------------------------------------------------------------------
+
 def weighed(got, want, tol, table, lens, page):
     """Blocks that hold tokens within the bound, the others as they were."""
     got = got.double().cpu()
@@ -229,7 +432,6 @@ def weighed(got, want, tol, table, lens, page):
     assert worst <= 1.0
 
 
-HEADS = [(1, 1), (8, 2), (5, 5), (16, 1), (24, 2), (40, 1), (6, 2)]
 WEIGHS = [  # lens, queries of each request
     ([1], [1]), ([0, 5], [1, 1]), ([63, 64, 65], [1, 1, 1]), ([130, 77, 300], [130, 1, 45]),
     ([500, 0, 20, 9], [3, 0, 20, 0]), ([5, 200], [9, 2]), ([700], [300]), ([1030, 4], [1, 4]),
