@@ -192,11 +192,16 @@ void kv8_weigh_op(Tensor weights, Tensor q, Tensor lse, Tensor kc, Tensor ks, Te
     if (q.numel() == 0 || n.B == 0) return;
     const Tensor qr = rows_of(q);
     const auto sq = strides2(qr);
+    const size_t bytes = kv8_weigh_workspace_bytes((int)n.T, (int)n.B, (int)n.Hq, c.Hkv, (int)max_q,
+                                                   (int)table.size(1), c.page);
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, kc.options());
     check_rc(kv8_weigh(weights.data_ptr<float>(), qr.data_ptr(), sq.data(), n.dt,
                        lse.data_ptr<float>(), (int)n.T, (int)n.B, (int)n.Hq, c.Hkv, c.D,
                        kc.data_ptr(), ks.data_ptr<float>(), c.pages, c.page, table.data_ptr<int>(),
                        table_stride(table), (int)table.size(1), lens.data_ptr<int>(), ints(cu_q),
-                       (int)max_q, (float)scale, causal, stream()));
+                       (int)max_q, (float)scale, causal, bytes ? ws.data_ptr() : nullptr, bytes,
+                       stream()));
 }
 
 std::vector<Tensor> kv8_evict_op(Tensor weights, Tensor table, Tensor lens, Tensor keep,

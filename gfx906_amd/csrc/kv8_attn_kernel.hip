@@ -51,20 +51,28 @@ __device__ __forceinline__ float lse_of(float m, float l) {
     return l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
 }
 
-// The V codes vc of a block of 64 keys (a lane's dims 16 ob + l%16, its 16 tokens), of which some
-// rows see only the keys below lim: a weight of 0 would not keep a NaN out of the sum of a row that
-// does not see it, so NaN codes become 0, and the sums of the rows that see one (a product of
-// who sees what with what is NaN) become NaN.
-template <int D, class T, int NB>
-__device__ __forceinline__ void take_nans(u32x4 (&vc)[D / 16], f32x4 (&oacc)[D / 16][NB], int key0,
-                                          const int (&lim)[NB], int g) {
-    using x8 = typename Elem<T>::x8;
+// V codes of a block of which some rows do not see all keys: a weight of 0 would not keep a NaN out
+// of the sum of a row that does not see it. NaN codes become 0; whether there were any (in the wave).
+template <int D>
+__device__ __forceinline__ bool strip_nans(u32x4 (&vc)[D / 16]) {
     unsigned any = 0;
 #pragma unroll
     for (int ob = 0; ob < D / 16; ++ob)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) any |= nan_bytes(vc[ob][e]);
-    if (__builtin_expect(!__any(any), 1)) return;
+        for (int e = 0; e < 4; ++e) {
+            const unsigned n = nan_bytes(vc[ob][e]);
+            any |= n;
+            vc[ob][e] &= ~((n >> 7) * 255u);
+        }
+    return __any(any);
+}
+
+// Afterwards: the sums of the rows that see a NaN of the block (its codes at vp, of this lane) become
+// NaN. Which do is a product too, of who sees what with what is NaN.
+template <int D, class T, int NB>
+__device__ __forceinline__ void give_nans(const uint8_t* vp, f32x4 (&oacc)[D / 16][NB], int key0,
+                                          const int (&lim)[NB], int g) {
+    using x8 = typename Elem<T>::x8;
     x8 sees[2][NB];
 #pragma unroll
     for (int half = 0; half < 2; ++half)
@@ -76,24 +84,21 @@ __device__ __forceinline__ void take_nans(u32x4 (&vc)[D / 16], f32x4 (&oacc)[D /
                     (T)(key0 + 32 * half + 16 * (e / 4) + 4 * g + (e & 3) < lim[nb] ? 1.f : 0.f);
 #pragma unroll
     for (int ob = 0; ob < D / 16; ++ob) {
-        unsigned one[4];
+        u32x4 x = *reinterpret_cast<const u32x4*>(vp + ob * 16 * kBlock);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const unsigned n = nan_bytes(vc[ob][e]) >> 7;
-            one[e] = n * 0x38u;  // 1.0
-            vc[ob][e] &= ~(n * 255u);
-        }
+        for (int e = 0; e < 4; ++e) x[e] = (nan_bytes(x[e]) >> 7) * 0x38u;  // 1.0
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             f32x4 count = {};
 #pragma unroll
             for (int half = 0; half < 2; ++half)
-                count = Elem<T>::mma16(expand<T>(one[2 * half], one[2 * half + 1], 1.f),
-                                       sees[half][nb], count);
+                count = Elem<T>::mma16(expand<T>(x[2 * half], x[2 * half + 1], 1.f), sees[half][nb],
+                                       count);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (count[e] > 0.f) oacc[ob][nb][e] = NAN;
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 #endif
@@ -275,6 +280,7 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
                 vc[ob] = *reinterpret_cast<const u32x4*>(p + (voff + ob * 16 * kBlock));
         };
         int c = c0 + wave, page = -1, next = -1;
+        bool nans = false;
         if (c < c1) {  // (a request without keys may have no table)
             page = page_of(c);
             next = page_of(c + NW);
@@ -309,7 +315,7 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
                 for (int nb = 0; nb < NB; ++nb) lim2[nb] = ok ? lim[nb] : 0;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) w.mask(S[half], key0 + 32 * half, lim2, g);
-                take_nans<D, T, NB>(vc, w.oacc, key0, lim2, g);
+                nans |= strip_nans<D>(vc) && ok;
             }
             const float s = ok ? vs : 1.f;  // (a scale that is NaN would reach every row)
 #pragma unroll
@@ -326,6 +332,14 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
                 __builtin_amdgcn_sched_barrier(0);
             }
             fetch_v(c + NW, page);
+        }
+        if (__builtin_expect(nans, 0)) {
+            for (c = c0 + wave; c < c1; c += NW) {
+                const int page = page_of(c);
+                if (c * 64 + 64 <= all_see || (unsigned)page >= (unsigned)a.c.pages) continue;
+                give_nans<D, T, NB>(a.c.vc + block_of(c, page) * (kBlock * D) + voff, w.oacc, c * 64, lim,
+                                    g);
+            }
         }
 
         // Merge the waves: a common max, then sums of 16 rows at a time through LDS.
@@ -777,12 +791,8 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             for (int x = max(c0, tile_see / 64); x < c1; ++x) {
                 const int page = page_of(x);
                 if (!good(x, page)) continue;
-                const uint8_t* p = a.c.vc + block_of(x, page) * (kBlock * D) + i * kBlock + 16 * g;
-                u32x4 vc[W::NO];
-#pragma unroll
-                for (int ob = 0; ob < W::NO; ++ob)
-                    vc[ob] = *reinterpret_cast<const u32x4*>(p + ob * 16 * kBlock);
-                take_nans<D, T, 2>(vc, w.oacc, x * 64, lim, g);
+                give_nans<D, T, 2>(a.c.vc + block_of(x, page) * (kBlock * D) + i * kBlock + 16 * g,
+                                   w.oacc, x * 64, lim, g);
             }
         }
 

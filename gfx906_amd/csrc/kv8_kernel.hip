@@ -294,37 +294,70 @@ struct LoadArgs {
     int T;
 };
 
-// 64 rows of a head a workgroup, 8 dims a lane: of V these are 8 bytes in as many lines, which
-// the rows of a block share. grid: rows / 64, heads x (K, V).
+// 64 rows of a head a workgroup, 8 dims a lane. Of V a row is D bytes in as many lines, so the
+// blocks that the rows lie in are read whole, one after the other, and the rows picked from
+// LDS. grid: rows / 64, heads x (K, V).
 template <class T, int D>
 __global__ void __launch_bounds__(256) load_kernel(const LoadArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int DL = D / 8, RW = 256 / DL;
-    const int h = blockIdx.y >> 1, dl = threadIdx.x % DL;
+    using x8 = typename Elem<T>::x8;
+    constexpr int DL = D / 8, RW = 256 / DL, PITCH = kBlock + 4;
+    __shared__ unsigned char vb[D * PITCH];
+    const int h = blockIdx.y >> 1, dl = threadIdx.x % DL, lane = threadIdx.x & 63;
     const bool is_v = blockIdx.y & 1;
+    const long long t0 = blockIdx.x * 64LL;
+    x8* const out = reinterpret_cast<x8*>(is_v ? a.v : a.k);
+    const int mine = t0 + lane < a.T ? a.slots[t0 + lane] : -1;  // (every wave has all 64)
+    const int part = a.c.page / kBlock;
+    // Number of the row's block among those of a head, -1 outside the cache.
+    const int block = mine >= 0 && mine < a.c.pages * (long long)a.c.page ? mine / kBlock : -1;
+    auto where = [&](int blk) { return block_at(a.c, blk / part, h, blk % part); };
+    auto put = [&](long long t, unsigned lo, unsigned hi, float s) {
+        out[(t * a.c.Hkv + h) * DL + dl] = expand<T>(lo, hi, s);
+    };
 #pragma unroll
     for (int n = 0; n < 64 / RW; ++n) {
-        const long long t = blockIdx.x * 64LL + n * RW + threadIdx.x / DL;
-        if (t >= a.T) continue;
-        const int slot = a.slots[t];
-        unsigned w[2] = {};
-        float s = 1.f;
-        if (slot >= 0 && slot < a.c.pages * (long long)a.c.page) {
-            const int page = slot / a.c.page, tok = slot % a.c.page;
-            const long long blk = block_at(a.c, page, h, tok / kBlock);
-            s = (is_v ? a.c.vs : a.c.ks)[blk];
-            if (is_v) {
-                const uint8_t* p = a.c.vc + blk * (kBlock * D) + 8 * dl * kBlock + place(tok % kBlock);
-#pragma unroll
-                for (int d = 0; d < 8; ++d) w[d / 4] |= (unsigned)p[d * kBlock] << (8 * (d & 3));
-            } else {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(
-                    a.c.kc + blk * (kBlock * D) + (tok % kBlock) * D + 8 * dl);
-                w[0] = x[0], w[1] = x[1];
-            }
+        const int r = n * RW + threadIdx.x / DL, blk = __shfl(block, r), slot = __shfl(mine, r);
+        if (t0 + r >= a.T) continue;
+        if (blk < 0) {
+            put(t0 + r, 0, 0, 1.f);
+        } else if (!is_v) {
+            const long long at = where(blk);
+            const u32x2 x = *reinterpret_cast<const u32x2*>(a.c.kc + at * (kBlock * D) +
+                                                            slot % kBlock * D + 8 * dl);
+            put(t0 + r, x[0], x[1], a.c.ks[at]);
         }
-        reinterpret_cast<typename Elem<T>::x8*>(is_v ? a.v : a.k)[(t * a.c.Hkv + h) * DL + dl] =
-            expand<T>(w[0], w[1], s);
+    }
+    if (!is_v) return;
+    for (unsigned long long left = __ballot(block >= 0); left;) {
+        const int blk = __shfl(block, (int)__ffsll(left) - 1);
+        const unsigned long long same = __ballot(block == blk);
+        left &= ~same;
+        const long long at = where(blk);
+        const float s = a.c.vs[at];
+        u32x4 x[D / 64];
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n)
+            x[n] = *reinterpret_cast<const u32x4*>(a.c.vc + at * (kBlock * D) + 4096 * n + 16 * threadIdx.x);
+        __syncthreads();  // (the block before has been read)
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) {
+            unsigned* p = reinterpret_cast<unsigned*>(vb + (64 * n + threadIdx.x / 4) * PITCH +
+                                                      16 * (threadIdx.x & 3));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = x[n][e];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 64 / RW; ++n) {
+            const int r = n * RW + threadIdx.x / DL, slot = __shfl(mine, r);
+            if (!(same >> r & 1)) continue;
+            const unsigned char* p = vb + 8 * dl * PITCH + place(slot % kBlock);
+            unsigned w[2] = {};
+#pragma unroll
+            for (int d = 0; d < 8; ++d) w[d / 4] |= (unsigned)p[d * PITCH] << (8 * (d & 3));
+            put(t0 + r, w[0], w[1], s);
+        }
     }
 #endif
 }
@@ -343,98 +376,263 @@ struct WeighArgs {
     const int* cu;
     int W, T, B, Hq, G, max_q, causal;
     float scale, qsign;  // log2_scale(); a negative scale negates q
+    int groups, split_rows, parts;  // of WeighPlan
+    float* sums;                    // [request][kv head][part][block]
 };
 
-// Weights of a block of 64 keys: its keys stay in registers as the matrix operand, the query
-// rows (a token's G heads beside each other) go by in tiles of 16, and each lane adds up the
-// exponentials of its rows and keys. SHARE waves of a workgroup have one block and every SHARE-th
-// tile of it (prompts), or four blocks (single tokens).
-//
-// grid: blocks of the table, kv heads, requests.
-template <int D, class T, int SHARE>
-__global__ void __launch_bounds__(256) weigh_kernel(const WeighArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using x8 = typename Elem<T>::x8;
-    constexpr int NJ = D / 64;
-    __shared__ float part[4];
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-    const int wave = uni(threadIdx.x >> 6);
-    const int hk = blockIdx.y, b = blockIdx.z;
-    const long long chunk = (long long)blockIdx.x * (4 / SHARE) + (SHARE == 1 ? wave : 0);
-    const Request req = request(a, b);
-    if (chunk * kBlock >= req.keys) return;  // (SHARE > 1: the same for all waves)
-    const int page = uni(a.table[b * a.table_stride + chunk * kBlock / a.c.page]);
-    if ((unsigned)page >= (unsigned)a.c.pages) return;
-    const int key0 = (int)chunk * kBlock;
-    const long long blk = block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock)));
-
-    // Keys 16 t + i, dims 64 j + 16 g + 8 n .. + 7.
-    x8 kf[4][NJ][2];
-    const float ks = ((ConstFloats)a.c.ks)[blk];
-    const uint8_t* kp = a.c.kc + blk * (kBlock * D) + i * D + 16 * g;
-    u32x4 raw[4][NJ];
+// Keys of a block as the matrix operand: keys 16 t + i, dims 64 j + 16 g + 8 n .. + 7 at step 2 j + n.
+template <int D, class T>
+__device__ __forceinline__ void load_keys(const Cache& c, long long blk, int i, int g,
+                                          typename Elem<T>::x8 (&kf)[4][D / 32]) {
+    const float ks = ((ConstFloats)c.ks)[blk];
+    const uint8_t* kp = c.kc + blk * (kBlock * D) + i * D + 16 * g;
+    u32x4 raw[4][D / 64];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < D / 64; ++j)
             raw[t][j] = *reinterpret_cast<const u32x4*>(kp + t * 16 * D + 64 * j);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            kf[t][j][0] = expand<T>(raw[t][j][0], raw[t][j][1], ks);
-            kf[t][j][1] = expand<T>(raw[t][j][2], raw[t][j][3], ks);
+        for (int j = 0; j < D / 64; ++j) {
+            kf[t][2 * j] = expand<T>(raw[t][j][0], raw[t][j][1], ks);
+            kf[t][2 * j + 1] = expand<T>(raw[t][j][2], raw[t][j][3], ks);
         }
-
-    const long long rows = (long long)req.m * a.G;
-    // The first query that sees the block's first key.
-    const long long q0 = a.causal ? max(0LL, key0 - (req.len - req.n)) : 0;
-    const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
-    float acc = 0.f;
-    for (long long r0 = (q0 * a.G & ~15LL) + (SHARE > 1 ? 16 * wave : 0); r0 < rows; r0 += 16 * SHARE) {
-        const long long r = r0 + i;
-        const int tok = (int)(r / a.G), h = hk * a.G + (int)(r - (long long)tok * a.G);
-        const bool ok = r < rows;
-        int lim = ok ? seen_by(a, req, tok) : 0;
-        const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh + 16 * g;
-        x8 qf[NJ][2];
+}
+// exp2 of 16 rows' scores with a block's keys less m (a lane's row), added to acc: those of keys below
+// lim, where not every row sees every key.
+template <int D, class T>
+__device__ __forceinline__ void add_weights(const typename Elem<T>::x8 (&kf)[4][D / 32],
+                                            const typename Elem<T>::x8 (&qf)[D / 32], float scale,
+                                            float m, bool all, int lim, int key0, int g,
+                                            float (&acc)[4]) {
+    f32x4 S[4] = {};
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+    for (int n = 0; n < D / 32; ++n)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                u32x4 x = {};
-                if (ok) x = *reinterpret_cast<const u32x4*>(q + 64 * j + 8 * n);
-                qf[j][n] = __builtin_bit_cast(x8, x ^ neg);
-            }
-        const float lse = ok ? a.lse[(long long)(req.first + tok) * a.Hq + h] : -INFINITY;
-        if (lse == -INFINITY) lim = 0;
-        const float m = lse * kLog2e;
-        f32x4 S[4] = {};
+        for (int t = 0; t < 4; ++t) S[t] = Elem<T>::mma16(kf[t][n], qf[n], S[t]);
+    if (all) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) S[t] = Elem<T>::mma16(kf[t][j][n], qf[j][n], S[t]);
+            for (int e = 0; e < 4; ++e) acc[e] += __builtin_amdgcn_exp2f(fmaf(S[t][e], scale, -m));
+    } else {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(S[t][e], a.scale, -m));
-                acc += key0 + 16 * t + 4 * g + e < lim ? p : 0.f;
+                const float p = __builtin_amdgcn_exp2f(fmaf(S[t][e], scale, -m));
+                acc[e] += key0 + 16 * t + 4 * g + e < lim ? p : 0.f;
             }
     }
-    acc = wave_sum(acc);
-    if constexpr (SHARE > 1) {
-        if (lane == 0) part[wave] = acc;
-        __syncthreads();
-        acc = part[0] + part[1] + part[2] + part[3];
-        if (wave) return;
-    }
-    // (once a block and call, so that its order is set; requests that share a page add in any)
-    if (lane == 0) atomicAdd(a.weights + blk, acc);
+}
+// What exp2 takes off: the lse in log2 units; infinity for a row of lse -inf (it sees nothing, or is
+// behind the last), which then weighs 0.
+__device__ __forceinline__ float shift_of(float lse) {
+    return lse == -INFINITY ? INFINITY : lse * kLog2e;
+}
 #endif
+
+// Few query rows (single tokens, drafts): a block of 64 keys a wave, its keys in registers, the rows
+// (a token's G heads beside each other) in tiles of 16. Bound by the bytes of the keys.
+//
+// grid: four blocks of the table, kv heads, requests.
+template <int D, class T>
+__global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using x8 = typename Elem<T>::x8;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const long long chunk = (long long)blockIdx.x * 4 + uni(threadIdx.x >> 6);
+    const Request req = request(a, b);
+    if (chunk * kBlock >= req.keys) return;
+    const int page = uni(a.table[b * a.table_stride + chunk * kBlock / a.c.page]);
+    if ((unsigned)page >= (unsigned)a.c.pages) return;
+    const int key0 = (int)chunk * kBlock;
+    const long long blk = block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock)));
+    x8 kf[4][D / 32];
+    load_keys<D, T>(a.c, blk, i, g, kf);
+    const int rows = req.m * a.G;
+    const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
+    float acc[4] = {};
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+        const int r = r0 + i, tok = (int)((unsigned)r / (unsigned)a.G), h = hk * a.G + r - tok * a.G;
+        const bool ok = r < rows;
+        const T* q = (const T*)a.q + (req.first + tok) * a.qt + h * a.qh + 16 * g;
+        x8 qf[D / 32];
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            u32x4 x = {};
+            if (ok) x = *reinterpret_cast<const u32x4*>(q + 64 * (n / 2) + 8 * (n % 2));
+            qf[n] = __builtin_bit_cast(x8, x ^ neg);
+        }
+        const float m = shift_of(ok ? a.lse[(long long)(req.first + tok) * a.Hq + h] : -INFINITY);
+        add_weights<D, T>(kf, qf, a.scale, m, false, ok ? seen_by(a, req, tok) : 0, key0, g, acc);
+    }
+    const float sum = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+    // (once a block and call, so that its order is set; requests that share a page add in any)
+    if (lane == 0) atomicAdd(a.weights + blk, sum);
+#endif
+}
+
+// Prompts: a workgroup has four blocks of 64 keys, one a wave in registers as above, and a part of the
+// query rows (a.split_rows), which go by through LDS 64 at a time, operand by operand (frag_slot()), the
+// next ones on their way while the four waves use them. Bound by the vector unit: a score costs a
+// product and sum, an exponential (four of the others) and an addition, 1.5 times what the matrix
+// pipe needs for it. Parts' sums go to the workspace, which weigh_join_kernel adds up, so that the
+// order of a sum is set.
+//
+// grid: parts x groups of four blocks, kv heads, requests.
+template <int D, class T>
+__global__ void __launch_bounds__(256, 3) weigh_prompt_kernel(const WeighArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using x8 = typename Elem<T>::x8;
+    constexpr int NS = D / 32, UN = D / 8, RW = 256 / UN, PER = 64 / RW;  // steps; 16-byte units a row;
+                                                                          // rows a load; loads a stage
+    __shared__ __attribute__((aligned(1024))) char qs[2][64 * 2 * D];
+    __shared__ float ms[2][64];
+    __shared__ int lims[2][64];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int wave = uni(tid >> 6), hk = blockIdx.y, b = blockIdx.z, G = a.G;
+    const int part = uni((int)(blockIdx.x / (unsigned)a.groups));
+    const long long group = blockIdx.x - (long long)part * a.groups;
+    const Request req = request(a, b);
+    const int rows = req.m * G;  // (the host has checked that it fits)
+    if (group * (4 * kBlock) >= req.keys || (long long)part * a.split_rows >= rows) return;
+    const long long chunk = group * 4 + wave;
+    const int key0 = (int)(chunk * kBlock);
+    int page = -1;
+    if (key0 < req.keys) page = uni(a.table[b * a.table_stride + key0 / a.c.page]);
+    const bool have = (unsigned)page < (unsigned)a.c.pages;
+    const long long blk = have ? block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock))) : 0;
+    x8 kf[4][NS] = {};
+    if (have) load_keys<D, T>(a.c, blk, i, g, kf);
+
+    // The part's rows; from the first query on that sees the group's first key.
+    const long long q0 = a.causal ? max(0LL, group * (4 * kBlock) - (req.len - req.n)) : 0;
+    const int end = min(rows, (part + 1) * a.split_rows);
+    int r0 = max(part * a.split_rows, (int)min(q0 * G, (long long)end) & ~63);
+    // This thread's rows of a stage: row r0 + lr + RW n, and their places in q, lse.
+    const int lr = tid / UN, u = tid % UN;
+    const int step_tok = uni((int)(64u / (unsigned)G)), step_h = 64 - step_tok * G;
+    int tok[PER], h[PER];
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+        const unsigned r = r0 + lr + RW * n;
+        tok[n] = (int)(r / (unsigned)G);
+        h[n] = (int)r - tok[n] * G;
+    }
+    int ltok = (int)((unsigned)(r0 + lane) / (unsigned)G), lh = r0 + lane - ltok * G;
+    // Unit u is dims 8 u ..: step 2 j + n and lane group of u = 8 j + 2 g + n.
+    const int at = (2 * (u >> 3) + (u & 1)) * 1024 + 16 * frag_slot(lr & 15, u >> 1 & 3, u & 1) +
+                   (lr >> 4) * (NS * 1024);
+    const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
+    u32x4 x[PER];
+    float m = 0.f;
+    int lim = 0;
+    auto advance = [&](int& t, int& hh) {
+        t += step_tok;
+        hh += step_h;
+        if (hh >= G) {
+            hh -= G;
+            ++t;
+        }
+    };
+    auto fetch = [&] {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            x[n] = u32x4{};
+            if (r0 + lr + RW * n < end)
+                x[n] = *reinterpret_cast<const u32x4*>(
+                    (const T*)a.q + (req.first + tok[n]) * a.qt + (hk * G + h[n]) * a.qh + 8 * u);
+            advance(tok[n], h[n]);
+        }
+        if (wave == 0) {
+            const bool ok = r0 + lane < end;
+            m = ok ? a.lse[(long long)(req.first + ltok) * a.Hq + hk * G + lh] : -INFINITY;
+            lim = ok ? seen_by(a, req, ltok) : 0;
+            advance(ltok, lh);
+        }
+    };
+    float acc[4] = {};
+    fetch();
+    for (int buf = 0; r0 < end; buf ^= 1) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n)
+            *reinterpret_cast<GFX906_LDS u32x4*>((GFX906_LDS char*)qs[buf] + at +
+                                                 n * (RW / 16) * (NS * 1024)) = x[n] ^ neg;
+        if (wave == 0) {
+            ms[buf][lane] = shift_of(m);
+            lims[buf][lane] = lim;
+        }
+        r0 += 64;
+        if (r0 < end) fetch();
+        lds_barrier();
+        if (!have) continue;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int l = lims[buf][16 * t + i];
+            if (!__any(l > key0)) continue;
+            x8 qf[NS];
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+                qf[n] = lds_read16<T>(qs[buf], (t * NS + n) * 1024 + 16 * frag_slot(i, g, n & 1));
+            const bool all = !__any(l < key0 + kBlock);
+            add_weights<D, T>(kf, qf, a.scale, ms[buf][16 * t + i], all, l, key0, g, acc);
+        }
+    }
+    if (!have) return;
+    const float sum = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+    if (lane) return;
+    if (a.parts == 1)
+        atomicAdd(a.weights + blk, sum);
+    else
+        a.sums[(((long long)b * a.c.Hkv + hk) * a.parts + part) * (4LL * a.groups) + chunk] = sum;
+#endif
+}
+
+// Adds up the parts of every block. grid: blocks of the table / 256, kv heads, requests.
+__global__ void __launch_bounds__(256) weigh_join_kernel(const WeighArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const long long chunk = blockIdx.x * 256LL + threadIdx.x;
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const Request req = request(a, b);
+    if (chunk * kBlock >= req.keys) return;
+    const int page = a.table[b * a.table_stride + chunk * kBlock / a.c.page];
+    if ((unsigned)page >= (unsigned)a.c.pages) return;
+    const int parts = min(a.parts, (req.m * a.G + a.split_rows - 1) / a.split_rows);
+    float sum = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p)
+        sum += a.sums[(((long long)b * a.c.Hkv + hk) * a.parts + p) * (4LL * a.groups) + chunk];
+    atomicAdd(a.weights + block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock))), sum);
+#endif
+}
+
+// How a call is launched: the rows of a part, so that there are up to 16 parts and workgroups for the
+// GPU, and what the parts' sums take.
+struct WeighPlan {
+    long long blocks, groups;  // of the table: blocks of 64 keys, groups of four
+    int split_rows, parts;
+    size_t bytes;
+};
+constexpr int kWeighFew = 64;  // query rows of a kv head that go to weigh_few_kernel
+WeighPlan weigh_plan(int B, int G, int Hkv, int W, int page, int max_q) {
+    WeighPlan p{};
+    p.blocks = (long long)W * (page / kBlock);
+    p.groups = (p.blocks + 3) / 4;
+    const long long rows = (long long)max_q * G;
+    if (rows <= kWeighFew) return p;
+    const long long room = std::max(1LL, (1LL << 24) / std::max(1LL, 4 * p.groups * Hkv * B));
+    const long long most = std::min({16LL, room, (rows + 511) / 512});
+    p.split_rows = (int)(((rows + most - 1) / most + 63) / 64 * 64);
+    p.parts = (int)((rows + p.split_rows - 1) / p.split_rows);
+    if (p.parts > 1) p.bytes = (size_t)(4 * p.groups * Hkv * B * p.parts) * sizeof(float);
+    return p;
 }
 
 // -- eviction -------------------------------------------------------------------------
@@ -452,13 +650,13 @@ struct EvictArgs {
     unsigned long long* keys;  // [B][W], for wide tables
 };
 
-constexpr int kEvictThreads = 512, kEvictLds = 4096;
+constexpr int kEvictThreads = 1024, kEvictLds = 4096;
 
 // A workgroup a request. How many pages every request gives back follows from lengths and
 // budgets alone, so each finds the place of its pages in the free list by adding up all of them.
 // Which ones: the `gone`-th smallest of the pages' weights, as 64-bit keys that order alike, by
 // histograms of 8 bits from the highest one in which they differ; mostly two or three
-// passes until a bin is taken whole. Then the row closes up, 512 columns at a time. Bound by
+// passes until a bin is taken whole. Then the row closes up, 1024 columns at a time. Bound by
 // latency (dependent steps in one workgroup).
 //
 // LDS: whether the keys are kept there or in the workspace.
@@ -518,19 +716,41 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a)
     const int c0 = a.first, c1 = n - a.recent;  // candidates
     const int per = a.Hkv * (a.page / kBlock);
     u64 any = 0, each = ~0ull;
-    for (int c = c0 + t; c < c1; c += NT) {
-        const int page = row[c];
-        u64 key = 0;
-        if ((unsigned)page < (unsigned)a.pages) {
-            const float* w = a.weights + (long long)page * per;
-            double sum = 0.0;
-            for (int x = 0; x < per; ++x) sum += (double)w[x];
-            const u64 u = (u64)__double_as_longlong(sum + 0.0);
-            key = sum != sum ? ~0ull : u >> 63 ? ~u : u | 1ull << 63;
+    // (two columns a thread at a time, the weights of both in flight)
+    for (int base = c0 + t; base < c1; base += 2 * NT) {
+        int page[2];
+        double sum[2] = {};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) page[u] = base + u * NT < c1 ? row[base + u * NT] : -1;
+        const float* w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            w[u] = a.weights + ((unsigned)page[u] < (unsigned)a.pages ? (long long)page[u] * per : 0);
+        if (a.pages) {
+            for (int x = 0; x < per; x += 8) {
+                float f[2][8];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) f[u][n] = w[u][min(x + n, per - 1)];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) sum[u] += x + n < per ? (double)f[u][n] : 0.0;
+            }
         }
-        keys[c] = key;
-        any |= key;
-        each &= key;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (base + u * NT >= c1) continue;
+            u64 key = 0;
+            if ((unsigned)page[u] < (unsigned)a.pages) {
+                const u64 v = (u64)__double_as_longlong(sum[u] + 0.0);
+                key = sum[u] != sum[u] ? ~0ull : v >> 63 ? ~v : v | 1ull << 63;
+            }
+            keys[base + u * NT] = key;
+            any |= key;
+            each &= key;
+        }
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
@@ -737,11 +957,17 @@ extern "C" int kv8_load(void* k, void* v, int dtype, int T, int Hkv, int D, cons
     return err.launched(who, hipGetLastError());
 }
 
+extern "C" size_t kv8_weigh_workspace_bytes(int T, int B, int Hq, int Hkv, int max_q, int W, int page) {
+    if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_q <= 0 || W <= 0 || page <= 0) return 0;
+    return weigh_plan(B, Hq / Hkv, Hkv, W, page, std::min(max_q, T)).bytes;
+}
+
 extern "C" int kv8_weigh(float* weights, const void* q, const long long* q_strides, int dtype,
                          const float* lse, int T, int B, int Hq, int Hkv, int D,
                          const void* k_codes, const float* k_scales, int pages, int page,
                          const int* table, long long table_stride, int W, const int* lens,
-                         const int* cu_q, int max_q, float scale, int causal, hipStream_t stream) {
+                         const int* cu_q, int max_q, float scale, int causal, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream) {
     const char* who = "kv8_weigh";
     LastError& err = last_error();
     err.text[0] = 0;
@@ -781,18 +1007,32 @@ extern "C" int kv8_weigh(float* weights, const void* q, const long long* q_strid
     a.causal = causal;
     a.scale = log2_scale(scale);
     a.qsign = scale < 0.f ? -1.f : 1.f;
-    const long long blocks = (long long)W * (page / kBlock);
-    const bool share = (long long)a.max_q * a.G > 64;
-    const long long gx = share ? blocks : (blocks + 3) / 4;
-    if (!launchable(gx * Hkv * B, 256)) return err.fail("%s: table too wide for so many heads", who);
+    if ((long long)a.max_q * a.G >= (1LL << 30)) return err.fail("%s: too many query rows", who);
+    const WeighPlan p = weigh_plan(B, a.G, Hkv, W, page, a.max_q);
+    if (B > 65535 || !launchable((p.parts ? p.parts * p.groups : p.groups) * Hkv * B, 256) ||
+        p.parts * p.groups >= (1LL << 31))
+        return err.fail("%s: table too wide for so many heads", who);
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes || !aligned(workspace, 4)))
+        return err.fail("%s: workspace misaligned or smaller than kv8_weigh_workspace_bytes()", who);
+    a.groups = (int)p.groups;
+    a.split_rows = p.split_rows;
+    a.parts = p.parts;
+    a.sums = (float*)workspace;
     for_types(dtype, D, [&](auto d, auto t) {
         constexpr int kD = decltype(d)::value;
-        const dim3 grid((unsigned)gx, (unsigned)Hkv, (unsigned)B);
-        if (share)
-            hipLaunchKernelGGL((weigh_kernel<kD, decltype(t), 4>), grid, dim3(256), 0, stream, a);
+        if (!p.parts)
+            hipLaunchKernelGGL((weigh_few_kernel<kD, decltype(t)>),
+                               dim3((unsigned)p.groups, (unsigned)Hkv, (unsigned)B), dim3(256), 0, stream,
+                               a);
         else
-            hipLaunchKernelGGL((weigh_kernel<kD, decltype(t), 1>), grid, dim3(256), 0, stream, a);
+            hipLaunchKernelGGL((weigh_prompt_kernel<kD, decltype(t)>),
+                               dim3((unsigned)(p.parts * p.groups), (unsigned)Hkv, (unsigned)B),
+                               dim3(256), 0, stream, a);
     });
+    if (p.parts > 1)
+        hipLaunchKernelGGL(weigh_join_kernel,
+                           dim3((unsigned)((p.blocks + 255) / 256), (unsigned)Hkv, (unsigned)B),
+                           dim3(256), 0, stream, a);
     return err.launched(who, hipGetLastError());
 }
 

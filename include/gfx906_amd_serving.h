@@ -112,11 +112,14 @@ int kv8_attn(const void* q, void* o, float* lse, const long long* q_strides,
  * arguments and its lse [T, Hq] (packed fp32), the attention that the block's tokens got.
  * weights: fp32 [pages, Hkv, page/64]. Queries past the first max_q of a request do not count. Rows
  * of lse -inf add nothing. Sums are fp32 in an order that sizes alone set; where requests share
- * a page, their sums are added in any order. */
+ * a page, their sums are added in any order. workspace: kv8_weigh_workspace_bytes() bytes (max_q = 1
+ * where cu_q is NULL; may be 0), 4-byte aligned. */
+size_t kv8_weigh_workspace_bytes(int T, int B, int Hq, int Hkv, int max_q, int W, int page);
 int kv8_weigh(float* weights, const void* q, const long long* q_strides, int dtype, const float* lse,
               int T, int B, int Hq, int Hkv, int D, const void* k_codes, const float* k_scales,
               int pages, int page, const int* table, long long table_stride, int W, const int* lens,
-              const int* cu_q, int max_q, float scale, int causal, hipStream_t stream);
+              const int* cu_q, int max_q, float scale, int causal, void* workspace,
+              size_t workspace_bytes, hipStream_t stream);
 
 /* Every request with more than keep[b] pages (n = ceil(lens[b] / page) of at most W) gives back
  * n - keep[b] of them (fewer, where fewer may go): those of least weight among its pages first ..
