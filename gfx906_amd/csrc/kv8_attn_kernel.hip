@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
     using W = Tile<D, T, NB, false, LSE>;
     using x8 = typename W::x8;
     constexpr int R = 16 * NB, NJ = D / 64, NW = 8, NT = 64 * NW;
-    __shared__ __attribute__((aligned(1024))) float stage[NW][16 * D];
+    __shared__ __attribute__((aligned(1024))) float stage[NW][R * D];
     __shared__ float ml_s[NW][R][3];
     __shared__ int run0[NT + 1];
     __shared__ int found;
@@ -149,42 +149,79 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
         return u.chunks ? (u.chunks + a.start_units) * u.tiles * a.c.Hkv : 0;
     };
     int b = 0, start = 0, u0 = 0, hi = 1;
+    // Up to 64 requests every lane keeps one, and no wave waits for another to find its run.
+    const bool few = a.B <= 64;
+    Request mine{};
+    auto get = [&](int x) __attribute__((always_inline)) {
+        if (!few) return request(a, x);
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, x); };
+        Request r;
+        r.first = of(mine.first);
+        r.n = of(mine.n);
+        r.m = of(mine.m);
+        r.len = of((int)mine.len);  // (an int is where it comes from)
+        r.keys = of(mine.keys);
+        return r;
+    };
     if constexpr (!DIRECT) {
-        const int per_run = (a.B + NT - 1) / NT;
-        int n = 0;
-        for (int x = tid * per_run; x < min(a.B, (tid + 1) * per_run); ++x)
-            n += count(units_of(request(a, x)));
-        int sum = n;
+        auto upto = [&](int sum) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(sum, o);
-            if (lane >= o) sum += x;
-        }
-        if (lane == 63) ml_s[wave][0][0] = __int_as_float(sum);
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) sum += __float_as_int(ml_s[w][0][0]);
-        run0[tid + 1] = sum;
-        if (tid == 0) run0[0] = 0;
-        __syncthreads();
-        const int all = run0[NT];
-        const int per = max(a.min_units, uni((int)((unsigned)(all + a.groups - 1) / (unsigned)a.groups)));
-        if (blockIdx.x == 0) {
-            n = run0[tid];
-            for (int x = tid * per_run; x < min(a.B, (tid + 1) * per_run); ++x) {
-                a.starts[x] = n;
-                n += count(units_of(request(a, x)));
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(sum, o);
+                if (lane >= o) sum += x;
             }
-            if (tid == 0) a.starts[a.B] = per;
+            return sum;
+        };
+        auto run = [&](int all) {
+            const int per =
+                max(a.min_units, uni((int)((unsigned)(all + a.groups - 1) / (unsigned)a.groups)));
+            // (the last run may end past 2^31 before it is cut)
+            const long long lo = (long long)blockIdx.x * per;
+            u0 = (int)min(lo, (long long)all);
+            hi = (int)min((long long)all, lo + per);
+            return per;
+        };
+        if (few) {
+            int n = 0;
+            if (lane < a.B) {
+                mine = request(a, lane);
+                n = count(units_of(mine));
+            }
+            const int sum = upto(n), per = run(uni(__shfl(sum, 63)));
+            if (blockIdx.x == 0 && wave == 0) {
+                if (lane < a.B) a.starts[lane] = sum - n;
+                if (lane == 0) a.starts[a.B] = per;
+            }
+            if (u0 >= hi) return;
+            b = uni((int)__ffsll(__ballot(sum > u0)) - 1);
+            start = __builtin_amdgcn_readlane(sum - n, b);
+        } else {
+            const int per_run = (a.B + NT - 1) / NT;
+            int n = 0;
+            for (int x = tid * per_run; x < min(a.B, (tid + 1) * per_run); ++x)
+                n += count(units_of(request(a, x)));
+            int sum = upto(n);
+            if (lane == 63) ml_s[wave][0][0] = __int_as_float(sum);
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) sum += __float_as_int(ml_s[w][0][0]);
+            run0[tid + 1] = sum;
+            if (tid == 0) run0[0] = 0;
+            __syncthreads();
+            const int per = run(run0[NT]);
+            if (blockIdx.x == 0) {
+                n = run0[tid];
+                for (int x = tid * per_run; x < min(a.B, (tid + 1) * per_run); ++x) {
+                    a.starts[x] = n;
+                    n += count(units_of(request(a, x)));
+                }
+                if (tid == 0) a.starts[a.B] = per;
+            }
+            if (u0 >= hi) return;
+            if (run0[tid] <= u0 && u0 < run0[tid + 1]) found = tid;
+            __syncthreads();
+            b = uni(found) * per_run;
+            start = uni(run0[uni(found)]);
         }
-        // (the last run may end past 2^31 before it is cut)
-        const long long lo = (long long)blockIdx.x * per;
-        if (lo >= all) return;
-        u0 = (int)lo;
-        hi = (int)min((long long)all, lo + per);
-        if (run0[tid] <= u0 && u0 < run0[tid + 1]) found = tid;
-        __syncthreads();
-        b = uni(found) * per_run;
-        start = uni(run0[uni(found)]);
     }
 
     while (u0 < hi) {
@@ -205,11 +242,11 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
             whole = true;
             u0 = hi;
         } else {
-            req = request(a, b);
+            req = get(b);
             Units un = units_of(req);
             while (start + count(un) <= u0) {
                 start += count(un);
-                req = request(a, ++b);
+                req = get(++b);
                 un = units_of(req);
             }
             chunks = un.chunks;
@@ -250,10 +287,9 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
 
         const ConstInts table = (ConstInts)(a.table + b * a.table_stride);
         const int shift = a.c.page == 64 ? 0 : a.c.page == 128 ? 1 : 2;
-        // (past the run: its last unit's page, read again and not used)
+        // (past the run: its last unit's page, which is not used)
         auto page_of = [&](int c) { return table[min(c, c1 - 1) >> shift]; };
-        // The loads are unconditional, so that the compiler waits for them where they are
-        // used: a page outside the cache reads page 0, and the unit's keys are masked.
+        // (a page outside the cache reads page 0, and the unit's keys are masked)
         auto block_of = [&](int c, int page) {
             const unsigned p = (unsigned)page < (unsigned)a.c.pages ? page : 0;
             return block_at(a.c, p, hk, c & ((1 << shift) - 1));
@@ -307,7 +343,7 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
                         S[t / 2][t % 2][nb] = Elem<T>::mma16(kf, w.qf[nb][n], S[t / 2][t % 2][nb]);
                 }
             __builtin_amdgcn_sched_barrier(0);
-            fetch_k(c + NW, page);
+            if (c + NW < c1) fetch_k(c + NW, page);
             const int key0 = c * 64;
             if (key0 + 64 > all_see || !ok) {
                 int lim2[NB];
@@ -331,7 +367,7 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            fetch_v(c + NW, page);
+            if (c + NW < c1) fetch_v(c + NW, page);
         }
         if (__builtin_expect(nans, 0)) {
             for (c = c0 + wave; c < c1; c += NW) {
@@ -342,7 +378,9 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
             }
         }
 
-        // Merge the waves: a common max, then sums of 16 rows at a time through LDS.
+        // Merge the waves: all rows through LDS, each wave's relative to its own max. (Barriers wait for
+        // LDS accesses only, not for the stores of partial results.)
+        auto* const buf = (GFX906_LDS float*)stage[wave];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const float l = quad_sum(w.lacc[nb][0]);
@@ -353,53 +391,44 @@ __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kern
                 ml_s[wave][16 * nb + i][1] = l;
                 ml_s[wave][16 * nb + i][2] = lu;
             }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            float mx = kNoMax;
-#pragma unroll
-            for (int x = 0; x < NW; ++x) mx = max2(mx, ml_s[x][16 * nb + i][0]);
-            const float f = __builtin_amdgcn_exp2f(w.m[nb] - mx);
-            auto* const buf = (GFX906_LDS float*)stage[wave];
 #pragma unroll
             for (int ob = 0; ob < W::NO; ++ob)
-                *reinterpret_cast<GFX906_LDS f32x4*>(buf + i * D + ((16 * ob + 4 * g) ^ (4 * i & (D - 4)))) =
-                    w.oacc[ob][nb] * f;
-            __syncthreads();
-            for (int e = tid; e < 4 * D; e += NT) {  // 16 rows x D/4 quads
-                const int r = e / (D / 4), d = (e - r * (D / 4)) * 4, x = d ^ (4 * r & (D - 4));
-                f32x4 acc = {};
-                float mr = kNoMax, lr = 0.f, lu = 0.f;
-#pragma unroll
-                for (int y = 0; y < NW; ++y) mr = max2(mr, ml_s[y][16 * nb + r][0]);
-#pragma unroll
-                for (int y = 0; y < NW; ++y) {
-                    const float f = __builtin_amdgcn_exp2f(ml_s[y][16 * nb + r][0] - mr);
-                    lr += ml_s[y][16 * nb + r][1] * f;
-                    lu += ml_s[y][16 * nb + r][2] * f;
-                    acc += *reinterpret_cast<const GFX906_LDS f32x4*>(
-                        (const GFX906_LDS float*)stage[y] + r * D + x);
-                }
-                const int row = rt * R + 16 * nb + r;
-                if (row >= rows) continue;
-                if (whole) {
-                    const int tok = row / a.G, h = hk * a.G + row - tok * a.G;
-                    T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh + d;
-                    acc *= lr != 0.f ? 1.f / lr : 0.f;
-                    const auto x0 = Elem<T>::cvt2(acc[0], acc[1]), x1 = Elem<T>::cvt2(acc[2], acc[3]);
-                    *reinterpret_cast<u32x2*>(o) =
-                        u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
-                    if (LSE && d == 0) a.lse[(long long)(req.first + tok) * a.Hq + h] = lse_of(mr, lu);
-                } else {
-                    *reinterpret_cast<f32x4*>(a.ws_o + (slot * R + 16 * nb + r) * D + d) = acc;
-                    if (d == 0)
-                        *reinterpret_cast<f32x4*>(a.ws_ml + (slot * R + 16 * nb + r) * 4) =
-                            f32x4{mr, lr, lu, 0.f};
-                }
-            }
-            __syncthreads();
+                *reinterpret_cast<GFX906_LDS f32x4*>(buf + (16 * nb + i) * D +
+                                                     ((16 * ob + 4 * g) ^ (4 * i & (D - 4)))) =
+                    w.oacc[ob][nb];
         }
+        lds_barrier();
+        const int n_rows = min(R, rows - rt * R);
+#pragma unroll 1
+        for (int e = tid; e < n_rows * (D / 4); e += NT) {
+            const int r = e / (D / 4), d = (e - r * (D / 4)) * 4, x = d ^ (4 * (r & 15) & (D - 4));
+            f32x4 acc = {};
+            float mr = kNoMax, lr = 0.f, lu = 0.f;
+#pragma unroll
+            for (int y = 0; y < NW; ++y) mr = max2(mr, ml_s[y][r][0]);
+#pragma unroll
+            for (int y = 0; y < NW; ++y) {
+                const float f = __builtin_amdgcn_exp2f(ml_s[y][r][0] - mr);
+                lr += ml_s[y][r][1] * f;
+                lu += ml_s[y][r][2] * f;
+                acc += *reinterpret_cast<const GFX906_LDS f32x4*>((const GFX906_LDS float*)stage[y] +
+                                                                  r * D + x) * f;
+            }
+            if (whole) {
+                const int row = rt * R + r, tok = row / a.G, h = hk * a.G + row - tok * a.G;
+                T* o = (T*)a.o + (req.first + tok) * a.ot + h * a.oh + d;
+                acc *= lr != 0.f ? 1.f / lr : 0.f;
+                const auto x0 = Elem<T>::cvt2(acc[0], acc[1]), x1 = Elem<T>::cvt2(acc[2], acc[3]);
+                *reinterpret_cast<u32x2*>(o) =
+                    u32x2{__builtin_bit_cast(unsigned, x0), __builtin_bit_cast(unsigned, x1)};
+                if (LSE && d == 0) a.lse[(long long)(req.first + tok) * a.Hq + h] = lse_of(mr, lu);
+            } else {
+                *reinterpret_cast<f32x4*>(a.ws_o + (slot * R + r) * D + d) = acc;
+                if (d == 0)
+                    *reinterpret_cast<f32x4*>(a.ws_ml + (slot * R + r) * 4) = f32x4{mr, lr, lu, 0.f};
+            }
+        }
+        lds_barrier();
     }
 #endif
 }
