@@ -381,26 +381,26 @@ struct WeighArgs {
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// Keys of a block as the matrix operand: keys 16 t + i, dims 64 j + 16 g + 8 n .. + 7 at step 2 j + n.
-template <int D, class T>
-__device__ __forceinline__ void load_keys(const Cache& c, long long blk, int i, int g,
-                                          typename Elem<T>::x8 (&kf)[4][D / 32]) {
-    const float ks = ((ConstFloats)c.ks)[blk];
-    const uint8_t* kp = c.kc + blk * (kBlock * D) + i * D + 16 * g;
+// Keys of a block as the matrix operand: keys 16 t + i, dims 64 j + 16 g + 8 n .. + 7 at step 2 j + n;
+// their codes first, and the operand of them.
+template <int D>
+struct Keys {
     u32x4 raw[4][D / 64];
+    float s;
+    __device__ __forceinline__ void load(const Cache& c, long long blk, int i, int g) {
+        s = ((ConstFloats)c.ks)[blk];
+        const uint8_t* kp = c.kc + blk * (kBlock * D) + i * D + 16 * g;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j)
-            raw[t][j] = *reinterpret_cast<const u32x4*>(kp + t * 16 * D + 64 * j);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-            kf[t][2 * j] = expand<T>(raw[t][j][0], raw[t][j][1], ks);
-            kf[t][2 * j + 1] = expand<T>(raw[t][j][2], raw[t][j][3], ks);
-        }
-}
+            for (int j = 0; j < D / 64; ++j)
+                raw[t][j] = *reinterpret_cast<const u32x4*>(kp + t * 16 * D + 64 * j);
+    }
+    template <class T>
+    __device__ __forceinline__ typename Elem<T>::x8 step(int t, int n) const {
+        return expand<T>(raw[t][n / 2][2 * (n % 2)], raw[t][n / 2][2 * (n % 2) + 1], s);
+    }
+};
 // exp2 of 16 rows' scores with a block's keys less m (a lane's row), added to acc: those of keys below
 // lim, where not every row sees every key.
 template <int D, class T>
@@ -435,27 +435,30 @@ __device__ __forceinline__ float shift_of(float lse) {
 }
 #endif
 
-// Few query rows (single tokens, drafts): a block of 64 keys a wave, its keys in registers, the rows
-// (a token's G heads beside each other) in tiles of 16. Bound by the bytes of the keys.
+// Few query rows (single tokens, drafts): a block of 64 keys a wave, the rows (a token's G heads beside
+// each other) in tiles of 16. Bound by the bytes of the keys: codes are expanded 16 keys at a time, so
+// that the registers are few and enough waves have theirs in flight. (A wave that goes over several
+// blocks, with the next one's codes on their way, has half as many waves beside it: 39 us and not 29
+// for 32 requests of 100 .. 16384 tokens.)
 //
-// grid: four blocks of the table, kv heads, requests.
+// grid: blocks of the table, kv heads, requests; one wave each, as ragged requests then fill the GPU best (four
+// to a workgroup: 29.5 us and not 27.4).
 template <int D, class T>
-__global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a) {
+__global__ void __launch_bounds__(64, D == 64 ? 8 : 4) weigh_few_kernel(const WeighArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using x8 = typename Elem<T>::x8;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     const int hk = blockIdx.y, b = blockIdx.z;
-    const long long chunk = (long long)blockIdx.x * 4 + uni(threadIdx.x >> 6);
     const Request req = request(a, b);
+    const long long chunk = blockIdx.x;
     if (chunk * kBlock >= req.keys) return;
-    const int page = uni(a.table[b * a.table_stride + chunk * kBlock / a.c.page]);
+    const int page = ((ConstInts)(a.table + b * a.table_stride))[chunk * kBlock / a.c.page];
     if ((unsigned)page >= (unsigned)a.c.pages) return;
-    const int key0 = (int)chunk * kBlock;
+    const int key0 = (int)chunk * kBlock, rows = req.m * a.G;
     const long long blk = block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock)));
-    x8 kf[4][D / 32];
-    load_keys<D, T>(a.c, blk, i, g, kf);
-    const int rows = req.m * a.G;
+    Keys<D> k;
+    k.load(a.c, blk, i, g);
     const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
     float acc[4] = {};
     for (int r0 = 0; r0 < rows; r0 += 16) {
@@ -470,7 +473,19 @@ __global__ void __launch_bounds__(256) weigh_few_kernel(const WeighArgs a) {
             qf[n] = __builtin_bit_cast(x8, x ^ neg);
         }
         const float m = shift_of(ok ? a.lse[(long long)(req.first + tok) * a.Hq + h] : -INFINITY);
-        add_weights<D, T>(kf, qf, a.scale, m, false, ok ? seen_by(a, req, tok) : 0, key0, g, acc);
+        const int lim = ok ? seen_by(a, req, tok) : 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x4 S = {};
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+                S = Elem<T>::mma16(k.template step<T>(t, n), qf[n], S);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(S[e], a.scale, -m));
+                acc[e] += key0 + 16 * t + 4 * g + e < lim ? p : 0.f;
+            }
+        }
     }
     const float sum = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
     // (once a block and call, so that its order is set; requests that share a page add in any)
@@ -510,7 +525,14 @@ __global__ void __launch_bounds__(256, 3) weigh_prompt_kernel(const WeighArgs a)
     const bool have = (unsigned)page < (unsigned)a.c.pages;
     const long long blk = have ? block_at(a.c, page, hk, (int)(chunk % (a.c.page / kBlock))) : 0;
     x8 kf[4][NS] = {};
-    if (have) load_keys<D, T>(a.c, blk, i, g, kf);
+    if (have) {
+        Keys<D> k;
+        k.load(a.c, blk, i, g);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) kf[t][n] = k.template step<T>(t, n);
+    }
 
     // The part's rows; from the first query on that sees the group's first key.
     const long long q0 = a.causal ? max(0LL, group * (4 * kBlock) - (req.len - req.n)) : 0;
@@ -573,16 +595,27 @@ __global__ void __launch_bounds__(256, 3) weigh_prompt_kernel(const WeighArgs a)
         if (r0 < end) fetch();
         lds_barrier();
         if (!have) continue;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int l = lims[buf][16 * t + i];
-            if (!__any(l > key0)) continue;
-            x8 qf[NS];
+        auto rows_of = [&](int t, x8 (&qf)[NS]) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < NS; ++n)
                 qf[n] = lds_read16<T>(qs[buf], (t * NS + n) * 1024 + 16 * frag_slot(i, g, n & 1));
-            const bool all = !__any(l < key0 + kBlock);
-            add_weights<D, T>(kf, qf, a.scale, ms[buf][16 * t + i], all, l, key0, g, acc);
+        };
+        const int least = lims[buf][lane];
+        if (!__any(least < key0 + kBlock)) {  // every row sees every key: the common case, without a branch
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                x8 qf[NS];
+                rows_of(t, qf);
+                add_weights<D, T>(kf, qf, a.scale, ms[buf][16 * t + i], true, 0, key0, g, acc);
+            }
+        } else if (__any(least > key0)) {
+#pragma unroll 1
+            for (int t = 0; t < 4; ++t) {
+                x8 qf[NS];
+                rows_of(t, qf);
+                add_weights<D, T>(kf, qf, a.scale, ms[buf][16 * t + i], false, lims[buf][16 * t + i], key0,
+                                  g, acc);
+            }
         }
     }
     if (!have) return;
@@ -1022,7 +1055,7 @@ extern "C" int kv8_weigh(float* weights, const void* q, const long long* q_strid
         constexpr int kD = decltype(d)::value;
         if (!p.parts)
             hipLaunchKernelGGL((weigh_few_kernel<kD, decltype(t)>),
-                               dim3((unsigned)p.groups, (unsigned)Hkv, (unsigned)B), dim3(256), 0, stream,
+                               dim3((unsigned)p.blocks, (unsigned)Hkv, (unsigned)B), dim3(64), 0, stream,
                                a);
         else
             hipLaunchKernelGGL((weigh_prompt_kernel<kD, decltype(t)>),
