@@ -538,17 +538,23 @@ __global__ void __launch_bounds__(256, 3) weigh_prompt_kernel(const WeighArgs a)
     const long long q0 = a.causal ? max(0LL, group * (4 * kBlock) - (req.len - req.n)) : 0;
     const int end = min(rows, (part + 1) * a.split_rows);
     int r0 = max(part * a.split_rows, (int)min(q0 * G, (long long)end) & ~63);
-    // This thread's rows of a stage: row r0 + lr + RW n, and their places in q, lse.
+    // This thread's rows of the stages are r0 + lr, RW further on with every load: its head of the kv
+    // head's and its place in q (a step of 64-bit places, another where a token's heads end); of the
+    // first wave's lanes also row r0 + lane, 64 further on with every stage, and its token and lse.
     const int lr = tid / UN, u = tid % UN;
-    const int step_tok = uni((int)(64u / (unsigned)G)), step_h = 64 - step_tok * G;
-    int tok[PER], h[PER];
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-        const unsigned r = r0 + lr + RW * n;
-        tok[n] = (int)(r / (unsigned)G);
-        h[n] = (int)r - tok[n] * G;
-    }
+    struct Step {
+        int tok, h;
+        long long far, wrap;
+    };
+    auto step_of = [&](int n, long long per_tok, long long per_head) {
+        const int t = uni((int)((unsigned)n / (unsigned)G)), h = n - t * G;
+        return Step{t, h, t * per_tok + h * per_head, per_tok - G * per_head};
+    };
+    const Step qstep = step_of(RW, a.qt, a.qh), lstep = step_of(64, a.Hq, 1);
+    int h = (int)((unsigned)(r0 + lr) % (unsigned)G), row = r0 + lr;
+    const T* q = (const T*)a.q + (req.first + (row - h) / G) * a.qt + (hk * G + h) * a.qh + 8 * u;
     int ltok = (int)((unsigned)(r0 + lane) / (unsigned)G), lh = r0 + lane - ltok * G;
+    const float* lse = a.lse + (long long)(req.first + ltok) * a.Hq + hk * G + lh;
     // Unit u is dims 8 u ..: step 2 j + n and lane group of u = 8 j + 2 g + n.
     const int at = (2 * (u >> 3) + (u & 1)) * 1024 + 16 * frag_slot(lr & 15, u >> 1 & 3, u & 1) +
                    (lr >> 4) * (NS * 1024);
@@ -556,28 +562,31 @@ __global__ void __launch_bounds__(256, 3) weigh_prompt_kernel(const WeighArgs a)
     u32x4 x[PER];
     float m = 0.f;
     int lim = 0;
-    auto advance = [&](int& t, int& hh) {
-        t += step_tok;
-        hh += step_h;
-        if (hh >= G) {
-            hh -= G;
-            ++t;
-        }
-    };
     auto fetch = [&] {
 #pragma unroll
         for (int n = 0; n < PER; ++n) {
             x[n] = u32x4{};
-            if (r0 + lr + RW * n < end)
-                x[n] = *reinterpret_cast<const u32x4*>(
-                    (const T*)a.q + (req.first + tok[n]) * a.qt + (hk * G + h[n]) * a.qh + 8 * u);
-            advance(tok[n], h[n]);
+            if (row < end) x[n] = *reinterpret_cast<const u32x4*>(q);
+            row += RW;
+            h += qstep.h;
+            q += qstep.far;
+            if (h >= G) {
+                h -= G;
+                q += qstep.wrap;
+            }
         }
         if (wave == 0) {
             const bool ok = r0 + lane < end;
-            m = ok ? a.lse[(long long)(req.first + ltok) * a.Hq + hk * G + lh] : -INFINITY;
+            m = ok ? *lse : -INFINITY;
             lim = ok ? seen_by(a, req, ltok) : 0;
-            advance(ltok, lh);
+            ltok += lstep.tok;
+            lh += lstep.h;
+            lse += lstep.far;
+            if (lh >= G) {
+                lh -= G;
+                ++ltok;
+                lse += lstep.wrap;
+            }
         }
     };
     float acc[4] = {};
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(256) weigh_join_kernel(const WeighArgs a) {
 #endif
 }
 
-// How a call is launched: the rows of a part, so that there are up to 16 parts and workgroups for the
+// How a call is launched: the rows of a part, so that there are up to 32 parts and workgroups for the
 // GPU, and what the parts' sums take.
 struct WeighPlan {
     long long blocks, groups;  // of the table: blocks of 64 keys, groups of four
@@ -661,7 +670,7 @@ WeighPlan weigh_plan(int B, int G, int Hkv, int W, int page, int max_q) {
     const long long rows = (long long)max_q * G;
     if (rows <= kWeighFew) return p;
     const long long room = std::max(1LL, (1LL << 24) / std::max(1LL, 4 * p.groups * Hkv * B));
-    const long long most = std::min({16LL, room, (rows + 511) / 512});
+    const long long most = std::min({32LL, room, (rows + 511) / 512});
     p.split_rows = (int)(((rows + most - 1) / most + 63) / 64 * 64);
     p.parts = (int)((rows + p.split_rows - 1) / p.split_rows);
     if (p.parts > 1) p.bytes = (size_t)(4 * p.groups * Hkv * B * p.parts) * sizeof(float);
