@@ -692,70 +692,50 @@ struct EvictArgs {
     unsigned long long* keys;  // [B][W], for wide tables
 };
 
-constexpr int kEvictThreads = 1024, kEvictLds = 4096;
+// Columns of a table whose keys fit LDS, and up to which a thread has one.
+constexpr int kEvictLds = 4096, kEvictNarrow = 512;
 
 // A workgroup a request. How many pages every request gives back follows from lengths and
 // budgets alone, so each finds the place of its pages in the free list by adding up all of them.
 // Which ones: the `gone`-th smallest of the pages' weights, as 64-bit keys that order alike, by
 // histograms of 8 bits from the highest one in which they differ; mostly two or three
-// passes until a bin is taken whole. Then the row closes up, 1024 columns at a time. Bound by
+// passes until a bin is taken whole. Then the row closes up, NT columns at a time. Bound by
 // latency (dependent steps in one workgroup).
 //
 // LDS: whether the keys are kept there or in the workspace.
-template <bool LDS>
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a) {
+template <int NT, bool LDS>
+__global__ void __launch_bounds__(NT) evict_kernel(const EvictArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef unsigned long long u64;
-    constexpr int NT = kEvictThreads, NW = NT / 64;
+    constexpr int NW = NT / 64;
     __shared__ u64 keys_s[LDS ? kEvictLds : 1];
-    __shared__ u64 red[NW][2];
+    __shared__ u64 red[4][NW];
     __shared__ int hist[256];
-    __shared__ int wave_n[NW];
+    __shared__ int wave_n[2][NW];
     __shared__ int chosen[3];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x;
-    auto pages_of = [&](int x) {
-        return (int)min(((long long)max(0, a.lens[x]) + a.page - 1) / a.page, (long long)a.W);
+    // Pages of a request, and how many of them it gives back.
+    auto pages_of = [&](int len) {
+        return (int)min(((long long)max(0, len) + a.page - 1) / a.page, (long long)a.W);
     };
-    auto gone_of = [&](int x) {
-        const long long n = pages_of(x);
-        return max(0LL, min(n - a.keep[x], n - a.recent - a.first));
+    auto gone_of = [&](int len, int keep) {
+        const long long n = pages_of(len);
+        return max(0LL, min(n - keep, n - a.recent - a.first));
     };
+    // (what needs no other value is loaded first)
+    const int len = b < a.B ? ((ConstInts)a.lens)[b] : 0, keep = b < a.B ? ((ConstInts)a.keep)[b] : 0;
+    const int had = ((ConstInts)a.used)[0];
     // Pages given back before this request, and by all.
     long long before = 0, all = 0;
     for (int x = t; x < a.B; x += NT) {
-        const long long n = gone_of(x);
+        const long long n = gone_of(a.lens[x], a.keep[x]);
         all += n;
         before += x < b ? n : 0;
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        all += __shfl_xor(all, o);
-        before += __shfl_xor(before, o);
-    }
-    if (lane == 0) {
-        red[wave][0] = (u64)before;
-        red[wave][1] = (u64)all;
-    }
-    __syncthreads();
-    before = all = 0;
-    for (int w = 0; w < NW; ++w) {
-        before += (long long)red[w][0];
-        all += (long long)red[w][1];
-    }
-    const int used = min(max(0, a.used[0]), a.n_free);
-    const int back = (int)max(0LL, used - all);
-    if (b == 0 && t == 0) {
-        a.used_out[0] = back;
-        a.lost[0] = (int)min(max(0LL, all - used), 0x7fffffffLL);
-    }
-    if (b >= a.B) return;
-    const int n = pages_of(b), gone = (int)gone_of(b);
-    if (t == 0) a.lens_out[b] = a.lens[b] - gone * a.page;
-    if (gone == 0) return;
-
+    const int n = pages_of(len), gone = (int)gone_of(len, keep);
     int* const row = a.table + b * a.table_stride;
     u64* const keys = LDS ? keys_s : a.keys + (long long)b * a.W;
-    const int c0 = a.first, c1 = n - a.recent;  // candidates
+    const int c0 = a.first, c1 = gone ? n - a.recent : 0;  // candidates
     const int per = a.Hkv * (a.page / kBlock);
     u64 any = 0, each = ~0ull;
     // (two columns a thread at a time, the weights of both in flight)
@@ -796,19 +776,44 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a)
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
+        all += __shfl_xor(all, o);
+        before += __shfl_xor(before, o);
         any |= __shfl_xor(any, o);
         each &= __shfl_xor(each, o);
     }
-    __syncthreads();
     if (lane == 0) {
-        red[wave][0] = any;
-        red[wave][1] = each;
+        red[0][wave] = (u64)before;
+        red[1][wave] = (u64)all;
+        red[2][wave] = any;
+        red[3][wave] = each;
     }
+    for (int x = t; x < 256; x += NT) hist[x] = 0;
     __syncthreads();
-    for (int w = 0; w < NW; ++w) {
-        any |= red[w][0];
-        each &= red[w][1];
+    {
+        // (a lane a wave's numbers, over the 16 or 8 lanes)
+        const int w = lane % NW;
+        before = (long long)red[0][w];
+        all = (long long)red[1][w];
+        any = red[2][w];
+        each = red[3][w];
+#pragma unroll
+        for (int o = NW / 2; o; o >>= 1) {
+            all += __shfl_xor(all, o);
+            before += __shfl_xor(before, o);
+            any |= __shfl_xor(any, o);
+            each &= __shfl_xor(each, o);
+        }
     }
+    const int used = min(max(0, had), a.n_free);
+    const int back = (int)max(0LL, used - all);
+    if (t == 0) {
+        if (b == 0) {
+            a.used_out[0] = back;
+            a.lost[0] = (int)min(max(0LL, all - used), 0x7fffffffLL);
+        }
+        if (b < a.B) a.lens_out[b] = len - gone * a.page;
+    }
+    if (gone == 0) return;
     // Of the keys whose bits from `hi` up are those of `limit`, the least `rem` go, and all below.
     u64 limit = each;
     int rem = gone, hi = any == each ? 0 : 64 - __clzll((long long)(any ^ each));
@@ -816,8 +821,6 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a)
     while (hi > 0) {
         const int lo = max(0, hi - 8);
         limit = hi < 64 ? limit & ~0ull << hi : 0;
-        for (int x = t; x < 256; x += NT) hist[x] = 0;
-        __syncthreads();
         for (int c = c0 + t; c < c1; c += NT) {
             const u64 k = keys[c];
             if (hi == 64 || k >> hi == limit >> hi)
@@ -853,26 +856,30 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a)
         rem = chosen[1];
         limit |= (u64)bin << lo;
         hi = lo;
-        __syncthreads();
         if (rem == held) {
             limit |= (1ull << lo) - 1;
             whole = true;
             break;
         }
+        for (int x = t; x < 256; x += NT) hist[x] = 0;
+        __syncthreads();
     }
 
     // The row closes up. Entries are read before the barriers behind which others are written
     // to their places or in front of them.
+    int turn = 0;
     auto scan = [&](bool x, int& total) {  // how many before this thread have x
         const u64 m = __ballot(x);
-        __syncthreads();
-        if (lane == 0) wave_n[wave] = __popcll(m);
+        turn ^= 1;  // (who still reads the counts of one scan has not reached the barrier of the next)
+        if (lane == 0) wave_n[turn][wave] = __popcll(m);
         __syncthreads();
         int at = __popcll(m & ((1ull << lane) - 1));
         total = 0;
+#pragma unroll
         for (int w = 0; w < NW; ++w) {
-            at += w < wave ? wave_n[w] : 0;
-            total += wave_n[w];
+            const int c = wave_n[turn][w];
+            at += w < wave ? c : 0;
+            total += c;
         }
         return at;
     };
@@ -882,11 +889,14 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictArgs a)
         const int page = c < n ? row[c] : -1;
         const bool may = c >= c0 && c < c1;
         const u64 key = may ? keys[c] : 0;
-        const bool equal = may && !whole && key == limit;
+        bool out = may && (whole ? key <= limit : key < limit);
         int total;
-        const int eq = equal0 + scan(equal, total);
-        equal0 += total;
-        const bool out = may && (whole ? key <= limit : key < limit || (equal && eq < rem));
+        if (!whole) {
+            const bool equal = may && key == limit;
+            const int at = equal0 + scan(equal, total);
+            equal0 += total;
+            out |= equal && at < rem;
+        }
         const int at = gone0 + scan(out, total);
         gone0 += total;
         if (out) {
@@ -1111,9 +1121,11 @@ extern "C" int kv8_evict(const float* weights, int pages, int Hkv, int page, int
                       n_free,  table, table_stride, lens, keep, free_pages, used, lens_out,
                       used_out, lost, (unsigned long long*)workspace};
     const dim3 grid((unsigned)std::max(B, 1));
-    if (W <= kEvictLds)
-        hipLaunchKernelGGL(evict_kernel<true>, grid, dim3(kEvictThreads), 0, stream, a);
+    if (W <= kEvictNarrow)
+        hipLaunchKernelGGL((evict_kernel<512, true>), grid, dim3(512), 0, stream, a);
+    else if (W <= kEvictLds)
+        hipLaunchKernelGGL((evict_kernel<1024, true>), grid, dim3(1024), 0, stream, a);
     else
-        hipLaunchKernelGGL(evict_kernel<false>, grid, dim3(kEvictThreads), 0, stream, a);
+        hipLaunchKernelGGL((evict_kernel<1024, false>), grid, dim3(1024), 0, stream, a);
     return err.launched(who, hipGetLastError());
 }
