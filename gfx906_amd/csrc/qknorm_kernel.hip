@@ -37,7 +37,7 @@ struct RotateArgs {
     unsigned B, S, N, groups;  // groups: of tokens
     int D, R, w32, heads;  // w32: weights are fp32; heads a wave goes over
     int tok_step, head_step, head_next;  // of a row group; from one round of a wave to the next
-    float eps;
+    float eps, inv_d;
 };
 
 // A row is 8 dims a lane in L = 2^k lanes (some idle where D is not 8 L), a wave 64 / L rows:
@@ -66,6 +66,25 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
     const bool live = t < a.B * a.S && 8 * l < a.D;
     const unsigned b = min(t, a.B * a.S - 1) / a.S, s = min(t, a.B * a.S - 1) - b * a.S;
 
+    const T* x = (const T*)p.x + b * p.xb + s * p.xs + 8 * l;
+    T* y = (T*)p.y + b * p.yb + s * p.ys + 8 * l;
+    int h = chunk * a.heads + grp * a.head_step;
+    const int h1 = min(p.H, (chunk + 1) * a.heads);
+    u32x4 raw[kUnroll];
+    auto fetch = [&](int from) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            raw[u] = u32x4{};
+            const int hh = from + u * a.head_next;
+            if (live && hh < h1) raw[u] = *reinterpret_cast<const u32x4*>(x + hh * p.xh);
+        }
+    };
+    // (the position's load and the first rows' are on their way together; angles and weights follow)
+    const bool turn = 8 * l < a.R;
+    const int half = a.R / 16;  // lanes between the numbers of a pair
+    long long at = s;
+    if (turn && a.pos) at = a.pos[b * a.pb + s * a.ps];
+    fetch(h);
     float w[8], c[NEAR ? 4 : 8], n[NEAR ? 4 : 8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = 1.f;
@@ -74,10 +93,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
         for (int e = 0; e < 8; ++e)
             w[e] = a.w32 ? ((const float*)p.w)[8 * l + e] : (float)((const T*)p.w)[8 * l + e];
     }
-    const bool turn = 8 * l < a.R;
-    const int half = a.R / 16;  // lanes between the numbers of a pair
     if (turn) {
-        const long long at = a.pos ? a.pos[b * a.pb + s * a.ps] : (long long)s;
         const bool ok = (unsigned long long)at < a.N;
         const long long off = (ok ? at : 0) * a.ab + (NEAR ? 4 * l : 8 * (l < half ? l : l - half));
         const float sign = NEAR || l >= half ? 1.f : -1.f;
@@ -97,20 +113,16 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
     }
     const int other = grp * L + (l < half ? l + half : l - half);
 
-    const T* x = (const T*)p.x + b * p.xb + s * p.xs + 8 * l;
-    T* y = (T*)p.y + b * p.yb + s * p.ys + 8 * l;
-    const int h0 = chunk * a.heads + grp * a.head_step, h1 = min(p.H, (chunk + 1) * a.heads);
-    for (int h = h0; __any(h < h1); h += kUnroll * a.head_next) {
-        u32x4 raw[kUnroll];
+    while (true) {
+        u32x4 now[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) now[u] = raw[u];
+        const int next = h + kUnroll * a.head_next;
+        const bool more = __any(next < h1);
+        if (more) fetch(next);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            raw[u] = u32x4{};
-            const int hh = h + u * a.head_next;
-            if (live && hh < h1) raw[u] = *reinterpret_cast<const u32x4*>(x + hh * p.xh);
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const x8 in = __builtin_bit_cast(x8, raw[u]);
+            const x8 in = __builtin_bit_cast(x8, now[u]);
             float v[8], sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -119,10 +131,10 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
             }
 #pragma unroll
             for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o);
-            float eps = a.eps;
-            if (__builtin_expect(__any(!(sum < INFINITY)), 0)) {
-                // Squares past fp32 (bf16 rows): the row times 2^-80.
-                const float f = sum < INFINITY ? 1.f : 0x1p-80f;
+            float mean = sum * a.inv_d + a.eps, r = __builtin_amdgcn_rsqf(mean);
+            if (__builtin_expect(__any(!(mean < INFINITY) || mean < 0x1p-100f), 0)) {
+                // Squares past fp32 (bf16 rows): the row times 2^-80. And what rsq is not made for.
+                const float f = mean < INFINITY ? 1.f : 0x1p-80f;
                 sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -131,9 +143,8 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
                 }
 #pragma unroll
                 for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o);
-                eps *= f * f;
+                r = 1.0f / sqrtf(sum * a.inv_d + a.eps * (f * f));
             }
-            const float r = 1.0f / sqrtf(sum / (float)a.D + eps);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
             if (a.R) {
@@ -162,6 +173,8 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
                 *reinterpret_cast<u32x4*>(y + hh * p.yh) = out;
             }
         }
+        if (!more) break;
+        h = next;
     }
 #endif
 }
@@ -251,6 +264,7 @@ extern "C" int qk_norm_rotate(const void* q, const void* k, void* q_out, void* k
     a.R = R;
     a.w32 = weight_f32;
     a.eps = eps;
+    a.inv_d = 1.f / D;
     const long long tasks = a.groups * (long long)(a.part[0].chunks + a.part[1].chunks);
     const long long grid = (tasks + 3) / 4;
     if (!launchable(grid, 256)) return g_err.fail("%s: too many rows for one call", who);
