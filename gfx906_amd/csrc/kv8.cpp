@@ -228,8 +228,8 @@ std::vector<Tensor> kv8_evict_op(Tensor weights, Tensor table, Tensor lens, Tens
     for (const Tensor* t : {&lens, &keep, &used, &weights}) at::assert_no_overlap(free_pages, *t);
     const c10::DeviceGuard guard(dev);
     const int W = (int)table.size(1);
-    const Tensor out = at::empty({B}, lens.options()), u = at::empty({1}, lens.options()),
-                 lost = at::empty({1}, lens.options());
+    const Tensor buf = at::empty({B + 2}, lens.options());
+    const Tensor out = part(buf, 0, {B}), u = part(buf, B, {1}), lost = part(buf, B + 1, {1});
     const size_t bytes = kv8_evict_workspace_bytes((int)B, W);
     Tensor ws;
     if (bytes) ws = at::empty({(int64_t)bytes}, lens.options().dtype(torch::kByte));

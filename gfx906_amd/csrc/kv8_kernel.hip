@@ -145,44 +145,67 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
     const unsigned task = (id >> 1) / (unsigned)a.c.Hkv;
     const int h = uni((int)((id >> 1) - task * a.c.Hkv));
     if (task >= a.tasks) return;
-    // The last request whose first number is at most `task`.
-    auto starts = [&](int b) { return b < a.B && (unsigned)((cu_at(a, b) >> 6) + 2 * b) <= task; };
-    const int step = (a.B + 63) / 64;
-    int b = uni(max(0, __popcll(__ballot(starts(lane * step))) - 1)) * step;
-    b += uni(max(0, __popcll(__ballot(lane < step && starts(b + lane))) - 1));
-    const Request r = request(a, b);
+    // The last request whose first number is at most `task`: one load of each lane's request up to 64
+    // of them, else two steps of 64.
+    auto first_of = [&](int x) { return (unsigned)((cu_at(a, x) >> 6) + 2 * x); };
+    Request r;
+    unsigned first;
+    int b;
+    if (a.B <= 64) {
+        Request mine{};
+        first = ~0u;
+        if (lane < a.B) {
+            mine = request(a, lane);
+            first = (unsigned)((mine.first >> 6) + 2 * lane);
+        }
+        b = uni(max(0, __popcll(__ballot(first <= task)) - 1));
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, b); };
+        r.first = of(mine.first);
+        r.n = of(mine.n);
+        r.len = of((int)mine.len);  // (an int is where it comes from)
+        first = (unsigned)of((int)first);
+    } else {
+        auto starts = [&](int x) { return x < a.B && first_of(x) <= task; };
+        const int step = (a.B + 63) / 64;
+        b = uni(max(0, __popcll(__ballot(starts(lane * step))) - 1)) * step;
+        b += uni(max(0, __popcll(__ballot(lane < step && starts(b + lane))) - 1));
+        r = request(a, b);
+        first = first_of(b);
+    }
     const long long old = r.len - r.n;  // tokens before the new ones (negative: rows too many)
-    const long long j = max(0LL, old) / kBlock + (task - (unsigned)((cu_at(a, b) >> 6) + 2 * b));
+    const long long j = max(0LL, old) / kBlock + (task - first);
     const long long p0 = max(old, j * kBlock), p1 = min(r.len, (j + 1) * kBlock);
-    if (p0 < 0 || p0 >= p1 || j * kBlock >= (long long)a.W * a.c.page) return;
-    const int page = a.table[b * a.table_stride + j * kBlock / a.c.page];
-    if ((unsigned)page >= (unsigned)a.c.pages) return;
+    if (p0 >= p1 || j * kBlock >= (long long)a.W * a.c.page) return;
     const int before = uni((int)(p0 - j * kBlock)), count = uni((int)(p1 - p0));
     const long long row0 = r.first + (p0 - old) - before;  // row of the block's token 0
+    const T* src = is_v ? (const T*)a.v + h * a.vh : (const T*)a.k + h * a.kh;
+    const long long st = is_v ? a.vt : a.kt;
+    constexpr int FEW = 4;
+    unsigned few[FEW] = {};  // (on their way while the page is looked up)
+    if (count <= FEW) {
+#pragma unroll
+        for (int n = 0; n < FEW; ++n)
+            if (n < count && 2 * lane < D)
+                few[n] = *reinterpret_cast<const unsigned*>(src + (row0 + before + n) * st + 2 * lane);
+    }
+    const int page = ((ConstInts)(a.table + b * a.table_stride))[j * kBlock / a.c.page];
+    if ((unsigned)page >= (unsigned)a.c.pages) return;
     const long long blk = block_at(a.c, page, h, (int)(j % (a.c.page / kBlock)));
     uint8_t* codes = const_cast<uint8_t*>(is_v ? a.c.vc : a.c.kc) + blk * (kBlock * D);
     float* scale = const_cast<float*>(is_v ? a.c.vs : a.c.ks) + blk;
-    const T* src = is_v ? (const T*)a.v + h * a.vh : (const T*)a.k + h * a.kh;
-    const long long st = is_v ? a.vt : a.kt;
     const int old_e =
         before ? min(kHigh, max(kLow, (int)(__float_as_uint(*scale) >> 23 & 255) - 127)) : kLow;
     if (!is_v && a.weights && before == 0 && lane == 0) a.weights[blk] = 0.f;
 
-    constexpr int FEW = 4;
     if (count <= FEW) {
-        unsigned x[FEW], m = 0;
+        unsigned m = 0;
 #pragma unroll
-        for (int n = 0; n < FEW; ++n) {
-            x[n] = 0;
-            if (n < count && 2 * lane < D)
-                x[n] = *reinterpret_cast<const unsigned*>(src + (row0 + before + n) * st + 2 * lane);
-            m = top2(m, x[n]);
-        }
+        for (int n = 0; n < FEW; ++n) m = top2(m, few[n]);
         m = wave_top(m);
         if (m > kMax16<T>) {
             m = 0;
 #pragma unroll
-            for (int n = 0; n < FEW; ++n) x[n] = tame<T>(x[n], m);
+            for (int n = 0; n < FEW; ++n) few[n] = tame<T>(few[n], m);
             m = wave_top(m);
         }
         const int e = max(old_e, exponent_for(f32_bits<T>(m)));
@@ -192,7 +215,7 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
 #pragma unroll
             for (int n = 0; n < FEW; ++n) {
                 if (n >= count || 2 * lane >= D) continue;
-                const unsigned w = pack2<T, false>(0, x[n], s);
+                const unsigned w = pack2<T, false>(0, few[n], s);
                 const int t = before + n;
                 if (is_v) {
                     codes[2 * lane * kBlock + place(t)] = (uint8_t)w;
@@ -329,17 +352,26 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadArgs a) {
         }
     }
     if (!is_v) return;
-    for (unsigned long long left = __ballot(block >= 0); left;) {
-        const int blk = __shfl(block, (int)__ffsll(left) - 1);
-        const unsigned long long same = __ballot(block == blk);
-        left &= ~same;
+    // (the next block's codes are on their way while rows are picked from one)
+    unsigned long long left = __ballot(block >= 0);
+    if (!left) return;
+    u32x4 x[D / 64];
+    float s = 0.f;
+    int blk = 0;
+    auto fetch = [&] {
+        blk = __builtin_amdgcn_readfirstlane(__shfl(block, (int)__ffsll(left) - 1));
         const long long at = where(blk);
-        const float s = a.c.vs[at];
-        u32x4 x[D / 64];
+        s = a.c.vs[at];
 #pragma unroll
         for (int n = 0; n < D / 64; ++n)
             x[n] = *reinterpret_cast<const u32x4*>(a.c.vc + at * (kBlock * D) + 4096 * n + 16 * threadIdx.x);
-        __syncthreads();  // (the block before has been read)
+    };
+    fetch();
+    while (true) {
+        const unsigned long long same = __ballot(block == blk);
+        const float unit = s;
+        left &= ~same;
+        lds_barrier();  // (the block before has been read)
 #pragma unroll
         for (int n = 0; n < D / 64; ++n) {
             unsigned* p = reinterpret_cast<unsigned*>(vb + (64 * n + threadIdx.x / 4) * PITCH +
@@ -347,7 +379,8 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) p[e] = x[n][e];
         }
-        __syncthreads();
+        if (left) fetch();
+        lds_barrier();
 #pragma unroll
         for (int n = 0; n < 64 / RW; ++n) {
             const int r = n * RW + threadIdx.x / DL, slot = __shfl(mine, r);
@@ -356,8 +389,9 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadArgs a) {
             unsigned w[2] = {};
 #pragma unroll
             for (int d = 0; d < 8; ++d) w[d / 4] |= (unsigned)p[d * PITCH] << (8 * (d & 3));
-            put(t0 + r, w[0], w[1], s);
+            put(t0 + r, w[0], w[1], unit);
         }
+        if (!left) return;
     }
 #endif
 }

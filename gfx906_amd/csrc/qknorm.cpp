@@ -72,6 +72,16 @@ std::vector<Tensor> norm_rotate_op(Tensor q, c10::optional<Tensor> k, c10::optio
     // [x, result] of q and of k, 4-D
     Tensor x[2], y[2], given[2];
     const c10::optional<Tensor>* out[2] = {&q_out, &k_out};
+    // Contiguous results of both lie in one buffer.
+    const bool both = k.has_value() && !q_out.has_value() && !k_out.has_value() &&
+                      (q.is_contiguous() || !q.is_non_overlapping_and_dense()) &&
+                      (k->is_contiguous() || !k->is_non_overlapping_and_dense());
+    Tensor buf;
+    const int64_t nq = (q.numel() + 7) / 8 * 8;
+    if (both) {
+        const c10::DeviceGuard guard(dev);
+        buf = at::empty({nq + k->numel()}, q.options());
+    }
     for (int i = 0; i < 2; ++i) {
         if (i == 1 && !k.has_value()) {
             TORCH_CHECK(!k_out.has_value(), who, ": a result for k without k");
@@ -88,7 +98,7 @@ std::vector<Tensor> norm_rotate_op(Tensor q, c10::optional<Tensor> k, c10::optio
                             given[i].sizes() == t.sizes(),
                         who, ": results must have the shape, type and device of their inputs");
         } else {
-            given[i] = at::empty_like(t);
+            given[i] = both ? part(buf, i ? nq : 0, t.sizes()) : at::empty_like(t);
         }
         x[i] = flat ? t.unsqueeze(0) : t;
         y[i] = flat ? given[i].unsqueeze(0) : given[i];

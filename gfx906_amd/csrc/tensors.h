@@ -40,6 +40,16 @@ inline std::array<long long, 2> strides2(const Tensor& t) {
     return {t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1)};
 }
 
+// A contiguous part of a one-dimensional buffer, made by hand: a view through the dispatcher takes
+// 0.7 us, as much as a tenth of a small call.
+inline Tensor part(const Tensor& buf, int64_t offset, at::IntArrayRef sizes) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(),
+                                                        buf.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
+
 inline hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
 
 }  // namespace gfx906_amd
