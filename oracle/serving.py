@@ -154,8 +154,10 @@ def decode(codes, scales, is_v):
 
 def attention(q, cache, table, lens, scale, cu=None, max_q=None, causal=True):
     """{row: (o [Hq, D], bound, lse [Hq], bound of lse)} of every computed row. The bound of o is
-    the one of the 4-bit cache's attention; an lse is off by its scores' errors and by 2^-21 of
-    exponentials, their sum and the logarithm, relative to the numbers that it is made of."""
+    the one of the 4-bit cache's attention. An lse is off by its scores' errors (D products added in
+    fp32) and by 2^-21 of the exponentials and their sum, and of its own size: it is ln 2 times the sum
+    of a maximum and a logarithm, so by 2^-23 (the logarithm, 1 ulp), 2^-24 (the sum), 2^-25 (ln 2) and
+    2^-24 (the product) of numbers no larger than |lse| and the scores, 2.3 * 2^-23 in all."""
     T, Hq, D = q.shape
     cu = list(range(T + 1)) if cu is None else [min(max(c, 0), T) for c in cu]
     G, out = Hq // cache.x[0].shape[1], {}
@@ -179,7 +181,8 @@ def attention(q, cache, table, lens, scale, cu=None, max_q=None, causal=True):
             tol[:, h] = tolerance(o, spread, size, q.dtype, D, keys, top)
             z = (x.double() @ k.T * scale).masked_fill(hide, -math.inf)
             lse[:, h] = torch.logsumexp(z, 1) if keys else -math.inf
-            ltol[:, h] = D * 2.0 ** -24 * size + 2.0 ** -21 * (1 + size)
+            own = lse[:, h].abs().nan_to_num(0.0, 0.0)
+            ltol[:, h] = D * 2.0 ** -24 * size + 2.0 ** -21 * (1 + size + own)
         for i in range(count):
             out[cu[b] + i] = (res[i], tol[i], lse[i], ltol[i])
     return out

@@ -566,3 +566,258 @@ def test_evict_refuses():
                 dict(lens=i32([1, 1]), keep=i32([1, 1]), table=t.expand(2, 2))):
         with pytest.raises(RuntimeError):
             kv8.evict(**(ok | bad))
+
+
+# -- what a program may do with all of it ---------------------------------------------------
+
+def test_caches_without_pages_and_requests_without_keys():
+    q = torch.randn(3, 4, 64, device=DEV).half()
+    empty = kv8.new_cache(0, 64, 2, 64)
+    for cache, table in ((empty, i32([[0], [0], [0]])), (kv8.new_cache(2, 64, 2, 64), i32([[], [], []]))):
+        out, lse = kv8.attn(q, cache, table, i32([5, 0, 70]), 0.1, lse=True)
+        assert out.eq(0).all() and lse.eq(-math.inf).all()
+        w = kv8.new_weights(cache)
+        kv8.weigh(w, q, lse, cache, table, i32([5, 0, 70]), 0.1)
+        kv8.store(cache, q[:, :2], q[:, :2], table, i32([5, 0, 70]), weights=w)
+        assert w.eq(0).all()
+    none = kv8.attn(q[:0], kv8.new_cache(2, 64, 2, 64), i32([]).view(0, 4), i32([]), 0.1, lse=True)
+    assert none[0].shape == (0, 4, 64) and none[1].shape == (0, 4)
+
+
+@pytest.mark.parametrize("news", [1, 4, 200])
+def test_hostile_lengths_tables_and_bounds_are_safe(news):
+    """Any int in lens, table and cu_q: no access outside, rows of others right."""
+    lens, H, D = [2 ** 31 - 1, -5, 130, 2 ** 31 - 1], 2, 64
+    cache, held, table = filled([130], 64, H, D, torch.float16, seed=1)
+    pages = len(cache.k)
+    wild = [[2 ** 31 - 1, -2 ** 31, pages, -1], [0, 1, 0, 1], table[0] + [-1] * (4 - len(table[0])),
+            [0, 0, 0, 0]]
+    cu = offsets([news] * 4)
+    q = torch.randn(cu[-1], 4, D, generator=torch.Generator().manual_seed(2)).half()
+    out, lse = kv8.attn(q.to(DEV), cache, i32(wild), i32(lens), 0.1, cu_q=i32(cu), max_q=news, lse=True)
+    rows = sv.attention(q[cu[2]:cu[3]], held, [wild[2]], [130], 0.1, [0, news])
+    check(out[cu[2]:cu[3]], lse[cu[2]:cu[3]], rows)
+    assert out[:cu[1]].eq(0).all() and out[cu[1]:cu[2]].eq(0).all()
+    w = kv8.new_weights(cache)
+    kv8.weigh(w, q.to(DEV), lse, cache, i32(wild), i32(lens), 0.1, cu_q=i32(cu), max_q=news)
+    for bounds in ([0, 5, 3, 2, 4], [-9, 2 ** 31 - 1, 0, -1, 3], [4, 3, 2, 1, 0]):
+        kv8.attn(q.to(DEV), cache, i32(wild), i32(lens), 0.1, cu_q=i32(bounds))
+        kv8.weigh(w, q.to(DEV), lse, cache, i32(wild), i32(lens), 0.1, cu_q=i32(bounds))
+    other = kv8.new_cache(pages, 64, H, D)
+    x = torch.randn(cu[-1], H, D, device=DEV).half()
+    wild[3] = [-1] * 4     # (page 0 is another request's)
+    for bounds in ([0, 5, 3, 2, 4], [-9, 2 ** 31 - 1, 0, -1, 3], [4, 3, 2, 1, 0], cu):
+        kv8.store(other, x, x, i32(wild), i32(lens), i32(bounds))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("n,news", [(200, 1), (2300, 2), (300, 200)])
+@pytest.mark.parametrize("scale", [0.0, 1e-37, -1e-37])
+def test_small_scales(scale, n, news):
+    """A scale of 0 weighs every key alike; so do those that leave scores below rounding."""
+    cache, held, table = filled([n], 64, 1, 64, torch.bfloat16, seed=n)
+    q = torch.randn(news, 2, 64, generator=torch.Generator().manual_seed(n)).bfloat16() * 100
+    out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32([n]), scale, cu_q=i32([0, news]), max_q=news,
+                        lse=True)
+    check(out, lse, sv.attention(q, held, table, [n], scale, [0, news]))
+
+
+@pytest.mark.parametrize("heads", [(4, 2), (32, 1)])
+@pytest.mark.parametrize("lens,news", [([700, 64, 3], [1, 1, 1]), ([900, 300], [260, 5])])
+def test_weights_of_all_blocks_add_up_to_the_rows(lens, news, heads):
+    """With attention's own lse every row's weights add up to 1, whatever way they are added."""
+    Hq, Hkv = heads
+    cache, _, table = filled(lens, 64, Hkv, 128, torch.bfloat16, seed=9)
+    cu = offsets(news)
+    q = torch.randn(cu[-1], Hq, 128, device=DEV).bfloat16()
+    _, lse = kv8.attn(q, cache, i32(table), i32(lens), 0.1, cu_q=i32(cu), max_q=max(news), lse=True)
+    for max_q in (max(news), 2000):        # (the room for more queries may take another form)
+        w = kv8.new_weights(cache)
+        kv8.weigh(w, q, lse, cache, i32(table), i32(lens), 0.1, cu_q=i32(cu), max_q=max_q)
+        got, rows = w.double().sum((0, 2)).cpu(), cu[-1] * Hq // Hkv
+        # an lse of some units is off by some 2^-21 and a score in fp32 by as much
+        assert ((got - rows).abs() <= rows * 2.0 ** -16).all(), got
+    again = kv8.new_weights(cache)
+    kv8.weigh(again, q, lse, cache, i32(table), i32(lens), 0.1, cu_q=i32(cu), max_q=2000)
+    assert torch.equal(again, w)
+
+
+def test_serving_with_eviction():
+    """Prompts, then single tokens, every step through page planning, norm and rotation, storing,
+    attention, weights and eviction; tokens, tables and pages against the oracle."""
+    from gfx906_amd import qknorm
+    B, Hq, Hkv, D, page, keep = 3, 4, 2, 64, 64, 4
+    g = torch.Generator().manual_seed(0)
+    cache, held = dirty_cache(24, page, Hkv, D), sv.Cache(24, page, Hkv, D)
+    weights = kv8.new_weights(cache).fill_(5.0)
+    table = torch.full((B, 8), -1, dtype=torch.int32, device=DEV)
+    free = torch.randperm(24, generator=g).int().to(DEV)
+    everything = sorted(free.tolist())
+    lens, used, told = i32([0] * B), i32([0]), [0] * B
+    cos, sin = qknorm.angles(4096, D // 2)
+    went = 0
+    for news in ([300, 70, 130], [1, 1, 1], [60, 1, 200], [1, 64, 1], [3, 100, 2], [1, 1, 1]):
+        plan = kv8.plan_pages(lens, i32(news), table, free, used, page, sum(news))
+        assert plan.missing.item() == 0
+        cu = offsets(news)
+        x = torch.randn(cu[-1], Hq + 2 * Hkv, D, generator=g).half().to(DEV)
+        pos = i32([told[b] + t for b in range(B) for t in range(news[b])])
+        told = [n + m for n, m in zip(told, news)]
+        q, k = qknorm.norm_rotate(x[:, :Hq], x[:, Hq:Hq + Hkv], cos=cos, sin=sin, positions=pos)
+        v = x[:, Hq + Hkv:]
+        kv8.store(cache, k, v, table, plan.lens, plan.cu_new, weights)
+        out, lse = kv8.attn(q, cache, table, plan.lens, D ** -0.5, cu_q=plan.cu_new, max_q=max(news),
+                            lse=True)
+        before = weights.clone()
+        kv8.weigh(weights, q, lse, cache, table, plan.lens, D ** -0.5, cu_q=plan.cu_new,
+                  max_q=max(news))
+        rows, n = table.tolist(), plan.lens.tolist()
+        held.store(k.cpu(), v.cpu(), rows, n, cu)
+        same(cache, held, rows, n)
+        check(out, lse, sv.attention(q.cpu(), held, rows, n, D ** -0.5, cu))
+        want, tol = sv.weigh(before.cpu(), q.cpu(), lse.cpu(), held, rows, n, D ** -0.5, cu)
+        weighed(weights, want, tol, rows, n, page)
+        w, f, u = weights.cpu(), free.tolist(), plan.used.item()
+        gone = kv8.evict(weights, table, plan.lens, i32([keep] * B), free, plan.used, first=1, recent=2)
+        want = sv.evict(w, page, rows, n, [keep] * B, f, u, 1, 2)
+        for a, b in zip((table, free, gone.lens, gone.used, gone.lost),
+                        (want[0], want[1], want[2], [want[3]], [want[4]])):
+            assert a.tolist() == b
+        went += u - gone.used.item()
+        lens, used = gone.lens, gone.used
+        # every page is free or some request's, once
+        mine = [p for r in table.tolist() for p in r if p >= 0]
+        assert sorted(mine + free[used.item():].tolist()) == everything
+    assert went > 0
+
+
+def test_captured_step_replays():
+    """A decoding step with all of it in one graph, replayed with new inputs in the same tensors;
+    eager work and synchronisations in between."""
+    B, Hq, Hkv, D, page = 3, 8, 2, 128, 64
+    lens0 = [300, 63, 128]
+    cache, _, rows = filled([n + 60 for n in lens0], page, Hkv, D, torch.float16, seed=3)
+    table0, lens, cu = i32(rows), i32(lens0), i32(list(range(B + 1)))
+    weights = kv8.new_weights(cache) + 1
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v = (torch.randn(B, h, D, device=DEV, generator=g).half() for h in (Hq, Hkv, Hkv))
+    out, table = torch.zeros_like(q), table0.clone()
+    free, used, keep = i32([0] * 9), i32([9]), i32([3] * B)
+    live = [cache.k, cache.k_scale, cache.v, cache.v_scale, weights, out, table, free]
+
+    def step():
+        kv8.store(cache, k, v, table, lens, cu, weights)
+        _, lse = kv8.attn(q, cache, table, lens, 0.1, cu_q=cu, max_q=1, out=out, lse=True)
+        kv8.weigh(weights, q, lse, cache, table, lens, 0.1, cu_q=cu, max_q=1)
+        return lse, kv8.evict(weights, table, lens, keep, free, used)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lse, gone = step()
+    for i in range(4):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, device=DEV, generator=g).half() * (1 + 3 * i))
+        table.copy_(table0)
+        lens.copy_(i32([n + i + 1 for n in lens0]))
+        saved = [t.clone() for t in live]
+        graph.replay()
+        got = [t.clone() for t in (*live, lse, *gone)]
+        torch.randn(1 << 18, device=DEV).sum().item()
+        for t, x in zip(live, saved):
+            t.copy_(x)
+        l2, g2 = step()
+        for a, b in zip(got, (*live, l2, *g2)):
+            assert torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0)), f"replay {i}"
+        torch.cuda.synchronize()
+
+
+def test_captured_prompts_replay():
+    lens, cu = [2500, 40, 700], [0, 150, 151, 300]
+    cache, _, table = filled(lens, 64, 2, 128, torch.bfloat16, seed=4)
+    table, n, cu = i32(table), i32(lens), i32(cu)
+    q = torch.randn(300, 8, 128, device=DEV).bfloat16()
+
+    def call():
+        out, lse = kv8.attn(q, cache, table, n, 0.1, cu_q=cu, max_q=150, lse=True)
+        w = kv8.new_weights(cache)
+        kv8.weigh(w, q, lse, cache, table, n, 0.1, cu_q=cu, max_q=150)
+        return out, lse, w
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device=DEV).bfloat16())
+        graph.replay()
+        torch.randn(1 << 18, device=DEV).sum().item()
+        assert all(torch.equal(a, b) for a, b in zip(got, call())), f"replay {i}"
+        torch.cuda.synchronize()
+
+
+def test_streams_at_once():
+    lens = [3000, 500, 1]
+    cache, _, table = filled(lens, 128, 2, 64, torch.float16, seed=6)
+    table, n = i32(table), i32(lens)
+    qs = [torch.randn(3, 8, 64, device=DEV).half() for _ in range(6)]
+    want = [kv8.attn(q, cache, table, n, 0.1, lse=True) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for i, q in enumerate(qs):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(kv8.attn(q, cache, table, n, 0.1, lse=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))
+
+
+def test_offsets_past_32_bits():
+    """Rows whose codes start past 2^32 bytes."""
+    page, D, Hkv = 256, 128, 8
+    pages = 2 ** 32 // (Hkv * page * D) + 3
+    cache, small = kv8.new_cache(pages, page, Hkv, D), kv8.new_cache(2, page, Hkv, D)
+    k, v = (torch.randn(300, Hkv, D, device=DEV).half() for _ in range(2))
+    at = torch.arange(300, dtype=torch.int32, device=DEV)
+    far, near, cu = i32([[pages - 1, pages - 2]]), i32([[0, 1]]), i32([0, 300])
+    for c, t in ((cache, far), (small, near)):
+        for a, b in ((0, 100), (100, 101), (101, 300)):     # parts of blocks, then a step
+            kv8.store(c, k[a:b], v[a:b], t, i32([b]), i32([0, b - a]))
+    slots = far[0, (at // page).long()] * page + at % page
+    for a, b in zip(kv8.load(cache, slots), kv8.load(small, at)):
+        assert torch.equal(a, b) and not a.eq(0).all()
+    q = torch.randn(300, 16, D, device=DEV).half()
+    for cu, m, n in ((None, 1, 1), (i32([0, 300]), 300, 300)):
+        got = []
+        for c, t in ((cache, far), (small, near)):
+            w = kv8.new_weights(c)
+            out, lse = kv8.attn(q[:n], c, t, i32([300]), 0.1, cu_q=cu, max_q=m, lse=True)
+            kv8.weigh(w, q[:n], lse, c, t, i32([300]), 0.1, cu_q=cu, max_q=m)
+            got.append((out, lse, w[t[0].long()]))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,W", [(32, 16, 4, 64), (64, 2, 2, 64), (32, 16, 4, 33), (40, 64, 1, 40),
+                                        (70, 4, 1, 50)])
+def test_single_tokens_with_room_for_more(B, Hq, Hkv, W):
+    """Without cu_q a request has one query, whatever max_q allows for: tables on either side
+    of the short form's limits, requests on either side of 64."""
+    g = torch.Generator().manual_seed(B + W)
+    lens = [int(n) for n in torch.randint(1, 300, (B,), generator=g)]
+    cache, held, table = filled(lens, 64, Hkv, 64, torch.float16, seed=B)
+    table = [(row + [-1] * W)[:W] for row in table]
+    q = torch.randn(B, Hq, 64, generator=g).half()
+    want = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), 0.125)
+    check(want, None, sv.attention(q, held, table, lens, 0.125))
+    for max_q in (2, 17, B, 1000, -1):
+        got = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), 0.125, max_q=max_q)
+        assert torch.equal(got, want), max_q
