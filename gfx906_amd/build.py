@@ -3,8 +3,8 @@
 Two shared objects and one program are produced under ``gfx906_amd/lib/``:
 
 * ``libgfx906_amd_attn.so`` -- the HIP kernels and the C ABIs declared in
-  ``include/gfx906_amd_attn.h``, ``include/gfx906_amd_serving.h`` and
-  ``include/gfx906_amd_conv3d.h``, compiled by ``hipcc --offload-arch=gfx950``. It plays the part of the reference's
+  ``include/gfx906_amd_attn.h`` and ``include/gfx906_amd_conv3d.h``, compiled
+  by ``hipcc --offload-arch=gfx950``. It plays the part of the reference's
   separately compiled kernel objects (``attn_kernel.gfx906.o``,
   ``conv3d_kernel.<arch>.o``; README.md:12, deploy/gfx906_attn.py:40-59).
 * ``gfx906_amd_attn_ext.so`` -- the PyTorch binding (``attn(q, k, v, scale)``,

@@ -1,12 +1,12 @@
 // PyTorch binding of the 8-bit key/value cache, its attention weights and eviction
-// (gfx906_amd_serving.h). The Python layer (gfx906_amd.kv8) documents the arguments. Every op runs
+// (gfx906_amd_attn.h). The Python layer (gfx906_amd.kv8) documents the arguments. Every op runs
 // on the current HIP stream of its tensors' device without synchronising; what cannot be run raises
 // RuntimeError.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 
 #include "bindings.h"
-#include "gfx906_amd_serving.h"
+#include "gfx906_amd_attn.h"
 #include "tensors.h"
 
 namespace {

@@ -1,8 +1,8 @@
 // What the kernels of the 8-bit cache share: the cache, its codes in the element types,
-// checks on the host. The format is described in gfx906_amd_serving.h. Internal.
+// checks on the host. The format is described in gfx906_amd_attn.h. Internal.
 #pragma once
 
-#include "gfx906_amd_serving.h"
+#include "gfx906_amd_attn.h"
 #include "longctx.h"
 
 namespace gfx906_amd {

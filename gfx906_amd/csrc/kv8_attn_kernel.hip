@@ -1,4 +1,4 @@
-// Attention over the 8-bit cache (gfx906_amd_serving.h) for AMD MI355X (gfx950).
+// Attention over the 8-bit cache (gfx906_amd_attn.h) for AMD MI355X (gfx950).
 //
 // How the work is dealt out is that of the 4-bit cache (kv4_kernel.hip, paged.h): few query
 // rows in equal runs of 64-token units, prompts in tiles of 128 rows. The codes are laid

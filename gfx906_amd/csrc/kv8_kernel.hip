@@ -1,6 +1,6 @@
 // Key/value cache in 8 bits for AMD MI355X (gfx950): storing and reading rows, the attention
 // weights of its blocks and eviction by them. The format and the entry points are
-// described in gfx906_amd_serving.h; the attention is in kv8_attn_kernel.hip.
+// described in gfx906_amd_attn.h; the attention is in kv8_attn_kernel.hip.
 //
 // gfx950 converts between pairs of E4M3 codes and fp16, bf16 or fp32 with a power-of-two
 // scale in one instruction (v_cvt_scalef32_*), rounding to nearest even.

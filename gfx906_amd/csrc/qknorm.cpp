@@ -1,12 +1,12 @@
 // PyTorch binding of the norms of queries and keys with the position rotation
-// (gfx906_amd_serving.h). The Python layer (gfx906_amd.qknorm) documents the arguments. Runs on
+// (gfx906_amd_attn.h). The Python layer (gfx906_amd.qknorm) documents the arguments. Runs on
 // the current HIP stream of the tensors' device without synchronising; what cannot be run raises
 // RuntimeError.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 
 #include "bindings.h"
-#include "gfx906_amd_serving.h"
+#include "gfx906_amd_attn.h"
 #include "tensors.h"
 
 namespace {

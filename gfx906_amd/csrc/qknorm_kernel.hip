@@ -1,6 +1,6 @@
 // Norms of queries and keys for each head with the position rotation in the same
 // pass, for AMD MI355X (gfx950). The entry point is described in
-// gfx906_amd_serving.h.
+// gfx906_amd_attn.h.
 //
 //   y = x / sqrt(mean(x^2) + eps) * w        over the D dims of a head
 //   (y_i, y_j) <- (c y_i - s y_j, s y_i + c y_j)   for the pairs of the first R dims
@@ -11,7 +11,7 @@
 
 #include <algorithm>
 
-#include "gfx906_amd_serving.h"
+#include "gfx906_amd_attn.h"
 
 namespace {
 

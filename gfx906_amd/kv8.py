@@ -14,7 +14,7 @@ of 2^-2. Requests, page tables and lengths are those of kv4, with its page plann
 and the next step goes on with ``gone.lens`` and ``gone.used``. Without eviction the weights, the lse and
 the last two calls are left out. Everything stays on the GPU: no call synchronises, and
 all of them may be captured into a HIP graph. The layout and what happens to values out of
-range is described in ``include/gfx906_amd_serving.h``. All calls run on the current
+range is described in ``include/gfx906_amd_attn.h``. All calls run on the current
 stream, raise ``RuntimeError`` for what they do not accept, and have no fallback. The
 reference has no counterpart.
 """

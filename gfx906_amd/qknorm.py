@@ -4,7 +4,7 @@ What models do with the rows of their projections before attention: an RMS norm 
 every head's dims, times a weight, then pairs of dims turned by angles of the token's
 position. The results are what :func:`gfx906_amd.attn`, :func:`gfx906_amd.kv4.store` and
 :func:`gfx906_amd.kv8.store` read. Formulas and the C ABI are in
-``include/gfx906_amd_serving.h``. The call runs on the current stream, raises
+``include/gfx906_amd_attn.h``. The call runs on the current stream, raises
 ``RuntimeError`` for what it does not accept, has no fallback and no gradient. The
 reference has no counterpart.
 """

@@ -1,7 +1,7 @@
 """CPU oracle of the serving operators (test infrastructure only): head norms with the
 position rotation, the 8-bit cache, attention over it, weights of its blocks, eviction.
 
-Plain loops in 64 bits over the definitions in ``include/gfx906_amd_serving.h``; nothing
+Plain loops in 64 bits over the definitions in ``include/gfx906_amd_attn.h``; nothing
 here comes from the kernels.
 """
 
