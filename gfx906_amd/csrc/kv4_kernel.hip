@@ -896,7 +896,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             for (int w = 0; w < wave; ++w) x += sum_s[w];
             return x;
         };
-        const long long n = scan(tid < a.B ? tiles_of(a, request(a, tid)) : 0);
+        const long long n = scan(tid < a.B ? tiles_of<kTileRows>(a, request(a, tid)) : 0);
         first_s[tid + 1] = (int)min(n, (long long)a.p_tiles);
         if (tid == 0) first_s[0] = 0;
         __syncthreads();
@@ -917,7 +917,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
                 else
                     hi = mid - 1;
             }
-            const int chunks = tile_chunks(a, request(a, lo), t - first_s[lo]);
+            const int chunks = tile_chunks<kTileRows>(a, request(a, lo), t - first_s[lo]);
             req[n] = lo;
             c[n] = chunks ? chunks + kPromptStart : 0;
             sum += c[n];
@@ -996,7 +996,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         }
         const Request req = request(a, b);
         const int rt = tile - t0;
-        const int end = uni(tile_end(a, req, rt)), chunks = (end + 63) / 64;
+        const int end = uni(tile_end<kTileRows>(a, req, rt)), chunks = (end + 63) / 64;
         const long long s = base * a.c.Hkv + hk * each + (p_cost(tile) - base);
         const int p0 = uni((int)(u0 - s)), p1 = uni((int)min((long long)chunks + kPromptStart, hi - s));
         u0 = s + p1;
@@ -1185,7 +1185,7 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
     auto head_of = [&](int r, int tok) {
         return hk * a.G + (int)((long long)rt * kTileRows + r - (long long)tok * a.G);
     };
-    const int end = tile_end(a, req, rt), chunks = (end + 63) / 64;
+    const int end = tile_end<kTileRows>(a, req, rt), chunks = (end + 63) / 64;
     int w0 = 0, w1 = 0;
     if (chunks) {
         const long long all = a.p_cost[a.p_first[a.B]] * a.c.Hkv;
@@ -1474,7 +1474,7 @@ extern "C" int kv4_attn(const void* q, void* o, const long long* q_strides,
                 hipLaunchKernelGGL((attn_prompt_kernel<kD, E, true>), dim3(pp.groups), dim3(256), 0,
                                    stream, a);
             } else {
-                hipLaunchKernelGGL(prompt_plan_kernel<AttnArgs>, dim3(1), dim3(1024), 0, stream, a);
+                hipLaunchKernelGGL((prompt_plan_kernel<kTileRows, AttnArgs>), dim3(1), dim3(1024), 0, stream, a);
                 hipLaunchKernelGGL((attn_prompt_kernel<kD, E, false>), dim3(pp.groups), dim3(256), 0,
                                    stream, a);
             }

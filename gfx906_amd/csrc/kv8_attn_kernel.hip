@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 
 // Attention of requests with many query rows, bound by the matrix rate.
 //
-// A tile is 128 query rows of a kv head (a token's G heads beside each other), 32 a wave; its keys
+// A tile is 32 NW query rows of a kv head (a token's G heads beside each other), 32 a wave; its keys
 // come in chunks of 64. The tiles' chunks are laid end to end and every workgroup takes an equal run;
 // prompt_combine_kernel merges tiles that lie in several runs. A chunk's codes are loaded by all
 // threads two chunks ahead, expanded on the way to LDS into the operands of both products, and then
@@ -547,12 +547,17 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 // the first product of the next but one around the softmax of the block between, one barrier a chunk.
 //
 // SELF: few tiles. Every workgroup adds up the tiles itself instead of a kernel before this one.
-template <int D, class T, bool SELF, bool LSE>
-__global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
+template <int D, class T, int NW, bool SELF, bool LSE>
+__global__ void __launch_bounds__(64 * NW, 2) attn_prompt_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using W = Tile<D, T, 2, true, LSE>;
     using x8 = typename W::x8;
-    constexpr int BYTES = 64 * W::RB, HALF = BYTES / 2, NX = D / 64;
+    constexpr int BYTES = 64 * W::RB, HALF = BYTES / 2, NT = 64 * NW, ROWS = 32 * NW;
+    // 16 bytes of codes a thread of K and of V, NX times; where there are threads enough (ALONE), of
+    // one of them.
+    constexpr int LOADS = 2 * 64 * D / 16;  // of a chunk
+    constexpr bool ALONE = LOADS <= NT;
+    constexpr int NX = ALONE ? 1 : LOADS / (2 * NT), FAR = 16 * NT;
     __shared__ __attribute__((aligned(1024))) char ka[BYTES];
     __shared__ __attribute__((aligned(1024))) char kb[BYTES];
     __shared__ __attribute__((aligned(1024))) char va[BYTES];
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
     __shared__ int first_s[SELF ? kSelfRequests + 1 : 1];
-    __shared__ long long cost_s[SELF ? kSelfTiles + 1 : 1], sum_s[4];
+    __shared__ long long cost_s[SELF ? kSelfTiles + 1 : 1], sum_s[NW];
     auto p_first = [&](int x) { return SELF ? first_s[x] : a.p_first[x]; };
     auto p_cost = [&](int x) { return SELF ? cost_s[x] : a.p_cost[x]; };
     if constexpr (SELF) {
@@ -579,12 +584,12 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             for (int w = 0; w < wave; ++w) x += sum_s[w];
             return x;
         };
-        const long long n = scan(tid < a.B ? tiles_of(a, request(a, tid)) : 0);
-        first_s[tid + 1] = (int)min(n, (long long)a.p_tiles);
+        const long long n = scan(tid < a.B ? tiles_of<ROWS>(a, request(a, tid)) : 0);
+        if (tid < kSelfRequests) first_s[tid + 1] = (int)min(n, (long long)a.p_tiles);
         if (tid == 0) first_s[0] = 0;
         __syncthreads();
         const int nt = first_s[a.B];
-        constexpr int PER = kSelfTiles / 256;
+        constexpr int PER = kSelfTiles / NT;
         long long c[PER], sum = 0;
         int req[PER];
 #pragma unroll
@@ -600,7 +605,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
                 else
                     hi = mid - 1;
             }
-            const int chunks = tile_chunks(a, request(a, lo), t - first_s[lo]);
+            const int chunks = tile_chunks<ROWS>(a, request(a, lo), t - first_s[lo]);
             req[n] = lo;
             c[n] = chunks ? chunks + kPromptStart : 0;
             sum += c[n];
@@ -616,11 +621,10 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             }
             at += c[n];
         }
-        if (tid == 255) cost_s[nt] = at;
+        if (tid == NT - 1) cost_s[nt] = at;
         if (blockIdx.x == 0) {
-            if (tid <= a.B) a.p_first[tid] = first_s[tid];
-            if (tid == 0 && a.B == 256) a.p_first[256] = first_s[256];
-            if (tid == 255) a.p_cost[nt] = at;
+            for (int x = tid; x <= a.B; x += NT) a.p_first[x] = first_s[x];
+            if (tid == NT - 1) a.p_cost[nt] = at;
         }
         __syncthreads();
     }
@@ -633,7 +637,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
     const long long hi = min(all, u0 + per);
     if (u0 >= hi) return;
     // The request, kv head and tile of unit u0.
-    for (int x = tid; x < a.B; x += 256)
+    for (int x = tid; x < a.B; x += NT)
         if (p_cost(p_first(x)) * a.c.Hkv <= u0 && u0 < p_cost(p_first(x + 1)) * a.c.Hkv) found = x;
     __syncthreads();
     int b = uni(found);
@@ -643,18 +647,25 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
     {
         const long long at = u0 - base * a.c.Hkv - hk * each;
         __syncthreads();
-        for (int x = t0 + tid; x < t1; x += 256)
+        for (int x = t0 + tid; x < t1; x += NT)
             if (p_cost(x) - base <= at && at < p_cost(x + 1) - base) found = x;
         __syncthreads();
     }
     int tile = uni(found);
 
-    // Where this thread's codes of a chunk go in LDS: 16 bytes each (and as many again 4 KB further
-    // on, at D = 128) of K, 16 dims of a key, and of V, 16 tokens of a dim. They are two operands'.
-    const int key = tid / (D / 16), unit = tid % (D / 16);
-    const int kst = (key / 32) * HALF + (4 * (unit >> 2) + (key >> 4 & 1)) * 1024 +
-                    16 * frag_slot(key & 15, unit & 3, unit >> 2);
-    const int vst = (tid / 64) * 1024 + 16 * frag_slot(tid / 4 & 15, tid & 3, 0);
+    // Where this thread's codes of a chunk go in LDS: of K 16 dims of a key, of V 16 tokens of a dim,
+    // which are two operands'; the next ones lie FAR bytes further on.
+    const bool has_v = !ALONE || tid >= NT / 2, has_k = !ALONE || !has_v;
+    const int slot16 = ALONE ? tid & (NT / 2 - 1) : tid;
+    auto kst = [&](int x) {
+        const int u = slot16 + x * NT, key = u / (D / 16), unit = u % (D / 16);
+        return (key / 32) * HALF + (4 * (unit >> 2) + (key >> 4 & 1)) * 1024 +
+               16 * frag_slot(key & 15, unit & 3, unit >> 2);
+    };
+    auto vst = [&](int x) {
+        const int u = slot16 + x * NT;
+        return (u / 64) * 1024 + 16 * frag_slot(u / 4 & 15, u & 3, 0);
+    };
 
     while (u0 < hi) {
         while (u0 >= base * a.c.Hkv + hk * each + (p_cost(tile + 1) - base)) {
@@ -673,7 +684,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         }
         const Request req = request(a, b);
         const int rt = tile - t0;
-        const int end = uni(tile_end(a, req, rt)), chunks = (end + 63) / 64;
+        const int end = uni(tile_end<ROWS>(a, req, rt)), chunks = (end + 63) / 64;
         const long long s = base * a.c.Hkv + hk * each + (p_cost(tile) - base);
         const int p0 = uni((int)(u0 - s)), p1 = uni((int)min((long long)chunks + kPromptStart, hi - s));
         u0 = s + p1;
@@ -687,7 +698,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         int lim[2];
         const long long rows = (long long)req.m * a.G;
         const unsigned neg = a.qsign < 0.f ? 0x80008000u : 0u;
-        const long long row0 = (long long)rt * kTileRows + wave * 32;
+        const long long row0 = (long long)rt * ROWS + wave * 32;
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
             const long long r = row0 + 16 * nb + i;
@@ -704,7 +715,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         const bool active = row0 < rows;  // (wave-uniform)
         const int all_see = active ? uni(seen_by(a, req, (int)(row0 / a.G))) : 0;
         // (of the tile: every row sees the chunks in front of it)
-        const int tile_see = uni(seen_by(a, req, (int)((long long)rt * kTileRows / a.G)));
+        const int tile_see = uni(seen_by(a, req, (int)((long long)rt * ROWS / a.G)));
 
         const ConstInts table = (ConstInts)(a.table + b * a.table_stride);
         const int shift = a.c.page == 64 ? 0 : a.c.page == 128 ? 1 : 2;
@@ -716,7 +727,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         };
         // Codes of chunks kc (K) and vc (V), on their way to LDS.
         struct Raw {
-            u32x4 kw[NX], vw[NX];
+            u32x4 kw[NX], vw[ALONE ? 1 : NX];  // (ALONE: kw is the one or the other)
             float ks, vs;
         };
         auto load = [&](int kc, int kpage, int vc, int vpage) __attribute__((always_inline)) {
@@ -724,10 +735,16 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             const long long kb = block_of(kc, kpage), vb = block_of(vc, vpage);
             r.ks = ((ConstFloats)a.c.ks)[kb];
             r.vs = ((ConstFloats)a.c.vs)[vb];
+            const uint8_t* kp = a.c.kc + kb * (kBlock * D) + 16 * slot16;
+            const uint8_t* vp = a.c.vc + vb * (kBlock * D) + 16 * slot16;
+            if constexpr (ALONE) {
+                r.kw[0] = *reinterpret_cast<const u32x4*>(has_v ? vp : kp);
+            } else {
 #pragma unroll
-            for (int x = 0; x < NX; ++x) {
-                r.kw[x] = *reinterpret_cast<const u32x4*>(a.c.kc + kb * (kBlock * D) + 4096 * x + 16 * tid);
-                r.vw[x] = *reinterpret_cast<const u32x4*>(a.c.vc + vb * (kBlock * D) + 4096 * x + 16 * tid);
+                for (int x = 0; x < NX; ++x) {
+                    r.kw[x] = *reinterpret_cast<const u32x4*>(kp + FAR * x);
+                    r.vw[x] = *reinterpret_cast<const u32x4*>(vp + FAR * x);
+                }
             }
             return r;
         };
@@ -735,31 +752,34 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             *reinterpret_cast<GFX906_LDS x8*>((GFX906_LDS char*)dst) = expand<T>(lo, hi, s);
         };
         auto put_k = [&](char* kd, const Raw& r) __attribute__((always_inline)) {
+            if (!has_k) return;
 #pragma unroll
-            for (int x = 0; x < NX; ++x) {  // (the next 4 KB are the other half's keys)
-                put(kd + kst + x * HALF, r.kw[x][0], r.kw[x][1], r.ks);
-                put(kd + kst + x * HALF + 2048, r.kw[x][2], r.kw[x][3], r.ks);
+            for (int x = 0; x < NX; ++x) {
+                put(kd + kst(x), r.kw[x][0], r.kw[x][1], r.ks);
+                put(kd + kst(x) + 2048, r.kw[x][2], r.kw[x][3], r.ks);
             }
         };
         // V of chunk c. Where some row does not see all of it, NaN is 0 for now.
         auto put_v = [&](char* vd, int c, int page, Raw& r) __attribute__((always_inline)) {
+            if (!has_v) return;
+            u32x4(&vw)[NX] = ALONE ? r.kw : reinterpret_cast<u32x4(&)[NX]>(r.vw);
             if (c * 64 + 64 > tile_see || !good(c, page)) {
                 unsigned any = 0;
 #pragma unroll
                 for (int x = 0; x < NX; ++x)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const unsigned n = nan_bytes(r.vw[x][e]);
+                        const unsigned n = nan_bytes(vw[x][e]);
                         any |= n;
-                        r.vw[x][e] &= ~((n >> 7) * 255u);
+                        vw[x][e] &= ~((n >> 7) * 255u);
                     }
                 if (any && good(c, page)) nans = 1;
                 if (!good(c, page)) r.vs = 1.f;  // (a scale that is NaN would reach every row)
             }
 #pragma unroll
-            for (int x = 0; x < NX; ++x) {  // (the next 4 KB are 64 dims on)
-                put(vd + vst + x * 4096, r.vw[x][0], r.vw[x][1], r.vs);
-                put(vd + vst + x * 4096 + HALF, r.vw[x][2], r.vw[x][3], r.vs);
+            for (int x = 0; x < NX; ++x) {
+                put(vd + vst(x), vw[x][0], vw[x][1], r.vs);
+                put(vd + vst(x) + HALF, vw[x][2], vw[x][3], r.vs);
             }
         };
         auto mask = [&](f32x4 (&S)[2][2], int c, int page, int half) __attribute__((always_inline)) {
@@ -785,7 +805,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
         put_k(ka, raw0);
         put_v(va, c0, g0, raw0);
         put_k(kb, raw1);
-        for (int z = tid; z < BYTES / 16; z += 256) *reinterpret_cast<u32x4*>(vb + 16 * z) = u32x4{};
+        for (int z = tid; z < BYTES / 16; z += NT) *reinterpret_cast<u32x4*>(vb + 16 * z) = u32x4{};
         __syncthreads();
         if (active) w.qk(ka, Sa);
 
@@ -832,7 +852,7 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
             float lu = l;
             if constexpr (LSE) lu = quad_sum(w.lsum[nb]);
             if (r >= rows) continue;
-            const long long at = slot * kTileRows + wave * 32 + 16 * nb + i;
+            const long long at = slot * ROWS + wave * 32 + 16 * nb + i;
             if (!whole) {
 #pragma unroll
                 for (int ob = 0; ob < W::NO; ++ob)
@@ -858,28 +878,28 @@ __global__ void __launch_bounds__(256, 2) attn_prompt_kernel(const AttnArgs a) {
 
 // Merges the runs of a tile and writes the zeros of tiles that see no key. One workgroup per 16
 // rows of a tile and kv head; behind these one per request and query row of attn_few_kernel's.
-template <int D, class T, bool LSE>
+template <int D, class T, int TILE, bool LSE>
 __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int ROWS = 16;
-    const int tile = blockIdx.x / (kTileRows / ROWS), hk = blockIdx.y, tid = threadIdx.x;
+    const int tile = blockIdx.x / (TILE / ROWS), hk = blockIdx.y, tid = threadIdx.x;
     if (tile >= a.p_tiles) {
-        const int e = blockIdx.x - a.p_tiles * (kTileRows / ROWS), few = e / kFewRows;
+        const int e = blockIdx.x - a.p_tiles * (TILE / ROWS), few = e / kFewRows;
         few_combine<D, T, 2, 256, LSE>(a, few, hk, e - few * kFewRows);
         return;
     }
-    const int r0 = blockIdx.x % (kTileRows / ROWS) * ROWS;
+    const int r0 = blockIdx.x % (TILE / ROWS) * ROWS;
     const int b = a.p_req[tile];
     if (tile >= a.p_first[a.B]) return;
     const int t0 = a.p_first[b], t1 = a.p_first[b + 1], rt = tile - t0;
     const Request req = request(a, b);
-    const int rows = (int)min(r0 + (long long)ROWS, (long long)req.m * a.G - (long long)rt * kTileRows);
+    const int rows = (int)min(r0 + (long long)ROWS, (long long)req.m * a.G - (long long)rt * TILE);
     if (r0 >= rows) return;
-    auto tok_of = [&](int r) { return (int)(((long long)rt * kTileRows + r) / a.G); };
+    auto tok_of = [&](int r) { return (int)(((long long)rt * TILE + r) / a.G); };
     auto head_of = [&](int r, int tok) {
-        return hk * a.G + (int)((long long)rt * kTileRows + r - (long long)tok * a.G);
+        return hk * a.G + (int)((long long)rt * TILE + r - (long long)tok * a.G);
     };
-    const int end = tile_end(a, req, rt), chunks = (end + 63) / 64;
+    const int end = tile_end<TILE>(a, req, rt), chunks = (end + 63) / 64;
     int w0 = 0, w1 = 0;
     if (chunks) {
         const long long all = a.p_cost[a.p_first[a.B]] * a.c.Hkv;
@@ -901,7 +921,7 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #pragma unroll
                 for (int n = 0; n < U; ++n) {
                     const int y = min(x + n, w1);
-                    const long long at = (2LL * y + (y == w0 ? 1 : 0)) * kTileRows + r;
+                    const long long at = (2LL * y + (y == w0 ? 1 : 0)) * TILE + r;
                     ml[n] = *reinterpret_cast<const f32x4*>(a.p_ml + at * 4);
                     p[n] = *reinterpret_cast<const f32x4*>(a.p_o + at * D + d);
                 }
@@ -929,13 +949,29 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #endif
 }
 
+// Waves of a prompt's tile, of 32 rows each: the more, the fewer times a chunk is expanded; but short
+// prompts fill large tiles badly. us with eight / four: 3 prompts of 77 .. 2111 queries behind 300 ..
+// 8192 tokens, 16/4 heads of 128, 192 / 207; one of 512 behind 16000, 8/2 heads, 64.4 / 67.9; 4 of 90 ..
+// 300 behind 100 .. 1000, 8/2 heads, 37.8 / 38.7; one of 150, 4/2 heads (300 rows), 25.6 / 24.6; one of
+// 300, 4/4 heads of 64, 26.9 / 22.1.
+constexpr int kWaves = 8, kWavesShort = 4;
+constexpr long long kLongRows = 512;
+int prompt_waves(int max_q, int G) {
+    return (long long)max_q * G >= kLongRows ? kWaves : kWavesShort;
+}
+// (eight waves a CU, as their registers allow)
+PromptPlan prompt_plan8(int T, int B, int G, int D, int max_q, size_t after) {
+    const int waves = prompt_waves(max_q, G);
+    return prompt_plan(T, B, G, D, max_q, after, 4, 32 * waves, 256 * 8 / waves);
+}
+
 }  // namespace
 
 extern "C" size_t kv8_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q,
                                            int max_len) {
     if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0 || max_q <= 0) return 0;
     const size_t few = few_plan(B, Hq / Hkv, Hkv, D, std::min(max_q, T), max_len, 4).bytes;
-    const PromptPlan p = prompt_plan(T, B, Hq / Hkv, D, std::min(max_q, T), few, 4);
+    const PromptPlan p = prompt_plan8(T, B, Hq / Hkv, D, std::min(max_q, T), few);
     return p.used ? p.bytes : few;
 }
 
@@ -972,10 +1008,11 @@ extern "C" int kv8_attn(const void* q, void* o, float* lse, const long long* q_s
     if (!good_scale(scale)) return err.fail("kv8_attn: scale must be finite, and below 2.3e38");
     const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page, 4);
     if (plan.units >= (1LL << 30)) return err.fail("kv8_attn: table too wide for so many heads");
-    const PromptPlan pp = prompt_plan(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes, 4);
+    const PromptPlan pp = prompt_plan8(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);
     const size_t need = pp.used ? pp.bytes : plan.bytes;
     const long long heads = (long long)B * Hkv;
-    const long long combines = pp.tiles * (long long)(kTileRows / 16) +
+    const int waves = prompt_waves(cu_q ? std::min(max_q, T) : 1, Hq / Hkv);
+    const long long combines = pp.tiles * (long long)(2 * waves) +
                                (plan.direct ? 0 : (long long)B * kFewRows);
     if (!(plan.direct ? launchable(heads * plan.tiles, 512)
                       : launchable(heads, plan.many ? 1024 : 256)) ||
@@ -1052,18 +1089,23 @@ extern "C" int kv8_attn(const void* q, void* o, float* lse, const long long* q_s
         else
             runs(attn_few_kernel<kD, E, 2, false, L>, few_combine_kernel<kD, E, 2, 256, L>,
                  few_combine_kernel<kD, E, 2, 1024, L>);
-        if (pp.used) {
+        auto prompts = [&](auto waves) {
+            constexpr int kW = decltype(waves)::value, kRows = 32 * kW;
             if (pp.self) {
-                hipLaunchKernelGGL((attn_prompt_kernel<kD, E, true, L>), dim3(pp.groups), dim3(256), 0,
-                                   stream, a);
+                hipLaunchKernelGGL((attn_prompt_kernel<kD, E, kW, true, L>), dim3(pp.groups),
+                                   dim3(64 * kW), 0, stream, a);
             } else {
-                hipLaunchKernelGGL(prompt_plan_kernel<AttnArgs>, dim3(1), dim3(1024), 0, stream, a);
-                hipLaunchKernelGGL((attn_prompt_kernel<kD, E, false, L>), dim3(pp.groups), dim3(256), 0,
-                                   stream, a);
+                hipLaunchKernelGGL((prompt_plan_kernel<kRows, AttnArgs>), dim3(1), dim3(1024), 0, stream,
+                                   a);
+                hipLaunchKernelGGL((attn_prompt_kernel<kD, E, kW, false, L>), dim3(pp.groups),
+                                   dim3(64 * kW), 0, stream, a);
             }
-            hipLaunchKernelGGL((prompt_combine_kernel<kD, E, L>), dim3((unsigned)combines, Hkv),
+            hipLaunchKernelGGL((prompt_combine_kernel<kD, E, kRows, L>), dim3((unsigned)combines, Hkv),
                                dim3(256), 0, stream, a);
-        }
+        };
+        if (!pp.used) return;
+        waves == kWaves ? prompts(std::integral_constant<int, kWaves>{})
+                        : prompts(std::integral_constant<int, kWavesShort>{});
     };
     auto by_dim = [&](auto t, auto with_lse) {
         D == 64 ? go(std::integral_constant<int, 64>{}, t, with_lse)

@@ -20,7 +20,7 @@ constexpr int kFewRows = 256;
 
 // A run is at least kPromptRun units: two prompts of 200 queries behind 800 tokens, 16/4 heads, 30
 // us in the prompt kernels with 5, 37 with 8, 53 with 16.
-constexpr int kTileRows = 128, kPromptStart = 4;
+constexpr int kTileRows = 128, kPromptStart = 4;  // (of the 4-bit cache's tiles)
 constexpr long long kPromptRun = kPromptStart + 1;
 constexpr int kSelfTiles = 1024, kSelfRequests = 256;  // SELF (attn_prompt_kernel)
 
@@ -57,25 +57,25 @@ __device__ __forceinline__ int seen_by(const A& a, const Request& r, int i) {
 }
 
 // Row tiles of a request, and the 64-key chunks that tile rt reads.
-template <class A>
+template <int ROWS, class A>
 __device__ __forceinline__ int tiles_of(const A& a, const Request& r) {
     const long long rows = (long long)r.m * a.G;
-    return rows > a.few_rows ? (int)((rows + kTileRows - 1) / kTileRows) : 0;
+    return rows > a.few_rows ? (int)((rows + ROWS - 1) / ROWS) : 0;
 }
-template <class A>
+template <int ROWS, class A>
 __device__ __forceinline__ int tile_end(const A& a, const Request& r, int rt) {
-    const long long last = min((long long)r.m * a.G, (rt + 1LL) * kTileRows) - 1;
+    const long long last = min((long long)r.m * a.G, (rt + 1LL) * ROWS) - 1;
     return seen_by(a, r, (int)(last / a.G));
 }
-template <class A>
+template <int ROWS, class A>
 __device__ __forceinline__ int tile_chunks(const A& a, const Request& r, int rt) {
-    return (tile_end(a, r, rt) + 63) / 64;
+    return (tile_end<ROWS>(a, r, rt) + 63) / 64;
 }
 #endif
 
 // Tiles of all requests and their units (chunks, and kPromptStart for the start and the
 // merge of a tile that has any), summed up. One workgroup.
-template <class A>
+template <int ROWS, class A>
 __global__ void __launch_bounds__(1024) prompt_plan_kernel(const A a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ int first[kPagedRequests + 1];
@@ -96,11 +96,11 @@ __global__ void __launch_bounds__(1024) prompt_plan_kernel(const A a) {
     // (requests whose rows overlap could have more tiles than there is room for)
     auto cap = [&](long long x) { return (int)min(x, (long long)a.p_tiles); };
     long long n = 0;
-    for (int b = b0; b < b1; ++b) n += tiles_of(a, request(a, b));
+    for (int b = b0; b < b1; ++b) n += tiles_of<ROWS>(a, request(a, b));
     n = scan(n) - n;
     for (int b = b0; b < b1; ++b) {
         first[b] = a.p_first[b] = cap(n);
-        n += tiles_of(a, request(a, b));
+        n += tiles_of<ROWS>(a, request(a, b));
     }
     __syncthreads();
     const int all = cap(part[1023]);
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(1024) prompt_plan_kernel(const A a) {
                 a.p_cost[i] = sum;
                 a.p_req[i] = x;
             }
-            const int c = tile_chunks(a, r, i - first[x]);
+            const int c = tile_chunks<ROWS>(a, r, i - first[x]);
             sum += c ? c + kPromptStart : 0;
         }
         if (!pass) {
@@ -180,26 +180,27 @@ inline FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len, in
 }
 
 // How attn_prompt_kernel is launched, and its part of the workspace behind the few
-// rows' one. tiles: the most there can be of T queries.
+// rows' one. tiles: the most there can be of T queries. rows: of a tile; groups: workgroups.
 struct PromptPlan {
     bool used;
     int groups, tiles;
     bool self;
     size_t cost_off, req_off, o_off, ml_off, bytes;
 };
-inline PromptPlan prompt_plan(int T, int B, int G, int D, int max_q, size_t after, int ml = 2) {
+inline PromptPlan prompt_plan(int T, int B, int G, int D, int max_q, size_t after, int ml = 2,
+                              int rows = kTileRows, int groups = 512) {
     PromptPlan p{};
     p.used = (long long)max_q * G > kFewRows;
     if (!p.used) return p;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    p.groups = 512;  // two a CU
-    p.tiles = (int)std::min<long long>((long long)T * G / kTileRows + B, (1LL << 27));
+    p.groups = groups;
+    p.tiles = (int)std::min<long long>((long long)T * G / rows + B, (1LL << 27));
     p.cost_off = up(after) + up((size_t)(B + 1) * sizeof(int));
     p.self = p.tiles <= kSelfTiles && B <= kSelfRequests;
     p.req_off = p.cost_off + up((size_t)(p.tiles + 1) * sizeof(long long));
     p.o_off = p.req_off + up((size_t)p.tiles * sizeof(int));
-    p.ml_off = p.o_off + (size_t)2 * p.groups * kTileRows * D * sizeof(float);
-    p.bytes = p.ml_off + (size_t)2 * p.groups * kTileRows * ml * sizeof(float);
+    p.ml_off = p.o_off + (size_t)2 * p.groups * rows * D * sizeof(float);
+    p.bytes = p.ml_off + (size_t)2 * p.groups * rows * ml * sizeof(float);
     return p;
 }
 

@@ -330,13 +330,14 @@ def test_many_requests(wide):
     check(out, lse, sv.attention(q, held, table, lens, 0.125))
 
 
-def test_prompts_among_many_requests():
+@pytest.mark.parametrize("longest", [700, 320])
+def test_prompts_among_many_requests(longest):
     """Three hundred requests, four of them prompts (their tiles are summed up by a kernel of
-    its own)."""
+    its own), long enough for large tiles or not."""
     g = torch.Generator().manual_seed(2)
     lens = [int(n) for n in torch.randint(0, 70, (300,), generator=g)]
     news = [min(1, n) for n in lens]
-    for b, n in ((5, 400), (6, 130), (170, 700), (299, 257)):
+    for b, n in ((5, 300), (6, 130), (170, longest), (299, 257)):
         lens[b], news[b] = n, max(129, n - 100)
     cache, held, table = filled(lens, 64, 1, 64, torch.bfloat16, seed=2)
     cu = offsets(news)
@@ -348,7 +349,7 @@ def test_prompts_among_many_requests():
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("news", [[5, 1], [150, 40]])
+@pytest.mark.parametrize("news", [[5, 1], [150, 40], [230, 130]])
 def test_nan_reaches_only_the_rows_that_see_it(news, D, dtype):
     """NaN and infinities among the keys and values of tokens that some rows do not see."""
     lens, page, H = [230, 130], 64, 2
@@ -364,7 +365,7 @@ def test_nan_reaches_only_the_rows_that_see_it(news, D, dtype):
     kv8.store(cache, k.to(DEV), v.to(DEV), i32(table), i32(lens), i32(cu))
     held.store(k, v, table, lens, cu)
     cu = offsets(news)
-    q = torch.randn(cu[-1], 4, D, generator=g).to(dtype)
+    q = torch.randn(cu[-1], 2 * (1 + len(news)) + 2, D, generator=g).to(dtype)[:, :6 if news[0] > 200 else 4]
     for causal in (True, False):
         out, lse = kv8.attn(q.to(DEV), cache, i32(table), i32(lens), 0.1, cu_q=i32(cu),
                             max_q=max(news), causal=causal, lse=True)
