@@ -696,7 +696,10 @@ struct WeighPlan {
     int split_rows, parts;
     size_t bytes;
 };
-constexpr int kWeighFew = 64;  // query rows of a kv head that go to weigh_few_kernel
+// Query rows of a kv head that go to weigh_few_kernel. 32 requests of 100 .. 16384 tokens, 32/8 heads, us
+// there / in weigh_prompt_kernel: 4 rows 27.3 / 45.8, 32 rows 34.8 / 46.4, 64 rows 47.0 / 44.2; one of
+// 131000, 16/2 heads, 64 rows 17.5 / 15.5.
+constexpr int kWeighFew = 32;
 WeighPlan weigh_plan(int B, int G, int Hkv, int W, int page, int max_q) {
     WeighPlan p{};
     p.blocks = (long long)W * (page / kBlock);
