@@ -949,6 +949,14 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 #endif
 }
 
+// Units of a head's start: fewer than for the 4-bit cache, whose units are half as many bytes. us with 4 /
+// 6 / 8 / 16: 32 requests of 100 .. 16384 tokens, 32/8 heads of 128, 50.6 / 45.0 / 44.3 / 45.7; 64 of 100 ..
+// 8000 52.2 / 46.8 / 45.5 / 49.3; 16 of 1000 .. 4000, three queries each, 16/4 heads, 17.5 / 17.4 / 17.2 / 19.1.
+constexpr int kStart = 8;
+// DIRECT reaches tables of 2048 tokens, no further with many heads: us there / in runs, 32 requests, 32/8
+// heads of 128: of 4000 tokens each 49.0 / 53.0, of 100 .. 4000 26.6 / 21.6; one request of 2000 14.8 / 15.0,
+// of 3000 19.8 / 15.1.
+constexpr int kFar = 1;
 // Waves of a prompt's tile, of 32 rows each: the more, the fewer times a chunk is expanded; but short
 // prompts fill large tiles badly. us with eight / four: 3 prompts of 77 .. 2111 queries behind 300 ..
 // 8192 tokens, 16/4 heads of 128, 192 / 207; one of 512 behind 16000, 8/2 heads, 64.4 / 67.9; 4 of 90 ..
@@ -970,7 +978,7 @@ PromptPlan prompt_plan8(int T, int B, int G, int D, int max_q, size_t after) {
 extern "C" size_t kv8_attn_workspace_bytes(int T, int B, int Hq, int Hkv, int D, int max_q,
                                            int max_len) {
     if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0 || max_q <= 0) return 0;
-    const size_t few = few_plan(B, Hq / Hkv, Hkv, D, std::min(max_q, T), max_len, 4).bytes;
+    const size_t few = few_plan(B, Hq / Hkv, Hkv, D, std::min(max_q, T), max_len, 4, kStart, kFar).bytes;
     const PromptPlan p = prompt_plan8(T, B, Hq / Hkv, D, std::min(max_q, T), few);
     return p.used ? p.bytes : few;
 }
@@ -1006,7 +1014,7 @@ extern "C" int kv8_attn(const void* q, void* o, float* lse, const long long* q_s
     const long long oe[2] = {T, Hq};
     if (!rows_apart(o_strides, oe, 2, D)) return err.fail("kv8_attn: o's rows overlap");
     if (!good_scale(scale)) return err.fail("kv8_attn: scale must be finite, and below 2.3e38");
-    const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page, 4);
+    const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page, 4, kStart, kFar);
     if (plan.units >= (1LL << 30)) return err.fail("kv8_attn: table too wide for so many heads");
     const PromptPlan pp = prompt_plan8(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);
     const size_t need = pp.used ? pp.bytes : plan.bytes;

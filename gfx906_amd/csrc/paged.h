@@ -154,8 +154,10 @@ struct FewPlan {
     long long units;
     size_t o_off, ml_off, bytes;  // of the workspace
 };
-// ml: floats of a row's statistics.
-inline FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len, int ml = 2) {
+// ml: floats of a row's statistics; start: units that the start of a head of up to 16 rows counts; far: by how
+// much DIRECT reaches further where there are heads enough.
+inline FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len, int ml = 2,
+                        int start = 16, int far = 2) {
     FewPlan p{};
     const long long rows = std::min<long long>((long long)max_q * G, kFewRows);
     p.nb = rows > 16 ? 2 : 1;
@@ -164,9 +166,9 @@ inline FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len, in
     // (a unit of 32 rows takes about as long as two of 16. 32 requests of 100 .. 16384 tokens,
     // one query each: 36.1 us with 8 units, 28.8 with 16, 30.5 with 24; 131072 tokens with 32
     // rows: 22.5 with 8, 24.0 with 16)
-    p.start = p.nb == 1 ? 16 : 8;
+    p.start = p.nb == 1 ? start : 8;
     p.units = segs * ((std::max(max_len, 1) + 63LL) / 64 + p.start);
-    p.direct = max_len <= (segs >= kDirectHeads ? 2 : 1) * kDirectTokens && segs < (1LL << 31);
+    p.direct = max_len <= (segs >= kDirectHeads ? far : 1) * kDirectTokens && segs < (1LL << 31);
     if (p.direct) return p;
     // A workgroup a CU, with a unit a wave at least. (Three of four waves, with 8 units for a
     // start: 32 ragged requests 29.3 us and not 28.8, 32 of 4000 tokens 33.5 and not 30.)
