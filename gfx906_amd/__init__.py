@@ -9,7 +9,9 @@ are not built or the inputs are not accepted; there is no fallback
 implementation.
 
 ``gfx906_amd.kv4`` holds a paged key/value cache in 4 bits with the attention over
-it, ``gfx906_amd.sparse`` attention over the key blocks that a score selects.
+it, ``gfx906_amd.sparse`` attention over the key blocks that a score selects,
+``gfx906_amd.kv8`` a cache in 8 bits with attention and eviction, and
+``gfx906_amd.qknorm`` the norms of queries and keys with the position rotation.
 """
 
 from .loader import (KERNEL_LIB, EXT_LIB, NotBuiltError, capi, extension,  # noqa: F401

@@ -117,6 +117,10 @@ __device__ __forceinline__ void give_nans(const uint8_t* vp, f32x4 (&oacc)[D / 1
 // key l%16, two steps' operands once they are expanded (Q has the same dims in the same steps).
 // V's 16 bytes are tokens of dim l%16 of 16, which is where the first product leaves their weights.
 // The next unit's K codes are loaded once the scores of one are done, its V codes at the end.
+//
+// 32 requests of 100 .. 16384 tokens, 8 kv heads of 128, one query each: 36.8 us (193 MB: 5.3 TB/s) and 4.6
+// for the merge; 131072 tokens, 2 kv heads, 32 rows: 18.9 and 5.0, of which the bytes take 11, a run's start
+// 4 and the waves' merge 2; 1024 tokens, 16 heads of 64, in DIRECT: 6.2.
 template <int D, class T, int NB, bool DIRECT, bool LSE>
 __global__ void __launch_bounds__(512, D == 64 && NB == 1 ? 4 : 2) attn_few_kernel(const AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -552,6 +556,10 @@ __global__ void __launch_bounds__(NT) few_combine_kernel(const AttnArgs a) {
 // used as attn_prompt_kernel of the 4-bit cache does: the second product of one block of 32 keys and
 // the first product of the next but one around the softmax of the block between, one barrier a chunk.
 //
+// 3 prompts of 77 .. 2111 queries behind 300 .. 8192 tokens, 16/4 heads of 128: 166 us (173 GFLOP: 1044
+// TFLOP/s; a library product of 8192 reaches 1240). The matrix pipe is busy for 44 % of the clocks, the
+// vector unit for 38, LDS for 36, without bank conflicts.
+//
 // SELF: few tiles. Every workgroup adds up the tiles itself instead of a kernel before this one.
 template <int D, class T, int NW, bool SELF, bool LSE>
 __global__ void __launch_bounds__(64 * NW, 2) attn_prompt_kernel(const AttnArgs a) {
@@ -956,8 +964,9 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(const AttnArgs a) {
 }
 
 // Units of a head's start: fewer than for the 4-bit cache, whose units are half as many bytes. us with 4 /
-// 6 / 8 / 16: 32 requests of 100 .. 16384 tokens, 32/8 heads of 128, 50.6 / 45.0 / 44.3 / 45.7; 64 of 100 ..
-// 8000 52.2 / 46.8 / 45.5 / 49.3; 16 of 1000 .. 4000, three queries each, 16/4 heads, 17.5 / 17.4 / 17.2 / 19.1.
+// 6 / 8 / 16 (codes loaded through the caches): 32 requests of 100 .. 16384 tokens, 32/8 heads of 128, 50.6 /
+// 45.0 / 44.3 / 45.7; 64 of 100 .. 8000 52.2 / 46.8 / 45.5 / 49.3; 16 of 1000 .. 4000, three queries each,
+// 16/4 heads, 17.5 / 17.4 / 17.2 / 19.1.
 constexpr int kStart = 8;
 // DIRECT reaches tables of 2048 tokens, no further with many heads: us there / in runs, 32 requests, 32/8
 // heads of 128: of 4000 tokens each 49.0 / 53.0, of 100 .. 4000 26.6 / 21.6; one request of 2000 14.8 / 15.0,
@@ -1020,7 +1029,8 @@ extern "C" int kv8_attn(const void* q, void* o, float* lse, const long long* q_s
     const long long oe[2] = {T, Hq};
     if (!rows_apart(o_strides, oe, 2, D)) return err.fail("kv8_attn: o's rows overlap");
     if (!good_scale(scale)) return err.fail("kv8_attn: scale must be finite, and below 2.3e38");
-    const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page, 4, kStart, kFar);
+    const FewPlan plan = few_plan(B, Hq / Hkv, Hkv, D, cu_q ? std::min(max_q, T) : 1, W * page, 4,
+                                  kStart, kFar);
     if (plan.units >= (1LL << 30)) return err.fail("kv8_attn: table too wide for so many heads");
     const PromptPlan pp = prompt_plan8(T, B, Hq / Hkv, D, cu_q ? std::min(max_q, T) : 1, plan.bytes);
     const size_t need = pp.used ? pp.bytes : plan.bytes;

@@ -154,8 +154,8 @@ struct FewPlan {
     long long units;
     size_t o_off, ml_off, bytes;  // of the workspace
 };
-// ml: floats of a row's statistics; start: units that the start of a head of up to 16 rows counts; far: by how
-// much DIRECT reaches further where there are heads enough.
+// ml: floats of a row's statistics; start: units that the start of a head of up to 16 rows counts;
+// far: how many times as far DIRECT reaches where there are heads enough.
 inline FewPlan few_plan(int B, int G, int Hkv, int D, int max_q, int max_len, int ml = 2,
                         int start = 16, int far = 2) {
     FewPlan p{};

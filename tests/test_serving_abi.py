@@ -208,7 +208,8 @@ def test_python_layer_refuses_on_the_cpu(lib):
         with pytest.raises(ValueError):
             kv8.new_cache(*bad, device="cpu")
     cache = kv8.new_cache(4, 128, 2, 64, device="cpu")
-    assert cache.page == 128 and cache.v.shape == (4, 2, 2, 64, 64) and kv8.new_weights(cache).shape == (4, 2, 2)
+    assert cache.page == 128 and cache.v.shape == (4, 2, 2, 64, 64)
+    assert kv8.new_weights(cache).shape == (4, 2, 2)
     assert sum(t.numel() * t.element_size() for t in (cache.k, cache.v)) == 4 * 2 * 128 * 64 * 2
     q, n = torch.zeros(1, 2, 64).half(), torch.ones(1, dtype=torch.int32)
     table, w = torch.zeros(1, 1, dtype=torch.int32), kv8.new_weights(cache)
