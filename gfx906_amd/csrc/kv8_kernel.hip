@@ -510,8 +510,9 @@ __global__ void __launch_bounds__(64, D == 64 ? 8 : 4) weigh_few_kernel(const We
             if (ok) x = *reinterpret_cast<const u32x4*>(q + 64 * (n / 2) + 8 * (n % 2));
             qf[n] = __builtin_bit_cast(x8, x ^ neg);
         }
-        const float m = shift_of(ok ? a.lse[(long long)(req.first + tok) * a.Hq + h] : -INFINITY);
-        const int lim = ok ? seen_by(a, req, tok) : 0;
+        const float lse = ok ? a.lse[(long long)(req.first + tok) * a.Hq + h] : -INFINITY;
+        const float m = shift_of(lse);
+        const int lim = lse == -INFINITY ? 0 : seen_by(a, req, tok);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 S = {};
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(256, 3) weigh_prompt_kernel(const WeighArgs a)
         if (wave == 0) {
             const bool ok = r0 + lane < end;
             m = ok ? *lse : -INFINITY;
-            lim = ok ? seen_by(a, req, ltok) : 0;
+            lim = m == -INFINITY ? 0 : seen_by(a, req, ltok);
             ltok += lstep.tok;
             lh += lstep.h;
             lse += lstep.far;

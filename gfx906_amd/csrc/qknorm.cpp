@@ -72,8 +72,9 @@ std::vector<Tensor> norm_rotate_op(Tensor q, c10::optional<Tensor> k, c10::optio
     // [x, result] of q and of k, 4-D
     Tensor x[2], y[2], given[2];
     const c10::optional<Tensor>* out[2] = {&q_out, &k_out};
-    // Contiguous results of both lie in one buffer.
+    // Small contiguous results of both lie in one buffer (an allocation is a tenth of such a call).
     const bool both = k.has_value() && !q_out.has_value() && !k_out.has_value() &&
+                      q.numel() + k->numel() <= (1 << 20) &&
                       (q.is_contiguous() || !q.is_non_overlapping_and_dense()) &&
                       (k->is_contiguous() || !k->is_non_overlapping_and_dense());
     Tensor buf;

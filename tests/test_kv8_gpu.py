@@ -485,6 +485,21 @@ def test_weigh_with_lost_pages_negative_scale_fewer_queries_and_nan():
         weighed(got, want, tol, table, [300, 130], 64)
 
 
+@pytest.mark.parametrize("news", [1, 30])
+def test_rows_that_see_nothing_weigh_nothing_whatever_the_keys_hold(news):
+    """An lse of -inf counts for the row, also where keys hold NaN."""
+    H, D, n = 1, 64, 100
+    k = torch.randn(n, H, D).half()
+    k[40] = math.nan
+    cache, table = kv8.new_cache(2, 64, H, D), i32([[1, 0]])
+    kv8.store(cache, k.to(DEV), k.nan_to_num().to(DEV), table, i32([n]), i32([0, n]))
+    q = torch.randn(news, 2, D, device=DEV).half()
+    lse = torch.full((news, 2), -math.inf, device=DEV)
+    w = kv8.new_weights(cache) + 3
+    kv8.weigh(w, q, lse, cache, table, i32([n]), 0.1, cu_q=i32([0, news]), max_q=news)
+    assert w.eq(3).all()
+
+
 def test_weigh_refuses():
     cache, _, table = filled([70], 64, 2, 64, torch.float16, seed=1)
     w, q = kv8.new_weights(cache), torch.zeros(1, 4, 64, device=DEV).half()
