@@ -12,6 +12,7 @@
 #include "longctx.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gfx906_amd_attn.h"
 
@@ -42,17 +43,18 @@ struct RotateArgs {
     float eps, inv_d;
 };
 
-// A row is 8 dims a lane in L = 2^k lanes (some idle where D is not 8 L), a wave 64 / L rows:
-// of one token's heads side by side, or of one head's tokens, whichever lie closer in memory
-// (tok_step, head_step). The wave then goes over `heads` heads with the same tokens' angles.
+// A row is 8 dims a lane in L = 2^k lanes (some idle where D is not 8 L), a wave 64 / L rows: of one
+// head's tokens, or of one token's heads (tok_step, head_step). The wave goes over `heads` heads with
+// the same tokens' angles; kUnroll rows a lane are in flight, of as many heads or, where there are too few
+// heads, of TS tokens.
 //
 // NEAR: pairs are neighbours (2i, 2i+1) and lie in one lane; else halves
 // (i, i + R/2), whose other number another lane holds.
-template <class T, int L, bool NEAR>
+template <class T, int L, bool NEAR, int TS>
 __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using x8 = typename Elem<T>::x8;
-    constexpr int RG = 64 / L;
+    constexpr int RG = 64 / L, HS = kUnroll / TS, NA = NEAR ? 4 : 8;
     const int lane = threadIdx.x & 63, l = lane % L, grp = lane / L;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned task = blockIdx.x * 4 + wave;
@@ -63,31 +65,38 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
     const bool is_k = chunk >= a.part[0].chunks;
     if (is_k) chunk -= a.part[0].chunks;
     const Rows& p = a.part[is_k];
-    // token of this lane, counted over batches
-    const unsigned t = a.tok_step ? tg * RG + grp : tg;
-    const bool live = t < a.B * a.S && 8 * l < a.D;
-    const unsigned b = min(t, a.B * a.S - 1) / a.S, s = min(t, a.B * a.S - 1) - b * a.S;
-
-    const T* x = (const T*)p.x + b * p.xb + s * p.xs + 8 * l;
-    T* y = (T*)p.y + b * p.yb + s * p.ys + 8 * l;
     int h = chunk * a.heads + grp * a.head_step;
     const int h1 = min(p.H, (chunk + 1) * a.heads);
+    // The lane's tokens, counted over batches, and where their rows and angles lie.
+    const bool turn = 8 * l < a.R;
+    const int half = a.R / 16;  // lanes between the numbers of a pair
+    bool live[TS];
+    const T* x[TS];
+    T* y[TS];
+    long long at[TS];
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        const unsigned t = a.tok_step ? (tg * TS + i) * RG + grp : tg, last = a.B * a.S - 1;
+        live[i] = t <= last && 8 * l < a.D;
+        const unsigned b = min(t, last) / a.S, s = min(t, last) - b * a.S;
+        x[i] = (const T*)p.x + b * p.xb + s * p.xs + 8 * l;
+        y[i] = (T*)p.y + b * p.yb + s * p.ys + 8 * l;
+        at[i] = s;
+        if (turn && a.pos) at[i] = a.pos[b * a.pb + s * a.ps];
+    }
     u32x4 raw[kUnroll];
     auto fetch = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             raw[u] = u32x4{};
-            const int hh = from + u * a.head_next;
-            if (live && hh < h1) raw[u] = *reinterpret_cast<const u32x4*>(x + hh * p.xh);
+            const int hh = from + u % HS * a.head_next;
+            if (live[u / HS] && hh < h1)
+                raw[u] = *reinterpret_cast<const u32x4*>(x[u / HS] + hh * p.xh);
         }
     };
-    // (the position's load and the first rows' are on their way together; angles and weights follow)
-    const bool turn = 8 * l < a.R;
-    const int half = a.R / 16;  // lanes between the numbers of a pair
-    long long at = s;
-    if (turn && a.pos) at = a.pos[b * a.pb + s * a.ps];
+    // (the positions' loads and the first rows' are on their way together; angles and weights follow)
     fetch(h);
-    float w[8], c[NEAR ? 4 : 8], n[NEAR ? 4 : 8];
+    float w[8], c[TS][NA], n[TS][NA];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = 1.f;
     if (p.w && 8 * l < a.D) {
@@ -95,23 +104,26 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
         for (int e = 0; e < 8; ++e)
             w[e] = a.w32 ? ((const float*)p.w)[8 * l + e] : (float)((const T*)p.w)[8 * l + e];
     }
-    if (turn) {
-        const bool ok = (unsigned long long)at < a.N;
-        const long long off = (ok ? at : 0) * a.ab + (NEAR ? 4 * l : 8 * (l < half ? l : l - half));
-        const float sign = NEAR || l >= half ? 1.f : -1.f;
 #pragma unroll
-        for (int e = 0; e < (NEAR ? 4 : 8); e += 4) {
-            const f32x4 cc = *reinterpret_cast<const f32x4*>(a.cos + off + e);
-            const f32x4 ss = *reinterpret_cast<const f32x4*>(a.sin + off + e);
+    for (int i = 0; i < TS; ++i) {
+        if (turn) {
+            const bool ok = (unsigned long long)at[i] < a.N;
+            const long long off = (ok ? at[i] : 0) * a.ab + (NEAR ? 4 * l : 8 * (l < half ? l : l - half));
+            const float sign = NEAR || l >= half ? 1.f : -1.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[e + i] = ok ? cc[i] : NAN;
-                n[e + i] = ok ? sign * ss[i] : NAN;
+            for (int e = 0; e < NA; e += 4) {
+                const f32x4 cc = *reinterpret_cast<const f32x4*>(a.cos + off + e);
+                const f32x4 ss = *reinterpret_cast<const f32x4*>(a.sin + off + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    c[i][e + k] = ok ? cc[k] : NAN;
+                    n[i][e + k] = ok ? sign * ss[k] : NAN;
+                }
             }
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int e = 0; e < (NEAR ? 4 : 8); ++e) c[e] = 1.f, n[e] = 0.f;
+            for (int e = 0; e < NA; ++e) c[i][e] = 1.f, n[i][e] = 0.f;
+        }
     }
     const int other = grp * L + (l < half ? l + half : l - half);
 
@@ -119,7 +131,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
         u32x4 now[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) now[u] = raw[u];
-        const int next = h + kUnroll * a.head_next;
+        const int next = h + HS * a.head_next;
         const bool more = __any(next < h1);
         if (more) fetch(next);
 #pragma unroll
@@ -154,25 +166,26 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
                 if constexpr (NEAR) {
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        z[e] = v[e] * c[e / 2] - v[e + 1] * n[e / 2];
-                        z[e + 1] = v[e] * n[e / 2] + v[e + 1] * c[e / 2];
+                        z[e] = v[e] * c[u / HS][e / 2] - v[e + 1] * n[u / HS][e / 2];
+                        z[e + 1] = v[e] * n[u / HS][e / 2] + v[e + 1] * c[u / HS][e / 2];
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = v[e] * c[e] + __shfl(v[e], other) * n[e];
+                    for (int e = 0; e < 8; ++e)
+                        z[e] = v[e] * c[u / HS][e] + __shfl(v[e], other) * n[u / HS][e];
                 }
                 if (turn) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = z[e];
                 }
             }
-            const int hh = h + u * a.head_next;
-            if (live && hh < h1) {
+            const int hh = h + u % HS * a.head_next;
+            if (live[u / HS] && hh < h1) {
                 u32x4 out;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     out[e] = __builtin_bit_cast(unsigned, Elem<T>::cvt2(v[2 * e], v[2 * e + 1]));
-                *reinterpret_cast<u32x4*>(y + hh * p.yh) = out;
+                *reinterpret_cast<u32x4*>(y[u / HS] + hh * p.yh) = out;
             }
         }
         if (!more) break;
@@ -231,20 +244,32 @@ extern "C" int qk_norm_rotate(const void* q, const void* k, void* q_out, void* k
     while (8 * L < D) L *= 2;
     RotateArgs a{};
     const int rg = 64 / L;
-    // Rows of a wave are a token's heads, or a head's tokens where those lie closer and there are
-    // enough of them.
+    // Rows of a wave are a token's heads, or a head's tokens where those lie closer or where heads would
+    // leave places empty, in the wave or in what is in flight. [B, S, H, D] of 40 M numbers, heads
+    // against tokens: D 64, 16 and 4 heads 60 us, 34, 32 and 8 heads 42 us, 33; D 128, 16 and 4 heads
+    // 48 us, 38, 32 and 8 heads 33 us, 36. One head: 334 us against 96, and 55 with four tokens in flight.
     const long long* st = Hq ? q_strides : k_strides;
-    const bool by_token = S >= rg && st[1] < st[2];
+    const long long tokens = (long long)B * S;
+    auto filled = [&](int H) {
+        return !H || (H >= std::max(2 * rg, kUnroll) && 8 * H >= 7 * ((H + rg - 1) / rg * rg));
+    };
+    const bool by_token = tokens >= rg && (st[1] < st[2] || !filled(Hq) || !filled(Hk));
+    // Four tokens a lane in flight take many tokens, lest waves are too few, and few heads, of which one
+    // round is then too little: D 128, 4 and 1 heads, 62500 tokens 51 us -> 41, 15625 tokens 14.6 us ->
+    // 16.3; 16 and 2 heads 37 us -> 38; one head, 15625 tokens 11.8 us -> 8.1, 7812 tokens 6.7 us -> 6.1.
+    const int least = Hq && Hk ? std::min(Hq, Hk) : std::max(Hq, Hk), most_heads = std::max(Hq, Hk);
+    const bool four = by_token && least < kUnroll && most_heads <= kUnroll &&
+                      tokens >= (most_heads == 1 ? 1024LL : 8192LL) * rg;
     a.tok_step = by_token;
     a.head_step = by_token ? 0 : 1;
     a.head_next = by_token ? 1 : rg;
-    const long long tokens = (long long)B * S;
-    a.groups = (unsigned)(by_token ? (tokens + rg - 1) / rg : tokens);
-    // Rounds of a wave: as many as keep 4096 waves (16 a CU) busy, kUnroll at least.
-    const int most = (std::max(Hq, Hk) + a.head_next - 1) / a.head_next;
+    const int set = by_token ? (four ? 4 : 1) * rg : 1;  // tokens of a wave
+    a.groups = (unsigned)((tokens + set - 1) / set);
+    // Rounds of a wave: as many as keep 4096 waves (16 a CU) busy, what is in flight at once at least.
+    const int most = (std::max(Hq, Hk) + a.head_next - 1) / a.head_next, once = four ? 1 : kUnroll;
     const long long rounds_all = a.groups * (long long)((Hq + Hk + a.head_next - 1) / a.head_next);
     const int rounds = (int)std::min<long long>(
-        most, rounds_all < 4096 ? 1 : std::max<long long>(kUnroll, rounds_all / 4096 / kUnroll * kUnroll));
+        most, rounds_all < 4096 ? 1 : std::max<long long>(once, rounds_all / 4096 / once * once));
     a.heads = rounds * a.head_next;
     a.part[0] = Rows{q, q_out, q_weight, 0, 0, 0, 0, 0, 0, Hq, (Hq + a.heads - 1) / a.heads};
     a.part[1] = Rows{k, k_out, k_weight, 0, 0, 0, 0, 0, 0, Hk, (Hk + a.heads - 1) / a.heads};
@@ -275,20 +300,22 @@ extern "C" int qk_norm_rotate(const void* q, const void* k, void* q_out, void* k
         auto run = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
         };
-#define GFX906_ROW(l)                                                                            \
-    case l:                                                                                      \
-        neighbours ? run(norm_rotate_kernel<T, l, true>) : run(norm_rotate_kernel<T, l, false>); \
-        break;
+        auto pick = [&](auto lanes) {
+            constexpr int l = decltype(lanes)::value;
+            if (four)
+                neighbours ? run(norm_rotate_kernel<T, l, true, 4>) : run(norm_rotate_kernel<T, l, false, 4>);
+            else
+                neighbours ? run(norm_rotate_kernel<T, l, true, 1>) : run(norm_rotate_kernel<T, l, false, 1>);
+        };
         switch (L) {
-            GFX906_ROW(1)
-            GFX906_ROW(2)
-            GFX906_ROW(4)
-            GFX906_ROW(8)
-            GFX906_ROW(16)
-            GFX906_ROW(32)
-            GFX906_ROW(64)
+            case 1: return pick(std::integral_constant<int, 1>{});
+            case 2: return pick(std::integral_constant<int, 2>{});
+            case 4: return pick(std::integral_constant<int, 4>{});
+            case 8: return pick(std::integral_constant<int, 8>{});
+            case 16: return pick(std::integral_constant<int, 16>{});
+            case 32: return pick(std::integral_constant<int, 32>{});
+            default: return pick(std::integral_constant<int, 64>{});
         }
-#undef GFX906_ROW
     };
     dtype == KV8_DTYPE_F16 ? go(f16{}) : go(bf16{});
     return g_err.launched(who, hipGetLastError());

@@ -64,6 +64,45 @@ def test_norm_rotate(case, dtype, neighbours):
     check(q, k, wq, wk, cos, sin, positions, 1e-5, neighbours, got)
 
 
+MANY = [  # B, S, Hq, Hk, D, R: few heads of many tokens, whole and with a ragged end
+    (1, 65600, 1, 1, 8, 8), (2, 16387, 1, 0, 16, 16), (3, 2731, 1, 1, 64, 64), (1, 4101, 1, 1, 128, 96),
+    (1, 2049, 1, 1, 200, 192), (3, 2731, 3, 1, 512, 512), (2, 8193, 2, 4, 248, 64), (1, 1024, 1, 0, 512, 0),
+]
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_few_heads_of_many_tokens(case, neighbours):
+    B, S, Hq, Hk, D, R = MANY[case]
+    R = R if neighbours else R // 16 * 16
+    print(f"norm_rotate {MANY[case]} neighbours {neighbours}", flush=True)
+    g = torch.Generator().manual_seed(case)
+    dtype = DTYPES[case % 2]
+    x = (torch.randn(B, S, Hq + 2 * Hk, D, generator=g) * 3).to(dtype).to(DEV)
+    q, k = x[:, :, :Hq], x[:, :, Hq:Hq + Hk] if Hk else None
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(DEV)
+    cos = sin = positions = None
+    if R:
+        cos, sin = qknorm.angles(max(S, 50), R // 2)
+        if case % 2:
+            positions = torch.randint(0, 50, (B, S), generator=g).int().to(DEV)
+            positions[-1, -1] = 2 ** 30          # (no such row: NaN, in its own rows only)
+    want_nan = positions is not None
+    got = qknorm.norm_rotate(q, k, w, w if Hk else None, cos, sin, positions, 1e-6, neighbours)
+    if not Hk:
+        got = (got,)
+    host = [None if t is None else t.cpu() for t in (cos, sin, positions)]
+    for name, t, y in zip("qk", (q, k), got):
+        want, tol = sv.norm_rotate(t.cpu(), w.cpu(), *host, 1e-6, neighbours)
+        assert want.isnan().any() == want_nan
+        close(y, want, tol, name)
+    # over the rows themselves
+    again = qknorm.norm_rotate(q, k, w, w if Hk else None, cos, sin, positions, 1e-6, neighbours,
+                               out=(q, k) if Hk else q)
+    for one, two in zip(got, again if Hk else (again,)):
+        assert torch.equal(one.nan_to_num(7.0), two.nan_to_num(7.0))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_flat_rows_one_tensor_and_no_weight(dtype):
     q = torch.randn(7, 4, 64, device=DEV).to(dtype)
