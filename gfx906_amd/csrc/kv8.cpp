@@ -143,12 +143,15 @@ std::vector<Tensor> kv8_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tenso
     const auto dev = kc.device();
     const Queries n(q, c, table, lens, cu_q, max_q, dev, who);
     Tensor o;
+    bool in_place = false;
     if (out.has_value()) {
         o = *out;
         TORCH_CHECK(o.device() == dev && o.dtype() == q.dtype() && o.sizes() == q.sizes(), who,
                     ": out must have q's shape, dtype and device");
         TORCH_CHECK(o.stride(2) == 1, who, ": out's head dim must be contiguous");
-        at::assert_no_partial_overlap(o, q);
+        in_place = o.data_ptr() == q.data_ptr() && strides2(o) == strides2(q);
+        TORCH_CHECK(in_place || !may_overlap(o.unsqueeze(0), q.unsqueeze(0)), who,
+                    ": out overlaps a part of q");
         for (const Tensor* t : {&kc, &ks, &vc, &vs, &table, &lens}) at::assert_no_overlap(o, *t);
         if (cu_q.has_value()) at::assert_no_overlap(o, *cu_q);
     } else {
@@ -159,7 +162,6 @@ std::vector<Tensor> kv8_attn_op(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tenso
     if (q.numel() == 0 || n.B == 0) return result;
     const c10::DeviceGuard guard(dev);
     // (a workgroup may read rows of q after another has written theirs: q is copied where out is q)
-    const bool in_place = o.data_ptr() == q.data_ptr();
     const Tensor qr = in_place ? q.clone(at::MemoryFormat::Contiguous) : rows_of(q);
     const auto sq = strides2(qr), so = strides2(o);
     const int W = (int)table.size(1);

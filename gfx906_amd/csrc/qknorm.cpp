@@ -15,43 +15,11 @@ using namespace gfx906_amd;
 
 const char* kWho = "norm_rotate";
 
-// {batch, token, head} of a [B, S, H, D] tensor.
-std::array<long long, 3> strides3(const Tensor& t) {
-    std::array<long long, 3> s;
-    for (int d = 0; d < 3; ++d) s[d] = t.size(d) <= 1 ? 0 : t.stride(d);
-    return s;
-}
 bool rows_ok(const Tensor& t) {
     bool ok = (t.size(3) <= 1 || t.stride(3) == 1) &&
               reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     for (long long s : strides3(t)) ok = ok && s >= 0 && s % 8 == 0;
     return ok;
-}
-
-// Whether elements of a and b (same B, S, D) may share memory: they do not where their
-// ranges lie apart, or where they are different parts of every batch's or every token's
-// elements (the projections of q, k and v are parts of one buffer).
-bool may_overlap(const Tensor& a, const Tensor& b) {
-    if (a.numel() == 0 || b.numel() == 0) return false;
-    auto at = [](const Tensor& t) {
-        return (long long)(reinterpret_cast<intptr_t>(t.data_ptr()) / t.element_size());
-    };
-    auto extent = [](const Tensor& t, int from) {  // elements that dims from.. span
-        long long n = 1;
-        for (int d = from; d < 4; ++d) n += (t.size(d) - 1) * t.stride(d);
-        return n;
-    };
-    const long long p = at(a), q = at(b);
-    if (p + extent(a, 0) <= q || q + extent(b, 0) <= p) return false;
-    auto apart = [&](long long period, int from) {
-        if (period <= 0) return false;
-        const long long d = ((q - p) % period + period) % period;
-        return d >= extent(a, from) && d + extent(b, from) <= period;
-    };
-    const auto sa = strides3(a), sb = strides3(b);
-    if (sa[0] == sb[0] && a.size(0) > 1 && apart(sa[0], 1)) return false;
-    return !(sa[1] == sb[1] && a.size(1) > 1 && (a.size(0) == 1 ||
-             (sa[0] == sb[0] && sa[1] > 0 && sa[0] % sa[1] == 0)) && apart(sa[1], 2));
 }
 
 }  // namespace

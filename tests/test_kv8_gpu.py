@@ -423,6 +423,21 @@ def test_attn_refuses():
             kv8.attn(**(ok | bad))
 
 
+def test_out_beside_q_in_one_buffer():
+    """Results may lie in another part of q's projection; a part of q is refused."""
+    cache, _, table = filled([70, 9], 64, 2, 64, torch.float16, seed=1)
+    x = torch.randn(2, 12, 64, device=DEV).half()
+    args = (cache, i32(table), i32([70, 9]), 0.1)
+    want = kv8.attn(x[:, :4].contiguous(), *args)
+    assert torch.equal(kv8.attn(x[:, :4], *args, out=x[:, 8:]), want)
+    assert torch.equal(x[:, 8:], want)
+    for out in (x[:, 1:5], x[:, 3:7], x.view(-1, 64)[:16].view(2, 8, 64)[:, :4]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            kv8.attn(x[:, :4], *args, out=out)
+    assert kv8.attn(x[:, :4], *args, out=x[:, :4]).data_ptr() == x.data_ptr()
+    assert torch.equal(x[:, :4], want)
+
+
 # -- weights of blocks --------------------------------------------------------------------
 
 def weighed(got, want, tol, table, lens, page):
