@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(NT) evict_kernel(const EvictArgs a) {
     const int n = pages_of(len), gone = (int)gone_of(len, keep);
     int* const row = a.table + b * a.table_stride;
     u64* const keys = LDS ? keys_s : a.keys + (long long)b * a.W;
-    const int c0 = a.first, c1 = gone ? n - a.recent : 0;  // candidates
+    const int c0 = gone ? a.first : 0, c1 = gone ? n - a.recent : 0;  // candidates
     const int per = a.Hkv * (a.page / kBlock);
     u64 any = 0, each = ~0ull;
     // (two columns a thread at a time, the weights of both in flight)
@@ -1161,6 +1161,10 @@ extern "C" int kv8_evict(const float* weights, int pages, int Hkv, int page, int
     const size_t need = kv8_evict_workspace_bytes(B, W);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
         return err.fail("%s: workspace misaligned or smaller than kv8_evict_workspace_bytes()", who);
+    // (more of them than a row has columns are as many as it has, and columns past the first ones
+    // then fit an int)
+    first = std::min(first, W);
+    recent = std::min(recent, std::max(W, 1));
     const EvictArgs a{weights, pages, Hkv,  page,       W,    B,        first,    recent,
                       n_free,  table, table_stride, lens, keep, free_pages, used, lens_out,
                       used_out, lost, (unsigned long long*)workspace};
