@@ -125,7 +125,8 @@ def evict(weights, table, lens, keep, free_pages, used, first=1, recent=1) -> Ev
     bits; of equal ones the earlier), but never its ``first`` first ones or its ``recent`` last ones.
 
     ``table`` (int32 ``[B, W]``) closes up in place; the pages go into ``free_pages`` in front of
-    entry ``used`` (int32 ``[1]``), from where :func:`plan_pages` takes them. What is left keeps its order,
-    and whole pages go, so nothing in the cache moves. A page that requests share goes back once for
+    entry ``used`` (int32 ``[1]``), from where :func:`plan_pages` takes them. Entries without a page, which
+    :func:`plan_pages` leaves when there are none, leave the rows before all others, and only pages go back.
+    What is left keeps its order, and whole pages go, so nothing in the cache moves. A page that requests share goes back once for
     each of them."""
     return Evicted(*extension().kv8_evict(weights, table, lens, keep, free_pages, used, first, recent))

@@ -411,15 +411,17 @@ int kv8_weigh(float* weights, const void* q, const long long* q_strides, int dty
               const int* cu_q, int max_q, float scale, int causal, void* workspace,
               size_t workspace_bytes, hipStream_t stream);
 
-/* Every request with more than keep[b] pages (n = ceil(lens[b] / page) of at most W) gives back
+/* Every request with more than keep[b] pages (n = ceil(lens[b] / page) of at most W) loses
  * n - keep[b] of them (fewer, where fewer may go): those of least weight among its pages first ..
  * n - recent - 1, of equal ones the earlier. A page's weight is the sum of weights[page] (fp32
- * [pages, Hkv, page/64]) over heads and blocks in fp64, NaN counting as largest; table entries
- * outside [0, pages) weigh least. The row closes up in place (-1 behind the last page that stays), lens_out[b]
- * = lens[b] less the evicted pages' tokens. The pages given back, in the order of the requests and
+ * [pages, Hkv, page/64]) over heads and blocks in fp64, NaN counting as largest. A table entry
+ * outside [0, pages), as kv4_plan_pages leaves where the free list ends, goes before all of them.
+ * The row closes up in place (-1 behind the last page that stays), lens_out[b] = lens[b] less the
+ * tokens of all that went. The pages that went, in the order of the requests and
  * of their rows, go before free_pages[*used], from where kv4_plan_pages takes pages:
  * into free_pages[*used_out .. *used), *used_out = *used less their number; *lost counts
- * those that had no room (the earlier ones go in). first >= 0, recent >= 1: the last page, which
+ * those that had no room (the earlier ones go in). Entries that name no page count in none of the
+ * three. first >= 0, recent >= 1: the last page, which
  * may be short, always stays. workspace: kv8_evict_workspace_bytes(), 8-byte aligned. */
 size_t kv8_evict_workspace_bytes(int B, int W);
 int kv8_evict(const float* weights, int pages, int Hkv, int page, int* table,

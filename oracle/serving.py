@@ -222,7 +222,8 @@ def weigh(weights, q, lse, cache, table, lens, scale, cu=None, max_q=None, causa
 # -- eviction -----------------------------------------------------------------------------
 
 def evict(weights, page, table, lens, keep, free_pages, used, first, recent):
-    """(table, free pages, lens, used, lost) as lists."""
+    """(table, free pages, lens, used, lost) as lists. Table entries without a page go first; they are
+    none that could be given back."""
     table, free, lens = [list(r) for r in table], list(free_pages), list(lens)
     used = min(max(used, 0), len(free))
     score = weights.double().flatten(1).sum(1).tolist() if len(weights) else []
@@ -239,7 +240,7 @@ def evict(weights, page, table, lens, keep, free_pages, used, first, recent):
             return (2, 0.0, c) if math.isnan(s) else (1, s, c)
 
         gone = sorted(sorted(may, key=rank)[:max(0, n - keep[b])])
-        given += [row[c] for c in gone]
+        given += [row[c] for c in gone if 0 <= row[c] < len(score)]
         left = [row[c] for c in range(n) if c not in set(gone)]
         row[:n] = left + [-1] * len(gone)
         lens[b] -= page * len(gone)

@@ -8,11 +8,23 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 
+# Tests that hold a value since shown to be wrong, and what is right. They run, and have to fail.
+WRONG = {
+    "test_serving_oracle.py::test_eviction_example":
+        "its last line has -1 given back as a page and page 3 lost for it: a table entry without a page "
+        "takes no place in the free list (test_evict_oracle.py)",
+}
+
+
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (gfx950) GPU")
 
 
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        for name, reason in WRONG.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
     try:
         import torch
         have_gpu = torch.cuda.is_available()
