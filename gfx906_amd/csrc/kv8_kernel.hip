@@ -1238,6 +1238,23 @@ extern "C" int kv8_evict(const float* weights, int pages, int Hkv, int page, int
     const size_t need = kv8_evict_workspace_bytes(B, W);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 8)))
         return err.fail("%s: workspace misaligned or smaller than kv8_evict_workspace_bytes()", who);
+    // Every workgroup reads inputs that others' results would overwrite.
+    struct Ints {
+        const int* at;
+        long long n;
+    };
+    const Ints outs[3] = {{lens_out, B}, {used_out, 1}, {lost, 1}};
+    const Ints ins[4] = {{lens, B}, {keep, B}, {used, 1}, {free_pages, n_free}};
+    auto apart = [](const Ints& x, const Ints& y) {
+        const uintptr_t p = (uintptr_t)x.at, q = (uintptr_t)y.at;
+        return !x.n || !y.n || p + 4 * x.n <= q || q + 4 * y.n <= p;
+    };
+    for (int i = 0; i < 3; ++i) {
+        for (const Ints& in : ins)
+            if (!apart(outs[i], in)) return err.fail("%s: results overlap the arguments", who);
+        for (int j = 0; j < i; ++j)
+            if (!apart(outs[i], outs[j])) return err.fail("%s: results overlap each other", who);
+    }
     // (more of them than a row has columns are as many as it has, and columns past the first ones
     // then fit an int)
     first = std::min(first, W);

@@ -422,7 +422,9 @@ int kv8_weigh(float* weights, const void* q, const long long* q_strides, int dty
  * into free_pages[*used_out .. *used), *used_out = *used less their number; *lost counts
  * those that had no room (the earlier ones go in). Entries that name no page count in none of the
  * three. first >= 0, recent >= 1: the last page, which
- * may be short, always stays. workspace: kv8_evict_workspace_bytes(), 8-byte aligned. */
+ * may be short, always stays. lens_out, used_out and lost must not overlap each other or anything else that is
+ * passed (what one request's work writes, another's may still read). workspace:
+ * kv8_evict_workspace_bytes(), 8-byte aligned. */
 size_t kv8_evict_workspace_bytes(int B, int W);
 int kv8_evict(const float* weights, int pages, int Hkv, int page, int* table,
               long long table_stride, int W, const int* lens, const int* keep, int B, int first,
