@@ -148,9 +148,10 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
             float mean = sum * a.inv_d + a.eps, r = __builtin_amdgcn_rsqf(mean);
             const bool big = !(mean < INFINITY), off = big || mean < 0x1p-100f;
             if (__builtin_expect(__any(off), 0)) {
-                // Squares past fp32 (bf16 rows): the row times 2^-80. And what rsq is not made for. (The
-                // wave's other rows keep what they have.)
-                const float f = big ? 0x1p-80f : 1.f;
+                // Squares past fp32 or below its range (bf16 rows): the row times 2^-80 or 2^80, and eps
+                // with its square, in two steps, as 2^160 is no fp32 number. (The wave's other rows
+                // keep what they have.)
+                const float f = big ? 0x1p-80f : off ? 0x1p80f : 1.f;
                 sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const RotateArgs a) {
                 }
 #pragma unroll
                 for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o);
-                if (off) r = 1.0f / sqrtf(sum * a.inv_d + a.eps * (f * f));
+                if (off) r = 1.0f / sqrtf(sum * a.inv_d + a.eps * f * f);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];

@@ -7,9 +7,19 @@ import pytest
 import torch
 
 from gfx906_amd import qknorm
+from oracle import serving as sv
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+def close(got, want, tol):
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.isinf(), want.isinf())
+    worst = ((got - want).abs() / tol)[torch.isfinite(want)].max().item()
+    print(f"  worst {worst:.3f} of the bound", flush=True)
+    assert worst <= 1.0
 
 
 @pytest.mark.parametrize("D", [8, 64, 128, 504])
@@ -25,3 +35,28 @@ def test_a_row_s_result_does_not_depend_on_others(odd, D):
     others = torch.ones(40000, 3, dtype=torch.bool, device=DEV)
     others[::3, 1] = False
     assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1e-25, 1e-20, 1e-16, 1e-15, 1e-10])
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-38])
+def test_small_rows(eps, size):
+    """Rows whose squares are below fp32's range, or have few bits there; of fp32's smallest numbers too."""
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn(1, 50, 2, 128, generator=g) * size).bfloat16()
+    x[0, 3, 0] = 0
+    x[0, 4, 1] = 0
+    x[0, 4, 1, 100] = 2.0 ** -133
+    x[0, 5, 0, :100] = 0
+    got = qknorm.norm_rotate(x.to(DEV), eps=eps)
+    want, tol = sv.norm_rotate(x, None, None, None, None, torch.tensor(eps).float().item(), False)
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e30, 3e38])
+def test_large_rows_and_large_eps(eps):
+    """Sums past fp32 that eps has a share in."""
+    x = torch.randn(1, 9, 2, 64, generator=torch.Generator().manual_seed(2))
+    x = (x * torch.logspace(10, 30, 9)[None, :, None, None]).bfloat16()
+    got = qknorm.norm_rotate(x.to(DEV), eps=eps)
+    want, tol = sv.norm_rotate(x, None, None, None, None, torch.tensor(eps).float().item(), False)
+    close(got, want, tol)
