@@ -68,6 +68,8 @@ std::vector<Tensor> norm_rotate_op(Tensor q, c10::optional<Tensor> k, c10::optio
                         who, ": results must have the shape, type and device of their inputs");
         } else {
             given[i] = both ? part(buf, i ? nq : 0, t.sizes()) : at::empty_like(t);
+            // (a dense input whose head dim is not the innermost one is copied; its order would not do)
+            if (t.numel() && given[i].stride(-1) != 1) given[i] = at::empty(t.sizes(), t.options());
         }
         x[i] = flat ? t.unsqueeze(0) : t;
         y[i] = flat ? given[i].unsqueeze(0) : given[i];

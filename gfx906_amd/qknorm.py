@@ -31,7 +31,8 @@ def norm_rotate(q, k=None, q_weight=None, k_weight=None, cos=None, sin=None, pos
 
     ``q`` is ``[T, Hq, D]`` or ``[B, S, Hq, D]``, ``k`` the same with its own heads (fp16 or bf16, D
     a multiple of 8 up to 512). Strides are free: pass parts of a fused projection as they are, and a
-    ``[B, H, S, D]`` tensor as ``x.transpose(1, 2)`` (results keep the order of dense inputs).
+    ``[B, H, S, D]`` tensor as ``x.transpose(1, 2)`` (results keep the order of dense inputs whose head dim
+    is contiguous; other rows are copied).
     Weights are ``[D]``, of the rows' type or fp32 (None: 1). ``cos`` and ``sin`` are fp32 ``[N, R/2]``
     (None: no rotation); a token's row is its entry in ``positions`` (int32 ``[T]`` or ``[B, S]``) or,
     without them, its place in the sequence. A position outside the tables gives NaN in the turned

@@ -60,3 +60,20 @@ def test_large_rows_and_large_eps(eps):
     got = qknorm.norm_rotate(x.to(DEV), eps=eps)
     want, tol = sv.norm_rotate(x, None, None, None, None, torch.tensor(eps).float().item(), False)
     close(got, want, tol)
+
+
+@pytest.mark.parametrize("tokens", [5, 3000])
+@pytest.mark.parametrize("flat", [False, True])
+def test_dense_rows_whose_dims_are_not_side_by_side(flat, tokens):
+    """[.., D, heads] in memory: copied, as every such input; the results are contiguous."""
+    g = torch.Generator(DEV).manual_seed(3)
+    lead = (tokens,) if flat else (2, tokens)
+    q, k = (torch.randn(*lead, 128, h, device=DEV, generator=g).half().transpose(-1, -2) for h in (6, 2))
+    cos, sin = qknorm.angles(tokens, 64)
+    got = qknorm.norm_rotate(q, k, cos=cos, sin=sin)
+    want = qknorm.norm_rotate(q.contiguous(), k.contiguous(), cos=cos, sin=sin)
+    for a, b, x in zip(got, want, (q, k)):
+        assert a.shape == x.shape and a.stride(-1) == 1 and torch.equal(a, b)
+    # heads last of all, batches between tokens
+    one = torch.randn(tokens, 2, 64, 3, device=DEV, generator=g).half().permute(1, 0, 3, 2)
+    assert torch.equal(qknorm.norm_rotate(one), qknorm.norm_rotate(one.contiguous()))
