@@ -47,30 +47,31 @@ inline std::array<long long, 3> strides3(const Tensor& t) {
     return s;
 }
 
-// Whether elements of a and b (same B, S, D) may share memory: they do not where their
-// ranges lie apart, or where they are different parts of every batch's or every token's
-// elements (the projections of q, k and v are parts of one buffer).
+// Whether elements of a and b, both [B, S, H, D] of one type, may share memory: they do not where their
+// ranges lie apart, nor where they do so modulo a period. Dims whose strides are multiples of the period
+// do not count for that, the others span a range: q, k and v are different parts of every
+// batch's, token's or head's elements of one buffer, in whatever order.
 inline bool may_overlap(const Tensor& a, const Tensor& b) {
     if (a.numel() == 0 || b.numel() == 0) return false;
     auto at = [](const Tensor& t) {
         return (long long)(reinterpret_cast<intptr_t>(t.data_ptr()) / t.element_size());
     };
-    auto extent = [](const Tensor& t, int from) {  // elements that dims from.. span
+    auto extent = [](const Tensor& t, long long period) {  // elements that t spans (0: of all dims)
         long long n = 1;
-        for (int d = from; d < 4; ++d) n += (t.size(d) - 1) * t.stride(d);
+        for (int d = 0; d < 4; ++d)
+            if (!period || t.stride(d) % period) n += (t.size(d) - 1) * t.stride(d);
         return n;
     };
     const long long p = at(a), q = at(b);
     if (p + extent(a, 0) <= q || q + extent(b, 0) <= p) return false;
-    auto apart = [&](long long period, int from) {
-        if (period <= 0) return false;
-        const long long d = ((q - p) % period + period) % period;
-        return d >= extent(a, from) && d + extent(b, from) <= period;
-    };
-    const auto sa = strides3(a), sb = strides3(b);
-    if (sa[0] == sb[0] && a.size(0) > 1 && apart(sa[0], 1)) return false;
-    return !(sa[1] == sb[1] && a.size(1) > 1 && (a.size(0) == 1 ||
-             (sa[0] == sb[0] && sa[1] > 0 && sa[0] % sa[1] == 0)) && apart(sa[1], 2));
+    for (const Tensor* t : {&a, &b})
+        for (int d = 0; d < 3; ++d) {
+            const long long period = t->stride(d);
+            if (period <= 0 || t->size(d) <= 1) continue;
+            const long long from = ((q - p) % period + period) % period;
+            if (from >= extent(a, period) && from + extent(b, period) <= period) return false;
+        }
+    return true;
 }
 
 // A contiguous part of a one-dimensional buffer, made by hand: a view through the dispatcher takes

@@ -77,3 +77,34 @@ def test_dense_rows_whose_dims_are_not_side_by_side(flat, tokens):
     # heads last of all, batches between tokens
     one = torch.randn(tokens, 2, 64, 3, device=DEV, generator=g).half().permute(1, 0, 3, 2)
     assert torch.equal(qknorm.norm_rotate(one), qknorm.norm_rotate(one.contiguous()))
+
+
+PLACES = {  # q and k of one buffer, by how it lies in memory
+    "each head's q, k and v": lambda B, S, H, D: ((B, S, H, 3, D), lambda x: (x[..., 0, :], x[..., 1, :])),
+    "each token's, heads first": lambda B, S, H, D: (
+        (B, H, S, 3, D), lambda x: tuple(x[..., i, :].transpose(1, 2) for i in range(2))),
+    "each batch's": lambda B, S, H, D: ((B, 3, S, H, D), lambda x: (x[:, 0], x[:, 1])),
+    "whole tensors": lambda B, S, H, D: ((3, B, S, H, D), lambda x: (x[0], x[1])),
+    "each token's": lambda B, S, H, D: ((B, S, 3, H, D), lambda x: (x[:, :, 0], x[:, :, 1])),
+}
+
+
+@pytest.mark.parametrize("B", [1, 2])
+@pytest.mark.parametrize("place", PLACES)
+def test_over_themselves_wherever_they_lie(place, B):
+    """q' and k' over q and k, however those share a buffer; the rest of it stays."""
+    S, H, D = 37, 5, 64
+    shape, parts = PLACES[place](B, S, H, D)
+    x = torch.randn(*shape, device=DEV, generator=torch.Generator(DEV).manual_seed(4)).half()
+    q, k = parts(x)
+    cos, sin = qknorm.angles(S, D // 2)
+    want = qknorm.norm_rotate(q, k, cos=cos, sin=sin)
+    y = x.clone()
+    for t, w in zip(parts(y), want):
+        t.copy_(w)
+    qknorm.norm_rotate(q, k, cos=cos, sin=sin, out=(q, k))
+    assert torch.equal(x, y)
+    # over parts that are not their own, or each other's
+    for out in ((k, q), (q, q), (k, None)):
+        with pytest.raises(RuntimeError):
+            qknorm.norm_rotate(q, k, cos=cos, sin=sin, out=out)
