@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using x8 = typename Elem<T>::x8;
     constexpr int DL = D / 8, RW = 256 / DL, PITCH = kBlock + 4;
-    __shared__ unsigned char vb[D * PITCH];
+    __shared__ __attribute__((aligned(16))) unsigned char vb[D * PITCH];  // (written as dwords)
     const int h = blockIdx.y >> 1, dl = threadIdx.x % DL, lane = threadIdx.x & 63;
     const bool is_v = blockIdx.y & 1;
     const long long t0 = blockIdx.x * 64LL;
@@ -486,7 +486,6 @@ __global__ void __launch_bounds__(64, D == 64 ? 8 : 4) weigh_few_kernel(const We
 #if defined(__HIP_DEVICE_COMPILE__)
     using x8 = typename Elem<T>::x8;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     const int hk = blockIdx.y, b = blockIdx.z;
     const Request req = request(a, b);
     const long long chunk = blockIdx.x;
