@@ -257,19 +257,20 @@ extern "C" int qk_norm_rotate(const void* q, const void* k, void* q_out, void* k
         return !H || (H >= std::max(2 * rg, kUnroll) && 8 * H >= 7 * ((H + rg - 1) / rg * rg));
     };
     const bool by_token = tokens >= rg && (st[1] < st[2] || !filled(Hq) || !filled(Hk));
-    // Four tokens a lane in flight take many tokens, lest waves are too few, and few heads, of which one
-    // round is then too little: D 128, 4 and 1 heads, 62500 tokens 51 us -> 41, 15625 tokens 14.6 us ->
-    // 16.3; 16 and 2 heads 37 us -> 38; one head, 15625 tokens 11.8 us -> 8.1, 7812 tokens 6.7 us -> 6.1.
-    const int least = Hq && Hk ? std::min(Hq, Hk) : std::max(Hq, Hk), most_heads = std::max(Hq, Hk);
-    const bool four = by_token && least < kUnroll && most_heads <= kUnroll &&
-                      tokens >= (most_heads == 1 ? 1024LL : 8192LL) * rg;
+    // Four tokens a lane in flight, where there is one head a token, of which one round is too little, and
+    // tokens enough for as many waves. 40 M numbers, us so / with one token, neighbours and halves, in a projection
+    // with far positions: D 40, 1 head of q and k each 62 75 / 84 94, D 128 46 55 / 58 65, 2 heads each 55 62 /
+    // 50 55, 39 46 / 37 41, 3 heads 63 64 / 41 44, 37 43 / 33 33, 4 and 1 57 65 / 44 49, 38 47 / 34 38. One head
+    // of 128, 15625 tokens 8.1 / 11.8, 7812 tokens 6.1 / 6.7.
+    const int most_heads = std::max(Hq, Hk);
+    const bool four = by_token && most_heads == 1 && tokens >= 1024LL * rg;
     a.tok_step = by_token;
     a.head_step = by_token ? 0 : 1;
     a.head_next = by_token ? 1 : rg;
     const int set = by_token ? (four ? 4 : 1) * rg : 1;  // tokens of a wave
     a.groups = (unsigned)((tokens + set - 1) / set);
     // Rounds of a wave: as many as keep 4096 waves (16 a CU) busy, what is in flight at once at least.
-    const int most = (std::max(Hq, Hk) + a.head_next - 1) / a.head_next, once = four ? 1 : kUnroll;
+    const int most = (most_heads + a.head_next - 1) / a.head_next, once = four ? 1 : kUnroll;
     const long long rounds_all = a.groups * (long long)((Hq + Hk + a.head_next - 1) / a.head_next);
     const int rounds = (int)std::min<long long>(
         most, rounds_all < 4096 ? 1 : std::max<long long>(once, rounds_all / 4096 / once * once));
