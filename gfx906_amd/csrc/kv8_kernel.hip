@@ -133,8 +133,8 @@ struct StoreArgs {
 // side by side in V, so that V is written in 16 or 8 bytes without an exchange. Up to four rows
 // (a decoding step) are written as they are where the scale stays, a dword of dims a lane.
 //
-// Bound by bytes: 8 prompts of 500 .. 4096 rows, 16 heads of 128, 41 us (49 without the loads past the
-// caches).
+// Bound by bytes: 8 prompts of 500 .. 4096 rows, 16 heads of 128, 36 us (4.9 TB/s; some 8 more without the
+// loads past the caches).
 template <class T, int D>
 __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -533,12 +533,12 @@ __global__ void __launch_bounds__(64, D == 64 ? 8 : 4) weigh_few_kernel(const We
 
 // Prompts: a workgroup has four blocks of 64 keys, one a wave in registers as above, and a part of the
 // query rows (a.split_rows), which go by through LDS 64 at a time, operand by operand (frag_slot()), the
-// next ones on their way while the four waves use them. Bound by the vector unit: a score costs a
-// product and sum, an exponential (four of the others) and an addition, 1.5 times what the matrix
-// pipe needs for it. Parts' sums go to the workspace, which weigh_join_kernel adds up, so that the
-// order of a sum is set. 3 prompts of 77 .. 2111 queries behind 300 .. 8192 tokens, 16/4 heads of 128: 101 us
-// (86 GFLOP; the vector unit is busy for 63 % of the clocks, the matrix pipe for 34) and 5 for the sums; 275
-// with every wave reading its rows from memory.
+// next ones on their way while the four waves use them. Bound by neither unit alone: a tile's products are
+// issued before its exponentials, so that a wave's matrix and vector work follow each other, and other waves
+// hardly fill the gaps: the vector unit is busy for 63 % of the clocks, the matrix pipe for 34, 97 in all.
+// Parts' sums go to the workspace, which weigh_join_kernel adds up, so that the
+// order of a sum is set. 3 prompts of 77 .. 2111 queries behind 300 .. 8192 tokens, 16/4 heads of 128: 101 to
+// 104 us (86 GFLOP) and 5 for the sums; 275 with every wave reading its rows from memory.
 //
 // grid: parts x groups of four blocks, kv heads, requests.
 template <int D, class T>
@@ -759,7 +759,7 @@ __device__ __forceinline__ int given_back(int gone, int bad) { return gone - min
 // Before several requests' rows close up: how many entries a row loses follows from its length and
 // budget, but which of them name a page only from the table, whose rows a workgroup each rewrites. So
 // the pages that every request gives back are counted first, into lens_out, a wave a request. 64 requests of
-// up to 512 pages 3.1 us.
+// up to 512 pages 3.0 us.
 __global__ void __launch_bounds__(256) evict_count_kernel(const EvictArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const int b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(256) evict_count_kernel(const EvictArgs a) {
 }
 
 // Then added up: lens_out becomes the pages that the requests in front of each give back, and the free
-// list's new end is set. One workgroup; 64 requests 2.3 us. (Counting in this one too: 64 requests of 512
+// list's new end is set. One workgroup; 64 requests 2.5 us. (Counting in this one too: 64 requests of 512
 // pages 15.6 us a call and not 14.1, 1000 of 64 pages 79 and not 18.)
 __global__ void __launch_bounds__(1024) evict_place_kernel(const EvictArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(1024) evict_place_kernel(const EvictArgs a) {
 // histograms of 8 bits from the highest one in which they differ; mostly two or three
 // passes until a bin is taken whole. Then the row closes up, NT columns at a time. Where a request's
 // pages go in the free list evict_place_kernel has written, but for a single request. Bound by
-// latency (dependent steps in one workgroup): 64 requests of up to 512 pages 8.8 us, one of 2048 14.9.
+// latency (dependent steps in one workgroup): 64 requests of up to 512 pages 8.4 us, one of 2048 14.6.
 //
 // LDS: whether the keys are kept there or in the workspace.
 template <int NT, bool LDS>

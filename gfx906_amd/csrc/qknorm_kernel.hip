@@ -7,8 +7,8 @@
 //
 // in fp32, rounded once. Bound by bytes: every row is read and written once, and a
 // token's angles are kept in registers while a wave goes over its heads. 2 x 8192 tokens, 24
-// heads of 64 each in q and k, 36 us: 5.6 TB/s. 32 tokens, 32 and 8 heads of 128: 5.5, a launch
-// and three loads that wait for each other.
+// heads of 64 each in q and k, 36 us in the kernel and 40 a call: 5.1 TB/s. 32 tokens, 32 and 8 heads of
+// 128: 5.4, a launch and three loads that wait for each other.
 #include "longctx.h"
 
 #include <algorithm>

@@ -402,7 +402,8 @@ int kv8_attn(const void* q, void* o, float* lse, const long long* q_strides,
  * arguments and its lse [T, Hq] (packed fp32), the attention that the block's tokens got.
  * weights: fp32 [pages, Hkv, page/64]. Queries past the first max_q of a request do not count. Rows
  * of lse -inf add nothing. Sums are fp32 in an order that sizes alone set; where requests share
- * a page, their sums are added in any order. workspace: kv8_weigh_workspace_bytes() bytes (max_q = 1
+ * a page, their sums are added in any order. Refused: max_q * Hq / Hkv of 2^30 and more, and tables of 2^26
+ * and more blocks over all requests and kv heads. workspace: kv8_weigh_workspace_bytes() bytes (max_q = 1
  * where cu_q is NULL; may be 0), 4-byte aligned. */
 size_t kv8_weigh_workspace_bytes(int T, int B, int Hq, int Hkv, int max_q, int W, int page);
 int kv8_weigh(float* weights, const void* q, const long long* q_strides, int dtype, const float* lse,
